@@ -386,6 +386,190 @@ int mtxc_softmax_lastdim(int dtype, void* dst, const void* src, uint64_t rows, u
                          uint64_t src_row_stride, uint64_t dst_row_stride);
 
 /* ------------------------------------------------------------------------------------------
+ * Row operators of a language model: the passes over HBM around its matrix products, and the rules
+ * applied to its logits before mtxc_softmax_lastdim / mtxc_reduce(ARGMAX) choose a token.  No counterpart
+ * in the reference, which would evaluate each as a trace of broadcast and reduction primitives.
+ *
+ * Common to all: dtype is MTXC_FLOAT, MTXC_FLOAT16 or MTXC_BFLOAT16 (others: MTXC_ERR_UNSUPPORTED_DTYPE).
+ * Arithmetic, sums and statistics are in 32 bits; a result is rounded once, when it is stored.  Strides are
+ * in elements and 64-bit; the innermost axis has unit stride, except where a stride for it is given.
+ * Addresses, sizes and strides need no alignment beyond the element's.  An output may be the very tensor
+ * (pointer and strides) of an input of the same shape; outputs and inputs must not overlap otherwise.
+ * Nothing is allocated; what the calls need of the thread's workspace is stated there.  Sums over rows run in a
+ * fixed order: equal calls give equal bits.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Dropout's random numbers.  Element (row, column) of a [rows, width] tensor takes the 16-bit lane
+ * (column % 8) of Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3",
+ * SC 2011) with the 64-bit key `seed` and the counter words (column / 8, row, offset low, offset high); lanes
+ * count from the low half of the first output word.  It is kept when the lane is below
+ * rint((1 - p) * 65536) and then multiplied by 65536 / that number, so the mean is exact for the probability
+ * that 16 bits can express.  Nothing is stored: a backward pass with the same seed and offset makes the same
+ * mask, whatever the dtype, the strides and the launch.  A step uses another offset (or seed) for each call;
+ * device_offset, if not NULL, is a device pointer to one more offset that is added to `offset` (modulo 2^64)
+ * when the kernel runs, so that a recorded graph can advance it. */
+typedef struct mtxc_dropout_state {
+    double p; /* 0 <= p <= 1; 0: nothing is dropped, 1: everything */
+    uint64_t seed;
+    uint64_t offset;
+    const uint64_t* device_offset;
+} mtxc_dropout_state;
+
+/* dst = dropout(src) on [rows, width]; also its backward pass (gradients in, gradients out).  rows and width
+ * below 2^31. */
+int mtxc_dropout(int dtype, void* dst, const void* src, uint64_t rows, uint64_t width, uint64_t dst_row_stride,
+                 uint64_t src_row_stride, const mtxc_dropout_state* drop);
+
+/* The norms after and before a transformer block, fused with the gate, the dropout and the residual between
+ * them.  For row t and column d, with weights w' = weight_offset + weight:
+ *     n = post_weight ? branch * r * post_w' : branch            r = rsqrt(mean(branch^2) + eps)
+ *     h = residual_scale * residual + branch_scale * gate[t / gate_rows] * dropout(n)
+ *     a = h * s * next_w'                                          s = rsqrt(mean(h^2) + eps)
+ * h goes to residual_out and a to normed, either of which may be NULL; a is computed from h before h is
+ * rounded.  branch NULL: h = residual_scale * residual (post_weight and gate must be NULL, and nothing is
+ * dropped).  post_weight NULL: no norm of the branch.  gate NULL: 1.  next_weight NULL: no second norm (normed
+ * must be NULL).  r and s go to post_rstd / next_rstd (rows floats each) where those are not NULL: the
+ * backward pass reads them.  Weights and gate have dtype weight_dtype / gate_dtype: the tensors' or
+ * MTXC_FLOAT.  The gate has ceil(rows / gate_rows) rows at gate_stride: gate_rows = rows for one gate per
+ * channel, 1 for one per token, a sequence's length for one per sequence.  rows and width below 2^31. */
+typedef struct mtxc_block_norm_args {
+    uint64_t rows, width;
+    const void* residual;
+    uint64_t residual_stride;
+    const void* branch;
+    uint64_t branch_stride;
+    const void* post_weight;
+    const void* next_weight;
+    const void* gate;
+    uint64_t gate_stride, gate_rows;
+    void* residual_out;
+    uint64_t residual_out_stride;
+    void* normed;
+    uint64_t normed_stride;
+    float* post_rstd;
+    float* next_rstd;
+    int weight_dtype, gate_dtype;
+    float residual_scale, branch_scale, weight_offset, eps;
+    mtxc_dropout_state drop;
+} mtxc_block_norm_args;
+int mtxc_block_norm(int dtype, const mtxc_block_norm_args* args);
+
+/* The gradients of mtxc_block_norm, given those of its outputs: d_residual_out (NULL: zero) and d_normed (NULL
+ * if and only if next_weight is NULL), with `residual_out` the stored h, branch, post_rstd and next_rstd of the
+ * forward call and its weights, gate, scales and dropout state.  With p = d_normed * next_w':
+ *     H = d_residual_out + s * p - h * s^3 * mean(p * h)                                (the gradient at h)
+ *     d_residual = residual_scale * H
+ *     q = branch_scale * gate * mask * H,  u = q * post_w'
+ *     d_branch = r * u - branch * r^3 * mean(u * branch)                     (q where there is no post norm)
+ *     d_next_weight = sum_t d_normed * h * s,   d_post_weight = sum_t q * branch * r          (float)
+ *     d_gate[group] = sum over its rows of branch_scale * mask * n * H                     (gate_dtype)
+ * d_residual, d_branch and the last three may each be NULL: not wanted.  d_gate has gate_stride's layout with
+ * its own stride d_gate_stride.  branch NULL (and with it d_branch, post_weight, gate): a norm alone.
+ * The sums over rows are made in 32 bits of per-block partials in the thread's workspace
+ * (MTXC_ERR_WORKSPACE when it cannot hold one block's). */
+typedef struct mtxc_block_norm_backward_args {
+    uint64_t rows, width;
+    const void* d_residual_out;
+    uint64_t d_residual_out_stride;
+    const void* d_normed;
+    uint64_t d_normed_stride;
+    const void* residual_out;
+    uint64_t residual_out_stride;
+    const void* branch;
+    uint64_t branch_stride;
+    const float* post_rstd;
+    const float* next_rstd;
+    const void* post_weight;
+    const void* next_weight;
+    const void* gate;
+    uint64_t gate_stride, gate_rows;
+    void* d_residual;
+    uint64_t d_residual_stride;
+    void* d_branch;
+    uint64_t d_branch_stride;
+    float* d_post_weight;
+    float* d_next_weight;
+    void* d_gate;
+    uint64_t d_gate_stride;
+    int weight_dtype, gate_dtype;
+    float residual_scale, branch_scale, weight_offset;
+    mtxc_dropout_state drop;
+} mtxc_block_norm_backward_args;
+int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backward_args* args);
+
+/* Rotary positions of one or two tensors of heads (queries and keys) in one launch.  Element (b, s, h, d) of
+ * tensor i lies at src[i] + b * src_strides[i][0] + s * src_strides[i][1] + h * src_strides[i][2] + d; heads[i]
+ * == 0: no such tensor (pointers ignored).  The first rotary_dim (even, <= head_dim) elements of a head are
+ * pairs (x, y): (j, j + rotary_dim / 2), or (2j, 2j + 1) with interleaved != 0, for j < rotary_dim / 2.  With
+ * t = positions[b, s] * frequencies[j] (t is negated with inverse != 0):
+ *     (x, y) -> scale * (x cos t - y sin t, x sin t + y cos t)
+ * and the rest of the head is copied.  inverse is the backward pass (the transpose of the rotation times
+ * scale).  frequencies: rotary_dim / 2 doubles on the device, in radians per position; the angle is reduced to
+ * one turn in 64 bits, so that it is right at any position.  positions: int32 or int64 (position_dtype) at
+ * b * position_strides[0] + s * position_strides[1] (0: shared). */
+typedef struct mtxc_rotary_args {
+    uint64_t batch, length;
+    uint32_t head_dim, rotary_dim;
+    uint32_t heads[2];
+    void* dst[2];
+    uint64_t dst_strides[2][3];
+    const void* src[2];
+    uint64_t src_strides[2][3];
+    const void* positions;
+    int position_dtype;
+    uint64_t position_strides[2];
+    const double* frequencies;
+    float scale;
+    int interleaved, inverse;
+} mtxc_rotary_args;
+int mtxc_rotary(int dtype, const mtxc_rotary_args* args);
+
+/* Fills count = rotary_dim / 2 frequencies (host doubles) base^(-2j / rotary_dim), stretched for a context
+ * `factor` times the one trained on, and *scale, the factor for the rotated elements (1 but for BY_PARTS):
+ *   NONE      as they are
+ *   LINEAR    divided by factor (positions interpolated)
+ *   BASE      base * factor^(rotary_dim / (rotary_dim - 2)): the fastest kept, the slowest divided by factor
+ *   BY_PARTS  each divided by factor, kept, or in between, by the number of turns it makes over
+ *             original_length positions: at most slow_turns, at least fast_turns, linear in between
+ *             (Peng, Quesnelle, Fan, Shippole: "YaRN", 2023); *scale = 0.1 ln(factor) + 1
+ * Host only. */
+enum { MTXC_ROTARY_NONE = 0, MTXC_ROTARY_LINEAR = 1, MTXC_ROTARY_BASE = 2, MTXC_ROTARY_BY_PARTS = 3 };
+int mtxc_rotary_frequencies(int scaling, uint32_t rotary_dim, double base, double factor, double original_length,
+                            double fast_turns, double slow_turns, double* frequencies, double* scale);
+
+/* Rules on logits [rows, vocab] before a token is chosen.  For row i, with its tokens tokens[i, 0 .. lengths[i]),
+ * of which the first prompt_lengths[i] are the prompt's and the others generated, and token v:
+ *   1. repetition: where v is among the tokens, l = l > 0 ? l / repetition[i] : l * repetition[i]
+ *   2. frequency, presence: l -= frequency[i] * c + (c ? presence[i] : 0), c = times v was generated
+ *   3. bias: l += bias_values[i, k] for the last k with bias_tokens[i, k] == v
+ *   4. mask: l = -infinity where bit v % 32 of mask[i, v / 32] is 0 (a row without a bit set: all -infinity)
+ * Every rule's pointers may be NULL: the rule is off.  lengths NULL: history for every row; prompt_lengths NULL:
+ * 0.  Both are cut to 0 .. history.  Tokens outside 0 .. vocab - 1 (padding) are passed over, in both lists.  The row
+ * strides of the lists and of the mask (32-bit words) may be 0: shared by all rows.  history and biases below 2^31,
+ * vocab below 2^31. */
+typedef struct mtxc_logits_args {
+    uint64_t rows, vocab;
+    void* dst;
+    uint64_t dst_stride;
+    const void* src;
+    uint64_t src_stride;
+    const int32_t* tokens;
+    uint64_t tokens_stride, history;
+    const int32_t* lengths;
+    const int32_t* prompt_lengths;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int32_t* bias_tokens;
+    uint64_t bias_tokens_stride;
+    const float* bias_values;
+    uint64_t bias_values_stride, biases;
+    const uint32_t* mask;
+    uint64_t mask_stride;
+} mtxc_logits_args;
+int mtxc_logits_rules(int dtype, const mtxc_logits_args* args);
+
+/* ------------------------------------------------------------------------------------------
  * Multi-GPU: one communicator per GPU for reductions over an axis sharded across the GPUs of a node
  * (benchmark configs 4 and 5b).  The reference drives a single Metal device through one GPUManager
  * (Mods/GPUManager.h:53-54); these entry points are the multi-device half of the layer that replaces

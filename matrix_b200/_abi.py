@@ -6,6 +6,7 @@ This is the binding a Python caller of the C ABI needs; it loads the in-tree lib
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libmtxc.so"
@@ -28,6 +29,42 @@ UNARY_OPS = {"exp": 0, "sqrt": 1}
 STATS = {"mean": 0, "rms": 1, "norm": 2}
 POINTWISE_OPS = {"greater": 0, "less": 1, "logical_and": 2, "where": 3, "floor": 4, "full": 5, "arctan2": 6,
                  "arcsin": 7}
+
+
+
+def _layout(*fields: str) -> struct.Struct:
+    """A C struct of include/mtxc.h as its fields in order, each "name:type" (struct module letters, native
+    alignment); packed bytes are passed as the pointer to it."""
+    return struct.Struct("@" + "".join(f.split(":")[1] for f in fields) + "0P")
+
+
+DROPOUT_FIELDS = ("p:d", "seed:Q", "offset:Q", "device_offset:P")
+DROPOUT_STATE = _layout(*DROPOUT_FIELDS)
+BLOCK_NORM_FIELDS = (
+    "rows:Q", "width:Q", "residual:P", "residual_stride:Q", "branch:P", "branch_stride:Q", "post_weight:P",
+    "next_weight:P", "gate:P", "gate_stride:Q", "gate_rows:Q", "residual_out:P", "residual_out_stride:Q", "normed:P",
+    "normed_stride:Q", "post_rstd:P", "next_rstd:P", "weight_dtype:i", "gate_dtype:i", "residual_scale:f",
+    "branch_scale:f", "weight_offset:f", "eps:f", *("drop." + f for f in DROPOUT_FIELDS))
+BLOCK_NORM_ARGS = _layout(*BLOCK_NORM_FIELDS)
+BLOCK_NORM_BACKWARD_FIELDS = (
+    "rows:Q", "width:Q", "d_residual_out:P", "d_residual_out_stride:Q", "d_normed:P", "d_normed_stride:Q",
+    "residual_out:P", "residual_out_stride:Q", "branch:P", "branch_stride:Q", "post_rstd:P", "next_rstd:P",
+    "post_weight:P", "next_weight:P", "gate:P", "gate_stride:Q", "gate_rows:Q", "d_residual:P", "d_residual_stride:Q",
+    "d_branch:P", "d_branch_stride:Q", "d_post_weight:P", "d_next_weight:P", "d_gate:P", "d_gate_stride:Q",
+    "weight_dtype:i", "gate_dtype:i", "residual_scale:f", "branch_scale:f", "weight_offset:f",
+    *("drop." + f for f in DROPOUT_FIELDS))
+BLOCK_NORM_BACKWARD_ARGS = _layout(*BLOCK_NORM_BACKWARD_FIELDS)
+ROTARY_FIELDS = (
+    "batch:Q", "length:Q", "head_dim:I", "rotary_dim:I", "heads:2I", "dst:2P", "dst_strides:6Q", "src:2P",
+    "src_strides:6Q", "positions:P", "position_dtype:i", "position_strides:2Q", "frequencies:P", "scale:f",
+    "interleaved:i", "inverse:i")
+ROTARY_ARGS = _layout(*ROTARY_FIELDS)
+LOGITS_FIELDS = (
+    "rows:Q", "vocab:Q", "dst:P", "dst_stride:Q", "src:P", "src_stride:Q", "tokens:P", "tokens_stride:Q", "history:Q",
+    "lengths:P", "prompt_lengths:P", "repetition:P", "frequency:P", "presence:P", "bias_tokens:P",
+    "bias_tokens_stride:Q", "bias_values:P", "bias_values_stride:Q", "biases:Q", "mask:P", "mask_stride:Q")
+LOGITS_ARGS = _layout(*LOGITS_FIELDS)
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "by_parts": 3}
 
 
 class MtxcError(RuntimeError):
@@ -99,6 +136,13 @@ def lib() -> C.CDLL:
             "mtxc_reduce_sharded": (i32, [i32, i32, vp, vp, u32, u32, u32, U32P, U32P, U32P, C.POINTER(C.c_int64)]),
             "mtxc_allreduce": (i32, [i32, i32, vp, u64]),
             "mtxc_arange": (i32, [i32, vp, vp, vp, u64]),
+            "mtxc_dropout": (i32, [i32, vp, vp, u64, u64, u64, u64, C.c_char_p]),
+            "mtxc_block_norm": (i32, [i32, C.c_char_p]),
+            "mtxc_block_norm_backward": (i32, [i32, C.c_char_p]),
+            "mtxc_rotary": (i32, [i32, C.c_char_p]),
+            "mtxc_rotary_frequencies": (i32, [i32, u32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double,
+                                              C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+            "mtxc_logits_rules": (i32, [i32, C.c_char_p]),
             "mtxc_graph_begin": (i32, []),
             "mtxc_graph_end": (i32, [C.POINTER(vp)]),
             "mtxc_graph_launch": (i32, [vp]),

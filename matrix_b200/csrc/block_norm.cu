@@ -56,6 +56,294 @@ struct Forward {
     DropArgs drop;
 };
 
+// ------------------------------------------------------------------------------------------
+// A thread's share of a row: chunks of eight elements.  VEC: eight consecutive columns, one access per chunk
+// (16 bytes of a half type, 32 of float); else a warp takes 256 consecutive columns and a lane every 32nd of
+// them, so that scalar accesses of rows of any width and alignment are contiguous across the warp.
+// ------------------------------------------------------------------------------------------
+template <typename T, bool VEC>
+struct Chunk {
+    uint32_t c;  // first column
+    // chunk k of thread `tid` of `threads` that share a row
+    __device__ __forceinline__ Chunk(uint32_t k, uint32_t threads, uint32_t tid)
+        : c(VEC ? (k * threads + tid) * 8 : (k * threads + (tid & ~31u)) * 8 + tid % 32) {}
+    __device__ __forceinline__ uint32_t column(int j) const { return VEC ? c + j : c + 32 * j; }
+    // whether element j lies in the row (VEC: all eight do or none)
+    __device__ __forceinline__ bool inside(int j, uint32_t width) const { return VEC ? c < width : c + 32 * j < width; }
+
+    __device__ __forceinline__ Eight<T> load(const T* row, uint32_t width) const {
+        Eight<T> v;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < (int)(2 * sizeof(T)); ++i) v.w[i] = 0;
+            if (c < width) v.load(row + c);
+        } else {
+            T e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = inside(j, width) ? row[c + 32 * j] : T(0.0f);
+            memcpy(v.w, e, sizeof(e));
+        }
+        return v;
+    }
+    __device__ __forceinline__ void store(T* row, uint32_t width, const float2 (&v)[4]) const {
+        Eight<T> o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.set2(j, v[j].x, v[j].y);
+        if constexpr (VEC) {
+            if (c < width) o.store(row + c);
+        } else {
+            T e[8];
+            memcpy(e, o.w, sizeof(e));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (inside(j, width)) row[c + 32 * j] = e[j];
+        }
+    }
+    // Eight values of a weight or gate row, shared by many rows and so left in L1 (0 outside the row).
+    __device__ __forceinline__ void param(const void* p, uint64_t at, bool is_float, uint32_t width, float2 (&v)[4]) const {
+        if constexpr (VEC) {
+            if (c >= width) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = make_float2(0.0f, 0.0f);
+            } else if (std::is_same_v<T, float> || is_float) {
+                const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + c);
+                const float4 a = __ldg(q), b = __ldg(q + 1);
+                v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w);
+                v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+            } else if constexpr (sizeof(T) == 2) {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + at + c));
+                const Eight<T> e{{a.x, a.y, a.z, a.w}};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = e.get2(j);
+            }
+        } else {
+            auto one = [&](int j) { return inside(j, width) ? mtxc::param<T>(p, at + c + 32 * j, is_float) : 0.0f; };
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = make_float2(one(2 * j), one(2 * j + 1));
+        }
+    }
+    // The column block whose counter this lane makes: its own, or one of the warp's 32.
+    __device__ __forceinline__ uint32_t block() const { return VEC ? c / 8 : c / 8 - threadIdx.x % 32 / 8 + threadIdx.x % 32; }
+};
+
+// Zeroes the dropped ones of a thread's K chunks of a row; the whole warp takes part.  Counters are made two
+// at a time: more would hold too many registers.
+template <typename T, bool VEC, int K>
+__device__ __forceinline__ void drop(const DropArgs& d, uint32_t row, uint32_t threads, uint32_t tid, float2 (&v)[K][4]) {
+    constexpr int N = K < 2 ? K : 2;
+    const Philox rng(d);
+    const uint32_t lane = threadIdx.x % 32;
+#pragma unroll
+    for (int k = 0; k < K; k += N) {
+        uint32_t block[N], rows[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) block[i] = Chunk<T, VEC>(k + i, threads, tid).block(), rows[i] = row;
+        Lanes l[N];
+        rng.make(block, rows, l);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (VEC) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[k + i][j].x = l[i].keeps(d, 2 * j) ? v[k + i][j].x : 0.0f;
+                    v[k + i][j].y = l[i].keeps(d, 2 * j + 1) ? v[k + i][j].y : 0.0f;
+                }
+            } else {  // each lane's eight bits go to the eight lanes that hold their columns
+                uint32_t own = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) own |= l[i].keeps(d, j) ? 1u << j : 0u;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t bits = __shfl_sync(0xffffffffu, own, j * 4 + lane / 8);
+                    float& e = j % 2 ? v[k + i][j / 2].y : v[k + i][j / 2].x;
+                    e = bits >> (lane % 8) & 1u ? e : 0.0f;
+                }
+            }
+        }
+    }
+}
+
+// Which of a thread's E elements of a row are kept, as bits; the whole warp takes part.
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ uint32_t kept_bits(const DropArgs& d, uint32_t row, uint32_t threads, uint32_t tid) {
+    constexpr int K = E / 8, N = K < 2 ? K : 2;
+    const Philox rng(d);
+    uint32_t own = 0, bits = 0;
+#pragma unroll
+    for (int k = 0; k < K; k += N) {
+        uint32_t block[N], rows[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) block[i] = Chunk<T, VEC>(k + i, threads, tid).block(), rows[i] = row;
+        Lanes l[N];
+        rng.make(block, rows, l);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) own |= l[i].keeps(d, j) ? 1u << (8 * (k + i) + j) : 0u;
+    }
+    if (VEC) return own;
+    const uint32_t lane = threadIdx.x % 32;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // each lane's bits go to the eight lanes that hold their columns
+        const uint32_t from = __shfl_sync(0xffffffffu, own, j * 4 + lane / 8) >> (lane % 8);
+#pragma unroll
+        for (int k = 0; k < K; ++k) bits |= (from >> (8 * k) & 1u) << (8 * k + j);
+    }
+    return bits;
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Sums N values over the threads that share a row: a warp (part unused), or a block of at most 1024 threads
+// through part[N][32], which no earlier sum of the row has used.
+template <int N, bool WARP>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* part) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    if constexpr (!WARP) {
+        const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[i * 32 + warp] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? part[i * 32 + lane] : 0.0f);
+    }
+}
+
+// Rows held in registers, E elements per thread: read once, written once.  WARP: a warp per row, eight rows
+// per block; else a block per row.
+template <typename T, int E, bool VEC, bool WARP, int BLOCK, int MIN>
+__global__ void __launch_bounds__(BLOCK, MIN) block_norm_kernel(const Forward f) {
+    constexpr int K = E / 8;
+    __shared__ float part[2][32];
+    const uint32_t threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x % 32 : threadIdx.x;
+    const uint32_t row = WARP ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+    if (WARP && row >= f.rows) return;
+    const uint32_t width = f.width;
+    Eight<T> x[K];
+    float2 h[K][4];  // first the branch, stage by stage, then h; arithmetic two elements at a time
+    if (f.b) {
+        Eight<T> b[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            b[k] = Chunk<T, VEC>(k, threads, tid).load(static_cast<const T*>(f.b) + row * f.bs, width);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            x[k] = Chunk<T, VEC>(k, threads, tid).load(static_cast<const T*>(f.x) + row * f.xs, width);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[k][j] = b[k].get2(j);
+        if (f.w_post) {
+            float2 q = both(0.0f);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q = __ffma2_rn(h[k][j], h[k][j], q);
+            float sum[1] = {q.x + q.y};
+            row_sum<1, WARP>(sum, part[0]);
+            const float r = rsqrtf(sum[0] / width + f.eps);
+            if (f.post_rstd && tid == 0) f.post_rstd[row] = r;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float2 w[4];
+                Chunk<T, VEC>(k, threads, tid).param(f.w_post, 0, f.w_float, width, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = __fmul2_rn(h[k][j], __ffma2_rn(both(r), w[j], both(r * f.w0)));
+            }
+        }
+        float beta = f.beta;
+        if (f.drop.on) {
+            beta *= f.drop.scale;
+            drop<T, VEC>(f.drop, row, threads, tid, h);
+        }
+        if (f.gate) {
+            const uint64_t g0 = row / f.gate_rows * f.gs;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float2 w[4];
+                Chunk<T, VEC>(k, threads, tid).param(f.gate, g0, f.g_float, width, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = __fmul2_rn(h[k][j], w[j]);
+            }
+        }
+        if (f.alpha == 1.0f) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = __ffma2_rn(both(beta), h[k][j], x[k].get2(j));
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = __ffma2_rn(both(beta), h[k][j], __fmul2_rn(both(f.alpha), x[k].get2(j)));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            x[k] = Chunk<T, VEC>(k, threads, tid).load(static_cast<const T*>(f.x) + row * f.xs, width);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[k][j] = __fmul2_rn(both(f.alpha), x[k].get2(j));
+    }
+    if (f.h) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            Chunk<T, VEC>(k, threads, tid).store(static_cast<T*>(f.h) + row * f.hs, width, h[k]);
+    }
+    if (!f.w_next) return;
+    float2 q = both(0.0f);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q = __ffma2_rn(h[k][j], h[k][j], q);
+    float sum[1] = {q.x + q.y};
+    row_sum<1, WARP>(sum, part[1]);
+    const float s = rsqrtf(sum[0] / width + f.eps);
+    if (f.a) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const Chunk<T, VEC> ch(k, threads, tid);
+            float2 w[4];
+            ch.param(f.w_next, 0, f.w_float, width, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[k][j] = __fmul2_rn(h[k][j], __ffma2_rn(both(s), w[j], both(s * f.w0)));
+            ch.store(static_cast<T*>(f.a) + row * f.as, width, h[k]);
+        }
+    }
+    if (f.next_rstd && tid == 0) f.next_rstd[row] = s;
+}
+
+// Elements per thread E, threads and blocks per SM, by width (measured on a B200 with a gate per channel, GB/s of
+// the bytes that have to move, the best against the next):
+//   a warp per row to 256 columns, and to 512 where accesses are vectors ([32768, 512] bf16 5446, a block 4699)
+//   half types, vectors: E = 16 to 1024 ([16384, 1024] bf16 with dropout 4471, E = 8 3847, a warp 3902), then 32, whose
+//     blocks of 256 hold more of a row in their registers ([16384, 2048] 5647, E = 16 5352, E = 8 4722)
+//   float, and scalar accesses: E = 8 to 4096 ([16384, 2047] bf16 2780, E = 16 2563, E = 32 1320), which needs the
+//     fewest registers, then 16 ([8192, 4097] bf16 2893, E = 8 in blocks of 1024 2340)
+// Wider rows return -1.
+template <typename T, bool VEC>
+int launch_forward(const Forward& f, cudaStream_t st) {
+    constexpr bool kHalfVec = VEC && sizeof(T) == 2;
+    auto threads = [&](uint32_t e) { return (f.width + 32 * e - 1) / (32 * e) * 32; };
+    const unsigned warps = (f.rows + 7) / 8;
+    if (f.width <= 256) block_norm_kernel<T, 8, VEC, true, 256, 1><<<warps, 256, 0, st>>>(f);
+    else if (f.width > 16384) return -1;
+    else if constexpr (kHalfVec) {
+        if (f.width <= 512) block_norm_kernel<T, 16, VEC, true, 256, 1><<<warps, 256, 0, st>>>(f);
+        else if (f.width <= 1024) block_norm_kernel<T, 16, VEC, false, 64, 1><<<f.rows, threads(16), 0, st>>>(f);
+        else if (f.width <= 8192) block_norm_kernel<T, 32, VEC, false, 256, 3><<<f.rows, threads(32), 0, st>>>(f);
+        else block_norm_kernel<T, 32, VEC, false, 512, 2><<<f.rows, threads(32), 0, st>>>(f);
+    } else {
+        if (f.width <= 4096) block_norm_kernel<T, 8, VEC, false, 512, 3><<<f.rows, threads(8), 0, st>>>(f);
+        else block_norm_kernel<T, 16, VEC, false, 1024, 1><<<f.rows, threads(16), 0, st>>>(f);
+    }
+    return check_launch("block_norm_kernel");
+}
+
 // Any width, stride and alignment: a block per row, which reads its row once for each sum.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) block_norm_any_kernel(const Forward f) {
@@ -77,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_any_kernel(const Forward 
             if (!f.b) return h;
             float n = to_float(b[c]);
             if (f.w_post) n *= r * (f.w0 + param<T>(f.w_post, c, f.w_float));
-            if (f.drop.on) n = Philox::lane(rng(c / 8, row), c % 8) < f.drop.kept ? n * f.drop.scale : 0.0f;
+            if (f.drop.on) n = rng(c / 8, row).at(c % 8) < f.drop.kept ? n * f.drop.scale : 0.0f;
             if (f.gate) n *= param<T>(f.gate, g0 + c, f.g_float);
             return h + f.beta * n;
         };
@@ -168,7 +456,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
             };
             auto mask = [&](uint32_t c) {
                 if (!f.drop.on) return f.beta;
-                return Philox::lane(rng(c / 8, row), c % 8) < f.drop.kept ? f.beta * f.drop.scale : 0.0f;
+                return rng(c / 8, row).at(c % 8) < f.drop.kept ? f.beta * f.drop.scale : 0.0f;
             };
             float sum[3] = {0.0f, 0.0f, 0.0f};
             for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
@@ -216,6 +504,267 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
     });
 }
 
+// The rows of a run: contiguous, so that the next ones can be fetched ahead across gate rows.
+__device__ __forceinline__ void run_rows(const Backward& f, uint32_t run, uint32_t& first, uint32_t& last) {
+    if (f.parts > 1) {
+        const uint64_t start = (uint64_t)(run / f.parts) * f.gate_rows, n = min((uint64_t)f.gate_rows, f.rows - start);
+        const uint32_t part = run % f.parts;
+        first = (uint32_t)(start + n * part / f.parts);
+        last = (uint32_t)(start + n * (part + 1) / f.parts);
+    } else {
+        first = (uint32_t)((uint64_t)f.groups * run / f.runs * f.gate_rows);
+        last = (uint32_t)min((uint64_t)f.groups * (run + 1) / f.runs * f.gate_rows, (uint64_t)f.rows);
+    }
+}
+
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+// The four rows that a row of the backward pass reads, as one thread's chunks.  VEC: copied to shared memory
+// `stages` rows ahead by the thread that reads them, which therefore needs no barrier; else in registers.
+template <typename T, int K, bool VEC>
+struct Inputs {
+    static constexpr int kPieces = sizeof(Eight<T>) / 16;
+    uint4* ring;  // this thread's first slot; slots of a block's threads lie side by side
+    uint32_t stride;
+    Eight<T> regs[VEC ? 1 : 4][VEC ? 1 : K];
+
+    __device__ __forceinline__ static const T* base(const Backward& f, int i) {
+        return static_cast<const T*>(i == 0 ? f.dh : i == 1 ? f.da : i == 2 ? f.h : f.b);
+    }
+    __device__ __forceinline__ static uint64_t row_stride(const Backward& f, int i) {
+        return i == 0 ? f.dhs : i == 1 ? f.das : i == 2 ? f.hs : f.bs;
+    }
+    __device__ __forceinline__ void fetch(const Backward& f, uint32_t row, uint32_t stage, uint32_t threads, uint32_t tid) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T* p = base(f, i);
+            if (!p) continue;
+            p += row * row_stride(f, i);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const Chunk<T, VEC> ch(k, threads, tid);
+                if constexpr (VEC) {
+                    if (ch.c >= f.width) continue;
+#pragma unroll
+                    for (int v = 0; v < kPieces; ++v)
+                        copy16(ring + (((stage * 4 + i) * K + k) * kPieces + v) * stride,
+                               reinterpret_cast<const uint4*>(p + ch.c) + v);
+                } else regs[i][k] = ch.load(p, f.width);
+            }
+        }
+    }
+    __device__ __forceinline__ Eight<T> get(int i, int k, uint32_t stage) const {
+        if constexpr (VEC) {
+            Eight<T> e;
+#pragma unroll
+            for (int v = 0; v < kPieces; ++v) {
+                const uint4 q = ring[(((stage * 4 + i) * K + k) * kPieces + v) * stride];
+                e.w[4 * v] = q.x, e.w[4 * v + 1] = q.y, e.w[4 * v + 2] = q.z, e.w[4 * v + 3] = q.w;
+            }
+            return e;
+        } else return regs[i][k];
+    }
+};
+
+// A thread's share of a partial-sum row.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_sums(const Chunk<T, VEC>& ch, float* row, uint32_t width, const float2 (&v)[4]) {
+    if constexpr (VEC) {
+        if (ch.c >= width) return;
+        float4* p = reinterpret_cast<float4*>(row + ch.c);
+        p[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        p[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (ch.inside(j, width)) row[ch.column(j)] = j % 2 ? v[j / 2].y : v[j / 2].x;
+    }
+}
+
+// Rows read once: E elements per thread, the sums over rows in registers.  A run of rows for each warp (WARP) or
+// block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.
+template <typename T, int E, bool VEC, bool WARP, bool MULTI, int BLOCK, int MIN>
+__global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t stages) {
+    constexpr int K = E / 8;
+    extern __shared__ uint4 ring[];
+    __shared__ float part[2][3 * 32];
+    const uint32_t threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x % 32 : threadIdx.x;
+    const uint32_t run = WARP ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+    if (WARP && run >= f.runs) return;
+    const uint32_t width = f.width;
+    uint32_t first, last;
+    run_rows(f, run, first, last);
+    Inputs<T, K, VEC> in;
+    in.ring = ring + threadIdx.x;
+    in.stride = blockDim.x;
+    if constexpr (VEC) {
+        for (uint32_t i = 0; i < stages; ++i) {
+            if (first + i < last) in.fetch(f, first + i, i, threads, tid);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    }
+    float2 A[K][4], S[K][4], W[MULTI ? K : 1][4];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            A[k][j] = S[k][j] = both(0.0f);
+            if (MULTI) W[k][j] = both(0.0f);
+        }
+    const bool has_b = f.b, has_post = f.w_post, has_next = f.w_next, has_gate = f.gate, drops = f.drop.on && has_b;
+    const bool want_s = f.part_post || f.dgate;
+    const float cf = drops ? f.beta * f.drop.scale : f.beta;
+    uint32_t group = first / f.gate_rows, group_left = f.gate_rows - first % f.gate_rows;
+    for (uint32_t row = first, stage = 0; row < last; ++row) {
+        if constexpr (VEC) {
+            if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        } else in.fetch(f, row, 0, threads, tid);
+        const uint64_t g0 = group * f.gs;
+        const float r = has_post ? f.post_rstd[row] : 1.0f, s = has_next ? f.next_rstd[row] : 0.0f;
+        const Eight<T> zero{};
+        uint32_t kept = 0xFFFFFFFFu;
+        if (drops) kept = kept_bits<T, E, VEC>(f.drop, row, threads, tid);
+        auto mask = [&](float2 v, int k, int j) {
+            return make_float2(kept >> (8 * k + 2 * j) & 1u ? v.x : 0.0f, kept >> (8 * k + 2 * j + 1) & 1u ? v.y : 0.0f);
+        };
+        float2 c1 = both(0.0f), su = both(0.0f), sv = both(0.0f);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const Chunk<T, VEC> ch(k, threads, tid);
+            if (VEC && ch.c >= width) continue;
+            const Eight<T> h = f.h ? in.get(2, k, stage) : zero;
+            float2 p[4] = {}, w[4];
+            if (has_next) {
+                const Eight<T> da = in.get(1, k, stage);
+                ch.param(f.w_next, 0, f.w_float, width, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] = __fmul2_rn(da.get2(j), __fadd2_rn(both(f.w0), w[j]));
+                    c1 = __ffma2_rn(p[j], h.get2(j), c1);
+                }
+            }
+            if (has_post) {
+                const Eight<T> b = in.get(3, k, stage), dh = f.dh ? in.get(0, k, stage) : zero;
+                float2 e[4];
+                ch.param(f.w_post, 0, f.w_float, width, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) e[j] = __fmul2_rn(b.get2(j), __fadd2_rn(both(f.w0), w[j]));
+                if (has_gate) {
+                    ch.param(f.gate, g0, f.g_float, width, w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = __fmul2_rn(e[j], w[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (drops) e[j] = mask(e[j], k, j);
+                    su = __ffma2_rn(e[j], __ffma2_rn(both(s), p[j], dh.get2(j)), su);
+                    sv = __ffma2_rn(e[j], h.get2(j), sv);
+                }
+            }
+        }
+        float sum[3] = {c1.x + c1.y, su.x + su.y, sv.x + sv.y};
+        row_sum<3, WARP>(sum, part[(row - first) % 2]);
+        const float kappa = s * s * s * (sum[0] / width);
+        const float c2 = r * r * r * (cf * (sum[1] - kappa * sum[2]) / width);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const Chunk<T, VEC> ch(k, threads, tid);
+            if (VEC && ch.c >= width) continue;
+            const Eight<T> h = f.h ? in.get(2, k, stage) : zero;
+            float2 H[4], w[4];
+            const Eight<T> dh = f.dh ? in.get(0, k, stage) : zero;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) H[j] = __ffma2_rn(both(-kappa), h.get2(j), dh.get2(j));
+            if (has_next) {
+                const Eight<T> da = in.get(1, k, stage);
+                ch.param(f.w_next, 0, f.w_float, width, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 d = __fmul2_rn(both(s), da.get2(j));
+                    H[j] = __ffma2_rn(d, __fadd2_rn(both(f.w0), w[j]), H[j]);
+                    A[k][j] = __ffma2_rn(d, h.get2(j), A[k][j]);
+                }
+            }
+            if (f.dx) {
+                float2 o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = __fmul2_rn(both(f.alpha), H[j]);
+                ch.store(static_cast<T*>(f.dx) + row * f.dxs, width, o);
+            }
+            if (has_b) {
+                const Eight<T> b = in.get(3, k, stage);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (drops) H[j] = mask(H[j], k, j);
+                    H[j] = __fmul2_rn(both(cf), H[j]);
+                    S[k][j] = __ffma2_rn(H[j], __fmul2_rn(both(r), b.get2(j)), S[k][j]);
+                }
+                if (has_gate) {
+                    ch.param(f.gate, g0, f.g_float, width, w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) H[j] = __fmul2_rn(H[j], w[j]);
+                }
+                if (has_post) {
+                    ch.param(f.w_post, 0, f.w_float, width, w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        H[j] = __ffma2_rn(__fmul2_rn(both(r), H[j]), __fadd2_rn(both(f.w0), w[j]),
+                                          __fmul2_rn(both(-c2), b.get2(j)));
+                }
+                if (f.db) ch.store(static_cast<T*>(f.db) + row * f.dbs, width, H);
+            }
+        }
+        if constexpr (VEC) {
+            if (row + stages < last) in.fetch(f, row + stages, stage, threads, tid);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            stage = stage + 1 == stages ? 0 : stage + 1;
+        }
+        if (--group_left == 0 || row + 1 == last) {  // the last of the gate row's rows in this run
+            if (MULTI && want_s) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const Chunk<T, VEC> ch(k, threads, tid);
+                    float2 w[4];
+                    ch.param(f.gate, g0, f.g_float, width, w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) W[MULTI ? k : 0][j] = __ffma2_rn(w[j], S[k][j], W[MULTI ? k : 0][j]);
+                    if (f.dgate) {
+                        if (has_post) {
+                            ch.param(f.w_post, 0, f.w_float, width, w);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) S[k][j] = __fmul2_rn(S[k][j], __fadd2_rn(both(f.w0), w[j]));
+                        }
+                        if (f.g_float) store_sums(ch, static_cast<float*>(f.dgate) + group * f.dgs, width, S[k]);
+                        else ch.store(static_cast<T*>(f.dgate) + group * f.dgs, width, S[k]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) S[k][j] = both(0.0f);
+                }
+            }
+            if (row + 1 < last) ++group, group_left = f.gate_rows;
+        }
+    }
+    if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const Chunk<T, VEC> ch(k, threads, tid);
+        if (f.part_next) store_sums(ch, f.part_next + (uint64_t)run * width, width, A[k]);
+        if (!MULTI && f.part_gate) store_sums(ch, f.part_gate + (uint64_t)run * width, width, S[k]);
+        if (f.part_post) {
+            if (!MULTI && has_gate) {
+                float2 w[4];
+                ch.param(f.gate, group * f.gs, f.g_float, width, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) S[k][j] = __fmul2_rn(w[j], S[k][j]);
+            }
+            store_sums(ch, f.part_post + (uint64_t)run * width, width, MULTI ? W[MULTI ? k : 0] : S[k]);
+        }
+    }
+}
+
 // Adds the blocks' partial sums in order: first the plain sums (dw_next, dw_post), then each gate row's.
 struct Finish {
     const float* part[2];
@@ -243,6 +792,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_finish_kernel(const Finis
     float v = 0.0f;
     if (c < f.width) {
         const uint32_t end = (uint32_t)((uint64_t)n * (warp + 1) / warps);
+#pragma unroll 8
         for (uint32_t i = (uint32_t)((uint64_t)n * warp / warps); i < end; ++i) v += part[(uint64_t)i * f.width + c];
     }
     sums[warp][lane] = v;
@@ -258,6 +808,68 @@ __global__ void __launch_bounds__(kThreads) block_norm_finish_kernel(const Finis
         else static_cast<T*>(f.dgate)[group * f.dgs + c] = from_float<T>(v);
     }
 }
+
+// Which backward kernel serves a width, and with what blocks.
+struct Plan {
+    int kind = -1;  // -1: block_norm_backward_any_kernel
+    uint32_t threads = kThreads, runs_per_block = 1, blocks_per_sm = 2, stages = 1;
+    size_t smem = 0;
+};
+
+constexpr size_t kMaxShared = 227 * 1024;
+
+template <typename T>
+Plan plan_backward(uint32_t width, bool vec) {
+    Plan p;
+    uint32_t e = 16, regs = 64;  // elements and registers of a thread
+    if (width <= 256) p.kind = 0, e = 8;
+    else if (vec && width <= 512) p.kind = 1;
+    else if (vec && width <= 8192) p.kind = 2, regs = 128;
+    else if (vec && width <= 16384) p.kind = 3;
+    else if (!vec && width <= 4096) p.kind = 4, e = 8, regs = 128;
+    else if (!vec && width <= 8192) p.kind = 5, e = 8;
+    else return p;
+    if (p.kind <= 1) p.threads = 256, p.runs_per_block = 8, regs = 96;
+    else p.threads = (width + 32 * e - 1) / (32 * e) * 32;
+    p.blocks_per_sm = std::min(2048 / p.threads, std::max(1u, 65536 / (p.threads * regs)));
+    if (vec) {
+        const size_t stage = (size_t)p.threads * 4 * e * sizeof(T);
+        if (stage > kMaxShared - 2048) return Plan();
+        p.stages = 2 * stage <= kMaxShared - 2048 ? 2 : 1;
+        p.smem = p.stages * stage;
+        p.blocks_per_sm = std::max<uint32_t>(1, std::min<uint32_t>(p.blocks_per_sm, kMaxShared / (p.smem + 2048)));
+    }
+    return p;
+}
+
+template <typename T, int E, bool VEC, bool WARP, bool MULTI, int BLOCK, int MIN>
+int launch_backward_kernel(const Backward& f, const Plan& p, cudaStream_t st) {
+    auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, BLOCK, MIN>;
+    if (p.smem > 46 * 1024) {  // the kernel has static shared memory too
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+        if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(block_norm_backward_kernel)");
+    }
+    kernel<<<(f.runs + p.runs_per_block - 1) / p.runs_per_block, p.threads, p.smem, st>>>(f, p.stages);
+    return check_launch("block_norm_backward_kernel");
+}
+
+template <typename T, bool MULTI>
+int launch_backward(const Backward& f, const Plan& p, bool vec, cudaStream_t st) {
+    switch (p.kind) {
+        case 0:
+            return vec ? launch_backward_kernel<T, 8, true, true, MULTI, 256, 2>(f, p, st)
+                       : launch_backward_kernel<T, 8, false, true, MULTI, 256, 2>(f, p, st);
+        case 1: return launch_backward_kernel<T, 16, true, true, MULTI, 256, 2>(f, p, st);
+        case 2: return launch_backward_kernel<T, 16, true, false, MULTI, 512, 1>(f, p, st);
+        case 3: return launch_backward_kernel<T, 16, true, false, MULTI, 1024, 1>(f, p, st);
+        case 4: return launch_backward_kernel<T, 8, false, false, MULTI, 512, 1>(f, p, st);
+        case 5: return launch_backward_kernel<T, 8, false, false, MULTI, 1024, 1>(f, p, st);
+        default: block_norm_backward_any_kernel<T><<<f.runs, kThreads, 0, st>>>(f); return check_launch("block_norm_backward_any_kernel");
+    }
+}
+
+// What eight consecutive parameters need for 16-byte accesses (any of the float-like types).
+bool param_aligned(const void* p, uint64_t stride) { return aligned16(p) && stride % 8 == 0; }
 
 // Checks what both directions share; returns MTXC_OK or an error status.
 int check_common(const std::string& who, int dtype, uint64_t rows, uint64_t width, bool branch, const void* post_weight,
@@ -325,11 +937,19 @@ extern "C" int mtxc_block_norm(int dtype, const mtxc_block_norm_args* a) {
     f.w0 = a->weight_offset;
     f.eps = a->eps;
     const unsigned grid = (unsigned)std::min<uint64_t>(f.rows, (uint64_t)ctx().sm_count * 8);
+    int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        block_norm_any_kernel<T><<<grid, kThreads, 0, ctx().stream()>>>(f);
+        const bool vec = f.width % 8 == 0 && eight_aligned<T>(f.x, f.xs) && eight_aligned<T>(f.b, f.bs) &&
+                         eight_aligned<T>(f.h, f.hs) && eight_aligned<T>(f.a, f.as) && param_aligned(f.w_post, 0) &&
+                         param_aligned(f.w_next, 0) && param_aligned(f.gate, f.gs);
+        rc = vec ? launch_forward<T, true>(f, ctx().stream()) : launch_forward<T, false>(f, ctx().stream());
+        if (rc == -1) {
+            block_norm_any_kernel<T><<<grid, kThreads, 0, ctx().stream()>>>(f);
+            rc = check_launch("block_norm_any_kernel");
+        }
     });
-    return check_launch("block_norm_any_kernel");
+    return rc;
 }
 
 extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backward_args* a) {
@@ -386,10 +1006,20 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     f.beta = a->branch_scale;
     f.w0 = a->weight_offset;
 
-    // blocks: two per SM, as many as there are rows and the workspace holds partial sums for
+    // runs of rows: what fills the GPU, no more than there are rows and the workspace holds partial sums for
+    bool vec = false;
+    Plan plan;
+    dispatch_float(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        vec = f.width % 8 == 0 && eight_aligned<T>(f.dh, f.dhs) && eight_aligned<T>(f.da, f.das) &&
+              eight_aligned<T>(f.h, f.hs) && eight_aligned<T>(f.b, f.bs) && eight_aligned<T>(f.dx, f.dxs) &&
+              eight_aligned<T>(f.db, f.dbs) && param_aligned(f.w_post, 0) && param_aligned(f.w_next, 0) &&
+              param_aligned(f.gate, f.gs) && eight_aligned<T>(f.dgate, f.dgs);
+        plan = plan_backward<T>(f.width, vec);
+    });
     const int sums = !!a->d_next_weight + !!a->d_post_weight + !!a->d_gate;
     const uint64_t row_bytes = (uint64_t)f.width * sizeof(float) * sums;
-    uint64_t runs = std::min<uint64_t>(f.rows, (uint64_t)ctx().sm_count * 2);
+    uint64_t runs = std::min<uint64_t>(f.rows, (uint64_t)ctx().sm_count * plan.blocks_per_sm * plan.runs_per_block);
     if (row_bytes) runs = std::min<uint64_t>(runs, ctx().workspace_bytes / row_bytes);
     if (runs == 0)
         return fail(MTXC_ERR_WORKSPACE, who + ": one block's partial sums need " + std::to_string(row_bytes) +
@@ -420,10 +1050,11 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     e.g_float = f.g_float;
     e.w0 = f.w0;
     const uint32_t jobs = e.plain + (f.part_gate && f.parts > 1 ? f.groups : 0);
+    int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        block_norm_backward_any_kernel<T><<<f.runs, kThreads, 0, st>>>(f);
-        if (jobs) block_norm_finish_kernel<T><<<dim3((f.width + 31) / 32, jobs), kThreads, 0, st>>>(e);
+        rc = f.gate && f.parts == 1 ? launch_backward<T, true>(f, plan, vec, st) : launch_backward<T, false>(f, plan, vec, st);
+        if (rc == MTXC_OK && jobs) block_norm_finish_kernel<T><<<dim3((f.width + 31) / 32, jobs), kThreads, 0, st>>>(e);
     });
-    return check_launch("block_norm_backward");
+    return rc == MTXC_OK ? check_launch("block_norm_finish_kernel") : rc;
 }

@@ -39,27 +39,42 @@ def _on_device(x: torch.Tensor, *others) -> int:
     return dev
 
 
-def _empty(shape, dtype: torch.dtype, dev: int, strides=None) -> torch.Tensor:
-    """A tensor from the memory of the stream that the kernels run on."""
-    raw = lib().mtxc_get_stream() or 0
-    if raw != torch._C._cuda_getCurrentRawStream(dev):
-        with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=dev)):
-            return _new(shape, dtype, dev, strides)
-    return _new(shape, dtype, dev, strides)
+def _own_memory(dev: int) -> bool:
+    """Whether torch's current stream is the one that the kernels run on."""
+    return (lib().mtxc_get_stream() or 0) == torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _new(shape, dtype, dev, strides):
-    device = torch.device("cuda", dev)
-    if strides is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+def _on_stream(dev: int):
+    """Makes the stream that the kernels run on torch's current one, so that new tensors come from its memory."""
+    return torch.cuda.stream(torch.cuda.ExternalStream(lib().mtxc_get_stream() or 0, device=dev))
+
+
+def _new(x: torch.Tensor, shape, dtype: torch.dtype, dev: int) -> torch.Tensor:
+    """A contiguous tensor on x's device, from the memory of the stream that the kernels run on."""
+    if _own_memory(dev):
+        return x.new_empty(shape, dtype=dtype)
+    with _on_stream(dev):
+        return x.new_empty(shape, dtype=dtype)
+
+
+def _new_like(x: torch.Tensor, dev: int) -> torch.Tensor:
+    """The same with x's shape and dtype."""
+    if x.is_contiguous():
+        if _own_memory(dev):
+            return torch.empty_like(x)
+        with _on_stream(dev):
+            return torch.empty_like(x)
+    return _new(x, x.shape, x.dtype, dev)
 
 
 def _row_stride(t: torch.Tensor, what: str, written: bool = False) -> int:
     """The stride from row to row of a tensor whose leading axes fold into one."""
-    shape, strides = t.shape, t.stride()
-    n = len(shape)
+    shape = t.shape
     width = shape[-1]
+    if t.is_contiguous():
+        return width
+    strides = t.stride()
+    n = len(shape)
     if width > 1 and strides[-1] != 1:
         raise ValueError(f"{what}: the last axis needs unit stride")
     stride, span = width, 0  # span: the extent so far times its stride, which the next axis out must continue
@@ -80,7 +95,7 @@ def _row_stride(t: torch.Tensor, what: str, written: bool = False) -> int:
 
 def _like(x: torch.Tensor, out: torch.Tensor | None, what: str, dev: int) -> torch.Tensor:
     if out is None:
-        return _empty(x.shape, x.dtype, dev)
+        return _new_like(x, dev)
     if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev:
         raise ValueError(f"{what}: expected a tensor of the input's shape, dtype and device")
     return out
@@ -110,13 +125,15 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int, *, device_offset:
     code = dtype_code(x.dtype)
     state = _abi.DROPOUT_STATE.pack(*_drop(p, seed, offset, device_offset, dev))
     out = _like(x, out, "out", dev)
-    if x.dim() == 0:
-        check(lib().mtxc_dropout(code, out.data_ptr(), x.data_ptr(), 1, 1, 1, 1, state))
+    n = x.numel()
+    if n == 0:
         return out
-    width = x.shape[-1]
-    rows = x.numel() // width if width else 0
-    check(lib().mtxc_dropout(code, out.data_ptr(), x.data_ptr(), rows, width, _row_stride(out, "out", True),
-                             _row_stride(x, "x"), state))
+    width = x.shape[-1] if x.dim() else 1
+    if out.is_contiguous() and x.is_contiguous():
+        xs = os = width
+    else:
+        xs, os = _row_stride(x, "x"), _row_stride(out, "out", True)
+    check(lib().mtxc_dropout(code, out.data_ptr(), x.data_ptr(), n // width, width, os, xs, state))
     return out
 
 
@@ -218,9 +235,9 @@ def block_norm(residual: torch.Tensor, branch: torch.Tensor | None = None, *, po
     post_rstd = next_rstd = None
     if save_rstd:
         if post_weight is not None:
-            post_rstd = _empty((rows,), torch.float32, dev)
+            post_rstd = _new(residual, (rows,), torch.float32, dev)
         if next_weight is not None:
-            next_rstd = _empty((rows,), torch.float32, dev)
+            next_rstd = _new(residual, (rows,), torch.float32, dev)
     g_ptr, g_stride, g_code, g_rows = _gate(gate, residual, rows)
     check(lib().mtxc_block_norm(code, _abi.BLOCK_NORM_ARGS.pack(
         rows, width, residual.data_ptr(), _row_stride(residual, "residual"),
@@ -264,12 +281,11 @@ def block_norm_backward(d_residual: torch.Tensor | None, d_normed: torch.Tensor 
         raise ValueError("post_weight and gate need a branch")
     width = residual.shape[-1]
     rows = residual.numel() // width if width else 0
-    dx = _empty(residual.shape, residual.dtype, dev)
-    db = _empty(residual.shape, residual.dtype, dev) if branch is not None else None
-    dp = _empty((width,), torch.float32, dev) if parameters and post_weight is not None else None
-    dn = _empty((width,), torch.float32, dev) if parameters and next_weight is not None else None
-    dg = _empty(gate.shape, gate.dtype, dev) if parameters and gate is not None else None
-
+    dx = _new(residual, residual.shape, residual.dtype, dev)
+    db = _new(residual, residual.shape, residual.dtype, dev) if branch is not None else None
+    dp = _new(residual, (width,), torch.float32, dev) if parameters and post_weight is not None else None
+    dn = _new(residual, (width,), torch.float32, dev) if parameters and next_weight is not None else None
+    dg = _new(gate, gate.shape, gate.dtype, dev) if parameters and gate is not None else None
     if rows == 0 and dg is not None:  # a sum over no rows (the call itself knows of no gate row then)
         check(lib().mtxc_memset(dg.data_ptr(), 0, dg.numel() * dg.element_size()))
 
@@ -313,7 +329,11 @@ def _heads(x: torch.Tensor | None, out: torch.Tensor | None, what: str, dev: int
     if x.shape[-1] > 1 and x.stride(-1) != 1:
         raise ValueError(f"{what}: the last axis needs unit stride")
     if out is None:
-        out = _empty_like(x, dev)
+        if _own_memory(dev):
+            out = torch.empty_like(x)
+        else:
+            with _on_stream(dev):
+                out = torch.empty_like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev:
         raise ValueError(f"{what}'s output: expected its shape, dtype and device")
     elif out.shape[-1] > 1 and out.stride(-1) != 1:
@@ -322,14 +342,6 @@ def _heads(x: torch.Tensor | None, out: torch.Tensor | None, what: str, dev: int
     if x.dim() == 3:
         xs, os = (0, *xs), (0, *os)
     return out, x.shape[-2], out.data_ptr(), x.data_ptr(), os, xs
-
-
-def _empty_like(x: torch.Tensor, dev: int) -> torch.Tensor:
-    raw = lib().mtxc_get_stream() or 0
-    if raw != torch._C._cuda_getCurrentRawStream(dev):
-        with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=dev)):
-            return torch.empty_like(x)
-    return torch.empty_like(x)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *,

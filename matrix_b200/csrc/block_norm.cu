@@ -163,34 +163,49 @@ __device__ __forceinline__ void drop(const DropArgs& d, uint32_t row, uint32_t t
     }
 }
 
-// Which of a thread's E elements of a row are kept, as bits; the whole warp takes part.
-template <typename T, int E, bool VEC>
-__device__ __forceinline__ uint32_t kept_bits(const DropArgs& d, uint32_t row, uint32_t threads, uint32_t tid) {
-    constexpr int K = E / 8, N = K < 2 ? K : 2;
-    const Philox rng(d);
-    uint32_t own = 0, bits = 0;
+// Which of a thread's K chunks of a row are kept, held for several uses: the lanes themselves where a chunk is one
+// counter's columns, else bits.  The whole warp makes them.
+template <typename T, int K, bool VEC>
+struct Kept {
+    Lanes lanes[VEC ? K : 1];
+    uint32_t bits = 0;
+
+    __device__ __forceinline__ void make(const DropArgs& d, uint32_t row, uint32_t threads, uint32_t tid) {
+        const Philox rng(d);
+        uint32_t block[K], rows[K];
 #pragma unroll
-    for (int k = 0; k < K; k += N) {
-        uint32_t block[N], rows[N];
+        for (int k = 0; k < K; ++k) block[k] = Chunk<T, VEC>(k, threads, tid).block(), rows[k] = row;
+        if constexpr (VEC) rng.make(block, rows, lanes);
+        else {
+            Lanes l[K];
+            rng.make(block, rows, l);
+            uint32_t own = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) block[i] = Chunk<T, VEC>(k + i, threads, tid).block(), rows[i] = row;
-        Lanes l[N];
-        rng.make(block, rows, l);
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+                for (int j = 0; j < 8; ++j) own |= l[k].keeps(d, j) ? 1u << (8 * k + j) : 0u;
+            const uint32_t lane = threadIdx.x % 32;
+            bits = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) own |= l[i].keeps(d, j) ? 1u << (8 * (k + i) + j) : 0u;
+            for (int j = 0; j < 8; ++j) {  // each lane's bits go to the eight lanes that hold their columns
+                const uint32_t from = __shfl_sync(0xffffffffu, own, j * 4 + lane / 8) >> (lane % 8);
+#pragma unroll
+                for (int k = 0; k < K; ++k) bits |= (from >> (8 * k) & 1u) << (8 * k + j);
+            }
+        }
     }
-    if (VEC) return own;
-    const uint32_t lane = threadIdx.x % 32;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {  // each lane's bits go to the eight lanes that hold their columns
-        const uint32_t from = __shfl_sync(0xffffffffu, own, j * 4 + lane / 8) >> (lane % 8);
-#pragma unroll
-        for (int k = 0; k < K; ++k) bits |= (from >> (8 * k) & 1u) << (8 * k + j);
+    __device__ __forceinline__ bool at(const DropArgs& d, int k, int j) const {
+        if constexpr (VEC) return lanes[k].keeps(d, j);
+        else return bits >> (8 * k + j) & 1u;
     }
-    return bits;
-}
+    __device__ __forceinline__ void zero_others(const DropArgs& d, int k, float2 (&v)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j].x = at(d, k, 2 * j) ? v[j].x : 0.0f;
+            v[j].y = at(d, k, 2 * j + 1) ? v[j].y : 0.0f;
+        }
+    }
+};
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
@@ -405,7 +420,8 @@ struct Backward {
     bool w_float, g_float;
     float alpha, beta, w0;
     DropArgs drop;
-    // partial sums, one row of `width` floats per block each; NULL: not wanted
+    // partial sums, one row of `width` floats per run each; NULL: not wanted.  Where runs share gate rows there is
+    // no part_post: S, in part_gate, gives both sums.
     float *part_next, *part_post, *part_gate;
     uint32_t groups, parts;  // gate rows (1 without a gate), blocks per gate row (1: blocks take whole gate rows)
     uint32_t runs;           // blocks
@@ -438,7 +454,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
         if (f.part_next) f.part_next[own + c] = 0.0f;
         if (f.part_post) f.part_post[own + c] = 0.0f;
     }
-    const bool want_s = f.part_post || f.dgate;
+    const bool want_s = f.part_post || f.part_gate;
     for_each_segment(f, blockIdx.x, [&](uint32_t group, uint32_t first, uint32_t last) {
         auto gate = [&](uint32_t c) { return f.gate ? param<T>(f.gate, group * f.gs + c, f.g_float) : 1.0f; };
         auto post = [&](uint32_t c) { return f.w_post ? f.w0 + param<T>(f.w_post, c, f.w_float) : 1.0f; };
@@ -530,11 +546,23 @@ struct Inputs {
     uint32_t stride;
     Eight<T> regs[VEC ? 1 : 4][VEC ? 1 : K];
 
+    // h serves the next norm alone (and the post norm's sums where there is one): without it, it is not read
     __device__ __forceinline__ static const T* base(const Backward& f, int i) {
-        return static_cast<const T*>(i == 0 ? f.dh : i == 1 ? f.da : i == 2 ? f.h : f.b);
+        return static_cast<const T*>(i == 0 ? f.dh : i == 1 ? f.da : i == 2 ? (f.w_next ? f.h : nullptr) : f.b);
     }
     __device__ __forceinline__ static uint64_t row_stride(const Backward& f, int i) {
         return i == 0 ? f.dhs : i == 1 ? f.das : i == 2 ? f.hs : f.bs;
+    }
+    // Zeros for what is never fetched: absent rows, and chunks outside the row.
+    __device__ __forceinline__ void absent(const Backward& f, uint32_t stages) {
+        if constexpr (VEC) {
+            for (uint32_t i = 0; i < stages * 4 * K * kPieces; ++i) ring[i * stride] = make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < K; ++k) regs[i][k] = Eight<T>{};
+        }
     }
     __device__ __forceinline__ void fetch(const Backward& f, uint32_t row, uint32_t stage, uint32_t threads, uint32_t tid) {
 #pragma unroll
@@ -584,8 +612,11 @@ __device__ __forceinline__ void store_sums(const Chunk<T, VEC>& ch, float* row, 
 }
 
 // Rows read once: E elements per thread, the sums over rows in registers.  A run of rows for each warp (WARP) or
-// block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.
-template <typename T, int E, bool VEC, bool WARP, bool MULTI, int BLOCK, int MIN>
+// block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.  SHARED: a
+// thread keeps its columns' w_next' and gate * w_post' in shared memory, as floats ready for use, for the run (or the
+// gate row); else they are made from the parameters for each row.  Inputs that the call does not have read as
+// zeros, weights as ones: fewer branches.
+template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool SHARED, int BLOCK, int MIN>
 __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t stages) {
     constexpr int K = E / 8;
     extern __shared__ uint4 ring[];
@@ -594,17 +625,63 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
     const uint32_t run = WARP ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
     if (WARP && run >= f.runs) return;
     const uint32_t width = f.width;
+    const bool has_b = f.b, has_post = f.w_post, has_next = f.w_next, has_gate = f.gate, drops = f.drop.on && has_b;
+    const bool want_s = f.part_post || f.dgate;
+    const float cf = drops ? f.beta * f.drop.scale : f.beta;
     uint32_t first, last;
     run_rows(f, run, first, last);
+    uint32_t group = first / f.gate_rows, group_left = f.gate_rows - first % f.gate_rows;
+
     Inputs<T, K, VEC> in;
     in.ring = ring + threadIdx.x;
     in.stride = blockDim.x;
+    uint4* const weights = in.ring + (VEC ? stages * 4 * K * Inputs<T, K, VEC>::kPieces : 0) * blockDim.x;
+    in.absent(f, stages);
     if constexpr (VEC) {
         for (uint32_t i = 0; i < stages; ++i) {
             if (first + i < last) in.fetch(f, first + i, i, threads, tid);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
+    // which = 0: w_next', 1: gate * w_post'
+    auto make_weights = [&](int which, int k, float2 (&w)[4]) {
+        const Chunk<T, VEC> ch(k, threads, tid);
+        const void* p = which ? f.w_post : f.w_next;
+        if (p) {
+            ch.param(p, 0, f.w_float, width, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __fadd2_rn(both(f.w0), w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = both(1.0f);
+        }
+        if (which && has_gate) {
+            float2 g[4];
+            ch.param(f.gate, group * f.gs, f.g_float, width, g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __fmul2_rn(g[j], w[j]);
+        }
+    };
+    auto keep_weights = [&](int which) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float2 w[4];
+            make_weights(which, k, w);
+            float4* q = reinterpret_cast<float4*>(weights + (which * K + k) * 2 * blockDim.x);
+            q[0] = make_float4(w[0].x, w[0].y, w[1].x, w[1].y);
+            q[blockDim.x] = make_float4(w[2].x, w[2].y, w[3].x, w[3].y);
+        }
+    };
+    auto get_weights = [&](int which, int k, float2 (&w)[4]) {
+        if constexpr (SHARED) {
+            const float4* q = reinterpret_cast<const float4*>(weights + (which * K + k) * 2 * blockDim.x);
+            const float4 a = q[0], b = q[blockDim.x];
+            w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
+            w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
+        } else make_weights(which, k, w);
+    };
+    if constexpr (SHARED) keep_weights(0), keep_weights(1);
+
     float2 A[K][4], S[K][4], W[MULTI ? K : 1][4];
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -613,56 +690,41 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             A[k][j] = S[k][j] = both(0.0f);
             if (MULTI) W[k][j] = both(0.0f);
         }
-    const bool has_b = f.b, has_post = f.w_post, has_next = f.w_next, has_gate = f.gate, drops = f.drop.on && has_b;
-    const bool want_s = f.part_post || f.dgate;
-    const float cf = drops ? f.beta * f.drop.scale : f.beta;
-    uint32_t group = first / f.gate_rows, group_left = f.gate_rows - first % f.gate_rows;
+    // the next row's deviations are on their way while a row is worked on
+    float next_r = 1.0f, next_s = 0.0f;
+    auto load_rstd = [&](uint32_t row) {
+        if (has_post) next_r = __ldg(f.post_rstd + row);
+        if (has_next) next_s = __ldg(f.next_rstd + row);
+    };
+    if (first < last) load_rstd(first);
     for (uint32_t row = first, stage = 0; row < last; ++row) {
+        const float r = next_r, s = next_s;
+        if (row + 1 < last) load_rstd(row + 1);
         if constexpr (VEC) {
             if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
             else asm volatile("cp.async.wait_group 0;" ::: "memory");
         } else in.fetch(f, row, 0, threads, tid);
-        const uint64_t g0 = group * f.gs;
-        const float r = has_post ? f.post_rstd[row] : 1.0f, s = has_next ? f.next_rstd[row] : 0.0f;
-        const Eight<T> zero{};
-        uint32_t kept = 0xFFFFFFFFu;
-        if (drops) kept = kept_bits<T, E, VEC>(f.drop, row, threads, tid);
-        auto mask = [&](float2 v, int k, int j) {
-            return make_float2(kept >> (8 * k + 2 * j) & 1u ? v.x : 0.0f, kept >> (8 * k + 2 * j + 1) & 1u ? v.y : 0.0f);
-        };
+        Kept<T, K, VEC> kept;
+        if (drops) kept.make(f.drop, row, threads, tid);
         float2 c1 = both(0.0f), su = both(0.0f), sv = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const Chunk<T, VEC> ch(k, threads, tid);
-            if (VEC && ch.c >= width) continue;
-            const Eight<T> h = f.h ? in.get(2, k, stage) : zero;
-            float2 p[4] = {}, w[4];
-            if (has_next) {
-                const Eight<T> da = in.get(1, k, stage);
-                ch.param(f.w_next, 0, f.w_float, width, w);
+            const Eight<T> dh = in.get(0, k, stage), da = in.get(1, k, stage), h = in.get(2, k, stage),
+                           b = in.get(3, k, stage);
+            float2 p[4], e[4];
+            get_weights(0, k, p);
+            get_weights(1, k, e);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[j] = __fmul2_rn(da.get2(j), __fadd2_rn(both(f.w0), w[j]));
-                    c1 = __ffma2_rn(p[j], h.get2(j), c1);
-                }
+            for (int j = 0; j < 4; ++j) {
+                p[j] = __fmul2_rn(da.get2(j), p[j]);
+                e[j] = __fmul2_rn(b.get2(j), e[j]);
             }
-            if (has_post) {
-                const Eight<T> b = in.get(3, k, stage), dh = f.dh ? in.get(0, k, stage) : zero;
-                float2 e[4];
-                ch.param(f.w_post, 0, f.w_float, width, w);
+            if (drops) kept.zero_others(f.drop, k, e);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e[j] = __fmul2_rn(b.get2(j), __fadd2_rn(both(f.w0), w[j]));
-                if (has_gate) {
-                    ch.param(f.gate, g0, f.g_float, width, w);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) e[j] = __fmul2_rn(e[j], w[j]);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (drops) e[j] = mask(e[j], k, j);
-                    su = __ffma2_rn(e[j], __ffma2_rn(both(s), p[j], dh.get2(j)), su);
-                    sv = __ffma2_rn(e[j], h.get2(j), sv);
-                }
+            for (int j = 0; j < 4; ++j) {
+                c1 = __ffma2_rn(p[j], h.get2(j), c1);
+                su = __ffma2_rn(e[j], __ffma2_rn(both(s), p[j], dh.get2(j)), su);
+                sv = __ffma2_rn(e[j], h.get2(j), sv);
             }
         }
         float sum[3] = {c1.x + c1.y, su.x + su.y, sv.x + sv.y};
@@ -672,63 +734,45 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const Chunk<T, VEC> ch(k, threads, tid);
-            if (VEC && ch.c >= width) continue;
-            const Eight<T> h = f.h ? in.get(2, k, stage) : zero;
-            float2 H[4], w[4];
-            const Eight<T> dh = f.dh ? in.get(0, k, stage) : zero;
+            const Eight<T> dh = in.get(0, k, stage), da = in.get(1, k, stage), h = in.get(2, k, stage),
+                           b = in.get(3, k, stage);
+            float2 H[4], w[4], o[4];
+            get_weights(0, k, w);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) H[j] = __ffma2_rn(both(-kappa), h.get2(j), dh.get2(j));
-            if (has_next) {
-                const Eight<T> da = in.get(1, k, stage);
-                ch.param(f.w_next, 0, f.w_float, width, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 d = __fmul2_rn(both(s), da.get2(j));
-                    H[j] = __ffma2_rn(d, __fadd2_rn(both(f.w0), w[j]), H[j]);
-                    A[k][j] = __ffma2_rn(d, h.get2(j), A[k][j]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                const float2 d = __fmul2_rn(both(s), da.get2(j));
+                A[k][j] = __ffma2_rn(d, h.get2(j), A[k][j]);
+                H[j] = __ffma2_rn(d, w[j], __ffma2_rn(both(-kappa), h.get2(j), dh.get2(j)));
+                o[j] = __fmul2_rn(both(f.alpha), H[j]);
             }
-            if (f.dx) {
-                float2 o[4];
+            if (f.dx) ch.store(static_cast<T*>(f.dx) + row * f.dxs, width, o);
+            if (!has_b) continue;
+            if (drops) kept.zero_others(f.drop, k, H);
+            get_weights(1, k, w);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = __fmul2_rn(both(f.alpha), H[j]);
-                ch.store(static_cast<T*>(f.dx) + row * f.dxs, width, o);
+            for (int j = 0; j < 4; ++j) {
+                H[j] = __fmul2_rn(both(cf * r), H[j]);
+                S[k][j] = __ffma2_rn(H[j], b.get2(j), S[k][j]);
+                H[j] = __fmul2_rn(H[j], w[j]);
             }
-            if (has_b) {
-                const Eight<T> b = in.get(3, k, stage);
+            if (has_post) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (drops) H[j] = mask(H[j], k, j);
-                    H[j] = __fmul2_rn(both(cf), H[j]);
-                    S[k][j] = __ffma2_rn(H[j], __fmul2_rn(both(r), b.get2(j)), S[k][j]);
-                }
-                if (has_gate) {
-                    ch.param(f.gate, g0, f.g_float, width, w);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) H[j] = __fmul2_rn(H[j], w[j]);
-                }
-                if (has_post) {
-                    ch.param(f.w_post, 0, f.w_float, width, w);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        H[j] = __ffma2_rn(__fmul2_rn(both(r), H[j]), __fadd2_rn(both(f.w0), w[j]),
-                                          __fmul2_rn(both(-c2), b.get2(j)));
-                }
-                if (f.db) ch.store(static_cast<T*>(f.db) + row * f.dbs, width, H);
+                for (int j = 0; j < 4; ++j) H[j] = __ffma2_rn(both(-c2), b.get2(j), H[j]);
             }
+            if (f.db) ch.store(static_cast<T*>(f.db) + row * f.dbs, width, H);
         }
         if constexpr (VEC) {
             if (row + stages < last) in.fetch(f, row + stages, stage, threads, tid);
             asm volatile("cp.async.commit_group;" ::: "memory");
             stage = stage + 1 == stages ? 0 : stage + 1;
         }
-        if (--group_left == 0 || row + 1 == last) {  // the last of the gate row's rows in this run
-            if (MULTI && want_s) {
+        if (MULTI && (--group_left == 0 || row + 1 == last)) {  // the last of the gate row's rows in this run
+            if (want_s) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const Chunk<T, VEC> ch(k, threads, tid);
                     float2 w[4];
-                    ch.param(f.gate, g0, f.g_float, width, w);
+                    ch.param(f.gate, group * f.gs, f.g_float, width, w);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) W[MULTI ? k : 0][j] = __ffma2_rn(w[j], S[k][j], W[MULTI ? k : 0][j]);
                     if (f.dgate) {
@@ -744,7 +788,10 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
                     for (int j = 0; j < 4; ++j) S[k][j] = both(0.0f);
                 }
             }
-            if (row + 1 < last) ++group, group_left = f.gate_rows;
+            if (row + 1 < last) {
+                ++group, group_left = f.gate_rows;
+                if constexpr (SHARED) keep_weights(1);
+            }
         }
     }
     if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -753,47 +800,47 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         const Chunk<T, VEC> ch(k, threads, tid);
         if (f.part_next) store_sums(ch, f.part_next + (uint64_t)run * width, width, A[k]);
         if (!MULTI && f.part_gate) store_sums(ch, f.part_gate + (uint64_t)run * width, width, S[k]);
-        if (f.part_post) {
-            if (!MULTI && has_gate) {
-                float2 w[4];
-                ch.param(f.gate, group * f.gs, f.g_float, width, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) S[k][j] = __fmul2_rn(w[j], S[k][j]);
-            }
-            store_sums(ch, f.part_post + (uint64_t)run * width, width, MULTI ? W[MULTI ? k : 0] : S[k]);
-        }
+        if (f.part_post) store_sums(ch, f.part_post + (uint64_t)run * width, width, MULTI ? W[MULTI ? k : 0] : S[k]);
     }
 }
 
-// Adds the blocks' partial sums in order: first the plain sums (dw_next, dw_post), then each gate row's.
+// Adds the runs' partial sums in order.  A job is one row of sums: dw_next; dw_post, from its own partial sums or,
+// where runs share gate rows, from the S of every run times the run's gate row; or the gradient of one gate row.
 struct Finish {
-    const float* part[2];
-    float* dst[2];
-    uint32_t plain;  // plain sums, `runs` partial rows each
-    uint32_t runs;
-    const float* part_gate;  // groups x parts partial rows
-    uint32_t parts;
-    void* dgate;
-    uint64_t dgs;
-    const void* w_post;
-    uint32_t width;
+    const float *part_next, *part_post, *part_gate;
+    float *d_next, *d_post;
+    void* dgate;  // NULL: not wanted, or written by the runs
+    const void *w_post, *gate;
+    uint64_t dgs, gs;
+    uint32_t width, runs, parts;
     bool w_float, g_float;
     float w0;
 };
 
+constexpr int kFinishThreads = 1024;  // a warp adds a 32nd of the partial rows of 32 columns
 template <typename T>
-__global__ void __launch_bounds__(kThreads) block_norm_finish_kernel(const Finish f) {
-    __shared__ float sums[kThreads / 32][32];
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = kThreads / 32;
+__global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const Finish f) {
+    constexpr uint32_t warps = kFinishThreads / 32;
+    __shared__ float sums[warps][32];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane;
-    const bool plain = blockIdx.y < f.plain;
-    const uint32_t group = blockIdx.y - f.plain, n = plain ? f.runs : f.parts;
-    const float* part = plain ? f.part[blockIdx.y] : f.part_gate + (uint64_t)group * f.parts * f.width;
+    uint32_t job = blockIdx.y;  // 0: next, 1: post, 2 + g: gate row g
+    if (!f.part_next) ++job;
+    if (!f.d_post && job >= 1) ++job;
+    const bool weighted = job == 1 && !f.part_post;
+    const uint32_t n = job < 2 ? f.runs : f.parts;
+    const float* part = job == 0 ? f.part_next : job == 1 && !weighted ? f.part_post : f.part_gate;
+    if (job >= 2) part += (uint64_t)(job - 2) * f.parts * f.width;
     float v = 0.0f;
     if (c < f.width) {
-        const uint32_t end = (uint32_t)((uint64_t)n * (warp + 1) / warps);
+        const uint32_t begin = (uint32_t)((uint64_t)n * warp / warps), end = (uint32_t)((uint64_t)n * (warp + 1) / warps);
+        if (weighted) {
+            for (uint32_t i = begin; i < end; ++i)
+                v += param<T>(f.gate, i / f.parts * f.gs + c, f.g_float) * part[(uint64_t)i * f.width + c];
+        } else {
 #pragma unroll 8
-        for (uint32_t i = (uint32_t)((uint64_t)n * warp / warps); i < end; ++i) v += part[(uint64_t)i * f.width + c];
+            for (uint32_t i = begin; i < end; ++i) v += part[(uint64_t)i * f.width + c];
+        }
     }
     sums[warp][lane] = v;
     __syncthreads();
@@ -801,11 +848,13 @@ __global__ void __launch_bounds__(kThreads) block_norm_finish_kernel(const Finis
     v = sums[0][lane];
 #pragma unroll
     for (uint32_t i = 1; i < warps; ++i) v += sums[i][lane];
-    if (plain) f.dst[blockIdx.y][c] = v;
+    if (job == 0) f.d_next[c] = v;
+    else if (job == 1) f.d_post[c] = v;
     else {
         if (f.w_post) v *= f.w0 + param<T>(f.w_post, c, f.w_float);
-        if (f.g_float) static_cast<float*>(f.dgate)[group * f.dgs + c] = v;
-        else static_cast<T*>(f.dgate)[group * f.dgs + c] = from_float<T>(v);
+        const uint64_t at = (job - 2) * f.dgs + c;
+        if (f.g_float) static_cast<float*>(f.dgate)[at] = v;
+        else static_cast<T*>(f.dgate)[at] = from_float<T>(v);
     }
 }
 
@@ -826,25 +875,25 @@ Plan plan_backward(uint32_t width, bool vec) {
     else if (vec && width <= 512) p.kind = 1;
     else if (vec && width <= 8192) p.kind = 2, regs = 128;
     else if (vec && width <= 16384) p.kind = 3;
-    else if (!vec && width <= 4096) p.kind = 4, e = 8, regs = 128;
+    else if (!vec && width <= 4096) p.kind = 4, e = 8;
     else if (!vec && width <= 8192) p.kind = 5, e = 8;
     else return p;
     if (p.kind <= 1) p.threads = 256, p.runs_per_block = 8, regs = 96;
     else p.threads = (width + 32 * e - 1) / (32 * e) * 32;
     p.blocks_per_sm = std::min(2048 / p.threads, std::max(1u, 65536 / (p.threads * regs)));
     if (vec) {
-        const size_t stage = (size_t)p.threads * 4 * e * sizeof(T);
-        if (stage > kMaxShared - 2048) return Plan();
-        p.stages = 2 * stage <= kMaxShared - 2048 ? 2 : 1;
-        p.smem = p.stages * stage;
-        p.blocks_per_sm = std::max<uint32_t>(1, std::min<uint32_t>(p.blocks_per_sm, kMaxShared / (p.smem + 2048)));
-    }
+        const size_t stage = (size_t)p.threads * 4 * e * sizeof(T), weights = p.kind == 3 ? 0 : p.threads * 2 * e * sizeof(float);
+        if (stage + weights > kMaxShared - 2048) return Plan();
+        p.stages = 2 * stage + weights <= kMaxShared - 2048 ? 2 : 1;
+        p.smem = p.stages * stage + weights;
+    } else p.smem = p.threads * 2 * e * sizeof(float);
+    p.blocks_per_sm = std::max<uint32_t>(1, std::min<uint32_t>(p.blocks_per_sm, kMaxShared / (p.smem + 2048)));
     return p;
 }
 
-template <typename T, int E, bool VEC, bool WARP, bool MULTI, int BLOCK, int MIN>
+template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool SHARED, int BLOCK, int MIN>
 int launch_backward_kernel(const Backward& f, const Plan& p, cudaStream_t st) {
-    auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, BLOCK, MIN>;
+    auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, SHARED, BLOCK, MIN>;
     if (p.smem > 46 * 1024) {  // the kernel has static shared memory too
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
         if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(block_norm_backward_kernel)");
@@ -857,13 +906,13 @@ template <typename T, bool MULTI>
 int launch_backward(const Backward& f, const Plan& p, bool vec, cudaStream_t st) {
     switch (p.kind) {
         case 0:
-            return vec ? launch_backward_kernel<T, 8, true, true, MULTI, 256, 2>(f, p, st)
-                       : launch_backward_kernel<T, 8, false, true, MULTI, 256, 2>(f, p, st);
-        case 1: return launch_backward_kernel<T, 16, true, true, MULTI, 256, 2>(f, p, st);
-        case 2: return launch_backward_kernel<T, 16, true, false, MULTI, 512, 1>(f, p, st);
-        case 3: return launch_backward_kernel<T, 16, true, false, MULTI, 1024, 1>(f, p, st);
-        case 4: return launch_backward_kernel<T, 8, false, false, MULTI, 512, 1>(f, p, st);
-        case 5: return launch_backward_kernel<T, 8, false, false, MULTI, 1024, 1>(f, p, st);
+            return vec ? launch_backward_kernel<T, 8, true, true, MULTI, true, 256, 2>(f, p, st)
+                       : launch_backward_kernel<T, 8, false, true, MULTI, true, 256, 2>(f, p, st);
+        case 1: return launch_backward_kernel<T, 16, true, true, MULTI, true, 256, 2>(f, p, st);
+        case 2: return launch_backward_kernel<T, 16, true, false, MULTI, true, 512, 1>(f, p, st);
+        case 3: return launch_backward_kernel<T, 16, true, false, MULTI, false, 1024, 1>(f, p, st);
+        case 4: return launch_backward_kernel<T, 8, false, false, MULTI, true, 512, 2>(f, p, st);
+        case 5: return launch_backward_kernel<T, 8, false, false, MULTI, true, 1024, 1>(f, p, st);
         default: block_norm_backward_any_kernel<T><<<f.runs, kThreads, 0, st>>>(f); return check_launch("block_norm_backward_any_kernel");
     }
 }
@@ -1033,28 +1082,33 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
         if (wanted) ws += (uint64_t)f.runs * f.width;
         return p;
     };
+    const bool shared_gate = f.gate && f.parts > 1;  // then S of each run gives both sums
     f.part_next = take(a->d_next_weight);
-    f.part_post = take(a->d_post_weight);
-    f.part_gate = take(a->d_gate);
+    f.part_post = take(a->d_post_weight && !shared_gate);
+    f.part_gate = take(a->d_gate || (a->d_post_weight && shared_gate));
     Finish e{};
-    if (f.part_next) e.part[e.plain] = f.part_next, e.dst[e.plain++] = a->d_next_weight;
-    if (f.part_post) e.part[e.plain] = f.part_post, e.dst[e.plain++] = a->d_post_weight;
-    e.runs = f.runs;
+    e.part_next = f.part_next;
+    e.part_post = f.part_post;
     e.part_gate = f.part_gate;
-    e.parts = f.parts;
-    e.dgate = f.dgate;
-    e.dgs = f.dgs;
+    e.d_next = a->d_next_weight;
+    e.d_post = a->d_post_weight;
+    e.dgate = shared_gate ? f.dgate : nullptr;
     e.w_post = f.w_post;
+    e.gate = f.gate;
+    e.dgs = f.dgs;
+    e.gs = f.gs;
     e.width = f.width;
+    e.runs = f.runs;
+    e.parts = f.parts;
     e.w_float = f.w_float;
     e.g_float = f.g_float;
     e.w0 = f.w0;
-    const uint32_t jobs = e.plain + (f.part_gate && f.parts > 1 ? f.groups : 0);
+    const uint32_t jobs = !!e.part_next + !!e.d_post + (e.dgate ? f.groups : 0);
     int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         rc = f.gate && f.parts == 1 ? launch_backward<T, true>(f, plan, vec, st) : launch_backward<T, false>(f, plan, vec, st);
-        if (rc == MTXC_OK && jobs) block_norm_finish_kernel<T><<<dim3((f.width + 31) / 32, jobs), kThreads, 0, st>>>(e);
+        if (rc == MTXC_OK && jobs) block_norm_finish_kernel<T><<<dim3((f.width + 31) / 32, jobs), kFinishThreads, 0, st>>>(e);
     });
     return rc == MTXC_OK ? check_launch("block_norm_finish_kernel") : rc;
 }

@@ -4,7 +4,8 @@ Run as ``python -m matrix_b200.build`` (or through ``__graft_entry__.build()``).
 cross-compiles without a GPU.  Objects go to ``matrix_b200/_build/``; the library to
 ``matrix_b200/lib/libmtxc.so``, which travels with the source tree to the GPU box.  The
 CUDA runtime is linked statically so the library does not depend on which libcudart the
-host process (e.g. PyTorch) loaded.
+host process (e.g. PyTorch) loaded.  ``binding/`` is compiled against the installed torch into the Python
+module ``lib/_lm.so``.
 """
 from __future__ import annotations
 
@@ -23,6 +24,8 @@ LIBDIR = PKG / "lib"
 LIB = LIBDIR / "libmtxc.so"
 HOST = PKG / "host"
 HOST_LIB = LIBDIR / "libmtx.so"
+BINDING = PKG / "binding"
+BINDING_LIB = LIBDIR / "_lm.so"
 INCLUDE = REPO / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -86,6 +89,20 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I", str(INCLUDE), "-I", str(HOST),
              "-I", str(cuda_include), "-o", str(HOST_LIB), *map(str, host_srcs), "-L", str(LIBDIR), "-lmtxc",
              "-ldl", "-Wl,-rpath,$ORIGIN"])
+    binding_srcs = sorted(BINDING.glob("*.cpp"))
+    if _stale(BINDING_LIB, [*binding_srcs, LIB, *headers]):
+        import sysconfig
+
+        import torch
+
+        torch_dir = Path(torch.__file__).resolve().parent
+        cuda_include = Path(nvcc()).resolve().parent.parent / "include"
+        run(["g++", *CXX_FLAGS, "-shared", "-I", str(torch_dir / "include"),
+             "-I", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+             "-I", sysconfig.get_paths()["include"], "-I", str(cuda_include),
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-o", str(BINDING_LIB),
+             *map(str, binding_srcs), "-L", str(LIBDIR), "-lmtxc", "-L", str(torch_dir / "lib"), "-ltorch_python",
+             "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"])
     return LIB
 
 

@@ -1,10 +1,11 @@
 // Rules on logits before a token is chosen (repeated-token penalties, biases, a grammar's bit mask), for
 // sm_100a: one pass over the logits, no counts kept from call to call.
 //
-// A block takes a slice of one row's vocabulary.  It scans the row's tokens and biases once (a few KB, from
-// L2 after the row's first block) and keeps what falls into its slice in shared memory: per token, how often
-// it was generated with the top bit for "also in the prompt", and the last bias entry that names it.  Both are
-// integer atomics, so the result does not depend on their order.  Then it streams its logits.
+// A block takes a slice of one row's vocabulary.  It starts the loads of its logits and of their mask bits, then
+// scans the row's tokens and biases (a few KB, from L2 after the row's first block) and keeps what falls into its slice
+// in shared memory: per token, how often it was generated with the top bit for "also in the prompt", and the last
+// bias entry that names it; and one bit for each token that has either, since most have neither and are only
+// masked.  All are integer atomics, so the result does not depend on their order.
 #include <algorithm>
 
 #include "rows.cuh"
@@ -13,11 +14,13 @@ namespace mtxc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr uint32_t kSlice = 4096;
+constexpr int kChunks = 2;                            // eights of a thread
+constexpr uint32_t kSlice = kThreads * kChunks * 8;   // tokens of a block
 constexpr uint32_t kPrompt = 1u << 31;
 
 struct Logits {
-    uint32_t rows, vocab, slices;
+    uint32_t first_row, vocab, slices;
+    FastDiv slices_div;
     void* dst;
     const void* src;
     uint64_t ds, ss;
@@ -34,58 +37,132 @@ struct Logits {
     uint64_t ms;
 };
 
-template <typename T>
+// Calls fn(index, token) for a thread's share of a list, four tokens' loads in flight.
+template <typename Fn>
+__device__ __forceinline__ void scan(const int32_t* list, uint32_t n, Fn&& fn) {
+    uint32_t i = threadIdx.x;
+    for (; i + 3 * kThreads < n; i += 4 * kThreads) {
+        int32_t t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = __ldg(list + i + k * kThreads);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) fn(i + k * kThreads, t[k]);
+    }
+    for (; i < n; i += kThreads) fn(i, __ldg(list + i));
+}
+
+// VEC: a thread's eights are eight consecutive tokens, one access each; else every 32nd of the warp's 256, so that
+// scalar accesses are contiguous across the warp.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) {
-    extern __shared__ uint32_t smem[];
-    uint32_t* count = smem;                          // kSlice words where there are tokens
-    uint32_t* entry = smem + (a.tokens ? kSlice : 0);  // kSlice words where there are biases: last entry + 1
-    for (uint64_t u = blockIdx.x; u < (uint64_t)a.rows * a.slices; u += gridDim.x) {
-        const uint32_t row = (uint32_t)(u / a.slices), first = (uint32_t)(u % a.slices) * kSlice;
-        const uint32_t n = min(kSlice, a.vocab - first);
-        __syncthreads();  // the last slice's counts are still read
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            if (a.tokens) count[i] = 0;
-            if (a.bias_tokens) entry[i] = 0;
+    extern __shared__ uint4 smem[];
+    uint32_t* const touched = reinterpret_cast<uint32_t*>(smem);  // kSlice bits
+    uint32_t* const count = touched + kSlice / 32;                // kSlice words where there are tokens
+    uint32_t* const entry = count + (a.tokens ? kSlice : 0);      // kSlice words where there are biases: last entry + 1
+    uint32_t row, slice;
+    a.slices_div.divmod(blockIdx.x, row, slice);
+    row += a.first_row;
+    const uint32_t first = slice * kSlice, n = min(kSlice, a.vocab - first);
+    const T* x = static_cast<const T*>(a.src) + row * a.ss + first;
+    T* y = static_cast<T*>(a.dst) + row * a.ds + first;
+    const uint32_t lane = threadIdx.x % 32;
+    auto at = [&](int k, int j) {  // element j of eight k, in the slice
+        const uint32_t c = k * (kThreads * 8);
+        return VEC ? c + threadIdx.x * 8 + j : c + (threadIdx.x - lane) * 8 + j * 32 + lane;
+    };
+    Eight<T> v[kChunks];
+    uint32_t allowed[kChunks];  // bit j for element j
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+        if constexpr (VEC) {
+            if (at(k, 0) < n) v[k].load(x + at(k, 0));
+        } else {
+            T e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = at(k, j) < n ? x[at(k, j)] : T(0.0f);
+            memcpy(v[k].w, e, sizeof(e));
         }
+        allowed[k] = 0xFF;
+        if (a.mask) {
+            const uint32_t* m = a.mask + row * a.ms + first / 32;
+            if constexpr (VEC) {
+                if (at(k, 0) < n) allowed[k] = __ldg(m + at(k, 0) / 32) >> (at(k, 0) % 32) & 0xFF;
+            } else {
+                allowed[k] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at(k, j) < n) allowed[k] |= (__ldg(m + at(k, j) / 32) >> lane & 1u) << j;
+            }
+        }
+    }
+    if (a.tokens || a.bias_tokens) {
+        const uint32_t words = kSlice / 32 + (a.tokens ? kSlice : 0) + (a.bias_tokens ? kSlice : 0);
+        for (uint32_t i = threadIdx.x; i < words / 4; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         if (a.tokens) {
-            const int32_t* t = a.tokens + row * a.ts;
             const uint32_t len = a.lengths ? min((uint32_t)max(a.lengths[row], 0), a.history) : a.history;
             const uint32_t prompt = a.prompt_lengths ? (uint32_t)max(a.prompt_lengths[row], 0) : 0;
-            for (uint32_t i = threadIdx.x; i < len; i += kThreads) {
-                const uint32_t v = (uint32_t)t[i] - first;
-                if (v < n) {
-                    if (i < prompt) atomicOr(&count[v], kPrompt);
-                    else atomicAdd(&count[v], 1u);
-                }
-            }
+            scan(a.tokens + row * a.ts, len, [&](uint32_t i, int32_t token) {
+                const uint32_t t = (uint32_t)token - first;
+                if (t >= n) return;
+                if (i < prompt) atomicOr(&count[t], kPrompt);
+                else atomicAdd(&count[t], 1u);
+                atomicOr(&touched[t / 32], 1u << (t % 32));
+            });
         }
         if (a.bias_tokens) {
-            const int32_t* t = a.bias_tokens + row * a.bts;
-            for (uint32_t i = threadIdx.x; i < a.biases; i += kThreads) {
-                const uint32_t v = (uint32_t)t[i] - first;
-                if (v < n) atomicMax(&entry[v], i + 1);
-            }
+            scan(a.bias_tokens + row * a.bts, a.biases, [&](uint32_t i, int32_t token) {
+                const uint32_t t = (uint32_t)token - first;
+                if (t >= n) return;
+                atomicMax(&entry[t], i + 1);
+                atomicOr(&touched[t / 32], 1u << (t % 32));
+            });
         }
         __syncthreads();
-        const T* x = static_cast<const T*>(a.src) + row * a.ss + first;
-        T* y = static_cast<T*>(a.dst) + row * a.ds + first;
-        const uint32_t* mask = a.mask ? a.mask + row * a.ms + first / 32 : nullptr;
-        const float rep = a.repetition ? a.repetition[row] : 1.0f;
-        const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            float l = to_float(x[i]);
-            const uint32_t c = a.tokens ? count[i] : 0;
-            if (c) {
-                if (a.repetition) l = l > 0.0f ? l / rep : l * rep;
-                if (c & ~kPrompt) {
-                    if (a.frequency) l -= freq * (float)(c & ~kPrompt);
-                    if (a.presence) l -= pres;
-                }
+    }
+    const float rep = a.repetition ? a.repetition[row] : 1.0f;
+    const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
+    auto ruled = [&](float l, uint32_t i) {
+        const uint32_t c = a.tokens ? count[i] : 0, made = c & ~kPrompt;
+        if (c && a.repetition) l = l > 0.0f ? l / rep : l * rep;
+        if (made) {
+            if (a.frequency) l -= freq * (float)made;
+            if (a.presence) l -= pres;
+        }
+        if (a.bias_tokens && entry[i]) l += a.bias_values[row * a.bvs + entry[i] - 1];
+        return l;
+    };
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+        uint32_t some = 0;  // bit j: element j has a count or a bias
+        if (a.tokens || a.bias_tokens) {
+            if constexpr (VEC) {
+                if (at(k, 0) < n) some = touched[at(k, 0) / 32] >> (at(k, 0) % 32) & 0xFF;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at(k, j) < n) some |= (touched[at(k, j) / 32] >> lane & 1u) << j;
             }
-            if (a.bias_tokens && entry[i]) l += a.bias_values[row * a.bvs + entry[i] - 1];
-            if (mask && !(mask[i / 32] >> (i % 32) & 1u)) l = -INFINITY;
-            y[i] = from_float<T>(l);
+        }
+        T e[8];
+        memcpy(e, v[k].w, sizeof(e));
+        if (some) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (some >> j & 1u) e[j] = from_float<T>(ruled(to_float(e[j]), at(k, j)));
+        }
+        if (allowed[k] != 0xFF) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(allowed[k] >> j & 1u)) e[j] = from_float<T>(-INFINITY);
+        }
+        if constexpr (VEC) {
+            memcpy(v[k].w, e, sizeof(e));
+            if (at(k, 0) < n) v[k].store(y + at(k, 0));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (at(k, j) < n) y[at(k, j)] = e[j];
         }
     }
 }
@@ -109,9 +186,9 @@ extern "C" int mtxc_logits_rules(int dtype, const mtxc_logits_args* a) {
     if (a->rows == 0 || a->vocab == 0) return MTXC_OK;
     if (!a->dst || !a->src) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null buffer");
     Logits l{};
-    l.rows = (uint32_t)a->rows;
     l.vocab = (uint32_t)a->vocab;
     l.slices = (l.vocab + kSlice - 1) / kSlice;
+    l.slices_div = FastDiv(l.slices);
     l.dst = a->dst;
     l.src = a->src;
     l.ds = a->dst_stride;
@@ -131,11 +208,20 @@ extern "C" int mtxc_logits_rules(int dtype, const mtxc_logits_args* a) {
     l.bvs = a->bias_values_stride;
     l.mask = a->mask;
     l.ms = a->mask_stride;
-    const unsigned grid = (unsigned)std::min<uint64_t>((uint64_t)l.rows * l.slices, (uint64_t)ctx().sm_count * 8);
-    const size_t smem = sizeof(uint32_t) * kSlice * ((l.tokens != nullptr) + (l.bias_tokens != nullptr));
-    dispatch_float(dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        logits_rules_kernel<T><<<grid, kThreads, smem, ctx().stream()>>>(l);
-    });
-    return check_launch("logits_rules_kernel");
+    const size_t smem = sizeof(uint32_t) * (kSlice / 32 + kSlice * ((l.tokens != nullptr) + (l.bias_tokens != nullptr)));
+    // launches of fewer than 2^31 blocks
+    const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / l.slices);
+    for (uint64_t row = 0; row < a->rows; row += most) {
+        l.first_row = (uint32_t)row;
+        const unsigned grid = (unsigned)(std::min(most, a->rows - row) * l.slices);
+        dispatch_float(dtype, [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (l.vocab % 8 == 0 && eight_aligned<T>(l.src, a->rows == 1 ? 0 : l.ss) &&
+                eight_aligned<T>(l.dst, a->rows == 1 ? 0 : l.ds))
+                logits_rules_kernel<T, true><<<grid, kThreads, smem, ctx().stream()>>>(l);
+            else logits_rules_kernel<T, false><<<grid, kThreads, smem, ctx().stream()>>>(l);
+        });
+        if (int rc = check_launch("logits_rules_kernel")) return rc;
+    }
+    return MTXC_OK;
 }

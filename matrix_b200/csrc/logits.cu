@@ -1,11 +1,13 @@
 // Rules on logits before a token is chosen (repeated-token penalties, biases, a grammar's bit mask), for
 // sm_100a: one pass over the logits, no counts kept from call to call.
 //
-// A block takes a slice of one row's vocabulary.  It starts the loads of its logits and of their mask bits, then
-// scans the row's tokens and biases (a few KB, from L2 after the row's first block) and keeps what falls into its slice
-// in shared memory: per token, how often it was generated with the top bit for "also in the prompt", and the last
-// bias entry that names it; and one bit for each token that has either, since most have neither and are only
-// masked.  All are integer atomics, so the result does not depend on their order.
+// A block takes a slice of one row's vocabulary.  Most tokens are in no list: they are only masked, and streamed
+// through registers.  Meanwhile the block scans the row's tokens and biases (a few KB, from L2 after the row's
+// first block) and keeps what falls into its slice in shared memory: per token, how often it was generated with the
+// top bit for "also in the prompt", the last bias entry that names it, and a list of the tokens that have either.
+// When the slice is written, the listed tokens, each once, are read again, ruled and written over; that also holds
+// where dst is src, since an allowed token's first write leaves its value.  The counts are integer atomics, and
+// the list's order changes nothing: equal calls give equal bits.
 #include <algorithm>
 
 #include "rows.cuh"
@@ -16,6 +18,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunks = 2;                            // eights of a thread
 constexpr uint32_t kSlice = kThreads * kChunks * 8;   // tokens of a block
+static_assert(kSlice <= 65536, "the list holds 16-bit positions");
 constexpr uint32_t kPrompt = 1u << 31;
 
 struct Logits {
@@ -56,9 +59,11 @@ __device__ __forceinline__ void scan(const int32_t* list, uint32_t n, Fn&& fn) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) {
     extern __shared__ uint4 smem[];
-    uint32_t* const touched = reinterpret_cast<uint32_t*>(smem);  // kSlice bits
+    __shared__ uint32_t listed;
+    uint32_t* const touched = reinterpret_cast<uint32_t*>(smem);  // kSlice bits: on the list
     uint32_t* const count = touched + kSlice / 32;                // kSlice words where there are tokens
     uint32_t* const entry = count + (a.tokens ? kSlice : 0);      // kSlice words where there are biases: last entry + 1
+    uint16_t* const list = reinterpret_cast<uint16_t*>(entry + (a.bias_tokens ? kSlice : 0));  // kSlice halves
     uint32_t row, slice;
     a.slices_div.divmod(blockIdx.x, row, slice);
     row += a.first_row;
@@ -95,10 +100,16 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
             }
         }
     }
-    if (a.tokens || a.bias_tokens) {
+    const bool lists = a.tokens || a.bias_tokens;
+    if (lists) {
+        if (threadIdx.x == 0) listed = 0;
         const uint32_t words = kSlice / 32 + (a.tokens ? kSlice : 0) + (a.bias_tokens ? kSlice : 0);
         for (uint32_t i = threadIdx.x; i < words / 4; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
+        auto touch = [&](uint32_t t) {
+            const uint32_t bit = 1u << (t % 32);
+            if (!(atomicOr(&touched[t / 32], bit) & bit)) list[atomicAdd(&listed, 1u)] = (uint16_t)t;
+        };
         if (a.tokens) {
             const uint32_t len = a.lengths ? min((uint32_t)max(a.lengths[row], 0), a.history) : a.history;
             const uint32_t prompt = a.prompt_lengths ? (uint32_t)max(a.prompt_lengths[row], 0) : 0;
@@ -107,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
                 if (t >= n) return;
                 if (i < prompt) atomicOr(&count[t], kPrompt);
                 else atomicAdd(&count[t], 1u);
-                atomicOr(&touched[t / 32], 1u << (t % 32));
+                touch(t);
             });
         }
         if (a.bias_tokens) {
@@ -115,42 +126,14 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
                 const uint32_t t = (uint32_t)token - first;
                 if (t >= n) return;
                 atomicMax(&entry[t], i + 1);
-                atomicOr(&touched[t / 32], 1u << (t % 32));
+                touch(t);
             });
         }
-        __syncthreads();
     }
-    const float rep = a.repetition ? a.repetition[row] : 1.0f;
-    const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
-    auto ruled = [&](float l, uint32_t i) {
-        const uint32_t c = a.tokens ? count[i] : 0, made = c & ~kPrompt;
-        if (c && a.repetition) l = l > 0.0f ? l / rep : l * rep;
-        if (made) {
-            if (a.frequency) l -= freq * (float)made;
-            if (a.presence) l -= pres;
-        }
-        if (a.bias_tokens && entry[i]) l += a.bias_values[row * a.bvs + entry[i] - 1];
-        return l;
-    };
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-        uint32_t some = 0;  // bit j: element j has a count or a bias
-        if (a.tokens || a.bias_tokens) {
-            if constexpr (VEC) {
-                if (at(k, 0) < n) some = touched[at(k, 0) / 32] >> (at(k, 0) % 32) & 0xFF;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (at(k, j) < n) some |= (touched[at(k, j) / 32] >> lane & 1u) << j;
-            }
-        }
         T e[8];
         memcpy(e, v[k].w, sizeof(e));
-        if (some) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (some >> j & 1u) e[j] = from_float<T>(ruled(to_float(e[j]), at(k, j)));
-        }
         if (allowed[k] != 0xFF) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -164,6 +147,25 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
             for (int j = 0; j < 8; ++j)
                 if (at(k, j) < n) y[at(k, j)] = e[j];
         }
+    }
+    if (!lists) return;
+    __syncthreads();  // the slice is written, the list complete
+    const uint32_t m = listed;
+    if (threadIdx.x >= m) return;
+    const float rep = a.repetition ? a.repetition[row] : 1.0f;
+    const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
+    for (uint32_t i = threadIdx.x; i < m; i += kThreads) {
+        const uint32_t t = list[i];
+        if (a.mask && !(a.mask[row * a.ms + (first + t) / 32] >> (t % 32) & 1u)) continue;
+        float l = to_float(x[t]);
+        const uint32_t c = a.tokens ? count[t] : 0, made = c & ~kPrompt;
+        if (c && a.repetition) l = l > 0.0f ? l / rep : l * rep;
+        if (made) {
+            if (a.frequency) l -= freq * (float)made;
+            if (a.presence) l -= pres;
+        }
+        if (a.bias_tokens && entry[t]) l += a.bias_values[row * a.bvs + entry[t] - 1];
+        y[t] = from_float<T>(l);
     }
 }
 
@@ -208,7 +210,8 @@ extern "C" int mtxc_logits_rules(int dtype, const mtxc_logits_args* a) {
     l.bvs = a->bias_values_stride;
     l.mask = a->mask;
     l.ms = a->mask_stride;
-    const size_t smem = sizeof(uint32_t) * (kSlice / 32 + kSlice * ((l.tokens != nullptr) + (l.bias_tokens != nullptr)));
+    const int lists = (l.tokens != nullptr) + (l.bias_tokens != nullptr);
+    const size_t smem = lists ? sizeof(uint32_t) * (kSlice / 32 + kSlice * lists + kSlice / 2) : 0;
     // launches of fewer than 2^31 blocks
     const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / l.slices);
     for (uint64_t row = 0; row < a->rows; row += most) {

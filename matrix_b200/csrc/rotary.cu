@@ -6,6 +6,7 @@
 // 32 bits would be off by up to 0.03 radians.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "rows.cuh"
 
@@ -13,16 +14,17 @@ namespace mtxc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 2;              // units of a thread whose loads are in flight together
-constexpr uint32_t kMaxHalf = 4096;     // a token's cosines and sines: 32 KB of shared memory
+constexpr uint32_t kMaxHalf = 4096;       // a token's cosines and sines: 32 KB of shared memory
 constexpr uint32_t kTableEntries = 2048;  // what a block's tokens share otherwise
-constexpr uint32_t kTileUnits = 4;        // units of a thread in all
+static const uint32_t kTileUnits = getenv("TU") ? atoi(getenv("TU")) : 8;        // units of a thread in all
+static const uint32_t kBlocksPerSm = getenv("BS") ? atoi(getenv("BS")) : 4;
 
 struct Rotary {
-    uint32_t tokens, tile;  // tokens of this launch, tokens of a block
-    uint32_t half, heads0, items_per_token;
-    FastDiv length, units, heads, half_div;  // units of a head, heads of both tensors
-    uint64_t first_batch;  // where the launch starts
+    uint32_t length, tile, tiles;  // tokens of a sequence, of a block; blocks of a sequence
+    uint32_t half, heads0;
+    uint32_t items, lanes, rows;   // units of a token; threads that take them side by side, and tokens side by side
+    FastDiv tiles_div, units, lanes_div, half_div;  // units: of a head
+    uint64_t first_batch;          // where the launch starts
     const void* src[2];
     void* dst[2];
     uint64_t ss[2][3], ds[2][3];
@@ -41,124 +43,135 @@ __device__ __forceinline__ void turn(const Rotary& r, double position, uint32_t 
     sn *= r.sin_scale;
 }
 
-// A block takes `tile` tokens.  It makes their cosines and sines once, in shared memory, for all heads -- with its
-// first loads already in flight -- and then turns units: VEC, eight pairs (two accesses of eight elements, half
-// a head apart) or, PAIRS (interleaved), eight elements of four pairs; else one pair.  What is not turned is copied in
-// units of eight elements, or one.
+// A block takes `tile` tokens of a sequence.  It makes their cosines and sines once, in shared memory, for all heads
+// -- with its first loads already in flight -- and then turns units: VEC, eight pairs (two accesses of eight elements,
+// half a head apart) or, PAIRS (interleaved), eight elements of four pairs; else one pair.  What is not turned is
+// copied in units of eight elements, or one.  A thread stays with one unit of one head for all its tokens, kUnroll at
+// a time, so that a unit's place is worked out once (worked out for each, it was two thirds of the instructions).
 template <typename T, bool VEC, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r) {
+    constexpr int kUnroll = VEC && !PAIRS ? 2 : 4;
     extern __shared__ float table[];  // [tile][half] cosines, then sines
-    const uint32_t first = blockIdx.x * r.tile, n = min(r.tile, r.tokens - first);
     float* const cosines = table;
     float* const sines = table + r.tile * r.half;
-    const uint32_t items = n * r.items_per_token;
+    uint32_t batch, t0;
+    r.tiles_div.divmod(blockIdx.x, batch, t0);
+    t0 *= r.tile;
+    const uint32_t n = min(r.tile, r.length - t0);
+    const uint64_t b = r.first_batch + batch;
     const uint32_t turned = VEC ? (PAIRS ? r.half / 4 : r.half / 8) : r.half;  // units of a head that are turned
+    uint32_t lane, token0;  // this thread's first unit and token
+    r.lanes_div.divmod(threadIdx.x, token0, lane);
+    const bool idle = token0 >= r.rows;
 
-    auto batch_and_s = [&](uint32_t token, uint64_t& b, uint64_t& s) {
-        uint32_t q, m;
-        r.length.divmod(token, q, m);
-        b = r.first_batch + q;
-        s = m;
-    };
     struct Unit {
-        uint64_t from, to;
-        uint32_t at;  // into the table; only for turned units
-        bool k, copy;
         Eight<T> a, b;
         T u, v;
     };
-    auto load = [&](uint32_t i, Unit& x) {
-        uint32_t q, unit, token, h;
-        r.units.divmod(i, q, unit);
-        r.heads.divmod(q, token, h);
-        uint64_t b, s;
-        batch_and_s(first + token, b, s);
-        x.k = h >= r.heads0;
-        const int k = x.k;
+    const T* src = nullptr;
+    T* dst = nullptr;
+    uint64_t src_step = 0, dst_step = 0;
+    uint32_t at = 0;  // the unit's first pair
+    bool copy = false;
+    // places a unit of the tile's first token
+    auto place = [&](uint32_t item) {
+        uint32_t h, unit;
+        r.units.divmod(item, h, unit);
+        const int k = h >= r.heads0;
         const uint64_t hh = k ? h - r.heads0 : h;
-        x.copy = unit >= turned;
-        // the unit's first element: turned units from 0 (half layout: their second half r.half further), copied
-        // ones from 2 * half
-        uint32_t c;
-        if (x.copy) c = 2 * r.half + (unit - turned) * (VEC ? 8 : 1);
-        else c = unit * (VEC ? 8 : PAIRS ? 2 : 1);
-        x.at = token * r.half + (VEC ? (PAIRS ? unit * 4 : unit * 8) : unit);
-        x.from = b * r.ss[k][0] + s * r.ss[k][1] + hh * r.ss[k][2] + c;
-        x.to = b * r.ds[k][0] + s * r.ds[k][1] + hh * r.ds[k][2] + c;
-        const T* src = static_cast<const T*>(r.src[k]) + x.from;
+        copy = unit >= turned;
+        const uint32_t c = copy ? 2 * r.half + (unit - turned) * (VEC ? 8 : 1) : unit * (VEC ? 8 : PAIRS ? 2 : 1);
+        at = VEC ? (PAIRS ? unit * 4 : unit * 8) : unit;
+        src = static_cast<const T*>(r.src[k]) + b * r.ss[k][0] + t0 * r.ss[k][1] + hh * r.ss[k][2] + c;
+        dst = static_cast<T*>(r.dst[k]) + b * r.ds[k][0] + t0 * r.ds[k][1] + hh * r.ds[k][2] + c;
+        src_step = r.ss[k][1];
+        dst_step = r.ds[k][1];
+    };
+    auto load = [&](uint32_t token, Unit& x) {
+        const T* p = src + token * src_step;
         if constexpr (VEC) {
-            x.a.load(src);
-            if (!PAIRS && !x.copy) x.b.load(src + r.half);
+            x.a.load(p);
+            if (!PAIRS && !copy) x.b.load(p + r.half);
         } else {
-            x.u = src[0];
-            if (!x.copy) x.v = src[PAIRS ? 1 : r.half];
+            x.u = p[0];
+            if (!copy) x.v = p[PAIRS ? 1 : r.half];
         }
     };
-    auto finish = [&](Unit& x) {
-        T* dst = static_cast<T*>(r.dst[x.k]) + x.to;
+    auto finish = [&](uint32_t token, Unit& x) {
+        T* p = dst + token * dst_step;
+        const float* cs = cosines + token * r.half + at;
+        const float* sn = sines + token * r.half + at;
         if constexpr (VEC) {
-            if (!x.copy) {
-                const float4* c4 = reinterpret_cast<const float4*>(cosines + x.at);
-                const float4* s4 = reinterpret_cast<const float4*>(sines + x.at);
+            if (!copy) {
+                const float4* c4 = reinterpret_cast<const float4*>(cs);
+                const float4* s4 = reinterpret_cast<const float4*>(sn);
                 if constexpr (PAIRS) {
                     const float4 c = c4[0], s = s4[0];
-                    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+                    const float cj[4] = {c.x, c.y, c.z, c.w}, sj[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float2 p = x.a.get2(j);
-                        x.a.set2(j, p.x * cs[j] - p.y * sn[j], p.x * sn[j] + p.y * cs[j]);
+                        const float2 q = x.a.get2(j);
+                        const float2 o = __ffma2_rn(make_float2(q.x, q.x), make_float2(cj[j], sj[j]),
+                                                    __fmul2_rn(make_float2(q.y, q.y), make_float2(-sj[j], cj[j])));
+                        x.a.set2(j, o.x, o.y);
                     }
                 } else {
                     const float4 c0 = c4[0], c1 = c4[1], s0 = s4[0], s1 = s4[1];
-                    const float2 cs[4] = {{c0.x, c0.y}, {c0.z, c0.w}, {c1.x, c1.y}, {c1.z, c1.w}};
-                    const float2 sn[4] = {{s0.x, s0.y}, {s0.z, s0.w}, {s1.x, s1.y}, {s1.z, s1.w}};
+                    const float2 cj[4] = {{c0.x, c0.y}, {c0.z, c0.w}, {c1.x, c1.y}, {c1.z, c1.w}};
+                    const float2 sj[4] = {{s0.x, s0.y}, {s0.z, s0.w}, {s1.x, s1.y}, {s1.z, s1.w}};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 u = x.a.get2(j), v = x.b.get2(j);
-                        const float2 vs = __fmul2_rn(v, sn[j]), vc = __fmul2_rn(v, cs[j]);
-                        const float2 p = __ffma2_rn(u, cs[j], make_float2(-vs.x, -vs.y)), q = __ffma2_rn(u, sn[j], vc);
+                        const float2 p = __ffma2_rn(u, cj[j], __fmul2_rn(v, make_float2(-sj[j].x, -sj[j].y)));
+                        const float2 q = __ffma2_rn(u, sj[j], __fmul2_rn(v, cj[j]));
                         x.a.set2(j, p.x, p.y);
                         x.b.set2(j, q.x, q.y);
                     }
-                    x.b.store(dst + r.half);
+                    x.b.store(p + r.half);
                 }
             }
-            x.a.store(dst);
-        } else if (x.copy) dst[0] = x.u;
+            x.a.store(p);
+        } else if (copy) p[0] = x.u;
         else {
-            const float cs = cosines[x.at], sn = sines[x.at], u = to_float(x.u), v = to_float(x.v);
-            dst[0] = from_float<T>(u * cs - v * sn);
-            dst[PAIRS ? 1 : r.half] = from_float<T>(u * sn + v * cs);
+            const float u = to_float(x.u), v = to_float(x.v);
+            p[0] = from_float<T>(u * cs[0] - v * sn[0]);
+            p[PAIRS ? 1 : r.half] = from_float<T>(u * sn[0] + v * cs[0]);
         }
     };
 
     Unit x[kUnroll];
+    uint32_t item = blockIdx.y * r.lanes + lane;  // blocks along y share a tile's units
+    const bool any = !idle && item < r.items;
+    if (any) {
+        place(item);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-        const uint32_t i = threadIdx.x + k * kThreads;
-        if (i < items) load(i, x[k]);
+        for (int k = 0; k < kUnroll; ++k)
+            if (token0 + k * r.rows < n) load(token0 + k * r.rows, x[k]);
     }
-    for (uint32_t e = threadIdx.x; e < n * r.half; e += kThreads) {
+    for (uint32_t e = threadIdx.x; e < n * r.half; e += blockDim.x) {
         uint32_t token, j;
         r.half_div.divmod(e, token, j);
-        uint64_t b, s;
-        batch_and_s(first + token, b, s);
-        const uint64_t at = b * r.ps[0] + s * r.ps[1];
-        const double position = r.wide_positions ? (double)static_cast<const long long*>(r.positions)[at]
-                                                 : (double)static_cast<const int*>(r.positions)[at];
+        const uint64_t p = b * r.ps[0] + (t0 + token) * r.ps[1];
+        const double position = r.wide_positions ? (double)static_cast<const long long*>(r.positions)[p]
+                                                 : (double)static_cast<const int*>(r.positions)[p];
         turn(r, position, j, cosines[e], sines[e]);
     }
     __syncthreads();
-    for (uint32_t base = threadIdx.x;; base += kUnroll * kThreads) {
+    if (!any) return;
+    for (uint32_t token = token0;;) {
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
-            if (base + k * kThreads < items) finish(x[k]);
-        if (base + kUnroll * kThreads >= items) break;
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const uint32_t i = base + (kUnroll + k) * kThreads;
-            if (i < items) load(i, x[k]);
+            if (token + k * r.rows < n) finish(token + k * r.rows, x[k]);
+        token += kUnroll * r.rows;
+        if (token >= n) {
+            item += gridDim.y * r.lanes;
+            if (item >= r.items) break;
+            place(item);
+            token = token0;
         }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+            if (token + k * r.rows < n) load(token + k * r.rows, x[k]);
     }
 }
 
@@ -179,8 +192,8 @@ extern "C" int mtxc_rotary(int dtype, const mtxc_rotary_args* a) {
     if (a->position_dtype != MTXC_INT32 && a->position_dtype != MTXC_INT64)
         return fail(MTXC_ERR_UNSUPPORTED_DTYPE, who + ": positions must be Int32 or Int64");
     const uint64_t heads = (uint64_t)a->heads[0] + a->heads[1];
-    if (heads * a->head_dim >> 27 || a->length >> 31)
-        return fail(MTXC_ERR_SHAPE, who + ": a token's elements must be below 2^27, the length below 2^31");
+    if (heads * a->head_dim >> 27 || a->length >> 31 || (a->length && a->batch > (1ull << 40) / a->length))
+        return fail(MTXC_ERR_SHAPE, who + ": a token's elements must be below 2^27, the length below 2^31, the tokens at most 2^40");
     if (a->batch == 0 || a->length == 0 || a->head_dim == 0 || heads == 0) return MTXC_OK;
     Rotary r{};
     r.half = a->rotary_dim / 2;
@@ -219,27 +232,36 @@ extern "C" int mtxc_rotary(int dtype, const mtxc_rotary_args* a) {
                 vec = vec && eight_aligned<T>(r.src[k], r.ss[k][i]) && eight_aligned<T>(r.dst[k], r.ds[k][i]);
         const uint32_t units = vec ? r.half / (pairs ? 4 : 8) + copied / 8 : r.half + copied;
         r.units = FastDiv(units);
-        r.heads = FastDiv((uint32_t)heads);
         r.half_div = FastDiv(std::max(1u, r.half));
-        r.items_per_token = units * (uint32_t)heads;
-        // launches of fewer than 2^31 tokens, whole sequences each
-        const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / a->length);
+        r.items = units * (uint32_t)heads;
+        r.length = (uint32_t)a->length;
+        // threads side by side: a token's units evenly in as few rounds as 256 threads allow, and as many tokens as fit
+        const uint32_t rounds = std::min<uint32_t>((r.items + kThreads - 1) / kThreads, 65535);
+        r.lanes = std::min<uint32_t>((r.items + rounds - 1) / rounds, kThreads);
+        r.lanes_div = FastDiv(r.lanes);
+        // tokens of a block: what gives a thread kTileUnits units, while every SM still has kBlocksPerSm blocks and the
+        // table fits
+        const uint64_t tokens = a->batch * a->length;
+        uint64_t tile = std::max<uint64_t>(1, kTileUnits * kThreads / r.items);
+        tile = std::min(tile, std::max<uint64_t>(1, tokens / (kBlocksPerSm * (uint64_t)ctx().sm_count)));
+        tile = std::min<uint64_t>({tile, std::max(1u, kTableEntries / std::max(1u, r.half)), r.length});
+        r.tiles = (uint32_t)((r.length + tile - 1) / tile);
+        r.tile = (r.length + r.tiles - 1) / r.tiles;
+        r.tiles_div = FastDiv(r.tiles);
+        r.rows = std::min(kThreads / r.lanes, r.tile);
+        const unsigned threads = (r.lanes * r.rows + 31) / 32 * 32;
+        const size_t smem = 2 * sizeof(float) * r.tile * r.half;
+        // launches of fewer than 2^31 blocks, whole sequences each
+        const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / r.tiles);
         for (uint64_t batch = 0; batch < a->batch && rc == MTXC_OK; batch += most) {
             r.first_batch = batch;
-            r.tokens = (uint32_t)(std::min(most, a->batch - batch) * a->length);
-            r.length = FastDiv((uint32_t)a->length);
-            // tokens of a block: what gives a thread kTileUnits units, while all SMs still have blocks and the table fits
-            uint32_t tile = std::max(1u, kThreads * kTileUnits / r.items_per_token);
-            tile = std::min(tile, std::max(1u, r.tokens / (4 * (uint32_t)ctx().sm_count)));
-            tile = std::min(tile, std::max(1u, kTableEntries / std::max(1u, r.half)));
-            r.tile = tile;
-            const unsigned grid = (r.tokens + tile - 1) / tile;
-            const size_t smem = 2 * sizeof(float) * tile * r.half;
+            const unsigned blocks = (unsigned)(std::min(most, a->batch - batch) * r.tiles);
+            const dim3 grid(blocks, blocks < (unsigned)ctx().sm_count ? rounds : 1);  // few tokens: no second round
             cudaStream_t st = ctx().stream();
-            if (vec && pairs) rotary_kernel<T, true, true><<<grid, kThreads, smem, st>>>(r);
-            else if (vec) rotary_kernel<T, true, false><<<grid, kThreads, smem, st>>>(r);
-            else if (pairs) rotary_kernel<T, false, true><<<grid, kThreads, smem, st>>>(r);
-            else rotary_kernel<T, false, false><<<grid, kThreads, smem, st>>>(r);
+            if (vec && pairs) rotary_kernel<T, true, true><<<grid, threads, smem, st>>>(r);
+            else if (vec) rotary_kernel<T, true, false><<<grid, threads, smem, st>>>(r);
+            else if (pairs) rotary_kernel<T, false, true><<<grid, threads, smem, st>>>(r);
+            else rotary_kernel<T, false, false><<<grid, threads, smem, st>>>(r);
             rc = check_launch("rotary_kernel");
         }
     });

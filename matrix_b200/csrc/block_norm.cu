@@ -209,21 +209,21 @@ struct Kept {
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Sums N values over the threads that share a row: a warp (part unused), or a block of at most 1024 threads
-// through part[N][32], which no earlier sum of the row has used.
+// Sums N values over the threads that share a row: a warp (part unused), or a team of `threads` (a block, or several
+// warps of one that have a named barrier of their own) through part[N][32], which no earlier sum of the row has used.
 template <int N, bool WARP>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* part) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float* part, uint32_t threads, uint32_t team) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
     if constexpr (!WARP) {
-        const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        const uint32_t lane = threadIdx.x % 32, warps = threads / 32, base = team * warps;
         if (lane == 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) part[i * 32 + warp] = v[i];
+            for (int i = 0; i < N; ++i) part[i * 32 + threadIdx.x / 32] = v[i];
         }
-        __syncthreads();
+        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? part[i * 32 + lane] : 0.0f);
+        for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? part[i * 32 + base + lane] : 0.0f);
     }
 }
 
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_kernel(const Forward f)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) q = __ffma2_rn(h[k][j], h[k][j], q);
             float sum[1] = {q.x + q.y};
-            row_sum<1, WARP>(sum, part[0]);
+            row_sum<1, WARP>(sum, part[0], threads, 0);
             const float r = rsqrtf(sum[0] / width + f.eps);
             if (f.post_rstd && tid == 0) f.post_rstd[row] = r;
 #pragma unroll
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_kernel(const Forward f)
 #pragma unroll
         for (int j = 0; j < 4; ++j) q = __ffma2_rn(h[k][j], h[k][j], q);
     float sum[1] = {q.x + q.y};
-    row_sum<1, WARP>(sum, part[1]);
+    row_sum<1, WARP>(sum, part[1], threads, 0);
     const float s = rsqrtf(sum[0] / width + f.eps);
     if (f.a) {
 #pragma unroll
@@ -611,25 +611,26 @@ __device__ __forceinline__ void store_sums(const Chunk<T, VEC>& ch, float* row, 
     }
 }
 
-// Rows read once: E elements per thread, the sums over rows in registers.  A run of rows for each warp (WARP) or
-// block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.  SHARED: a
+// Rows read once: E elements per thread, the sums over rows in registers.  A run of rows for each team: a warp
+// (WARP), or `threads` threads; a block's teams add their sums in shared memory, so that there is one row of partial
+// sums for each block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.  SHARED: a
 // thread keeps its columns' w_next' and gate * w_post' in shared memory, as floats ready for use, for the run (or the
 // gate row); else they are made from the parameters for each row.  Inputs that the call does not have read as
 // zeros, weights as ones: fewer branches.
 template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool SHARED, int BLOCK, int MIN>
-__global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t stages) {
+__global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t team_threads, uint32_t stages) {
     constexpr int K = E / 8;
     extern __shared__ uint4 ring[];
     __shared__ float part[2][3 * 32];
-    const uint32_t threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x % 32 : threadIdx.x;
-    const uint32_t run = WARP ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-    if (WARP && run >= f.runs) return;
+    const uint32_t threads = WARP ? 32 : team_threads, teams = blockDim.x / threads;
+    const uint32_t team = threadIdx.x / threads, tid = threadIdx.x - team * threads;
+    const uint32_t run = blockIdx.x * teams + team;
     const uint32_t width = f.width;
     const bool has_b = f.b, has_post = f.w_post, has_next = f.w_next, has_gate = f.gate, drops = f.drop.on && has_b;
     const bool want_s = f.part_post || f.dgate;
     const float cf = drops ? f.beta * f.drop.scale : f.beta;
-    uint32_t first, last;
-    run_rows(f, run, first, last);
+    uint32_t first = 0, last = 0;
+    if (run < f.runs) run_rows(f, run, first, last);
     uint32_t group = first / f.gate_rows, group_left = f.gate_rows - first % f.gate_rows;
 
     Inputs<T, K, VEC> in;
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             }
         }
         float sum[3] = {c1.x + c1.y, su.x + su.y, sv.x + sv.y};
-        row_sum<3, WARP>(sum, part[(row - first) % 2]);
+        row_sum<3, WARP>(sum, part[(row - first) % 2], threads, team);
         const float kappa = s * s * s * (sum[0] / width);
         const float c2 = r * r * r * (cf * (sum[1] - kappa * sum[2]) / width);
 #pragma unroll
@@ -795,16 +796,52 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         }
     }
     if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+    float* const out_a = f.part_next ? f.part_next + (uint64_t)blockIdx.x * width : nullptr;
+    float* out_s = MULTI || !f.part_gate ? f.part_post : f.part_gate;
+    if (out_s) out_s += (uint64_t)blockIdx.x * width;
+    if (!SHARED || teams == 1) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const Chunk<T, VEC> ch(k, threads, tid);
+            if (out_a) store_sums(ch, out_a, width, A[k]);
+            if (out_s) store_sums(ch, out_s, width, MULTI ? W[MULTI ? k : 0] : S[k]);
+        }
+        return;
+    }
+    // each thread's sums into its own slots of the weights, then piece by piece over the teams, in order
+    float4* const own = reinterpret_cast<float4*>(weights);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const Chunk<T, VEC> ch(k, threads, tid);
-        if (f.part_next) store_sums(ch, f.part_next + (uint64_t)run * width, width, A[k]);
-        if (!MULTI && f.part_gate) store_sums(ch, f.part_gate + (uint64_t)run * width, width, S[k]);
-        if (f.part_post) store_sums(ch, f.part_post + (uint64_t)run * width, width, MULTI ? W[MULTI ? k : 0] : S[k]);
+        const float2(&v)[4] = MULTI ? W[MULTI ? k : 0] : S[k];
+        own[(2 * k) * blockDim.x] = make_float4(A[k][0].x, A[k][0].y, A[k][1].x, A[k][1].y);
+        own[(2 * k + 1) * blockDim.x] = make_float4(A[k][2].x, A[k][2].y, A[k][3].x, A[k][3].y);
+        own[(2 * K + 2 * k) * blockDim.x] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        own[(2 * K + 2 * k + 1) * blockDim.x] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    }
+    __syncthreads();
+    for (uint32_t piece = team; piece < 4 * K; piece += teams) {
+        float* out = piece < 2 * K ? out_a : out_s;
+        if (!out) continue;
+        const Chunk<T, VEC> ch(piece / 2 % K, threads, tid);
+        const float4* slot = own + piece * blockDim.x - team * threads;
+        float4 sum = slot[0];
+        for (uint32_t t = 1; t < teams; ++t) {
+            const float4 o = slot[t * threads];
+            sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
+        }
+        const int j = piece % 2 * 4;
+        if constexpr (VEC) {
+            if (ch.c < width) *reinterpret_cast<float4*>(out + ch.c + j) = sum;
+        } else {
+            const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ch.inside(j + i, width)) out[ch.column(j + i)] = e[i];
+        }
     }
 }
 
-// Adds the runs' partial sums in order.  A job is one row of sums: dw_next; dw_post, from its own partial sums or,
+// Adds the blocks' partial sums in order.  A job is one row of sums: dw_next; dw_post, from its own partial sums or,
 // where runs share gate rows, from the S of every run times the run's gate row; or the gradient of one gate row.
 struct Finish {
     const float *part_next, *part_post, *part_gate;
@@ -812,7 +849,7 @@ struct Finish {
     void* dgate;  // NULL: not wanted, or written by the runs
     const void *w_post, *gate;
     uint64_t dgs, gs;
-    uint32_t width, runs, parts;
+    uint32_t width, runs, parts;  // rows of partial sums in all, and for a gate row
     bool w_float, g_float;
     float w0;
 };
@@ -861,44 +898,45 @@ __global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const
 // Which backward kernel serves a width, and with what blocks.
 struct Plan {
     int kind = -1;  // -1: block_norm_backward_any_kernel
-    uint32_t threads = kThreads, runs_per_block = 1, blocks_per_sm = 2, stages = 1;
-    size_t smem = 0;
+    uint32_t team = kThreads, teams = 1, blocks_per_sm = 2, stages = 1;
+    size_t team_smem = 0;
 };
 
-constexpr size_t kMaxShared = 227 * 1024;
+constexpr size_t kMaxShared = 227 * 1024 - 2048;  // less the kernels' static part
 
 template <typename T>
 Plan plan_backward(uint32_t width, bool vec) {
     Plan p;
-    uint32_t e = 16, regs = 64;  // elements and registers of a thread
-    if (width <= 256) p.kind = 0, e = 8;
-    else if (vec && width <= 512) p.kind = 1;
-    else if (vec && width <= 8192) p.kind = 2, regs = 128;
-    else if (vec && width <= 16384) p.kind = 3;
-    else if (!vec && width <= 4096) p.kind = 4, e = 8;
-    else if (!vec && width <= 8192) p.kind = 5, e = 8;
+    uint32_t e = 16, block = 512, regs = 128;  // elements of a thread, threads of a block, registers
+    if (width <= 256) p.kind = 0, e = 8, block = 256;
+    else if (vec && width <= 512) p.kind = 1, block = 256;
+    else if (vec && width <= 8192) p.kind = 2;
+    else if (vec && width <= 16384) p.kind = 3, block = 1024, regs = 64;
+    else if (!vec && width <= 4096) p.kind = 4, e = 8, regs = 64;
+    else if (!vec && width <= 8192) p.kind = 5, e = 8, block = 1024, regs = 64;
     else return p;
-    if (p.kind <= 1) p.threads = 256, p.runs_per_block = 8, regs = 96;
-    else p.threads = (width + 32 * e - 1) / (32 * e) * 32;
-    p.blocks_per_sm = std::min(2048 / p.threads, std::max(1u, 65536 / (p.threads * regs)));
-    if (vec) {
-        const size_t stage = (size_t)p.threads * 4 * e * sizeof(T), weights = p.kind == 3 ? 0 : p.threads * 2 * e * sizeof(float);
-        if (stage + weights > kMaxShared - 2048) return Plan();
-        p.stages = 2 * stage + weights <= kMaxShared - 2048 ? 2 : 1;
-        p.smem = p.stages * stage + weights;
-    } else p.smem = p.threads * 2 * e * sizeof(float);
-    p.blocks_per_sm = std::max<uint32_t>(1, std::min<uint32_t>(p.blocks_per_sm, kMaxShared / (p.smem + 2048)));
+    p.team = p.kind <= 1 ? 32 : (width + 32 * e - 1) / (32 * e) * 32;
+    // the rows of a stage, and the weights
+    const size_t stage = vec ? (size_t)p.team * 4 * e * sizeof(T) : 0, weights = p.kind == 3 ? 0 : p.team * 2 * e * sizeof(float);
+    if (stage + weights > kMaxShared) return Plan();
+    p.stages = 2 * stage + weights <= kMaxShared ? 2 : 1;
+    p.team_smem = p.stages * stage + weights;
+    p.teams = p.kind == 3 ? 1 : (uint32_t)std::min<size_t>({block / p.team, std::max<size_t>(1, kMaxShared / std::max<size_t>(1, p.team_smem)), 15});
+    const uint32_t threads = p.team * p.teams;
+    p.blocks_per_sm = std::max<uint32_t>(
+        1, std::min<size_t>({2048 / threads, 65536 / (threads * regs), kMaxShared / (p.team_smem * p.teams + 2048)}));
     return p;
 }
 
 template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool SHARED, int BLOCK, int MIN>
 int launch_backward_kernel(const Backward& f, const Plan& p, cudaStream_t st) {
     auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, SHARED, BLOCK, MIN>;
-    if (p.smem > 46 * 1024) {  // the kernel has static shared memory too
-        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+    const size_t smem = p.team_smem * p.teams;
+    if (smem > 46 * 1024) {  // the kernel has static shared memory too
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(block_norm_backward_kernel)");
     }
-    kernel<<<(f.runs + p.runs_per_block - 1) / p.runs_per_block, p.threads, p.smem, st>>>(f, p.stages);
+    kernel<<<(f.runs + p.teams - 1) / p.teams, p.team * p.teams, smem, st>>>(f, p.team, p.stages);
     return check_launch("block_norm_backward_kernel");
 }
 
@@ -1068,18 +1106,26 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     });
     const int sums = !!a->d_next_weight + !!a->d_post_weight + !!a->d_gate;
     const uint64_t row_bytes = (uint64_t)f.width * sizeof(float) * sums;
-    uint64_t runs = std::min<uint64_t>(f.rows, (uint64_t)ctx().sm_count * plan.blocks_per_sm * plan.runs_per_block);
-    if (row_bytes) runs = std::min<uint64_t>(runs, ctx().workspace_bytes / row_bytes);
-    if (runs == 0)
+    // teams that the GPU holds; a block's teams share a gate row, or each has whole ones; few rows: fewer teams in a
+    // block, so that all SMs have some
+    const uint64_t most = (uint64_t)ctx().sm_count * plan.blocks_per_sm * plan.teams;
+    f.groups = (uint32_t)(((uint64_t)f.rows + f.gate_rows - 1) / f.gate_rows);
+    plan.teams = (uint32_t)std::min<uint64_t>(plan.teams, std::max<uint64_t>(1, f.rows / ctx().sm_count));
+    if (f.gate && most >= f.groups) plan.teams = (uint32_t)std::min<uint64_t>(plan.teams, most / f.groups);
+    uint64_t blocks = most / plan.teams;
+    if (row_bytes) blocks = std::min<uint64_t>(blocks, ctx().workspace_bytes / row_bytes);
+    if (blocks == 0)
         return fail(MTXC_ERR_WORKSPACE, who + ": one block's partial sums need " + std::to_string(row_bytes) +
                                             " bytes of workspace, the thread has " + std::to_string(ctx().workspace_bytes));
-    f.groups = (uint32_t)(((uint64_t)f.rows + f.gate_rows - 1) / f.gate_rows);
-    f.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(runs / f.groups, f.gate_rows));
+    const uint64_t runs = std::min<uint64_t>(f.rows, blocks * plan.teams);
+    f.parts = (uint32_t)(std::min<uint64_t>(runs / f.groups, f.gate_rows) / plan.teams * plan.teams);
+    if (f.parts <= 1) f.parts = 1;
     f.runs = f.parts > 1 ? f.groups * f.parts : (uint32_t)std::min<uint64_t>(runs, f.groups);
+    const uint32_t partial_rows = (f.runs + plan.teams - 1) / plan.teams;
     float* ws = static_cast<float*>(ctx().workspace);
     auto take = [&](bool wanted) {
         float* p = wanted ? ws : nullptr;
-        if (wanted) ws += (uint64_t)f.runs * f.width;
+        if (wanted) ws += (uint64_t)partial_rows * f.width;
         return p;
     };
     const bool shared_gate = f.gate && f.parts > 1;  // then S of each run gives both sums
@@ -1098,8 +1144,8 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     e.dgs = f.dgs;
     e.gs = f.gs;
     e.width = f.width;
-    e.runs = f.runs;
-    e.parts = f.parts;
+    e.runs = partial_rows;
+    e.parts = std::max(1u, f.parts / plan.teams);
     e.w_float = f.w_float;
     e.g_float = f.g_float;
     e.w0 = f.w0;

@@ -62,42 +62,59 @@ __global__ void __launch_bounds__(kThreads) dropout_vec_kernel(const Dropout a) 
 
 // Any width, stride and alignment.  A lane makes the mask of one counter; the warp's 32 x 8 elements are then
 // read and written 32 consecutive slots at a time (slot s belongs to the counter of lane s / 8), with the mask
-// bits of a slot from the lane that owns it.
+// bits of a slot from the lane that owns it.  Where the warp's counters are all of one row the slots' places need no
+// exchange.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const Dropout a) {
     const Philox rng(a.drop);
     const uint32_t lane = threadIdx.x % 32;
     const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-    uint32_t row = 0, block = 0, keep = 0;  // keep: bit j for element j, only of elements inside the row
-    uint32_t inside = 0;
+    uint32_t row = a.first_row, block = 0;
     if (i < a.items) {
         a.per_row.divmod(i, row, block);
         row += a.first_row;
-        inside = min(8u, a.width - block * 8);
-        const Lanes w = rng(block, row);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) keep |= (uint32_t)(!a.drop.on || w.keeps(a.drop, j)) << j;
     }
     T x[8];
-    uint32_t r[8], c[8];
-    uint32_t valid = 0, kept = 0;
+    uint64_t to[8];
+    uint32_t valid = 0;
+    const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0), block0 = __shfl_sync(0xffffffffu, block, 0);
+    if (__all_sync(0xffffffffu, i < a.items && row == row0)) {
+        const uint32_t c0 = block0 * 8 + lane;
+        const T* src = static_cast<const T*>(a.src) + row0 * a.ss + c0;
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-        const uint32_t from = j * 4 + lane / 8, e = lane % 8;
-        r[j] = __shfl_sync(0xffffffffu, row, from);
-        c[j] = __shfl_sync(0xffffffffu, block, from) * 8 + e;
-        const uint32_t bits = __shfl_sync(0xffffffffu, keep | inside << 8, from);
-        kept |= (bits >> e & 1u) << j;
-        if (e < bits >> 8) {
-            valid |= 1u << j;
-            x[j] = static_cast<const T*>(a.src)[r[j] * a.ss + c[j]];
+        for (uint32_t j = 0; j < 8; ++j) {
+            to[j] = row0 * a.ds + c0 + 32 * j;
+            if (c0 + 32 * j < a.width) {
+                valid |= 1u << j;
+                x[j] = src[32 * j];
+            }
+        }
+    } else {
+        const uint32_t inside = i < a.items ? min(8u, a.width - block * 8) : 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t from = j * 4 + lane / 8, e = lane % 8;
+            const uint32_t r = __shfl_sync(0xffffffffu, row, from), c = __shfl_sync(0xffffffffu, block, from) * 8 + e;
+            to[j] = r * a.ds + c;
+            if (e < __shfl_sync(0xffffffffu, inside, from)) {
+                valid |= 1u << j;
+                x[j] = static_cast<const T*>(a.src)[r * a.ss + c];
+            }
         }
     }
+    uint32_t keep = 0xFF;  // bit j for element j of this lane's counter
+    if (a.drop.on) {
+        const Lanes w = rng(block, row);
+        keep = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j) keep |= (uint32_t)w.keeps(a.drop, j) << j;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        const bool kept = __shfl_sync(0xffffffffu, keep, j * 4 + lane / 8) >> (lane % 8) & 1u;
         if (valid >> j & 1u)
-            static_cast<T*>(a.dst)[r[j] * a.ds + c[j]] =
-                from_float<T>(kept >> j & 1u ? to_float(x[j]) * a.drop.scale : 0.0f);
+            static_cast<T*>(a.dst)[to[j]] = from_float<T>(kept ? to_float(x[j]) * a.drop.scale : 0.0f);
+    }
 }
 
 }  // namespace

@@ -2,12 +2,13 @@
 // sm_100a: one pass over the logits, no counts kept from call to call.
 //
 // A block takes a slice of one row's vocabulary.  Most tokens are in no list: they are only masked, and streamed
-// through registers.  Meanwhile the block scans the row's tokens and biases (a few KB, from L2 after the row's
-// first block) and keeps what falls into its slice in shared memory: per token, how often it was generated with the
-// top bit for "also in the prompt", the last bias entry that names it, and a list of the tokens that have either.
-// When the slice is written, the listed tokens, each once, are read again, ruled and written over; that also holds
-// where dst is src, since an allowed token's first write leaves its value.  The counts are integer atomics, and
-// the list's order changes nothing: equal calls give equal bits.
+// through registers.  While their loads are on the way the block scans the row's tokens and biases (a few KB, from L2
+// after the row's first block) and keeps what falls into its slice in shared memory: per token, how often it was
+// generated, with the top bit for "also in the prompt"; one bit for the tokens that a bias names; and a list of the
+// tokens with a count.  When the slice is written, each token of the list without a bias, and then each last entry of
+// a biased token, is read again, ruled and written over; that also holds where dst is src, since an allowed token's
+// first write leaves its value.  The counts are integer atomics, and the list's order changes nothing: equal calls
+// give equal bits.
 #include <algorithm>
 
 #include "rows.cuh"
@@ -16,13 +17,14 @@ namespace mtxc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunks = 2;                            // eights of a thread
-constexpr uint32_t kSlice = kThreads * kChunks * 8;   // tokens of a block
+// Eights of a thread.  More mean fewer scans of the lists but fewer blocks to hide them: [256, 131072] bf16 with a
+// history of 2,048 takes 65 us with 1, 45 with 2, 47 with 3, 46 with 4 and 61 with 8.
+constexpr int kChunks = 2;
+constexpr uint32_t kSlice = kThreads * kChunks * 8;  // tokens of a block
 static_assert(kSlice <= 65536, "the list holds 16-bit positions");
-constexpr uint32_t kPrompt = 1u << 31;
 
 struct Logits {
-    uint32_t first_row, vocab, slices;
+    uint32_t first_row, vocab;
     FastDiv slices_div;
     void* dst;
     const void* src;
@@ -40,43 +42,72 @@ struct Logits {
     uint64_t ms;
 };
 
-// Calls fn(index, token) for a thread's share of a list, four tokens' loads in flight.
-template <typename Fn>
-__device__ __forceinline__ void scan(const int32_t* list, uint32_t n, Fn&& fn) {
-    uint32_t i = threadIdx.x;
-    for (; i + 3 * kThreads < n; i += 4 * kThreads) {
-        int32_t t[4];
+// A thread's share of a list: its first four entries, whose loads start before their number is known, then the rest,
+// four loads in flight.
+struct Share {
+    const int32_t* list;
+    int32_t t[4];
+    __device__ __forceinline__ Share(const int32_t* p, uint32_t most) : list(p) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = __ldg(list + i + k * kThreads);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) fn(i + k * kThreads, t[k]);
+        for (int k = 0; k < 4; ++k) t[k] = threadIdx.x + k * kThreads < most ? __ldg(list + threadIdx.x + k * kThreads) : -1;
     }
-    for (; i < n; i += kThreads) fn(i, __ldg(list + i));
-}
+    // fn(index, token) for the entries below n
+    template <typename Fn>
+    __device__ __forceinline__ void each(uint32_t n, Fn&& fn) {
+        for (uint32_t i = threadIdx.x;;) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k * kThreads < n) fn(i + k * kThreads, t[k]);
+            i += 4 * kThreads;
+            if (i >= n) break;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k * kThreads < n) t[k] = __ldg(list + i + k * kThreads);
+        }
+    }
+};
+
+// One token's count: of type C in shared memory, 16 bits while the history is shorter than 2^15.
+template <typename C>
+struct Counts {
+    static constexpr uint32_t kPrompt = 1u << (8 * sizeof(C) - 1);
+    uint32_t* words;
+    // Both return whether the token had no count before.
+    __device__ __forceinline__ bool generated(uint32_t t) const { return add(t, false); }
+    __device__ __forceinline__ bool prompt(uint32_t t) const { return add(t, true); }
+    __device__ __forceinline__ uint32_t at(uint32_t t) const { return reinterpret_cast<const C*>(words)[t]; }
+
+private:
+    __device__ __forceinline__ bool add(uint32_t t, bool prompt) const {
+        const uint32_t shift = sizeof(C) == 2 ? t % 2 * 16 : 0;
+        uint32_t* w = words + (sizeof(C) == 2 ? t / 2 : t);
+        const uint32_t old = prompt ? atomicOr(w, kPrompt << shift) : atomicAdd(w, 1u << shift);
+        return (C)(old >> shift) == 0;
+    }
+};
 
 // VEC: a thread's eights are eight consecutive tokens, one access each; else every 32nd of the warp's 256, so that
-// scalar accesses are contiguous across the warp.
-template <typename T, bool VEC>
+// scalar accesses are contiguous across the warp.  C: the counts' type.
+template <typename T, bool VEC, typename C>
 __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) {
     extern __shared__ uint4 smem[];
     __shared__ uint32_t listed;
-    uint32_t* const touched = reinterpret_cast<uint32_t*>(smem);  // kSlice bits: on the list
-    uint32_t* const count = touched + kSlice / 32;                // kSlice words where there are tokens
-    uint32_t* const entry = count + (a.tokens ? kSlice : 0);      // kSlice words where there are biases: last entry + 1
-    uint16_t* const list = reinterpret_cast<uint16_t*>(entry + (a.bias_tokens ? kSlice : 0));  // kSlice halves
+    uint32_t* const biased = reinterpret_cast<uint32_t*>(smem);  // kSlice bits
+    const Counts<C> count{biased + kSlice / 32};                 // kSlice counts
+    uint16_t* const list = reinterpret_cast<uint16_t*>(reinterpret_cast<C*>(count.words) + kSlice);  // kSlice positions
     uint32_t row, slice;
     a.slices_div.divmod(blockIdx.x, row, slice);
     row += a.first_row;
     const uint32_t first = slice * kSlice, n = min(kSlice, a.vocab - first);
     const T* x = static_cast<const T*>(a.src) + row * a.ss + first;
     T* y = static_cast<T*>(a.dst) + row * a.ds + first;
+    const uint32_t* mask = a.mask ? a.mask + row * a.ms + first / 32 : nullptr;
     const uint32_t lane = threadIdx.x % 32;
     auto at = [&](int k, int j) {  // element j of eight k, in the slice
         const uint32_t c = k * (kThreads * 8);
         return VEC ? c + threadIdx.x * 8 + j : c + (threadIdx.x - lane) * 8 + j * 32 + lane;
     };
     Eight<T> v[kChunks];
-    uint32_t allowed[kChunks];  // bit j for element j
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
         if constexpr (VEC) {
@@ -87,86 +118,114 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
             for (int j = 0; j < 8; ++j) e[j] = at(k, j) < n ? x[at(k, j)] : T(0.0f);
             memcpy(v[k].w, e, sizeof(e));
         }
-        allowed[k] = 0xFF;
-        if (a.mask) {
-            const uint32_t* m = a.mask + row * a.ms + first / 32;
-            if constexpr (VEC) {
-                if (at(k, 0) < n) allowed[k] = __ldg(m + at(k, 0) / 32) >> (at(k, 0) % 32) & 0xFF;
-            } else {
-                allowed[k] = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (at(k, j) < n) allowed[k] |= (__ldg(m + at(k, j) / 32) >> lane & 1u) << j;
-            }
-        }
     }
+    const float rep = a.repetition ? __ldg(a.repetition + row) : 1.0f;
+    const float freq = a.frequency ? __ldg(a.frequency + row) : 0.0f, pres = a.presence ? __ldg(a.presence + row) : 0.0f;
     const bool lists = a.tokens || a.bias_tokens;
     if (lists) {
+        uint32_t len = a.history, prompt = 0;
+        if (a.lengths) len = min((uint32_t)max(__ldg(a.lengths + row), 0), a.history);
+        if (a.prompt_lengths) prompt = (uint32_t)max(__ldg(a.prompt_lengths + row), 0);
+        Share tokens(a.tokens + row * a.ts, a.tokens ? a.history : 0);
         if (threadIdx.x == 0) listed = 0;
-        const uint32_t words = kSlice / 32 + (a.tokens ? kSlice : 0) + (a.bias_tokens ? kSlice : 0);
-        for (uint32_t i = threadIdx.x; i < words / 4; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
+        const uint32_t bytes = kSlice / 8 + (a.tokens ? kSlice * sizeof(C) : 0);
+        for (uint32_t i = threadIdx.x; i < bytes / 16; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        auto touch = [&](uint32_t t) {
-            const uint32_t bit = 1u << (t % 32);
-            if (!(atomicOr(&touched[t / 32], bit) & bit)) list[atomicAdd(&listed, 1u)] = (uint16_t)t;
-        };
         if (a.tokens) {
-            const uint32_t len = a.lengths ? min((uint32_t)max(a.lengths[row], 0), a.history) : a.history;
-            const uint32_t prompt = a.prompt_lengths ? (uint32_t)max(a.prompt_lengths[row], 0) : 0;
-            scan(a.tokens + row * a.ts, len, [&](uint32_t i, int32_t token) {
+            tokens.each(len, [&](uint32_t i, int32_t token) {
                 const uint32_t t = (uint32_t)token - first;
-                if (t >= n) return;
-                if (i < prompt) atomicOr(&count[t], kPrompt);
-                else atomicAdd(&count[t], 1u);
-                touch(t);
+                if (t < n && (i < prompt ? count.prompt(t) : count.generated(t))) list[atomicAdd(&listed, 1u)] = (uint16_t)t;
             });
         }
         if (a.bias_tokens) {
-            scan(a.bias_tokens + row * a.bts, a.biases, [&](uint32_t i, int32_t token) {
-                const uint32_t t = (uint32_t)token - first;
-                if (t >= n) return;
-                atomicMax(&entry[t], i + 1);
-                touch(t);
-            });
+            const int32_t* names = a.bias_tokens + row * a.bts;
+            for (uint32_t i = threadIdx.x; i < a.biases; i += kThreads) {
+                const uint32_t t = (uint32_t)__ldg(names + i) - first;
+                if (t < n) atomicOr(&biased[t / 32], 1u << (t % 32));
+            }
         }
     }
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-        T e[8];
-        memcpy(e, v[k].w, sizeof(e));
-        if (allowed[k] != 0xFF) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!(allowed[k] >> j & 1u)) e[j] = from_float<T>(-INFINITY);
-        }
         if constexpr (VEC) {
-            memcpy(v[k].w, e, sizeof(e));
-            if (at(k, 0) < n) v[k].store(y + at(k, 0));
-        } else {
+            if (at(k, 0) >= n) continue;
+            if (mask) {
+                const uint32_t allowed = __ldg(mask + at(k, 0) / 32) >> (at(k, 0) % 32);
+                T e[8];
+                memcpy(e, v[k].w, sizeof(e));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (at(k, j) < n) y[at(k, j)] = e[j];
+                for (int j = 0; j < 8; ++j)
+                    if (!(allowed >> j & 1u)) e[j] = from_float<T>(-INFINITY);
+                memcpy(v[k].w, e, sizeof(e));
+            }
+            v[k].store(y + at(k, 0));
+        } else {
+            T e[8];
+            memcpy(e, v[k].w, sizeof(e));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (at(k, j) >= n) continue;
+                if (mask && !(__ldg(mask + at(k, j) / 32) >> lane & 1u)) e[j] = from_float<T>(-INFINITY);
+                y[at(k, j)] = e[j];
+            }
         }
     }
     if (!lists) return;
-    __syncthreads();  // the slice is written, the list complete
-    const uint32_t m = listed;
-    if (threadIdx.x >= m) return;
-    const float rep = a.repetition ? a.repetition[row] : 1.0f;
-    const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
-    for (uint32_t i = threadIdx.x; i < m; i += kThreads) {
-        const uint32_t t = list[i];
-        if (a.mask && !(a.mask[row * a.ms + (first + t) / 32] >> (t % 32) & 1u)) continue;
+    __syncthreads();  // the slice is written, the list and the bits are complete
+    auto rule = [&](uint32_t t, float bias) {
+        if (mask && !(mask[t / 32] >> (t % 32) & 1u)) return;
         float l = to_float(x[t]);
-        const uint32_t c = a.tokens ? count[t] : 0, made = c & ~kPrompt;
+        const uint32_t c = a.tokens ? count.at(t) : 0, made = c & ~Counts<C>::kPrompt;
         if (c && a.repetition) l = l > 0.0f ? l / rep : l * rep;
         if (made) {
             if (a.frequency) l -= freq * (float)made;
             if (a.presence) l -= pres;
         }
-        if (a.bias_tokens && entry[t]) l += a.bias_values[row * a.bvs + entry[t] - 1];
-        y[t] = from_float<T>(l);
+        y[t] = from_float<T>(l + bias);
+    };
+    if (a.tokens) {
+        for (uint32_t i = threadIdx.x, m = listed; i < m; i += kThreads) {
+            const uint32_t t = list[i];
+            if (!a.bias_tokens || !(biased[t / 32] >> (t % 32) & 1u)) rule(t, 0.0f);
+        }
     }
+    if (a.bias_tokens) {
+        // from the list's end, 256 entries at a time: an entry counts if its token still has its bit and no later entry
+        // of these names it too
+        const int32_t* names = a.bias_tokens + row * a.bts;
+        for (uint32_t base = (a.biases - 1) / kThreads * kThreads;; base -= kThreads) {
+            const uint32_t i = base + threadIdx.x, end = min(base + kThreads, a.biases);
+            const int32_t token = i < end ? names[i] : -1;
+            const uint32_t t = (uint32_t)token - first;
+            bool last = i < end && t < n && (biased[t / 32] >> (t % 32) & 1u);
+            for (uint32_t k = i + 1; last && k < end; ++k) last = names[k] != token;
+            if (last) rule(t, a.bias_values[row * a.bvs + i]);
+            if (base == 0) break;
+            __syncthreads();
+            if (last) atomicAnd(&biased[t / 32], ~(1u << (t % 32)));
+            __syncthreads();
+        }
+    }
+}
+
+// Launches of fewer than 2^31 blocks.
+template <typename T, bool VEC, typename C>
+int launch(Logits l, uint64_t rows, cudaStream_t st) {
+    const size_t smem = l.tokens ? kSlice / 8 + kSlice * (sizeof(C) + sizeof(uint16_t)) : l.bias_tokens ? kSlice / 8 : 0;
+    const uint32_t slices = (l.vocab + kSlice - 1) / kSlice;
+    const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / slices);
+    l.slices_div = FastDiv(slices);
+    for (uint64_t row = 0; row < rows; row += most) {
+        l.first_row = (uint32_t)row;
+        logits_rules_kernel<T, VEC, C><<<(unsigned)(std::min(most, rows - row) * slices), kThreads, smem, st>>>(l);
+        if (int rc = check_launch("logits_rules_kernel")) return rc;
+    }
+    return MTXC_OK;
+}
+
+template <typename T, bool VEC>
+int launch(const Logits& l, uint64_t rows, cudaStream_t st) {
+    return l.history < 32768 ? launch<T, VEC, uint16_t>(l, rows, st) : launch<T, VEC, uint32_t>(l, rows, st);
 }
 
 }  // namespace
@@ -189,8 +248,6 @@ extern "C" int mtxc_logits_rules(int dtype, const mtxc_logits_args* a) {
     if (!a->dst || !a->src) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null buffer");
     Logits l{};
     l.vocab = (uint32_t)a->vocab;
-    l.slices = (l.vocab + kSlice - 1) / kSlice;
-    l.slices_div = FastDiv(l.slices);
     l.dst = a->dst;
     l.src = a->src;
     l.ds = a->dst_stride;
@@ -210,21 +267,12 @@ extern "C" int mtxc_logits_rules(int dtype, const mtxc_logits_args* a) {
     l.bvs = a->bias_values_stride;
     l.mask = a->mask;
     l.ms = a->mask_stride;
-    const int lists = (l.tokens != nullptr) + (l.bias_tokens != nullptr);
-    const size_t smem = lists ? sizeof(uint32_t) * (kSlice / 32 + kSlice * lists + kSlice / 2) : 0;
-    // launches of fewer than 2^31 blocks
-    const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / l.slices);
-    for (uint64_t row = 0; row < a->rows; row += most) {
-        l.first_row = (uint32_t)row;
-        const unsigned grid = (unsigned)(std::min(most, a->rows - row) * l.slices);
-        dispatch_float(dtype, [&](auto* t) {
-            using T = std::remove_pointer_t<decltype(t)>;
-            if (l.vocab % 8 == 0 && eight_aligned<T>(l.src, a->rows == 1 ? 0 : l.ss) &&
-                eight_aligned<T>(l.dst, a->rows == 1 ? 0 : l.ds))
-                logits_rules_kernel<T, true><<<grid, kThreads, smem, ctx().stream()>>>(l);
-            else logits_rules_kernel<T, false><<<grid, kThreads, smem, ctx().stream()>>>(l);
-        });
-        if (int rc = check_launch("logits_rules_kernel")) return rc;
-    }
-    return MTXC_OK;
+    const bool vec_shape = l.vocab % 8 == 0;
+    int rc = MTXC_OK;
+    dispatch_float(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const bool vec = vec_shape && eight_aligned<T>(l.src, a->rows == 1 ? 0 : l.ss) && eight_aligned<T>(l.dst, a->rows == 1 ? 0 : l.ds);
+        rc = vec ? launch<T, true>(l, a->rows, ctx().stream()) : launch<T, false>(l, a->rows, ctx().stream());
+    });
+    return rc;
 }

@@ -6,7 +6,7 @@
 // 32 bits would be off by up to 0.03 radians.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
+
 
 #include "rows.cuh"
 
@@ -16,8 +16,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kMaxHalf = 4096;       // a token's cosines and sines: 32 KB of shared memory
 constexpr uint32_t kTableEntries = 2048;  // what a block's tokens share otherwise
-static const uint32_t kTileUnits = getenv("TU") ? atoi(getenv("TU")) : 8;        // units of a thread in all
-static const uint32_t kBlocksPerSm = getenv("BS") ? atoi(getenv("BS")) : 4;
+constexpr uint32_t kTileUnits = 12;        // units of a thread in all
+constexpr uint32_t kBlocksPerSm = 4;
 
 struct Rotary {
     uint32_t length, tile, tiles;  // tokens of a sequence, of a block; blocks of a sequence

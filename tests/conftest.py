@@ -23,7 +23,7 @@ def _build_once():
         oracle_build.build_port()
     from matrix_b200 import build as lib_build
 
-    if not lib_build.LIB.exists():
+    if not lib_build.LIB.exists() or not lib_build.BINDING_LIB.exists():
         lib_build.build()
 
 

@@ -332,24 +332,28 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_kernel(const Forward f)
     if (f.next_rstd && tid == 0) f.next_rstd[row] = s;
 }
 
-// Elements per thread E, threads and blocks per SM, by width (measured on a B200 with a gate per channel, GB/s of
-// the bytes that have to move, the best against the next):
-//   a warp per row to 256 columns, and to 512 where accesses are vectors ([32768, 512] bf16 5446, a block 4699)
-//   half types, vectors: E = 16 to 1024 ([16384, 1024] bf16 with dropout 4471, E = 8 3847, a warp 3902), then 32, whose
-//     blocks of 256 hold more of a row in their registers ([16384, 2048] 5647, E = 16 5352, E = 8 4722)
-//   float, and scalar accesses: E = 8 to 4096 ([16384, 2047] bf16 2780, E = 16 2563, E = 32 1320), which needs the
-//     fewest registers, then 16 ([8192, 4097] bf16 2893, E = 8 in blocks of 1024 2340)
+// Elements per thread E, threads and blocks per SM (measured on a B200, the best against the next):
+//   a warp per row to 256 columns, and to 512 for vectors of half types ([32768, 512] bf16 5446 GB/s, a block 4699)
+//   few elements, up to 10,240 per SM: E = 8, the shortest way through one row ([300, 2048] bf16 3.2 us on the device,
+//     E = 16 3.6, E = 32 4.4; [300, 8192], which is more, 7.8, 6.4 and 6.0)
+//   half types, vectors: E = 16 to 1024 columns ([16384, 1024] bf16 with dropout 4471 GB/s, E = 8 3847, a warp 3902) and
+//     up to 57,344 elements per SM ([2000, 4096] 13.3 us, E = 32 13.6, E = 8 14.7; [4000, 4096] 26.9, 22.9, 28.5), then
+//     32, whose blocks hold more of a row in their registers ([16384, 2048] 5647 GB/s, E = 16 5352, E = 8 4722)
+//   float, and scalar accesses: E = 8 to 4096 ([16384, 2047] bf16 2780 GB/s, E = 16 2563, E = 32 1320), which needs
+//     the fewest registers, then 16 ([8192, 4097] bf16 2893, E = 8 in blocks of 1024 2340)
 // Wider rows return -1.
 template <typename T, bool VEC>
-int launch_forward(const Forward& f, cudaStream_t st) {
-    constexpr bool kHalfVec = VEC && sizeof(T) == 2;
+int launch_forward(const Forward& f, cudaStream_t st, int sms) {
     auto threads = [&](uint32_t e) { return (f.width + 32 * e - 1) / (32 * e) * 32; };
     const unsigned warps = (f.rows + 7) / 8;
+    const uint64_t per_sm = (uint64_t)f.rows * f.width / sms;
+    constexpr bool kHalfVec = VEC && sizeof(T) == 2;
     if (f.width <= 256) block_norm_kernel<T, 8, VEC, true, 256, 1><<<warps, 256, 0, st>>>(f);
     else if (f.width > 16384) return -1;
+    else if (f.width <= 8192 && per_sm <= 10240) block_norm_kernel<T, 8, VEC, false, 1024, 1><<<f.rows, threads(8), 0, st>>>(f);
     else if constexpr (kHalfVec) {
         if (f.width <= 512) block_norm_kernel<T, 16, VEC, true, 256, 1><<<warps, 256, 0, st>>>(f);
-        else if (f.width <= 1024) block_norm_kernel<T, 16, VEC, false, 64, 1><<<f.rows, threads(16), 0, st>>>(f);
+        else if (f.width <= 1024 || per_sm <= 57344) block_norm_kernel<T, 16, VEC, false, 1024, 1><<<f.rows, threads(16), 0, st>>>(f);
         else if (f.width <= 8192) block_norm_kernel<T, 32, VEC, false, 256, 3><<<f.rows, threads(32), 0, st>>>(f);
         else block_norm_kernel<T, 32, VEC, false, 512, 2><<<f.rows, threads(32), 0, st>>>(f);
     } else {
@@ -1030,7 +1034,8 @@ extern "C" int mtxc_block_norm(int dtype, const mtxc_block_norm_args* a) {
         const bool vec = f.width % 8 == 0 && eight_aligned<T>(f.x, f.xs) && eight_aligned<T>(f.b, f.bs) &&
                          eight_aligned<T>(f.h, f.hs) && eight_aligned<T>(f.a, f.as) && param_aligned(f.w_post, 0) &&
                          param_aligned(f.w_next, 0) && param_aligned(f.gate, f.gs);
-        rc = vec ? launch_forward<T, true>(f, ctx().stream()) : launch_forward<T, false>(f, ctx().stream());
+        rc = vec ? launch_forward<T, true>(f, ctx().stream(), ctx().sm_count)
+                 : launch_forward<T, false>(f, ctx().stream(), ctx().sm_count);
         if (rc == -1) {
             block_norm_any_kernel<T><<<grid, kThreads, 0, ctx().stream()>>>(f);
             rc = check_launch("block_norm_any_kernel");

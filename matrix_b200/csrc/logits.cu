@@ -22,6 +22,7 @@ constexpr int kThreads = 256;
 constexpr int kChunks = 2;
 constexpr uint32_t kSlice = kThreads * kChunks * 8;  // tokens of a block
 static_assert(kSlice <= 65536, "the list holds 16-bit positions");
+static_assert(kThreads <= 256, "an entry holds 8-bit threads");
 
 struct Logits {
     uint32_t first_row, vocab;
@@ -91,7 +92,8 @@ private:
 template <typename T, bool VEC, typename C>
 __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) {
     extern __shared__ uint4 smem[];
-    __shared__ uint32_t listed;
+    __shared__ uint32_t listed, named;
+    __shared__ uint32_t entries[kThreads];  // of the biases looked at together: position << 8 | thread
     uint32_t* const biased = reinterpret_cast<uint32_t*>(smem);  // kSlice bits
     const Counts<C> count{biased + kSlice / 32};                 // kSlice counts
     uint16_t* const list = reinterpret_cast<uint16_t*>(reinterpret_cast<C*>(count.words) + kSlice);  // kSlice positions
@@ -122,12 +124,21 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
     const float rep = a.repetition ? __ldg(a.repetition + row) : 1.0f;
     const float freq = a.frequency ? __ldg(a.frequency + row) : 0.0f, pres = a.presence ? __ldg(a.presence + row) : 0.0f;
     const bool lists = a.tokens || a.bias_tokens;
+    // The biases, kThreads at a time from the list's end; this thread's of these: its position (n or more: not in the
+    // slice), entered for the others to see.
+    const int32_t* names = a.bias_tokens + row * a.bts;
+    const uint32_t last_names = a.bias_tokens ? (a.biases - 1) / kThreads * kThreads : 0;
+    uint32_t named_here = 0xFFFFFFFFu;
+    auto enter = [&](uint32_t t) {
+        named_here = t;
+        if (t < n) entries[atomicAdd(&named, 1u)] = t << 8 | threadIdx.x;
+    };
     if (lists) {
         uint32_t len = a.history, prompt = 0;
         if (a.lengths) len = min((uint32_t)max(__ldg(a.lengths + row), 0), a.history);
         if (a.prompt_lengths) prompt = (uint32_t)max(__ldg(a.prompt_lengths + row), 0);
         Share tokens(a.tokens + row * a.ts, a.tokens ? a.history : 0);
-        if (threadIdx.x == 0) listed = 0;
+        if (threadIdx.x == 0) listed = named = 0;
         const uint32_t bytes = kSlice / 8 + (a.tokens ? kSlice * sizeof(C) : 0);
         for (uint32_t i = threadIdx.x; i < bytes / 16; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -138,10 +149,10 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
             });
         }
         if (a.bias_tokens) {
-            const int32_t* names = a.bias_tokens + row * a.bts;
             for (uint32_t i = threadIdx.x; i < a.biases; i += kThreads) {
                 const uint32_t t = (uint32_t)__ldg(names + i) - first;
                 if (t < n) atomicOr(&biased[t / 32], 1u << (t % 32));
+                if (i >= last_names) enter(t);
             }
         }
     }
@@ -190,19 +201,19 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
         }
     }
     if (a.bias_tokens) {
-        // from the list's end, 256 entries at a time: an entry counts if its token still has its bit and no later entry
-        // of these names it too
-        const int32_t* names = a.bias_tokens + row * a.bts;
-        for (uint32_t base = (a.biases - 1) / kThreads * kThreads;; base -= kThreads) {
-            const uint32_t i = base + threadIdx.x, end = min(base + kThreads, a.biases);
-            const int32_t token = i < end ? names[i] : -1;
-            const uint32_t t = (uint32_t)token - first;
-            bool last = i < end && t < n && (biased[t / 32] >> (t % 32) & 1u);
-            for (uint32_t k = i + 1; last && k < end; ++k) last = names[k] != token;
-            if (last) rule(t, a.bias_values[row * a.bvs + i]);
+        // an entry counts if its token still has its bit and no later entry of these names it too
+        for (uint32_t base = last_names;; base -= kThreads) {
+            const uint32_t t = named_here;
+            bool last = t < n && (biased[t / 32] >> (t % 32) & 1u);
+            for (uint32_t k = 0, m = last ? named : 0; k < m; ++k)
+                if (entries[k] >> 8 == t && (entries[k] & 255) > threadIdx.x) last = false;
+            if (last) rule(t, a.bias_values[row * a.bvs + base + threadIdx.x]);
             if (base == 0) break;
             __syncthreads();
             if (last) atomicAnd(&biased[t / 32], ~(1u << (t % 32)));
+            if (threadIdx.x == 0) named = 0;
+            __syncthreads();
+            enter((uint32_t)__ldg(names + base - kThreads + threadIdx.x) - first);
             __syncthreads();
         }
     }

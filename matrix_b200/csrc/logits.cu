@@ -16,13 +16,7 @@
 namespace mtxc {
 namespace {
 
-constexpr int kThreads = 256;
-// Eights of a thread.  More mean fewer scans of the lists but fewer blocks to hide them: [256, 131072] bf16 with a
-// history of 2,048 takes 65 us with 1, 45 with 2, 47 with 3, 46 with 4 and 61 with 8.
-constexpr int kChunks = 2;
-constexpr uint32_t kSlice = kThreads * kChunks * 8;  // tokens of a block
-static_assert(kSlice <= 65536, "the list holds 16-bit positions");
-static_assert(kThreads <= 256, "an entry holds 8-bit threads");
+constexpr int kChunks = 2;  // eights of a thread
 
 struct Logits {
     uint32_t first_row, vocab;
@@ -45,12 +39,13 @@ struct Logits {
 
 // A thread's share of a list: its first four entries, whose loads start before their number is known, then the rest,
 // four loads in flight.
+template <int THREADS>
 struct Share {
     const int32_t* list;
     int32_t t[4];
     __device__ __forceinline__ Share(const int32_t* p, uint32_t most) : list(p) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = threadIdx.x + k * kThreads < most ? __ldg(list + threadIdx.x + k * kThreads) : -1;
+        for (int k = 0; k < 4; ++k) t[k] = threadIdx.x + k * THREADS < most ? __ldg(list + threadIdx.x + k * THREADS) : -1;
     }
     // fn(index, token) for the entries below n
     template <typename Fn>
@@ -58,12 +53,12 @@ struct Share {
         for (uint32_t i = threadIdx.x;;) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (i + k * kThreads < n) fn(i + k * kThreads, t[k]);
-            i += 4 * kThreads;
+                if (i + k * THREADS < n) fn(i + k * THREADS, t[k]);
+            i += 4 * THREADS;
             if (i >= n) break;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (i + k * kThreads < n) t[k] = __ldg(list + i + k * kThreads);
+                if (i + k * THREADS < n) t[k] = __ldg(list + i + k * THREADS);
         }
     }
 };
@@ -89,11 +84,13 @@ private:
 
 // VEC: a thread's eights are eight consecutive tokens, one access each; else every 32nd of the warp's 256, so that
 // scalar accesses are contiguous across the warp.  C: the counts' type.
-template <typename T, bool VEC, typename C>
-__global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) {
+template <typename T, bool VEC, int THREADS, typename C>
+__global__ void __launch_bounds__(THREADS) logits_rules_kernel(const Logits a) {
+    constexpr uint32_t kSlice = THREADS * kChunks * 8;  // tokens of a block
+    static_assert(kSlice <= 65536 && THREADS <= 1024, "the list holds 16-bit positions, an entry 10-bit threads");
     extern __shared__ uint4 smem[];
     __shared__ uint32_t listed, named;
-    __shared__ uint32_t entries[kThreads];  // of the biases looked at together: position << 8 | thread
+    __shared__ uint32_t entries[THREADS];  // of the biases looked at together: position << 10 | thread
     uint32_t* const biased = reinterpret_cast<uint32_t*>(smem);  // kSlice bits
     const Counts<C> count{biased + kSlice / 32};                 // kSlice counts
     uint16_t* const list = reinterpret_cast<uint16_t*>(reinterpret_cast<C*>(count.words) + kSlice);  // kSlice positions
@@ -106,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
     const uint32_t* mask = a.mask ? a.mask + row * a.ms + first / 32 : nullptr;
     const uint32_t lane = threadIdx.x % 32;
     auto at = [&](int k, int j) {  // element j of eight k, in the slice
-        const uint32_t c = k * (kThreads * 8);
+        const uint32_t c = k * (THREADS * 8);
         return VEC ? c + threadIdx.x * 8 + j : c + (threadIdx.x - lane) * 8 + j * 32 + lane;
     };
     Eight<T> v[kChunks];
@@ -124,23 +121,23 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
     const float rep = a.repetition ? __ldg(a.repetition + row) : 1.0f;
     const float freq = a.frequency ? __ldg(a.frequency + row) : 0.0f, pres = a.presence ? __ldg(a.presence + row) : 0.0f;
     const bool lists = a.tokens || a.bias_tokens;
-    // The biases, kThreads at a time from the list's end; this thread's of these: its position (n or more: not in the
+    // The biases, THREADS at a time from the list's end; this thread's of these: its position (n or more: not in the
     // slice), entered for the others to see.
     const int32_t* names = a.bias_tokens + row * a.bts;
-    const uint32_t last_names = a.bias_tokens ? (a.biases - 1) / kThreads * kThreads : 0;
+    const uint32_t last_names = a.bias_tokens ? (a.biases - 1) / THREADS * THREADS : 0;
     uint32_t named_here = 0xFFFFFFFFu;
     auto enter = [&](uint32_t t) {
         named_here = t;
-        if (t < n) entries[atomicAdd(&named, 1u)] = t << 8 | threadIdx.x;
+        if (t < n) entries[atomicAdd(&named, 1u)] = t << 10 | threadIdx.x;
     };
     if (lists) {
         uint32_t len = a.history, prompt = 0;
         if (a.lengths) len = min((uint32_t)max(__ldg(a.lengths + row), 0), a.history);
         if (a.prompt_lengths) prompt = (uint32_t)max(__ldg(a.prompt_lengths + row), 0);
-        Share tokens(a.tokens + row * a.ts, a.tokens ? a.history : 0);
+        Share<THREADS> tokens(a.tokens + row * a.ts, a.tokens ? a.history : 0);
         if (threadIdx.x == 0) listed = named = 0;
         const uint32_t bytes = kSlice / 8 + (a.tokens ? kSlice * sizeof(C) : 0);
-        for (uint32_t i = threadIdx.x; i < bytes / 16; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
+        for (uint32_t i = threadIdx.x; i < bytes / 16; i += THREADS) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         if (a.tokens) {
             tokens.each(len, [&](uint32_t i, int32_t token) {
@@ -149,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
             });
         }
         if (a.bias_tokens) {
-            for (uint32_t i = threadIdx.x; i < a.biases; i += kThreads) {
+            for (uint32_t i = threadIdx.x; i < a.biases; i += THREADS) {
                 const uint32_t t = (uint32_t)__ldg(names + i) - first;
                 if (t < n) atomicOr(&biased[t / 32], 1u << (t % 32));
                 if (i >= last_names) enter(t);
@@ -195,48 +192,60 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const Logits a) 
         y[t] = from_float<T>(l + bias);
     };
     if (a.tokens) {
-        for (uint32_t i = threadIdx.x, m = listed; i < m; i += kThreads) {
+        for (uint32_t i = threadIdx.x, m = listed; i < m; i += THREADS) {
             const uint32_t t = list[i];
             if (!a.bias_tokens || !(biased[t / 32] >> (t % 32) & 1u)) rule(t, 0.0f);
         }
     }
     if (a.bias_tokens) {
         // an entry counts if its token still has its bit and no later entry of these names it too
-        for (uint32_t base = last_names;; base -= kThreads) {
+        for (uint32_t base = last_names;; base -= THREADS) {
             const uint32_t t = named_here;
             bool last = t < n && (biased[t / 32] >> (t % 32) & 1u);
             for (uint32_t k = 0, m = last ? named : 0; k < m; ++k)
-                if (entries[k] >> 8 == t && (entries[k] & 255) > threadIdx.x) last = false;
+                if (entries[k] >> 10 == t && (entries[k] & 1023) > threadIdx.x) last = false;
             if (last) rule(t, a.bias_values[row * a.bvs + base + threadIdx.x]);
             if (base == 0) break;
             __syncthreads();
             if (last) atomicAnd(&biased[t / 32], ~(1u << (t % 32)));
             if (threadIdx.x == 0) named = 0;
             __syncthreads();
-            enter((uint32_t)__ldg(names + base - kThreads + threadIdx.x) - first);
+            enter((uint32_t)__ldg(names + base - THREADS + threadIdx.x) - first);
             __syncthreads();
         }
     }
 }
 
 // Launches of fewer than 2^31 blocks.
-template <typename T, bool VEC, typename C>
+template <typename T, bool VEC, int THREADS, typename C>
 int launch(Logits l, uint64_t rows, cudaStream_t st) {
+    constexpr uint32_t kSlice = THREADS * kChunks * 8;
     const size_t smem = l.tokens ? kSlice / 8 + kSlice * (sizeof(C) + sizeof(uint16_t)) : l.bias_tokens ? kSlice / 8 : 0;
+    auto kernel = logits_rules_kernel<T, VEC, THREADS, C>;
+    if (smem > 40 * 1024) {  // the kernel has static shared memory too
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(logits_rules_kernel)");
+    }
     const uint32_t slices = (l.vocab + kSlice - 1) / kSlice;
     const uint64_t most = std::max<uint64_t>(1, ((1ull << 31) - 1) / slices);
     l.slices_div = FastDiv(slices);
     for (uint64_t row = 0; row < rows; row += most) {
         l.first_row = (uint32_t)row;
-        logits_rules_kernel<T, VEC, C><<<(unsigned)(std::min(most, rows - row) * slices), kThreads, smem, st>>>(l);
+        kernel<<<(unsigned)(std::min(most, rows - row) * slices), THREADS, smem, st>>>(l);
         if (int rc = check_launch("logits_rules_kernel")) return rc;
     }
     return MTXC_OK;
 }
 
+// Threads of a block, and with them its slice: larger slices scan the lists less often, smaller ones hide the scan
+// behind more blocks.  On a B200: [256, 131072] bf16 with a history of 2,048 takes 47 us with 256 threads, 42 with 512, 44
+// with 1024; [100, 131072] float with 1,000 26, 29 and 32; [256, 50257] bf16 (scalar accesses) 29, 35 and 41;
+// [64, 131072] bf16 with 40,000 85, 58 and 45.
 template <typename T, bool VEC>
 int launch(const Logits& l, uint64_t rows, cudaStream_t st) {
-    return l.history < 32768 ? launch<T, VEC, uint16_t>(l, rows, st) : launch<T, VEC, uint32_t>(l, rows, st);
+    if (l.history >= 32768) return launch<T, VEC, 1024, uint32_t>(l, rows, st);
+    if ((VEC && sizeof(T) == 2) || l.history > 8192) return launch<T, VEC, 512, uint16_t>(l, rows, st);
+    return launch<T, VEC, 256, uint16_t>(l, rows, st);
 }
 
 }  // namespace

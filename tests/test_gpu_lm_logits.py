@@ -63,7 +63,8 @@ def test_vocabularies(lm, dtype, vocab):
     check(lm, normal(3, vocab, dtype), inputs(3, vocab, 50, 9))
 
 
-@pytest.mark.parametrize("rows,history,biases", [(1, 1, 1), (1, 3000, 300), (40, 17, 2), (700, 5, 3), (2, 4097, 1)])
+@pytest.mark.parametrize("rows,history,biases", [(1, 1, 1), (1, 3000, 300), (40, 17, 2), (700, 5, 3), (2, 4097, 1),
+                                                 (2, 40000, 1), (3, 5, 2500)])
 def test_rows_and_lists(lm, rows, history, biases):
     check(lm, normal(rows, 500, torch.float32), inputs(rows, 500, history, biases))
 

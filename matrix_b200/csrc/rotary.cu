@@ -21,7 +21,7 @@ constexpr uint32_t kBlocksPerSm = 4;
 
 struct Rotary {
     uint32_t length, tile, tiles;  // tokens of a sequence, of a block; blocks of a sequence
-    uint32_t half, heads0;
+    uint32_t half, heads0, far;    // far: between the two accesses of a copied unit, 0: it has one
     uint32_t items, lanes, rows;   // units of a token; threads that take them side by side, and tokens side by side
     FastDiv tiles_div, units, lanes_div, half_div;  // units: of a head
     uint64_t first_batch;          // where the launch starts
@@ -43,14 +43,29 @@ __device__ __forceinline__ void turn(const Rotary& r, double position, uint32_t 
     sn *= r.sin_scale;
 }
 
+template <int M>
+__device__ __forceinline__ void read_table(const float* p, float (&v)[M]) {
+    if constexpr (M % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < M; i += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p + i);
+            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        }
+    } else if constexpr (M == 2) {
+        const float2 q = *reinterpret_cast<const float2*>(p);
+        v[0] = q.x, v[1] = q.y;
+    } else v[0] = p[0];
+}
+
 // A block takes `tile` tokens of a sequence.  It makes their cosines and sines once, in shared memory, for all heads
-// -- with its first loads already in flight -- and then turns units: VEC, eight pairs (two accesses of eight elements,
-// half a head apart) or, PAIRS (interleaved), eight elements of four pairs; else one pair.  What is not turned is
-// copied in units of eight elements, or one.  A thread stays with one unit of one head for all its tokens, kUnroll at
+// -- with its first loads already in flight -- and then turns units: N pairs (two accesses of N = 8 or 4 elements, half
+// a head apart) or, PAIRS (interleaved), N elements of N / 2 pairs; N = 0: one pair.  What is not turned is copied in units of
+// N elements, without PAIRS two such r.far apart where they divide so, or one element.  A thread stays with one unit of one head for all its tokens, kUnroll at
 // a time, so that a unit's place is worked out once (worked out for each, it was two thirds of the instructions).
-template <typename T, bool VEC, bool PAIRS>
+template <typename T, int N, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r) {
-    constexpr int kUnroll = VEC && !PAIRS ? 2 : 4;
+    constexpr int kUnroll = N && !PAIRS ? 2 : 4;
+    constexpr int kStep = N ? N : 1, kPairs = N == 0 ? 1 : PAIRS ? N / 2 : N;  // elements of a copy, pairs of a unit
     extern __shared__ float table[];  // [tile][half] cosines, then sines
     float* const cosines = table;
     float* const sines = table + r.tile * r.half;
@@ -59,19 +74,19 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r) {
     t0 *= r.tile;
     const uint32_t n = min(r.tile, r.length - t0);
     const uint64_t b = r.first_batch + batch;
-    const uint32_t turned = VEC ? (PAIRS ? r.half / 4 : r.half / 8) : r.half;  // units of a head that are turned
+    const uint32_t turned = r.half / kPairs;  // units of a head that are turned
     uint32_t lane, token0;  // this thread's first unit and token
     r.lanes_div.divmod(threadIdx.x, token0, lane);
     const bool idle = token0 >= r.rows;
 
     struct Unit {
-        Eight<T> a, b;
+        Few<T, N ? N : 4> a, b;
         T u, v;
     };
     const T* src = nullptr;
     T* dst = nullptr;
     uint64_t src_step = 0, dst_step = 0;
-    uint32_t at = 0;  // the unit's first pair
+    uint32_t at = 0, far = 0;  // the unit's first pair; from its first access to its second (0: none)
     bool copy = false;
     // places a unit of the tile's first token
     auto place = [&](uint32_t item) {
@@ -80,8 +95,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r) {
         const int k = h >= r.heads0;
         const uint64_t hh = k ? h - r.heads0 : h;
         copy = unit >= turned;
-        const uint32_t c = copy ? 2 * r.half + (unit - turned) * (VEC ? 8 : 1) : unit * (VEC ? 8 : PAIRS ? 2 : 1);
-        at = VEC ? (PAIRS ? unit * 4 : unit * 8) : unit;
+        far = copy ? r.far : PAIRS ? (N ? 0 : 1) : r.half;
+        at = unit * kPairs;
+        const uint32_t c = copy ? 2 * r.half + (unit - turned) * kStep : at * (PAIRS ? 2 : 1);
         src = static_cast<const T*>(r.src[k]) + b * r.ss[k][0] + t0 * r.ss[k][1] + hh * r.ss[k][2] + c;
         dst = static_cast<T*>(r.dst[k]) + b * r.ds[k][0] + t0 * r.ds[k][1] + hh * r.ds[k][2] + c;
         src_step = r.ss[k][1];
@@ -89,53 +105,50 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r) {
     };
     auto load = [&](uint32_t token, Unit& x) {
         const T* p = src + token * src_step;
-        if constexpr (VEC) {
+        if constexpr (N) {
             x.a.load(p);
-            if (!PAIRS && !copy) x.b.load(p + r.half);
+            if (!PAIRS && far) x.b.load(p + far);
         } else {
             x.u = p[0];
-            if (!copy) x.v = p[PAIRS ? 1 : r.half];
+            if (far) x.v = p[far];
         }
     };
     auto finish = [&](uint32_t token, Unit& x) {
         T* p = dst + token * dst_step;
-        const float* cs = cosines + token * r.half + at;
-        const float* sn = sines + token * r.half + at;
-        if constexpr (VEC) {
-            if (!copy) {
-                const float4* c4 = reinterpret_cast<const float4*>(cs);
-                const float4* s4 = reinterpret_cast<const float4*>(sn);
-                if constexpr (PAIRS) {
-                    const float4 c = c4[0], s = s4[0];
-                    const float cj[4] = {c.x, c.y, c.z, c.w}, sj[4] = {s.x, s.y, s.z, s.w};
+        if (!copy) {
+            float cs[kPairs], sn[kPairs];
+            read_table(cosines + token * r.half + at, cs);
+            read_table(sines + token * r.half + at, sn);
+            if constexpr (N == 0) {
+                const float u = to_float(x.u), v = to_float(x.v);
+                x.u = from_float<T>(u * cs[0] - v * sn[0]);
+                x.v = from_float<T>(u * sn[0] + v * cs[0]);
+            } else if constexpr (PAIRS) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 q = x.a.get2(j);
-                        const float2 o = __ffma2_rn(make_float2(q.x, q.x), make_float2(cj[j], sj[j]),
-                                                    __fmul2_rn(make_float2(q.y, q.y), make_float2(-sj[j], cj[j])));
-                        x.a.set2(j, o.x, o.y);
-                    }
-                } else {
-                    const float4 c0 = c4[0], c1 = c4[1], s0 = s4[0], s1 = s4[1];
-                    const float2 cj[4] = {{c0.x, c0.y}, {c0.z, c0.w}, {c1.x, c1.y}, {c1.z, c1.w}};
-                    const float2 sj[4] = {{s0.x, s0.y}, {s0.z, s0.w}, {s1.x, s1.y}, {s1.z, s1.w}};
+                for (int j = 0; j < kPairs; ++j) {
+                    const float2 q = x.a.get2(j);
+                    const float2 o = __ffma2_rn(make_float2(q.x, q.x), make_float2(cs[j], sn[j]),
+                                                __fmul2_rn(make_float2(q.y, q.y), make_float2(-sn[j], cs[j])));
+                    x.a.set2(j, o.x, o.y);
+                }
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 u = x.a.get2(j), v = x.b.get2(j);
-                        const float2 p = __ffma2_rn(u, cj[j], __fmul2_rn(v, make_float2(-sj[j].x, -sj[j].y)));
-                        const float2 q = __ffma2_rn(u, sj[j], __fmul2_rn(v, cj[j]));
-                        x.a.set2(j, p.x, p.y);
-                        x.b.set2(j, q.x, q.y);
-                    }
-                    x.b.store(p + r.half);
+                for (int j = 0; j < kPairs / 2; ++j) {
+                    const float2 u = x.a.get2(j), v = x.b.get2(j);
+                    const float2 c = make_float2(cs[2 * j], cs[2 * j + 1]), s = make_float2(sn[2 * j], sn[2 * j + 1]);
+                    const float2 p = __ffma2_rn(u, c, __fmul2_rn(v, make_float2(-s.x, -s.y)));
+                    const float2 q = __ffma2_rn(u, s, __fmul2_rn(v, c));
+                    x.a.set2(j, p.x, p.y);
+                    x.b.set2(j, q.x, q.y);
                 }
             }
+        }
+        if constexpr (N) {
             x.a.store(p);
-        } else if (copy) p[0] = x.u;
-        else {
-            const float u = to_float(x.u), v = to_float(x.v);
-            p[0] = from_float<T>(u * cs[0] - v * sn[0]);
-            p[PAIRS ? 1 : r.half] = from_float<T>(u * sn[0] + v * cs[0]);
+            if (!PAIRS && far) x.b.store(p + far);
+        } else {
+            p[0] = x.u;
+            if (far) p[far] = x.v;
         }
     };
 
@@ -226,11 +239,18 @@ extern "C" int mtxc_rotary(int dtype, const mtxc_rotary_args* a) {
     int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        bool vec = r.half % (pairs ? 4 : 8) == 0 && copied % 8 == 0;
-        for (int k = 0; k < 2; ++k)
-            for (int i = 0; a->heads[k] && i < 3; ++i)
-                vec = vec && eight_aligned<T>(r.src[k], r.ss[k][i]) && eight_aligned<T>(r.dst[k], r.ds[k][i]);
-        const uint32_t units = vec ? r.half / (pairs ? 4 : 8) + copied / 8 : r.half + copied;
+        // elements of an access: what the sizes, strides and addresses all divide by
+        auto fits = [&](auto count) {
+            constexpr int N = decltype(count)::value;
+            bool ok = r.half % (pairs ? N / 2 : N) == 0 && copied % N == 0;
+            for (int k = 0; k < 2; ++k)
+                for (int i = 0; a->heads[k] && i < 3; ++i)
+                    ok = ok && few_aligned<T, N>(r.src[k], r.ss[k][i]) && few_aligned<T, N>(r.dst[k], r.ds[k][i]);
+            return ok;
+        };
+        const uint32_t step = fits(std::integral_constant<int, 8>()) ? 8 : fits(std::integral_constant<int, 4>()) ? 4 : 1;
+        r.far = !pairs && copied % (2 * step) == 0 ? copied / 2 : 0;
+        const uint32_t units = r.half / (step == 1 ? 1 : pairs ? step / 2 : step) + copied / step / (r.far ? 2 : 1);
         r.units = FastDiv(units);
         r.half_div = FastDiv(std::max(1u, r.half));
         r.items = units * (uint32_t)heads;
@@ -258,10 +278,13 @@ extern "C" int mtxc_rotary(int dtype, const mtxc_rotary_args* a) {
             const unsigned blocks = (unsigned)(std::min(most, a->batch - batch) * r.tiles);
             const dim3 grid(blocks, blocks < (unsigned)ctx().sm_count ? rounds : 1);  // few tokens: no second round
             cudaStream_t st = ctx().stream();
-            if (vec && pairs) rotary_kernel<T, true, true><<<grid, threads, smem, st>>>(r);
-            else if (vec) rotary_kernel<T, true, false><<<grid, threads, smem, st>>>(r);
-            else if (pairs) rotary_kernel<T, false, true><<<grid, threads, smem, st>>>(r);
-            else rotary_kernel<T, false, false><<<grid, threads, smem, st>>>(r);
+            auto run = [&](auto count) {
+                if (pairs) rotary_kernel<T, decltype(count)::value, true><<<grid, threads, smem, st>>>(r);
+                else rotary_kernel<T, decltype(count)::value, false><<<grid, threads, smem, st>>>(r);
+            };
+            if (step == 8) run(std::integral_constant<int, 8>());
+            else if (step == 4) run(std::integral_constant<int, 4>());
+            else run(std::integral_constant<int, 0>());
             rc = check_launch("rotary_kernel");
         }
     });

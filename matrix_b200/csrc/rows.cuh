@@ -105,30 +105,32 @@ struct Philox {
 };
 
 // ------------------------------------------------------------------------------------------
-// Eight consecutive elements: 16 bytes of a half type, 32 of float (one 256-bit access).
+// N consecutive elements in one access of 8, 16 or 32 bytes (eight floats: one 256-bit access).
 // ------------------------------------------------------------------------------------------
-template <typename T>
-struct Eight {
-    uint32_t w[2 * sizeof(T)];
+template <typename T, int N>
+struct Few {
+    static constexpr int kBytes = N * (int)sizeof(T);
+    uint32_t w[kBytes / 4];
 
     // Streaming read, past L1.  Not volatile, as load_stream: read before anything writes it.
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (sizeof(T) == 4)
+        if constexpr (kBytes == 32)
             asm("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                 : "l"(p));
-        else
+        else if constexpr (kBytes == 16)
             asm("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                 : "l"(p));
+        else asm("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
     }
     __device__ __forceinline__ void store(T* p) const {
-        if constexpr (sizeof(T) == 4)
+        if constexpr (kBytes == 32)
             asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                          "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                          : "memory");
-        else
-            __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        else if constexpr (kBytes == 16) __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        else __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
     }
     __device__ __forceinline__ float get(int i) const {
         if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[i]);
@@ -152,10 +154,15 @@ struct Eight {
         }
     }
 };
-// What a pointer and its row stride (elements) need for Eight's accesses.
 template <typename T>
-inline bool eight_aligned(const void* p, uint64_t stride) {
-    return reinterpret_cast<uintptr_t>(p) % sizeof(Eight<T>) == 0 && stride % 8 == 0;
+using Eight = Few<T, 8>;
+
+// What a pointer and its row stride (elements) need for Few's accesses.
+template <typename T, int N>
+inline bool few_aligned(const void* p, uint64_t stride) {
+    return reinterpret_cast<uintptr_t>(p) % sizeof(Few<T, N>) == 0 && stride % N == 0;
 }
+template <typename T>
+inline bool eight_aligned(const void* p, uint64_t stride) { return few_aligned<T, 8>(p, stride); }
 
 }  // namespace mtxc

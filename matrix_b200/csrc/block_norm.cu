@@ -11,6 +11,8 @@
 // projection of s p on h, never longer than s p: the difference loses no more than H itself does.)
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "rows.cuh"
 
 namespace mtxc {
@@ -64,9 +66,9 @@ struct Forward {
 template <typename T, bool VEC>
 struct Chunk {
     uint32_t c;  // first column
-    // chunk k of thread `tid` of `threads` that share a row
-    __device__ __forceinline__ Chunk(uint32_t k, uint32_t threads, uint32_t tid)
-        : c(VEC ? (k * threads + tid) * 8 : (k * threads + (tid & ~31u)) * 8 + tid % 32) {}
+    // chunk k of thread `tid` of `threads` that share the columns from `from` (a multiple of 256)
+    __device__ __forceinline__ Chunk(uint32_t k, uint32_t threads, uint32_t tid, uint32_t from = 0)
+        : c(from + (VEC ? (k * threads + tid) * 8 : (k * threads + (tid & ~31u)) * 8 + tid % 32)) {}
     __device__ __forceinline__ uint32_t column(int j) const { return VEC ? c + j : c + 32 * j; }
     // whether element j lies in the row (VEC: all eight do or none)
     __device__ __forceinline__ bool inside(int j, uint32_t width) const { return VEC ? c < width : c + 32 * j < width; }
@@ -170,11 +172,11 @@ struct Kept {
     Lanes lanes[VEC ? K : 1];
     uint32_t bits = 0;
 
-    __device__ __forceinline__ void make(const DropArgs& d, uint32_t row, uint32_t threads, uint32_t tid) {
+    __device__ __forceinline__ void make(const DropArgs& d, uint32_t row, uint32_t threads, uint32_t tid, uint32_t from) {
         const Philox rng(d);
         uint32_t block[K], rows[K];
 #pragma unroll
-        for (int k = 0; k < K; ++k) block[k] = Chunk<T, VEC>(k, threads, tid).block(), rows[k] = row;
+        for (int k = 0; k < K; ++k) block[k] = Chunk<T, VEC>(k, threads, tid, from).block(), rows[k] = row;
         if constexpr (VEC) rng.make(block, rows, lanes);
         else {
             Lanes l[K];
@@ -428,7 +430,8 @@ struct Backward {
     // no part_post: S, in part_gate, gives both sums.
     float *part_next, *part_post, *part_gate;
     uint32_t groups, parts;  // gate rows (1 without a gate), blocks per gate row (1: blocks take whole gate rows)
-    uint32_t runs;           // blocks
+    uint32_t runs;           // teams
+    uint32_t cluster, cols;  // blocks that share a row, and a block's columns
 };
 
 // The rows of block `run`, gate row by gate row: calls fn(group, first, last) for each.
@@ -524,6 +527,8 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
     });
 }
 
+constexpr uint32_t kMaxCluster = 8;
+
 // The rows of a run: contiguous, so that the next ones can be fetched ahead across gate rows.
 __device__ __forceinline__ void run_rows(const Backward& f, uint32_t run, uint32_t& first, uint32_t& last) {
     if (f.parts > 1) {
@@ -568,7 +573,8 @@ struct Inputs {
                 for (int k = 0; k < K; ++k) regs[i][k] = Eight<T>{};
         }
     }
-    __device__ __forceinline__ void fetch(const Backward& f, uint32_t row, uint32_t stage, uint32_t threads, uint32_t tid) {
+    __device__ __forceinline__ void fetch(const Backward& f, uint32_t row, uint32_t stage, uint32_t threads, uint32_t tid,
+                                          uint32_t from, uint32_t limit) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const T* p = base(f, i);
@@ -576,14 +582,14 @@ struct Inputs {
             p += row * row_stride(f, i);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const Chunk<T, VEC> ch(k, threads, tid);
+                const Chunk<T, VEC> ch(k, threads, tid, from);
                 if constexpr (VEC) {
-                    if (ch.c >= f.width) continue;
+                    if (ch.c >= limit) continue;
 #pragma unroll
                     for (int v = 0; v < kPieces; ++v)
                         copy16(ring + (((stage * 4 + i) * K + k) * kPieces + v) * stride,
                                reinterpret_cast<const uint4*>(p + ch.c) + v);
-                } else regs[i][k] = ch.load(p, f.width);
+                } else regs[i][k] = ch.load(p, limit);
             }
         }
     }
@@ -617,19 +623,22 @@ __device__ __forceinline__ void store_sums(const Chunk<T, VEC>& ch, float* row, 
 
 // Rows read once: E elements per thread, the sums over rows in registers.  A run of rows for each team: a warp
 // (WARP), or `threads` threads; a block's teams add their sums in shared memory, so that there is one row of partial
-// sums for each block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.  SHARED: a
-// thread keeps its columns' w_next' and gate * w_post' in shared memory, as floats ready for use, for the run (or the
-// gate row); else they are made from the parameters for each row.  Inputs that the call does not have read as
-// zeros, weights as ones: fewer branches.
-template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool SHARED, int BLOCK, int MIN>
+// sums for each block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.  CLUSTER: a
+// row's columns are shared by the blocks of a cluster (one team each), f.cols to a block, which exchange their sums
+// through distributed shared memory: one cluster barrier per row.  A thread keeps its columns' w_next' and
+// gate * w_post' in shared memory, as floats ready for use, for the run (or the gate row).  Inputs that the call does
+// not have read as zeros, weights as ones: fewer branches.
+template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool CLUSTER, int BLOCK, int MIN>
 __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t team_threads, uint32_t stages) {
     constexpr int K = E / 8;
     extern __shared__ uint4 ring[];
     __shared__ float part[2][3 * 32];
+    __shared__ float from_rank[2][kMaxCluster][3];  // CLUSTER: the blocks' sums of a row
     const uint32_t threads = WARP ? 32 : team_threads, teams = blockDim.x / threads;
     const uint32_t team = threadIdx.x / threads, tid = threadIdx.x - team * threads;
-    const uint32_t run = blockIdx.x * teams + team;
-    const uint32_t width = f.width;
+    const uint32_t rank = CLUSTER ? blockIdx.x % f.cluster : 0;
+    const uint32_t run = CLUSTER ? blockIdx.x / f.cluster : blockIdx.x * teams + team;
+    const uint32_t from = CLUSTER ? rank * f.cols : 0, limit = CLUSTER ? min(f.width, from + f.cols) : f.width;
     const bool has_b = f.b, has_post = f.w_post, has_next = f.w_next, has_gate = f.gate, drops = f.drop.on && has_b;
     const bool want_s = f.part_post || f.dgate;
     const float cf = drops ? f.beta * f.drop.scale : f.beta;
@@ -644,16 +653,16 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
     in.absent(f, stages);
     if constexpr (VEC) {
         for (uint32_t i = 0; i < stages; ++i) {
-            if (first + i < last) in.fetch(f, first + i, i, threads, tid);
+            if (first + i < last) in.fetch(f, first + i, i, threads, tid, from, limit);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
     // which = 0: w_next', 1: gate * w_post'
     auto make_weights = [&](int which, int k, float2 (&w)[4]) {
-        const Chunk<T, VEC> ch(k, threads, tid);
+        const Chunk<T, VEC> ch(k, threads, tid, from);
         const void* p = which ? f.w_post : f.w_next;
         if (p) {
-            ch.param(p, 0, f.w_float, width, w);
+            ch.param(p, 0, f.w_float, limit, w);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = __fadd2_rn(both(f.w0), w[j]);
         } else {
@@ -662,7 +671,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         }
         if (which && has_gate) {
             float2 g[4];
-            ch.param(f.gate, group * f.gs, f.g_float, width, g);
+            ch.param(f.gate, group * f.gs, f.g_float, limit, g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = __fmul2_rn(g[j], w[j]);
         }
@@ -678,14 +687,12 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         }
     };
     auto get_weights = [&](int which, int k, float2 (&w)[4]) {
-        if constexpr (SHARED) {
             const float4* q = reinterpret_cast<const float4*>(weights + (which * K + k) * 2 * blockDim.x);
             const float4 a = q[0], b = q[blockDim.x];
             w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
             w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
-        } else make_weights(which, k, w);
     };
-    if constexpr (SHARED) keep_weights(0), keep_weights(1);
+    keep_weights(0), keep_weights(1);
 
     float2 A[K][4], S[K][4], W[MULTI ? K : 1][4];
 #pragma unroll
@@ -702,15 +709,16 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         if (has_next) next_s = __ldg(f.next_rstd + row);
     };
     if (first < last) load_rstd(first);
+    if constexpr (CLUSTER) cooperative_groups::this_cluster().sync();  // every block runs before the first is written to
     for (uint32_t row = first, stage = 0; row < last; ++row) {
         const float r = next_r, s = next_s;
         if (row + 1 < last) load_rstd(row + 1);
         if constexpr (VEC) {
             if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
             else asm volatile("cp.async.wait_group 0;" ::: "memory");
-        } else in.fetch(f, row, 0, threads, tid);
+        } else in.fetch(f, row, 0, threads, tid, from, limit);
         Kept<T, K, VEC> kept;
-        if (drops) kept.make(f.drop, row, threads, tid);
+        if (drops) kept.make(f.drop, row, threads, tid, from);
         float2 c1 = both(0.0f), su = both(0.0f), sv = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -734,11 +742,23 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         }
         float sum[3] = {c1.x + c1.y, su.x + su.y, sv.x + sv.y};
         row_sum<3, WARP>(sum, part[(row - first) % 2], threads, team);
-        const float kappa = s * s * s * (sum[0] / width);
-        const float c2 = r * r * r * (cf * (sum[1] - kappa * sum[2]) / width);
+        if constexpr (CLUSTER) {
+            // double buffered like part: a block that writes a row's slots again has passed the barrier of the row between
+            cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+            float(&slots)[kMaxCluster][3] = from_rank[(row - first) % 2];
+            if (threadIdx.x < f.cluster) {
+                float* to = cluster.map_shared_rank(slots[rank], threadIdx.x);
+                to[0] = sum[0], to[1] = sum[1], to[2] = sum[2];
+            }
+            cluster.sync();
+            sum[0] = sum[1] = sum[2] = 0.0f;
+            for (uint32_t i = 0; i < f.cluster; ++i) sum[0] += slots[i][0], sum[1] += slots[i][1], sum[2] += slots[i][2];
+        }
+        const float kappa = s * s * s * (sum[0] / f.width);
+        const float c2 = r * r * r * (cf * (sum[1] - kappa * sum[2]) / f.width);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const Chunk<T, VEC> ch(k, threads, tid);
+            const Chunk<T, VEC> ch(k, threads, tid, from);
             const Eight<T> dh = in.get(0, k, stage), da = in.get(1, k, stage), h = in.get(2, k, stage),
                            b = in.get(3, k, stage);
             float2 H[4], w[4], o[4];
@@ -750,7 +770,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
                 H[j] = __ffma2_rn(d, w[j], __ffma2_rn(both(-kappa), h.get2(j), dh.get2(j)));
                 o[j] = __fmul2_rn(both(f.alpha), H[j]);
             }
-            if (f.dx) ch.store(static_cast<T*>(f.dx) + row * f.dxs, width, o);
+            if (f.dx) ch.store(static_cast<T*>(f.dx) + row * f.dxs, limit, o);
             if (!has_b) continue;
             if (drops) kept.zero_others(f.drop, k, H);
             get_weights(1, k, w);
@@ -764,10 +784,10 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
 #pragma unroll
                 for (int j = 0; j < 4; ++j) H[j] = __ffma2_rn(both(-c2), b.get2(j), H[j]);
             }
-            if (f.db) ch.store(static_cast<T*>(f.db) + row * f.dbs, width, H);
+            if (f.db) ch.store(static_cast<T*>(f.db) + row * f.dbs, limit, H);
         }
         if constexpr (VEC) {
-            if (row + stages < last) in.fetch(f, row + stages, stage, threads, tid);
+            if (row + stages < last) in.fetch(f, row + stages, stage, threads, tid, from, limit);
             asm volatile("cp.async.commit_group;" ::: "memory");
             stage = stage + 1 == stages ? 0 : stage + 1;
         }
@@ -775,19 +795,19 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             if (want_s) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    const Chunk<T, VEC> ch(k, threads, tid);
+                    const Chunk<T, VEC> ch(k, threads, tid, from);
                     float2 w[4];
-                    ch.param(f.gate, group * f.gs, f.g_float, width, w);
+                    ch.param(f.gate, group * f.gs, f.g_float, limit, w);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) W[MULTI ? k : 0][j] = __ffma2_rn(w[j], S[k][j], W[MULTI ? k : 0][j]);
                     if (f.dgate) {
                         if (has_post) {
-                            ch.param(f.w_post, 0, f.w_float, width, w);
+                            ch.param(f.w_post, 0, f.w_float, limit, w);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) S[k][j] = __fmul2_rn(S[k][j], __fadd2_rn(both(f.w0), w[j]));
                         }
-                        if (f.g_float) store_sums(ch, static_cast<float*>(f.dgate) + group * f.dgs, width, S[k]);
-                        else ch.store(static_cast<T*>(f.dgate) + group * f.dgs, width, S[k]);
+                        if (f.g_float) store_sums(ch, static_cast<float*>(f.dgate) + group * f.dgs, limit, S[k]);
+                        else ch.store(static_cast<T*>(f.dgate) + group * f.dgs, limit, S[k]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) S[k][j] = both(0.0f);
@@ -795,20 +815,20 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             }
             if (row + 1 < last) {
                 ++group, group_left = f.gate_rows;
-                if constexpr (SHARED) keep_weights(1);
+                keep_weights(1);
             }
         }
     }
     if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
-    float* const out_a = f.part_next ? f.part_next + (uint64_t)blockIdx.x * width : nullptr;
+    float* const out_a = f.part_next ? f.part_next + (uint64_t)(CLUSTER ? run : blockIdx.x) * f.width : nullptr;
     float* out_s = MULTI || !f.part_gate ? f.part_post : f.part_gate;
-    if (out_s) out_s += (uint64_t)blockIdx.x * width;
-    if (!SHARED || teams == 1) {
+    if (out_s) out_s += (uint64_t)(CLUSTER ? run : blockIdx.x) * f.width;
+    if (CLUSTER || teams == 1) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const Chunk<T, VEC> ch(k, threads, tid);
-            if (out_a) store_sums(ch, out_a, width, A[k]);
-            if (out_s) store_sums(ch, out_s, width, MULTI ? W[MULTI ? k : 0] : S[k]);
+            const Chunk<T, VEC> ch(k, threads, tid, from);
+            if (out_a) store_sums(ch, out_a, limit, A[k]);
+            if (out_s) store_sums(ch, out_s, limit, MULTI ? W[MULTI ? k : 0] : S[k]);
         }
         return;
     }
@@ -826,7 +846,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
     for (uint32_t piece = team; piece < 4 * K; piece += teams) {
         float* out = piece < 2 * K ? out_a : out_s;
         if (!out) continue;
-        const Chunk<T, VEC> ch(piece / 2 % K, threads, tid);
+        const Chunk<T, VEC> ch(piece / 2 % K, threads, tid, from);
         const float4* slot = own + piece * blockDim.x - team * threads;
         float4 sum = slot[0];
         for (uint32_t t = 1; t < teams; ++t) {
@@ -835,12 +855,12 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         }
         const int j = piece % 2 * 4;
         if constexpr (VEC) {
-            if (ch.c < width) *reinterpret_cast<float4*>(out + ch.c + j) = sum;
+            if (ch.c < limit) *reinterpret_cast<float4*>(out + ch.c + j) = sum;
         } else {
             const float e[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (ch.inside(j + i, width)) out[ch.column(j + i)] = e[i];
+                if (ch.inside(j + i, limit)) out[ch.column(j + i)] = e[i];
         }
     }
 }
@@ -899,10 +919,11 @@ __global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const
     }
 }
 
-// Which backward kernel serves a width, and with what blocks.
+// Which backward kernel serves a width, and with what blocks.  Rows of more than 8192 elements go to clusters of 2 to 8
+// blocks, of more than 65,536 to block_norm_backward_any_kernel.
 struct Plan {
     int kind = -1;  // -1: block_norm_backward_any_kernel
-    uint32_t team = kThreads, teams = 1, blocks_per_sm = 2, stages = 1;
+    uint32_t team = kThreads, teams = 1, blocks_per_sm = 2, stages = 1, cluster = 1, cols = 0;
     size_t team_smem = 0;
 };
 
@@ -911,51 +932,72 @@ constexpr size_t kMaxShared = 227 * 1024 - 2048;  // less the kernels' static pa
 template <typename T>
 Plan plan_backward(uint32_t width, bool vec) {
     Plan p;
+    while (p.cluster < kMaxCluster && width > 8192 * p.cluster) p.cluster *= 2;
+    p.cols = p.cluster > 1 ? ((width + p.cluster - 1) / p.cluster + 255) / 256 * 256 : width;
+    if (p.cols > 8192) return Plan();
     uint32_t e = 16, block = 512, regs = 128;  // elements of a thread, threads of a block, registers
-    if (width <= 256) p.kind = 0, e = 8, block = 256;
-    else if (vec && width <= 512) p.kind = 1, block = 256;
-    else if (vec && width <= 8192) p.kind = 2;
-    else if (vec && width <= 16384) p.kind = 3, block = 1024, regs = 64;
-    else if (!vec && width <= 4096) p.kind = 4, e = 8, regs = 64;
-    else if (!vec && width <= 8192) p.kind = 5, e = 8, block = 1024, regs = 64;
-    else return p;
-    p.team = p.kind <= 1 ? 32 : (width + 32 * e - 1) / (32 * e) * 32;
+    if (p.cols <= 256) p.kind = 0, e = 8, block = 256;
+    else if (vec && p.cols <= 512) p.kind = 1, block = 256;
+    else if (vec) p.kind = 2;
+    else if (p.cols <= 4096) p.kind = 3, e = 8, regs = 64;
+    else p.kind = 4, e = 8, block = 1024, regs = 64;
+    p.team = p.kind <= 1 ? 32 : (p.cols + 32 * e - 1) / (32 * e) * 32;
     // the rows of a stage, and the weights
-    const size_t stage = vec ? (size_t)p.team * 4 * e * sizeof(T) : 0, weights = p.kind == 3 ? 0 : p.team * 2 * e * sizeof(float);
-    if (stage + weights > kMaxShared) return Plan();
+    const size_t stage = vec ? (size_t)p.team * 4 * e * sizeof(T) : 0, weights = p.team * 2 * e * sizeof(float);
     p.stages = 2 * stage + weights <= kMaxShared ? 2 : 1;
     p.team_smem = p.stages * stage + weights;
-    p.teams = p.kind == 3 ? 1 : (uint32_t)std::min<size_t>({block / p.team, std::max<size_t>(1, kMaxShared / std::max<size_t>(1, p.team_smem)), 15});
+    if (p.cluster == 1) p.teams = (uint32_t)std::min<size_t>({block / p.team, kMaxShared / p.team_smem, 15});
     const uint32_t threads = p.team * p.teams;
     p.blocks_per_sm = std::max<uint32_t>(
         1, std::min<size_t>({2048 / threads, 65536 / (threads * regs), kMaxShared / (p.team_smem * p.teams + 2048)}));
     return p;
 }
 
-template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool SHARED, int BLOCK, int MIN>
+template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool CLUSTER, int BLOCK, int MIN>
 int launch_backward_kernel(const Backward& f, const Plan& p, cudaStream_t st) {
-    auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, SHARED, BLOCK, MIN>;
+    auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, CLUSTER, BLOCK, MIN>;
     const size_t smem = p.team_smem * p.teams;
-    if (smem > 46 * 1024) {  // the kernel has static shared memory too
-        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(block_norm_backward_kernel)");
+    cudaError_t err = cudaSuccess;
+    if (smem > 46 * 1024)  // the kernel has static shared memory too
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(block_norm_backward_kernel)");
+    if constexpr (CLUSTER) {
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = p.cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(f.runs * p.cluster);
+        config.blockDim = dim3(p.team);
+        config.dynamicSmemBytes = smem;
+        config.stream = st;
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        err = cudaLaunchKernelEx(&config, kernel, f, p.team, p.stages);
+        if (err != cudaSuccess) return cuda_fail(err, "block_norm_backward_kernel");
+        return MTXC_OK;
+    } else {
+        kernel<<<(f.runs + p.teams - 1) / p.teams, p.team * p.teams, smem, st>>>(f, p.team, p.stages);
+        return check_launch("block_norm_backward_kernel");
     }
-    kernel<<<(f.runs + p.teams - 1) / p.teams, p.team * p.teams, smem, st>>>(f, p.team, p.stages);
-    return check_launch("block_norm_backward_kernel");
 }
 
 template <typename T, bool MULTI>
 int launch_backward(const Backward& f, const Plan& p, bool vec, cudaStream_t st) {
+    if (p.cluster > 1) {
+        if (vec) return launch_backward_kernel<T, 16, true, false, MULTI, true, 512, 1>(f, p, st);
+        return launch_backward_kernel<T, 8, false, false, MULTI, true, 1024, 1>(f, p, st);
+    }
     switch (p.kind) {
         case 0:
-            return vec ? launch_backward_kernel<T, 8, true, true, MULTI, true, 256, 2>(f, p, st)
-                       : launch_backward_kernel<T, 8, false, true, MULTI, true, 256, 2>(f, p, st);
-        case 1: return launch_backward_kernel<T, 16, true, true, MULTI, true, 256, 2>(f, p, st);
-        case 2: return launch_backward_kernel<T, 16, true, false, MULTI, true, 512, 1>(f, p, st);
-        case 3: return launch_backward_kernel<T, 16, true, false, MULTI, false, 1024, 1>(f, p, st);
-        case 4: return launch_backward_kernel<T, 8, false, false, MULTI, true, 512, 2>(f, p, st);
-        case 5: return launch_backward_kernel<T, 8, false, false, MULTI, true, 1024, 1>(f, p, st);
-        default: block_norm_backward_any_kernel<T><<<f.runs, kThreads, 0, st>>>(f); return check_launch("block_norm_backward_any_kernel");
+            return vec ? launch_backward_kernel<T, 8, true, true, MULTI, false, 256, 2>(f, p, st)
+                       : launch_backward_kernel<T, 8, false, true, MULTI, false, 256, 2>(f, p, st);
+        case 1: return launch_backward_kernel<T, 16, true, true, MULTI, false, 256, 2>(f, p, st);
+        case 2: return launch_backward_kernel<T, 16, true, false, MULTI, false, 512, 1>(f, p, st);
+        case 3: return launch_backward_kernel<T, 8, false, false, MULTI, false, 512, 2>(f, p, st);
+        case 4: return launch_backward_kernel<T, 8, false, false, MULTI, false, 1024, 1>(f, p, st);
+        default:
+            block_norm_backward_any_kernel<T><<<f.runs, kThreads, 0, st>>>(f);
+            return check_launch("block_norm_backward_any_kernel");
     }
 }
 
@@ -1113,7 +1155,9 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     const uint64_t row_bytes = (uint64_t)f.width * sizeof(float) * sums;
     // teams that the GPU holds; a block's teams share a gate row, or each has whole ones; few rows: fewer teams in a
     // block, so that all SMs have some
-    const uint64_t most = (uint64_t)ctx().sm_count * plan.blocks_per_sm * plan.teams;
+    f.cluster = plan.cluster;
+    f.cols = plan.cols;
+    const uint64_t most = std::max<uint64_t>(1, (uint64_t)ctx().sm_count * plan.blocks_per_sm * plan.teams / plan.cluster);
     f.groups = (uint32_t)(((uint64_t)f.rows + f.gate_rows - 1) / f.gate_rows);
     plan.teams = (uint32_t)std::min<uint64_t>(plan.teams, std::max<uint64_t>(1, f.rows / ctx().sm_count));
     if (f.gate && most >= f.groups) plan.teams = (uint32_t)std::min<uint64_t>(plan.teams, most / f.groups);

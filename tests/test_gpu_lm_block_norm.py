@@ -131,6 +131,15 @@ def test_backward_widths(lm, dtype, width):
     Case((2, width), dtype, gate="token").check_backward(lm)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [8193, 16385, 32776, 50001, 65536, 65544, 70001])
+def test_backward_of_wide_rows(lm, dtype, width):
+    """Rows shared by 2, 4 and 8 blocks, and rows past 65,536."""
+    Case((7, width), dtype, gate="channel", drop=0.2, alpha=0.5).check_backward(lm)
+    Case((3, 2, width), dtype, gate="sequence").check_backward(lm)
+    Case((300, width // 8 + 8192), dtype).check_backward(lm)
+
+
 @pytest.mark.parametrize("width", [64, 100, 2048, 2049])
 @pytest.mark.parametrize("rows", [1, 3, 147, 149, 300, 1500])
 def test_rows(lm, rows, width):

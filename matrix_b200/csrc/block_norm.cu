@@ -73,6 +73,10 @@ struct Chunk {
     // whether element j lies in the row (VEC: all eight do or none)
     __device__ __forceinline__ bool inside(int j, uint32_t width) const { return VEC ? c < width : c + 32 * j < width; }
 
+    // whether the warp's 256 columns all lie in the row: then scalar accesses need no comparisons, which were a third of
+    // the instructions of a row of half types
+    __device__ __forceinline__ bool whole(uint32_t width) const { return c - threadIdx.x % 32 + 256 <= width; }
+
     __device__ __forceinline__ Eight<T> load(const T* row, uint32_t width) const {
         Eight<T> v;
         if constexpr (VEC) {
@@ -81,8 +85,14 @@ struct Chunk {
             if (c < width) v.load(row + c);
         } else {
             T e[8];
+            const T* p = row + c;
+            if (whole(width)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = inside(j, width) ? row[c + 32 * j] : T(0.0f);
+                for (int j = 0; j < 8; ++j) e[j] = p[32 * j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = inside(j, width) ? p[32 * j] : T(0.0f);
+            }
             memcpy(v.w, e, sizeof(e));
         }
         return v;
@@ -96,9 +106,15 @@ struct Chunk {
         } else {
             T e[8];
             memcpy(e, o.w, sizeof(e));
+            T* p = row + c;
+            if (whole(width)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (inside(j, width)) row[c + 32 * j] = e[j];
+                for (int j = 0; j < 8; ++j) p[32 * j] = e[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (inside(j, width)) p[32 * j] = e[j];
+            }
         }
     }
     // Eight values of a weight or gate row, shared by many rows and so left in L1 (0 outside the row).
@@ -119,9 +135,19 @@ struct Chunk {
                 for (int j = 0; j < 4; ++j) v[j] = e.get2(j);
             }
         } else {
-            auto one = [&](int j) { return inside(j, width) ? mtxc::param<T>(p, at + c + 32 * j, is_float) : 0.0f; };
+            auto all = [&](auto* q) {
+                q += at + c;
+                if (whole(width)) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = make_float2(one(2 * j), one(2 * j + 1));
+                    for (int j = 0; j < 4; ++j) v[j] = make_float2(to_float(q[64 * j]), to_float(q[64 * j + 32]));
+                } else {
+                    auto one = [&](int j) { return inside(j, width) ? to_float(q[32 * j]) : 0.0f; };
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = make_float2(one(2 * j), one(2 * j + 1));
+                }
+            };
+            if (is_float) all(static_cast<const float*>(p));
+            else all(static_cast<const T*>(p));
         }
     }
     // The column block whose counter this lane makes: its own, or one of the warp's 32.

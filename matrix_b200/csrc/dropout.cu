@@ -82,12 +82,18 @@ __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const Dropout a) 
         const uint32_t c0 = block0 * 8 + lane;
         const T* src = static_cast<const T*>(a.src) + row0 * a.ss + c0;
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            to[j] = row0 * a.ds + c0 + 32 * j;
-            if (c0 + 32 * j < a.width) {
-                valid |= 1u << j;
-                x[j] = src[32 * j];
-            }
+        for (uint32_t j = 0; j < 8; ++j) to[j] = row0 * a.ds + c0 + 32 * j;
+        if (block0 * 8 + 256 <= a.width) {  // the whole warp inside the row: no comparisons
+            valid = 0xFF;
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) x[j] = src[32 * j];
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (c0 + 32 * j < a.width) {
+                    valid |= 1u << j;
+                    x[j] = src[32 * j];
+                }
         }
     } else {
         const uint32_t inside = i < a.items ? min(8u, a.width - block * 8) : 0;

@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(const Logits a) {
         const uint32_t c = k * (THREADS * 8);
         return VEC ? c + threadIdx.x * 8 + j : c + (threadIdx.x - lane) * 8 + j * 32 + lane;
     };
+    // scalar accesses: whether the warp's 256 tokens of eight k all lie in the slice, and need no comparisons
+    auto whole = [&](int k) { return at(k, 0) - lane + 256 <= n; };
     Eight<T> v[kChunks];
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
@@ -113,8 +115,14 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(const Logits a) {
             if (at(k, 0) < n) v[k].load(x + at(k, 0));
         } else {
             T e[8];
+            const T* p = x + at(k, 0);
+            if (whole(k)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = at(k, j) < n ? x[at(k, j)] : T(0.0f);
+                for (int j = 0; j < 8; ++j) e[j] = p[32 * j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = at(k, j) < n ? p[32 * j] : T(0.0f);
+            }
             memcpy(v[k].w, e, sizeof(e));
         }
     }
@@ -170,11 +178,15 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(const Logits a) {
         } else {
             T e[8];
             memcpy(e, v[k].w, sizeof(e));
+            T* p = y + at(k, 0);
+            const uint32_t* m = mask ? mask + at(k, 0) / 32 : nullptr;  // the warp's eight words, one for each element
+            if (whole(k)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (at(k, j) >= n) continue;
-                if (mask && !(__ldg(mask + at(k, j) / 32) >> lane & 1u)) e[j] = from_float<T>(-INFINITY);
-                y[at(k, j)] = e[j];
+                for (int j = 0; j < 8; ++j) p[32 * j] = m && !(__ldg(m + j) >> lane & 1u) ? from_float<T>(-INFINITY) : e[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at(k, j) < n) p[32 * j] = m && !(__ldg(m + j) >> lane & 1u) ? from_float<T>(-INFINITY) : e[j];
             }
         }
     }

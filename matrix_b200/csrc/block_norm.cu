@@ -391,7 +391,7 @@ int launch_forward(const Forward& f, cudaStream_t st, int sms) {
     return check_launch("block_norm_kernel");
 }
 
-// Any width, stride and alignment: a block per row, which reads its row once for each sum.
+// Any width (in use: above 16,384), stride and alignment: a block per row, which reads its row once for each sum.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) block_norm_any_kernel(const Forward f) {
     __shared__ float part[32];
@@ -438,10 +438,10 @@ __global__ void __launch_bounds__(kThreads) block_norm_any_kernel(const Forward 
 }
 
 // ------------------------------------------------------------------------------------------
-// Backward.  The rows are cut into one contiguous run for each block; a block adds its rows' shares of the
-// sums over rows into rows of its own in the workspace, and a second kernel adds the blocks' in order.  Where
-// there is a gate, runs respect its rows: either a block has whole gate rows (parts == 1) and writes their
-// gradients itself, or `parts` blocks share one gate row and leave their S to the second kernel.
+// Backward.  The rows are cut into contiguous runs, one for each team of threads (a block, or a part of one); a
+// block leaves its teams' sums over rows as one row of partial sums in the workspace, and a second kernel adds the
+// blocks' in order.  Where there is a gate, runs respect its rows: either a run has whole gate rows (parts == 1) and
+// writes their gradients itself, or `parts` runs share one gate row and leave their S to the second kernel.
 // ------------------------------------------------------------------------------------------
 struct Backward {
     const void *dh, *da, *h, *b, *w_post, *w_next, *gate;
@@ -452,11 +452,11 @@ struct Backward {
     bool w_float, g_float;
     float alpha, beta, w0;
     DropArgs drop;
-    // partial sums, one row of `width` floats per run each; NULL: not wanted.  Where runs share gate rows there is
+    // partial sums, one row of `width` floats per block each; NULL: not wanted.  Where runs share gate rows there is
     // no part_post: S, in part_gate, gives both sums.
     float *part_next, *part_post, *part_gate;
-    uint32_t groups, parts;  // gate rows (1 without a gate), blocks per gate row (1: blocks take whole gate rows)
-    uint32_t runs;           // teams
+    uint32_t groups, parts;  // gate rows (1 without a gate), runs per gate row (1: runs take whole gate rows)
+    uint32_t runs;
     uint32_t cluster, cols;  // blocks that share a row, and a block's columns
 };
 
@@ -477,7 +477,8 @@ __device__ __forceinline__ void for_each_segment(const Backward& f, uint32_t run
     }
 }
 
-// Any width, stride and alignment: the rows are read twice and the sums over rows live in the workspace.
+// Any width (in use: above 65,536), stride and alignment: the rows are read twice and the sums over rows live in the
+// workspace.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const Backward f) {
     __shared__ float part[3 * 32];
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
             const T* b = static_cast<const T*>(f.b) + row * f.bs;
             const float r = f.w_post ? f.post_rstd[row] : 1.0f, s = f.w_next ? f.next_rstd[row] : 0.0f;
             auto upper = [&](uint32_t c) { return f.dh ? to_float(dh[c]) : 0.0f; };
+            auto stream = [&](uint32_t c) { return f.w_next ? to_float(h[c]) : 0.0f; };  // serves the next norm alone
             auto p_of = [&](uint32_t c) {
                 return f.w_next ? to_float(da[c]) * (f.w0 + param<T>(f.w_next, c, f.w_float)) : 0.0f;
             };
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
             };
             float sum[3] = {0.0f, 0.0f, 0.0f};
             for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
-                const float p = p_of(c), hv = to_float(h[c]);
+                const float p = p_of(c), hv = stream(c);
                 sum[0] += p * hv;
                 if (f.w_post) {
                     const float e = mask(c) * gate(c) * post(c) * to_float(b[c]);
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
             const float kappa = s * s * s * (sum[0] / f.width);
             const float c2 = (sum[1] - kappa * sum[2]) / f.width;
             for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
-                const float hv = to_float(h[c]);
+                const float hv = stream(c);
                 const float g_next = f.w_next ? to_float(da[c]) * hv * s : 0.0f;
                 const float H = upper(c) + s * p_of(c) - hv * kappa;
                 if (f.b) {
@@ -713,10 +715,10 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         }
     };
     auto get_weights = [&](int which, int k, float2 (&w)[4]) {
-            const float4* q = reinterpret_cast<const float4*>(weights + (which * K + k) * 2 * blockDim.x);
-            const float4 a = q[0], b = q[blockDim.x];
-            w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
-            w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
+        const float4* q = reinterpret_cast<const float4*>(weights + (which * K + k) * 2 * blockDim.x);
+        const float4 a = q[0], b = q[blockDim.x];
+        w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
+        w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
     };
     keep_weights(0), keep_weights(1);
 

@@ -390,6 +390,34 @@ def test_refusals(lm):
         assert e.value.code == code
 
 
+@pytest.mark.parametrize("width", [64, 4096, 70000])
+def test_gradients_in_place_and_of_a_scaled_stream(lm, gpu, width):
+    """Through the C ABI: gradients written over the tensors they are made from; and without norm and branch, where
+    the call needs no residual_out at all."""
+    from matrix_b200 import _abi
+
+    lib = _abi.lib()
+    c = Case((6, width), torch.float32)
+    h, r, s = c.stored()
+    dh, da, b, hd = (t.cuda() for t in (c.dh, c.da, c.b, h))
+    kept = [t.cuda() for t in (r, s, c.post, c.next)]
+    want = lm.block_norm_backward(dh, da, hd, b, post_rstd=kept[0], next_rstd=kept[1], post_weight=kept[2],
+                                  next_weight=kept[3], parameters=False)
+    at = [t.data_ptr() for t in kept]
+    drop = (0.0, 0, 0, 0)
+    _abi.check(lib.mtxc_block_norm_backward(0, _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
+        6, width, dh.data_ptr(), width, da.data_ptr(), width, hd.data_ptr(), width, b.data_ptr(), width, *at, 0, 0, 0,
+        dh.data_ptr(), width, b.data_ptr(), width, 0, 0, 0, 0, 0, 0, 1.0, 1.0, 0.0, *drop)))
+    gpu.sync()
+    assert torch.equal(dh, want.residual) and torch.equal(b, want.branch)
+    dx = torch.empty_like(dh)
+    _abi.check(lib.mtxc_block_norm_backward(0, _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
+        6, width, dh.data_ptr(), width, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, dx.data_ptr(), width, 0, 0, 0, 0, 0, 0, 0, 0,
+        0.5, 1.0, 0.0, *drop)))
+    gpu.sync()
+    assert torch.equal(dx, dh * 0.5)
+
+
 def test_workspace_refusal(lm, gpu):
     """Partial sums that do not fit the thread's workspace: refused, and nothing is written."""
     from matrix_b200 import MtxcError, _abi

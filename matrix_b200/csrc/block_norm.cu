@@ -745,6 +745,17 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
             else asm volatile("cp.async.wait_group 0;" ::: "memory");
         } else in.fetch(f, row, 0, threads, tid, from, limit);
+        // a gate row that ends with this row: the next one's way from HBM starts now
+        if (MULTI && group_left == 1 && row + 1 < last) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const Chunk<T, VEC> ch(k, threads, tid, from);
+                const uint64_t at = (group + 1) * f.gs + ch.c;
+                const void* p = f.g_float ? static_cast<const void*>(static_cast<const float*>(f.gate) + at)
+                                          : static_cast<const void*>(static_cast<const T*>(f.gate) + at);
+                if (ch.c < limit) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+            }
+        }
         Kept<T, K, VEC> kept;
         if (drops) kept.make(f.drop, row, threads, tid, from);
         float2 c1 = both(0.0f), su = both(0.0f), sv = both(0.0f);
@@ -902,27 +913,38 @@ struct Finish {
     const void *w_post, *gate;
     uint64_t dgs, gs;
     uint32_t width, runs, parts;  // rows of partial sums in all, and for a gate row
+    uint32_t split_log;
     bool w_float, g_float;
     float w0;
 };
 
-constexpr int kFinishThreads = 1024;  // a warp adds a 32nd of the partial rows of 32 columns
+constexpr uint32_t kFinishThreads = 1024;
+// A block takes kFinishThreads >> split_log columns of a job, whose partial rows it shares out over 1 << split_log groups
+// of threads: 32 for the plain sums, fewer for gate rows of few partial rows.
 template <typename T>
 __global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const Finish f) {
-    constexpr uint32_t warps = kFinishThreads / 32;
-    __shared__ float sums[warps][32];
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const uint32_t c = blockIdx.x * 32 + lane;
-    uint32_t job = blockIdx.y;  // 0: next, 1: post, 2 + g: gate row g
-    if (!f.part_next) ++job;
-    if (!f.d_post && job >= 1) ++job;
+    __shared__ float sums[kFinishThreads];
+    const uint32_t plain = (f.part_next ? 1 : 0) + (f.d_post ? 1 : 0), plain_blocks = (f.width + 31) / 32;
+    uint32_t job, block = blockIdx.x, split_log = 5;  // job 0: next, 1: post, 2 + g: gate row g
+    if (block < plain * plain_blocks) {
+        job = block / plain_blocks + (f.part_next ? 0 : 1);
+        block %= plain_blocks;
+    } else {
+        block -= plain * plain_blocks;
+        split_log = f.split_log;
+        const uint32_t blocks = (uint32_t)((((uint64_t)f.width << split_log) + kFinishThreads - 1) / kFinishThreads);
+        job = 2 + block / blocks;
+        block %= blocks;
+    }
+    const uint32_t cols = kFinishThreads >> split_log, part_of = threadIdx.x >> (10 - split_log);
+    const uint32_t c = block * cols + (threadIdx.x & (cols - 1));
     const bool weighted = job == 1 && !f.part_post;
     const uint32_t n = job < 2 ? f.runs : f.parts;
     const float* part = job == 0 ? f.part_next : job == 1 && !weighted ? f.part_post : f.part_gate;
     if (job >= 2) part += (uint64_t)(job - 2) * f.parts * f.width;
     float v = 0.0f;
     if (c < f.width) {
-        const uint32_t begin = (uint32_t)((uint64_t)n * warp / warps), end = (uint32_t)((uint64_t)n * (warp + 1) / warps);
+        const uint32_t begin = n * part_of >> split_log, end = n * (part_of + 1) >> split_log;
         if (weighted) {
             for (uint32_t i = begin; i < end; ++i)
                 v += param<T>(f.gate, i / f.parts * f.gs + c, f.g_float) * part[(uint64_t)i * f.width + c];
@@ -931,12 +953,15 @@ __global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const
             for (uint32_t i = begin; i < end; ++i) v += part[(uint64_t)i * f.width + c];
         }
     }
-    sums[warp][lane] = v;
+    sums[threadIdx.x] = v;
     __syncthreads();
-    if (warp || c >= f.width) return;
-    v = sums[0][lane];
+    if (part_of || c >= f.width) return;
+    if (split_log == 5) {
 #pragma unroll
-    for (uint32_t i = 1; i < warps; ++i) v += sums[i][lane];
+        for (uint32_t i = 1; i < 32; ++i) v += sums[i * 32 + threadIdx.x];
+    } else {
+        for (uint32_t i = 1; i < 1u << split_log; ++i) v += sums[i * cols + threadIdx.x];
+    }
     if (job == 0) f.d_next[c] = v;
     else if (job == 1) f.d_post[c] = v;
     else {
@@ -1226,12 +1251,14 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     e.w_float = f.w_float;
     e.g_float = f.g_float;
     e.w0 = f.w0;
-    const uint32_t jobs = !!e.part_next + !!e.d_post + (e.dgate ? f.groups : 0);
+    while (e.split_log < 5 && 4u << e.split_log < e.parts) ++e.split_log;
+    const uint64_t finish = (uint64_t)(!!e.part_next + !!e.d_post) * ((f.width + 31) / 32) +
+                            (e.dgate ? (uint64_t)f.groups * ((((uint64_t)f.width << e.split_log) + kFinishThreads - 1) / kFinishThreads) : 0);
     int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         rc = f.gate && f.parts == 1 ? launch_backward<T, true>(f, plan, vec, st) : launch_backward<T, false>(f, plan, vec, st);
-        if (rc == MTXC_OK && jobs) block_norm_finish_kernel<T><<<dim3((f.width + 31) / 32, jobs), kFinishThreads, 0, st>>>(e);
+        if (rc == MTXC_OK && finish) block_norm_finish_kernel<T><<<(unsigned)finish, kFinishThreads, 0, st>>>(e);
     });
     return rc == MTXC_OK ? check_launch("block_norm_finish_kernel") : rc;
 }

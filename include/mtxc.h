@@ -506,8 +506,8 @@ int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backward_args* arg
  *     (x, y) -> scale * (x cos t - y sin t, x sin t + y cos t)
  * and the rest of the head is copied.  inverse is the backward pass (the transpose of the rotation times
  * scale).  frequencies: rotary_dim / 2 doubles on the device, in radians per position; the angle is reduced to
- * one turn in 64 bits (in 32 it would be off by up to 0.03 radians at position 10^6).  positions: int32 or int64 (position_dtype) at
- * b * position_strides[0] + s * position_strides[1] (0: shared). */
+ * one turn in 64 bits (in 32 it would be off by up to 0.03 radians at position 10^6).  positions: int32 or
+ * int64 (position_dtype) at b * position_strides[0] + s * position_strides[1] (0: shared). */
 typedef struct mtxc_rotary_args {
     uint64_t batch, length;
     uint32_t head_dim, rotary_dim;

@@ -73,8 +73,8 @@ struct Chunk {
     // whether element j lies in the row (VEC: all eight do or none)
     __device__ __forceinline__ bool inside(int j, uint32_t width) const { return VEC ? c < width : c + 32 * j < width; }
 
-    // whether the warp's 256 columns all lie in the row: then scalar accesses need no comparisons, which were a third of
-    // the instructions of a row of half types
+    // whether the warp's 256 columns all lie in the row: then scalar accesses need no comparisons, which were a
+    // third of the instructions of a row of half types
     __device__ __forceinline__ bool whole(uint32_t width) const { return c - threadIdx.x % 32 + 256 <= width; }
 
     __device__ __forceinline__ Eight<T> load(const T* row, uint32_t width) const {
@@ -255,8 +255,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* part, uint32_t thr
     }
 }
 
-// Rows held in registers, E elements per thread: read once, written once.  WARP: a warp per row, eight rows
-// per block; else a block per row.
+// Rows held in registers, E elements per thread: read once, written once.  WARP: a warp per row, eight rows per
+// block; else a block per row.  Bound by HBM ([8192, 4096] bf16 46 us, 5.8 TB/s), with dropout by the generator's
+// integer work ([8192, 8192] bf16 with a gate per channel 109 us, 4.9 TB/s).  A grid of resident blocks that
+// copies the next row ahead was slower (47 -> 51 us, 109 -> 122): more blocks hide a row's two reductions better.
 template <typename T, int E, bool VEC, bool WARP, int BLOCK, int MIN>
 __global__ void __launch_bounds__(BLOCK, MIN) block_norm_kernel(const Forward f) {
     constexpr int K = E / 8;
@@ -650,12 +652,13 @@ __device__ __forceinline__ void store_sums(const Chunk<T, VEC>& ch, float* row, 
 }
 
 // Rows read once: E elements per thread, the sums over rows in registers.  A run of rows for each team: a warp
-// (WARP), or `threads` threads; a block's teams add their sums in shared memory, so that there is one row of partial
-// sums for each block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of) one gate row.  CLUSTER: a
-// row's columns are shared by the blocks of a cluster (one team each), f.cols to a block, which exchange their sums
-// through distributed shared memory: one cluster barrier per row.  A thread keeps its columns' w_next' and
-// gate * w_post' in shared memory, as floats ready for use, for the run (or the gate row).  Inputs that the call does
-// not have read as zeros, weights as ones: fewer branches.
+// (WARP), or `threads` threads; a block's teams add their sums in shared memory, so that there is one row of
+// partial sums for each block.  MULTI: a run has whole gate rows and writes their gradients; else it has (part of)
+// one gate row.  CLUSTER: a row's columns are shared by the blocks of a cluster (one team each), f.cols to a
+// block, which exchange their sums through distributed shared memory: one cluster barrier per row.  A thread keeps
+// its columns' w_next' and gate * w_post' in shared memory, as floats ready for use, for the run (or the gate
+// row).  Inputs that the call does not have read as zeros, weights as ones: fewer branches.  Bound by latency at
+// 16 warps per SM: [8192, 4096] bf16 with gate and dropout 88 us with the finish, 4.6 TB/s.
 template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool CLUSTER, int BLOCK, int MIN>
 __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t team_threads, uint32_t stages) {
     constexpr int K = E / 8;
@@ -782,7 +785,8 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
         float sum[3] = {c1.x + c1.y, su.x + su.y, sv.x + sv.y};
         row_sum<3, WARP>(sum, part[(row - first) % 2], threads, team);
         if constexpr (CLUSTER) {
-            // double buffered like part: a block that writes a row's slots again has passed the barrier of the row between
+            // double buffered like part: a block that writes a row's slots again has passed the barrier of the row
+            // between
             cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
             float(&slots)[kMaxCluster][3] = from_rank[(row - first) % 2];
             if (threadIdx.x < f.cluster) {
@@ -919,8 +923,8 @@ struct Finish {
 };
 
 constexpr uint32_t kFinishThreads = 1024;
-// A block takes kFinishThreads >> split_log columns of a job, whose partial rows it shares out over 1 << split_log groups
-// of threads: 32 for the plain sums, fewer for gate rows of few partial rows.
+// A block takes kFinishThreads >> split_log columns of a job, whose partial rows it shares out over 1 << split_log
+// groups of threads: 32 for the plain sums, fewer for gate rows of few partial rows.
 template <typename T>
 __global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const Finish f) {
     __shared__ float sums[kFinishThreads];
@@ -972,8 +976,13 @@ __global__ void __launch_bounds__(kFinishThreads) block_norm_finish_kernel(const
     }
 }
 
-// Which backward kernel serves a width, and with what blocks.  Rows of more than 8192 elements go to clusters of 2 to 8
-// blocks, of more than 65,536 to block_norm_backward_any_kernel.
+// Which backward kernel serves a width, and with what blocks.  Rows of more than 8192 elements go to clusters of 2
+// to 8 blocks, each with 4,352 to 8,192 columns (kinds 2 and 4: the cluster kernels have their elements per
+// thread), of more than 65,536 to block_norm_backward_any_kernel.  Larger clusters than a width needs measured
+// slower ([2048, 8192] bf16 48 us with one block, 59 with two, 86 with four).  Vectors take 16 elements a thread
+// at 128 registers ([8192, 4096] bf16 with gate and dropout 98 us when 8 at 64 registers took 115, 16 at 80
+// registers 124), scalar accesses 8 at 64 ([8192, 1001] bf16 45 us, with the next row ahead in registers and half
+// the blocks 57).
 struct Plan {
     int kind = -1;  // -1: block_norm_backward_any_kernel
     uint32_t team = kThreads, teams = 1, blocks_per_sm = 2, stages = 1, cluster = 1, cols = 0;

@@ -9,6 +9,9 @@
 // a biased token, is read again, ruled and written over; that also holds where dst is src, since an allowed token's
 // first write leaves its value.  The counts are integer atomics, and the list's order changes nothing: equal calls
 // give equal bits.
+//
+// [256, 131072] bf16 with a mask takes 18 us without lists (7.6 TB/s, partly from L2), 25 with 16 biases and 41
+// with a history of 2,048 tokens a row too: the scans are what is left, and they are bound by issue.
 #include <algorithm>
 
 #include "rows.cuh"
@@ -250,9 +253,9 @@ int launch(Logits l, uint64_t rows, cudaStream_t st) {
 }
 
 // Threads of a block, and with them its slice: larger slices scan the lists less often, smaller ones hide the scan
-// behind more blocks.  On a B200: [256, 131072] bf16 with a history of 2,048 takes 47 us with 256 threads, 42 with 512, 44
-// with 1024; [100, 131072] float with 1,000 26, 29 and 32; [256, 50257] bf16 (scalar accesses) 29, 35 and 41;
-// [64, 131072] bf16 with 40,000 85, 58 and 45.
+// behind more blocks.  On a B200: [256, 131072] bf16 with a history of 2,048 takes 47 us with 256 threads, 42 with
+// 512, 44 with 1024; [100, 131072] float with 1,000 26, 29 and 32; [256, 50257] bf16 (scalar accesses) 29, 35 and
+// 41; [64, 131072] bf16 with 40,000 85, 58 and 45.
 template <typename T, bool VEC>
 int launch(const Logits& l, uint64_t rows, cudaStream_t st) {
     if (l.history >= 32768) return launch<T, VEC, 1024, uint32_t>(l, rows, st);

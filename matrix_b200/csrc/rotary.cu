@@ -56,11 +56,13 @@ __device__ __forceinline__ void read_table(const float* p, float (&v)[M]) {
     } else v[0] = p[0];
 }
 
-// A block takes `tile` tokens of a sequence.  It makes their cosines and sines once, in shared memory, for all heads
-// -- with its first loads already in flight -- and then turns units: N pairs (two accesses of N = 8 or 4 elements, half
-// a head apart) or, PAIRS (interleaved), N elements of N / 2 pairs; N = 0: one pair.  What is not turned is copied in units of
-// N elements, without PAIRS two such r.far apart where they divide so, or one element.  A thread stays with one unit of one head for all its tokens, kUnroll at
-// a time, so that a unit's place is worked out once (worked out for each, it was two thirds of the instructions).
+// A block takes `tile` tokens of a sequence.  It makes their cosines and sines once, in shared memory, for all
+// heads -- with its first loads already in flight -- and then turns units: N pairs (two accesses of N = 8 or 4
+// elements, half a head apart) or, PAIRS (interleaved), N elements of N / 2 pairs; N = 0: one pair.  What is not
+// turned is copied in units of N elements, without PAIRS two such r.far apart where they divide so, or one
+// element.  A thread stays with one unit of one head for all its tokens, kUnroll at a time, so that a unit's place
+// is worked out once (worked out for each, it was two thirds of the instructions).  Bound by HBM: 16,384 tokens x
+// 40 heads of 128 bf16 56 us, 6.0 TB/s.
 template <typename T, int N, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r) {
     constexpr int kUnroll = N && !PAIRS ? 2 : 4;
@@ -254,13 +256,15 @@ extern "C" int mtxc_rotary(int dtype, const mtxc_rotary_args* a) {
         r.half_div = FastDiv(std::max(1u, r.half));
         r.items = units * (uint32_t)heads;
         r.length = (uint32_t)a->length;
-        // threads side by side: a token's units evenly in as few rounds as 256 threads allow, and as many tokens as fit
+        // threads side by side: a token's units evenly in as few rounds as 256 threads allow, and as many tokens
+        // as fit
         const uint32_t rounds = std::min<uint32_t>((r.items + kThreads - 1) / kThreads, 65535);
         r.lanes = std::min<uint32_t>((r.items + rounds - 1) / rounds, kThreads);
         r.lanes_div = FastDiv(r.lanes);
-        // tokens of a block: what gives a thread 6 units of two accesses or 10 of one, in whole rounds of the unrolled loads,
-        // while every SM still has kBlocksPerSm blocks and the table fits (16,384 tokens x 40 heads of 128 bf16: 57 us with 6,
-        // 63 with 8, 66 with 12; interleaved 56 us with 10, 60 with 16, 98 with 4)
+        // tokens of a block: what gives a thread 6 units of two accesses or 10 of one, in whole rounds of the
+        // unrolled loads, while every SM still has kBlocksPerSm blocks and the table fits (16,384 tokens x 40
+        // heads of 128 bf16: 57 us with 6, 63 with 8, 66 with 12; interleaved 56 us with 10, 60 with 16, 98 with
+        // 4)
         const uint64_t tokens = a->batch * a->length;
         const uint32_t round = std::max(1u, kThreads / r.lanes) * (step > 1 && !pairs ? 2 : 4);
         uint64_t tile = std::max<uint64_t>(1, (step > 1 && !pairs ? 6 : 10) * kThreads / r.items);

@@ -479,8 +479,8 @@ __device__ __forceinline__ void for_each_segment(const Backward& f, uint32_t run
     }
 }
 
-// Any width (in use: above 65,536), stride and alignment: the rows are read twice and the sums over rows live in the
-// workspace.
+// Any width (in use: above 65,536, and where a gradient is written over a gate per token, which is here read before the
+// row's stores), stride and alignment: the rows are read twice and the sums over rows live in the workspace.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const Backward f) {
     __shared__ float part[3 * 32];
@@ -524,34 +524,28 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
             block_sum(sum, part);
             const float kappa = s * s * s * (sum[0] / f.width);
             const float c2 = (sum[1] - kappa * sum[2]) / f.width;
+            const bool ends = f.part_gate && row + 1 == last;
             for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
-                const float hv = stream(c);
+                const float hv = stream(c), g = gate(c);
                 const float g_next = f.w_next ? to_float(da[c]) * hv * s : 0.0f;
                 const float H = upper(c) + s * p_of(c) - hv * kappa;
                 if (f.b) {
-                    const float bv = to_float(b[c]), t = mask(c) * H, u = t * gate(c) * post(c);
+                    const float bv = to_float(b[c]), t = mask(c) * H, w = post(c), u = t * g * w;
                     if (f.db)
                         static_cast<T*>(f.db)[row * f.dbs + c] = from_float<T>(f.w_post ? r * u - bv * (r * r * r * c2) : u);
                     if (want_s) {
                         // one row's S at a time is enough where the run's S is not kept
-                        const float S = t * (bv * r);
-                        if (f.part_gate) f.part_gate[own + c] += S;
-                        else if (f.part_post) f.part_post[own + c] += gate(c) * S;
+                        float S = t * (bv * r);
+                        if (f.part_gate) S = f.part_gate[own + c] += S;
+                        if (f.part_post && (ends || !f.part_gate)) f.part_post[own + c] += g * S;
+                        if (ends && f.parts == 1) {
+                            if (f.g_float) static_cast<float*>(f.dgate)[group * f.dgs + c] = w * S;
+                            else static_cast<T*>(f.dgate)[group * f.dgs + c] = from_float<T>(w * S);
+                        }
                     }
                 }
                 if (f.dx) static_cast<T*>(f.dx)[row * f.dxs + c] = from_float<T>(f.alpha * H);
                 if (f.part_next) f.part_next[own + c] += g_next;
-            }
-        }
-        if (f.part_gate) {
-            for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
-                const float S = f.part_gate[own + c];
-                if (f.part_post) f.part_post[own + c] += gate(c) * S;
-                if (f.parts == 1) {
-                    const float d = post(c) * S;
-                    if (f.g_float) static_cast<float*>(f.dgate)[group * f.dgs + c] = d;
-                    else static_cast<T*>(f.dgate)[group * f.dgs + c] = from_float<T>(d);
-                }
             }
         }
     });
@@ -1213,6 +1207,9 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
               param_aligned(f.gate, f.gs) && eight_aligned<T>(f.dgate, f.dgs);
         plan = plan_backward<T>(f.width, vec);
     });
+    // The other kernels read a gate row once more after its rows' stores: read before them it is held across the
+    // row's work, which cost the kernels of scalar accesses 10 to 22 % in spills ([8192, 1001] f16 77 -> 93 us).
+    if (f.gate && (f.dx == f.gate || f.db == f.gate)) plan = Plan();
     const int sums = !!a->d_next_weight + !!a->d_post_weight + !!a->d_gate;
     const uint64_t row_bytes = (uint64_t)f.width * sizeof(float) * sums;
     // teams that the GPU holds; a block's teams share a gate row, or each has whole ones; few rows: fewer teams in a

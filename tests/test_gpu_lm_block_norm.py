@@ -439,3 +439,29 @@ def test_workspace_refusal(lm, gpu):
         torch.cuda.synchronize()
         _abi.check(lib.mtxc_shutdown())
         gpu.init(0)
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 10)])
+@pytest.mark.parametrize("rows,width", [(1, 4096), (300, 64), (7, 1000), (300, 4096), (300, 4097), (40, 8200), (40, 12001), (100, 70000)])
+@pytest.mark.parametrize("over", ["branch", "residual"])
+def test_gradients_written_over_a_gate_per_token(lm, gpu, dtype, code, rows, width, over):
+    """Through the C ABI: a gate per token has the rows' shape, so that a gradient may be written over it.  The sums
+    over rows take the gate as it was."""
+    from matrix_b200 import _abi
+
+    c = Case((rows, width), dtype, gate="token", drop=0.1)
+    h, r, s = c.stored()
+    dh, da, hd, b, gate = (t.cuda() for t in (c.dh, c.da, h, c.b, c.gate))
+    kept = [t.cuda() for t in (r, s, c.post, c.next)]
+    got = {"residual": torch.empty_like(hd), "branch": torch.empty_like(hd), over: gate, "gate": torch.empty_like(hd),
+           "post_weight": torch.empty(width, device="cuda"), "next_weight": torch.empty(width, device="cuda")}
+    at = lambda t: (t.data_ptr(), width)  # noqa: E731
+    _abi.check(_abi.lib().mtxc_block_norm_backward(code, _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
+        rows, width, *at(dh), *at(da), *at(hd), *at(b), *(t.data_ptr() for t in kept), *at(gate), 1, *at(got["residual"]),
+        *at(got["branch"]), got["post_weight"].data_ptr(), got["next_weight"].data_ptr(), *at(got["gate"]), code, code,
+        1.0, 1.0, 0.0, 0.1, SEED, OFFSET, 0)))
+    gpu.sync()
+    want = ref.block_norm_backward(c.flat(c.dh), c.flat(c.da), c.flat(h), c.flat(c.b), r.double(), s.double(), c.post.double(),
+                                   c.flat(c.gate), 1, c.next.double(), 1.0, 1.0, 0.0, c.mask)
+    for name, (exact, magnitude) in want.items():
+        ref.assert_within(got[name], exact, magnitude, f"{(rows, width)} {dtype} d_{name}")

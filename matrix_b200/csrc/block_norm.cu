@@ -9,6 +9,8 @@
 // mean(u b) needs H, which needs mean(p h): with e = beta mask g w_post b it is
 // mean(e (dh + s p)) - kappa mean(e h), so one reduction of three sums serves both.  (kappa h is the
 // projection of s p on h, never longer than s p: the difference loses no more than H itself does.)
+// A deviation's cube passes the range of 32 bits where a row's root mean square passes 1e12 either way, and the
+// gradients do not: kappa is made one factor at a time, and b r^3 mean(u b) as (b r) (r (r mean(u b))).
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -522,8 +524,8 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
                 }
             }
             block_sum(sum, part);
-            const float kappa = s * s * s * (sum[0] / f.width);
-            const float c2 = (sum[1] - kappa * sum[2]) / f.width;
+            const float kappa = s * (s * (s * (sum[0] / f.width)));
+            const float c2 = r * (r * ((sum[1] - kappa * sum[2]) / f.width));
             const bool ends = f.part_gate && row + 1 == last;
             for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
                 const float hv = stream(c), g = gate(c);
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
                 if (f.b) {
                     const float bv = to_float(b[c]), t = mask(c) * H, w = post(c), u = t * g * w;
                     if (f.db)
-                        static_cast<T*>(f.db)[row * f.dbs + c] = from_float<T>(f.w_post ? r * u - bv * (r * r * r * c2) : u);
+                        static_cast<T*>(f.db)[row * f.dbs + c] = from_float<T>(f.w_post ? r * u - (bv * r) * c2 : u);
                     if (want_s) {
                         // one row's S at a time is enough where the run's S is not kept
                         float S = t * (bv * r);
@@ -791,8 +793,8 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             sum[0] = sum[1] = sum[2] = 0.0f;
             for (uint32_t i = 0; i < f.cluster; ++i) sum[0] += slots[i][0], sum[1] += slots[i][1], sum[2] += slots[i][2];
         }
-        const float kappa = s * s * s * (sum[0] / f.width);
-        const float c2 = r * r * r * (cf * (sum[1] - kappa * sum[2]) / f.width);
+        const float kappa = s * (s * (s * (sum[0] / f.width)));
+        const float c2 = r * (r * (cf * (sum[1] - kappa * sum[2]) / f.width));
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const Chunk<T, VEC> ch(k, threads, tid, from);
@@ -819,7 +821,7 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             }
             if (has_post) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) H[j] = __ffma2_rn(both(-c2), b.get2(j), H[j]);
+                for (int j = 0; j < 4; ++j) H[j] = __ffma2_rn(both(-c2), __fmul2_rn(both(r), b.get2(j)), H[j]);
             }
             if (f.db) ch.store(static_cast<T*>(f.db) + row * f.dbs, limit, H);
         }

@@ -465,3 +465,28 @@ def test_gradients_written_over_a_gate_per_token(lm, gpu, dtype, code, rows, wid
                                    c.flat(c.gate), 1, c.next.double(), 1.0, 1.0, 0.0, c.mask)
     for name, (exact, magnitude) in want.items():
         ref.assert_within(got[name], exact, magnitude, f"{(rows, width)} {dtype} d_{name}")
+
+
+class Scaled(Case):
+    """Rows of any magnitude, the first of them zero; eps is a hundredth of their mean square."""
+
+    def __init__(self, shape, dtype, scale, **more):
+        super().__init__(shape, dtype, **more)
+        self.x, self.b = (self.x.double() * scale).to(dtype), (self.b.double() * scale).to(dtype)
+        self.x[0], self.b[0] = 0, 0
+        self.eps = (0.1 * scale) ** 2
+
+    def stored(self):
+        r, s = ((self.flat(t).square().mean(1) + self.eps).rsqrt().float() for t in (self.b, self.x))
+        return self.x, r, s
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale,widths", [(1e14, (64, 1000, 4096, 8200, 12001, 70000)), (1e-14, (64, 1000, 4096, 8200, 12001, 70000)),
+                                          (1e16, (64, 1000, 4096)), (1e-17, (64, 1000, 4096))])
+@pytest.mark.parametrize("gate", ["channel", "token"])
+def test_gradients_of_very_large_and_very_small_rows(lm, dtype, scale, widths, gate):
+    """Where the cube of a deviation passes the range of 32 bits, and the gradients do not."""
+    for width in widths:
+        Scaled((5, width), dtype, scale, gate=gate, drop=0.2).check_backward(lm)
+        Scaled((5, width), dtype, scale, gate=gate).check_backward(lm, dh=False)

@@ -228,6 +228,13 @@ struct Kept {
         if constexpr (VEC) return lanes[k].keeps(d, j);
         else return bits >> (8 * k + j) & 1u;
     }
+    __device__ __forceinline__ void zero_others(const DropArgs& d, int k, Eight<T>& v) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (sizeof(T) == 4) v.w[j] = at(d, k, j) ? v.w[j] : 0;
+            else v.w[j / 2] &= at(d, k, j) ? 0xFFFFFFFFu : j % 2 ? 0xFFFFu : 0xFFFF0000u;
+        }
+    }
     __device__ __forceinline__ void zero_others(const DropArgs& d, int k, float2 (&v)[4]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -493,6 +500,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
         if (f.part_post) f.part_post[own + c] = 0.0f;
     }
     const bool want_s = f.part_post || f.part_gate;
+    const float cf = f.drop.on ? f.beta * f.drop.scale : f.beta;
     for_each_segment(f, blockIdx.x, [&](uint32_t group, uint32_t first, uint32_t last) {
         auto gate = [&](uint32_t c) { return f.gate ? param<T>(f.gate, group * f.gs + c, f.g_float) : 1.0f; };
         auto post = [&](uint32_t c) { return f.w_post ? f.w0 + param<T>(f.w_post, c, f.w_float) : 1.0f; };
@@ -509,16 +517,13 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
             auto p_of = [&](uint32_t c) {
                 return f.w_next ? to_float(da[c]) * (f.w0 + param<T>(f.w_next, c, f.w_float)) : 0.0f;
             };
-            auto mask = [&](uint32_t c) {
-                if (!f.drop.on) return f.beta;
-                return rng(c / 8, row).at(c % 8) < f.drop.kept ? f.beta * f.drop.scale : 0.0f;
-            };
+            auto keeps = [&](uint32_t c) { return !f.drop.on || rng(c / 8, row).at(c % 8) < f.drop.kept; };
             float sum[3] = {0.0f, 0.0f, 0.0f};
             for (uint32_t c = threadIdx.x; c < f.width; c += kThreads) {
                 const float p = p_of(c), hv = stream(c);
                 sum[0] += p * hv;
                 if (f.w_post) {
-                    const float e = mask(c) * gate(c) * post(c) * to_float(b[c]);
+                    const float e = keeps(c) ? cf * gate(c) * post(c) * to_float(b[c]) : 0.0f;
                     sum[1] += e * (upper(c) + s * p);
                     sum[2] += e * hv;
                 }
@@ -532,12 +537,14 @@ __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const
                 const float g_next = f.w_next ? to_float(da[c]) * hv * s : 0.0f;
                 const float H = upper(c) + s * p_of(c) - hv * kappa;
                 if (f.b) {
-                    const float bv = to_float(b[c]), t = mask(c) * H, w = post(c), u = t * g * w;
+                    // what is dropped may be infinite or NaN: a zero all the same
+                    const bool kept = keeps(c);
+                    const float bv = to_float(b[c]), t = kept ? cf * H : 0.0f, w = post(c), u = t * g * w;
                     if (f.db)
                         static_cast<T*>(f.db)[row * f.dbs + c] = from_float<T>(f.w_post ? r * u - (bv * r) * c2 : u);
                     if (want_s) {
                         // one row's S at a time is enough where the run's S is not kept
-                        float S = t * (bv * r);
+                        float S = kept ? t * (bv * r) : 0.0f;
                         if (f.part_gate) S = f.part_gate[own + c] += S;
                         if (f.part_post && (ends || !f.part_gate)) f.part_post[own + c] += g * S;
                         if (ends && f.parts == 1) {
@@ -629,6 +636,14 @@ struct Inputs {
             }
             return e;
         } else return regs[i][k];
+    }
+    __device__ __forceinline__ void put(int i, int k, uint32_t stage, const Eight<T>& e) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int v = 0; v < kPieces; ++v)
+                ring[(((stage * 4 + i) * K + k) * kPieces + v) * stride] =
+                    make_uint4(e.w[4 * v], e.w[4 * v + 1], e.w[4 * v + 2], e.w[4 * v + 3]);
+        } else regs[i][k] = e;
     }
 };
 
@@ -756,7 +771,19 @@ __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const B
             }
         }
         Kept<T, K, VEC> kept;
-        if (drops) kept.make(f.drop, row, threads, tid, from);
+        if (drops) {
+            kept.make(f.drop, row, threads, tid, from);
+            // What is dropped may be infinite or NaN: a zero to the gate's sums below all the same.  (With a post norm such
+            // an element has spoilt its whole row's deviation already.)
+            if (want_s && !has_post) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    Eight<T> b = in.get(3, k, stage);
+                    kept.zero_others(f.drop, k, b);
+                    in.put(3, k, stage, b);
+                }
+            }
+        }
         float2 c1 = both(0.0f), su = both(0.0f), sv = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {

@@ -490,3 +490,25 @@ def test_gradients_of_very_large_and_very_small_rows(lm, dtype, scale, widths, g
     for width in widths:
         Scaled((5, width), dtype, scale, gate=gate, drop=0.2).check_backward(lm)
         Scaled((5, width), dtype, scale, gate=gate).check_backward(lm, dh=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [64, 333, 1000, 4096, 8200, 12001, 70000])
+@pytest.mark.parametrize("gate", [None, "channel", "token"])
+def test_dropped_elements_hold_anything(lm, dtype, width, gate):
+    """Where an element is dropped the branch and the gradient above it may be infinite or NaN: what is dropped is a
+    zero in both directions.  (Without a norm of the branch, whose mean square every element enters.)"""
+    c = Case((7, width), dtype, gate=gate, post=False, next=False, drop=0.5)
+    gone = (c.mask == 0).view(c.shape)
+    b, dh = c.b.clone(), c.dh.clone()
+    b[gone] = torch.tensor([float("inf"), float("nan"), float("-inf")], dtype=dtype).repeat(b.numel())[:int(gone.sum())]
+    want = lm.block_norm_backward(c.dh.cuda(), None, c.x.cuda(), c.b.cuda(), **c.params())
+    got = lm.block_norm_backward(c.dh.cuda(), None, c.x.cuda(), b.cuda(), **c.params())
+    assert torch.equal(got.branch, want.branch) and torch.equal(got.residual, want.residual)
+    assert gate is None or torch.equal(got.gate, want.gate)
+    dh[gone] = torch.tensor([float("nan"), float("inf")], dtype=dtype).repeat(b.numel())[:int(gone.sum())]
+    got = lm.block_norm_backward(dh.cuda(), None, c.x.cuda(), b.cuda(), **c.params())
+    assert torch.equal(got.branch, want.branch)
+    assert gate is None or torch.equal(got.gate, want.gate)
+    forward = [lm.block_norm(c.x.cuda(), t.cuda(), **c.params()).residual for t in (c.b, b)]
+    assert torch.equal(*forward)

@@ -404,10 +404,11 @@ int mtxc_softmax_lastdim(int dtype, void* dst, const void* src, uint64_t rows, u
  * SC 2011) with the 64-bit key `seed` and the counter words (column / 8, row, offset low, offset high); lanes
  * count from the low half of the first output word.  It is kept when the lane is below
  * rint((1 - p) * 65536) and then multiplied by 65536 / that number, so the mean is exact for the probability
- * that 16 bits can express; a dropped element counts as 0 in both directions, infinite or NaN as it may be.  Nothing is stored: a backward pass with the same seed and offset makes the same
- * mask, whatever the dtype, the strides and the launch.  A step uses another offset (or seed) for each call;
- * device_offset, if not NULL, is a device pointer to one more offset that is added to `offset` (modulo 2^64)
- * when the kernel runs, so that a recorded graph can advance it. */
+ * that 16 bits can express; a dropped element counts as 0 in both directions, infinite or NaN as it may be.
+ * Nothing is stored: a backward pass with the same seed and offset makes the same mask, whatever the dtype, the
+ * strides and the launch.  A step uses another offset (or seed) for each call; device_offset, if not NULL, is a
+ * device pointer to one more offset that is added to `offset` (modulo 2^64) when the kernel runs, so that a
+ * recorded graph can advance it. */
 typedef struct mtxc_dropout_state {
     double p; /* 0 <= p <= 1; 0: nothing is dropped, 1: everything */
     uint64_t seed;

@@ -1043,8 +1043,10 @@ int launch_backward_kernel(const Backward& f, const Plan& p, cudaStream_t st) {
     auto kernel = block_norm_backward_kernel<T, E, VEC, WARP, MULTI, CLUSTER, BLOCK, MIN>;
     const size_t smem = p.team_smem * p.teams;
     cudaError_t err = cudaSuccess;
-    if (smem > 46 * 1024)  // the kernel has static shared memory too
-        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // The limit belongs to the kernel, not to the call, and several threads may call: always the same one, which never
+    // undoes another's.  (46 KB: the kernel has static shared memory too.)
+    if (smem > 46 * 1024)
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(block_norm_backward_kernel)");
     if constexpr (CLUSTER) {
         cudaLaunchAttribute attr{};

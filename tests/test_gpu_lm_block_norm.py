@@ -512,3 +512,50 @@ def test_dropped_elements_hold_anything(lm, dtype, width, gate):
     assert gate is None or torch.equal(got.gate, want.gate)
     forward = [lm.block_norm(c.x.cuda(), t.cuda(), **c.params()).residual for t in (c.b, b)]
     assert torch.equal(*forward)
+
+
+def test_calls_from_two_threads(lm, gpu):
+    """Two threads with streams and workspaces of their own call one kernel with blocks of different shared memory:
+    every call is accepted and every result is that of one thread by itself."""
+    import threading
+
+    from matrix_b200 import _abi
+
+    lib, at = _abi.lib(), lambda t: (t.data_ptr(), 4096)  # noqa: E731
+    jobs = []
+    for rows in (100, 900):  # one team in a block, two
+        c = Case((rows, 4096), torch.bfloat16)
+        h, r, s = c.stored()
+        t = [v.cuda() for v in (c.dh, c.da, h, c.b, r, s, c.post, c.next)]
+        want = lm.block_norm_backward(*t[:4], post_rstd=t[4], next_rstd=t[5], post_weight=t[6], next_weight=t[7])
+        got = [torch.empty_like(v) for v in (want.residual, want.branch, want.post_weight, want.next_weight)]
+        args = _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
+            rows, 4096, *at(t[0]), *at(t[1]), *at(t[2]), *at(t[3]), *(v.data_ptr() for v in t[4:]), 0, 0, 0, *at(got[0]),
+            *at(got[1]), got[2].data_ptr(), got[3].data_ptr(), 0, 0, 10, 10, 1.0, 1.0, 0.0, 0.0, 0, 0, 0)
+        jobs.append((args, got, want, t))
+    torch.cuda.synchronize()
+    failed, start = [], threading.Barrier(2)
+
+    def work(args):
+        try:
+            _abi.check(lib.mtxc_init(0))
+            start.wait(60)
+            for i in range(4000):
+                _abi.check(lib.mtxc_block_norm_backward(10, args))
+                if i % 200 == 199:
+                    _abi.check(lib.mtxc_sync())
+        except Exception as e:
+            failed.append(str(e))
+        finally:
+            lib.mtxc_sync()
+            lib.mtxc_shutdown()
+
+    threads = [threading.Thread(target=work, args=(job[0],)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for _, got, want, _ in jobs:
+        for g, w in zip(got, (want.residual, want.branch, want.post_weight, want.next_weight)):
+            assert torch.equal(g, w)

@@ -410,8 +410,11 @@ PyObject* rotary(PyObject* const* a) {
         const Tensor* given = maybe(a[7 + i], names[i]);
         if (!x) continue;
         if (x->size(-1) > 1 && x->stride(-1) != 1) throw invalid(quoted(names[i], "the last axis needs unit stride"));
-        if (!given) out[i] = x->is_contiguous() ? memory.like(*x) : at::empty_like(*x);
-        else {
+        if (!given) {
+            // heads stored as x stores them; x's axes may overlap, and then their order does not say which is the innermost
+            out[i] = x->is_contiguous() ? memory.like(*x) : at::empty_like(*x);
+            if (x->size(-1) > 1 && out[i].stride(-1) != 1) out[i] = memory.like(*x);
+        } else {
             if (given->sizes() != x->sizes() || given->scalar_type() != x->scalar_type() || !given->is_cuda() ||
                 given->get_device() != dev || (x->size(-1) > 1 && given->stride(-1) != 1))
                 throw invalid(quoted(names[i], "expected an output of its shape, dtype and device, with unit stride in its last axis"));

@@ -216,3 +216,14 @@ def test_refusals(lm):
     with pytest.raises(MtxcError) as e:
         lm.rotary(q.int(), None, pos, freq)
     assert e.value.code == _abi.ERR_UNSUPPORTED_DTYPE
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_heads_that_overlap(lm, interleaved):
+    """Heads that are windows of one buffer, a stride of one element apart: the output is a tensor of its own."""
+    freq = lm.rotary_frequencies(8, device="cpu")[0]
+    base = normal(64).cuda()
+    for shape, strides in (((1, 5, 2, 8), (64, 1, 8, 1)), ((1, 3, 4, 8), (64, 0, 1, 1)), ((2, 3, 2, 8), (1, 16, 8, 1))):
+        x = torch.as_strided(base, shape, strides)
+        positions = torch.arange(shape[1], dtype=torch.int32).expand(shape[:2]).contiguous()
+        check(lm, x, x, positions, freq, f"strides {strides}", interleaved=interleaved)

@@ -18,6 +18,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <utility>
 
 #include "mtxc.h"
 
@@ -368,6 +369,22 @@ void put_strides(const Tensor& t, uint64_t (&to)[3]) {
     for (int64_t i = 0; i < 3; ++i) to[i] = i + lead >= 3 ? (uint64_t)t.stride(i + lead - 3) : 0;
 }
 
+// Refuses an output of heads with two elements at one address: from the innermost axis out, each stride has to pass
+// what lies inside it.  (The last axis has unit stride.)
+void no_overlap(const Tensor& t, const char* what) {
+    std::pair<int64_t, int64_t> axes[3];  // stride, size
+    int n = 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1) axes[n++] = {t.stride(i), t.size(i)};
+    if (t.numel() == 0) return;
+    std::sort(axes, axes + n);
+    int64_t span = t.size(-1);
+    for (int i = 0; i < n; ++i) {
+        if (axes[i].first < span) throw invalid(quoted(what, "its elements overlap"));
+        span += axes[i].first * (axes[i].second - 1);
+    }
+}
+
 PyObject* rotary(PyObject* const* a) {
     const Tensor& q = tensor(a[0], "q");
     const Tensor* k = maybe(a[1], "k");
@@ -418,6 +435,7 @@ PyObject* rotary(PyObject* const* a) {
             if (given->sizes() != x->sizes() || given->scalar_type() != x->scalar_type() || !given->is_cuda() ||
                 given->get_device() != dev || (x->size(-1) > 1 && given->stride(-1) != 1))
                 throw invalid(quoted(names[i], "expected an output of its shape, dtype and device, with unit stride in its last axis"));
+            no_overlap(*given, names[i]);
             out[i] = *given;
         }
         m.heads[i] = (uint32_t)x->size(-2);

@@ -227,3 +227,18 @@ def test_heads_that_overlap(lm, interleaved):
         x = torch.as_strided(base, shape, strides)
         positions = torch.arange(shape[1], dtype=torch.int32).expand(shape[:2]).contiguous()
         check(lm, x, x, positions, freq, f"strides {strides}", interleaved=interleaved)
+
+
+def test_outputs_that_overlap_are_refused(lm):
+    """Two elements of an output at one address."""
+    freq, pos = lm.rotary_frequencies(64)[0], torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 3, 4, 64, device="cuda")
+    base = torch.zeros(4096, device="cuda")
+    for strides in ((0, 256, 64, 1), (768, 0, 64, 1), (768, 256, 0, 1), (768, 256, 63, 1), (768, 255, 64, 1), (767, 256, 64, 1),
+                    (64, 384, 128, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            lm.rotary(q, None, pos, freq, out=(torch.as_strided(base, q.shape, strides), None))
+    for strides in ((768, 256, 64, 1), (1024, 256, 64, 1), (64, 128, 512, 1), (64, 512, 128, 1)):  # orders of the axes, and room between
+        out = torch.as_strided(torch.zeros(4096, device="cuda"), q.shape, strides)
+        assert lm.rotary(q + 1, None, pos, freq, out=(out, None))[0] is out
+        assert torch.equal(out, lm.rotary(q + 1, None, pos, freq)[0])

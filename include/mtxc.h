@@ -394,7 +394,8 @@ int mtxc_softmax_lastdim(int dtype, void* dst, const void* src, uint64_t rows, u
  * Arithmetic, sums and statistics are in 32 bits; a result is rounded once, when it is stored.  Strides are
  * in elements and 64-bit; the innermost axis has unit stride, except where a stride for it is given.
  * Addresses, sizes and strides need no alignment beyond the element's.  An output may be the very tensor
- * (pointer and strides) of an input of the same shape; outputs and inputs must not overlap otherwise.
+ * (pointer and strides) of an input of the same shape; outputs and inputs must not overlap otherwise (one pointer
+ * for two outputs: MTXC_ERR_INVALID_ARGUMENT).
  * Nothing is allocated; what the calls need of the thread's workspace is stated there.  Sums over rows run in a
  * fixed order: equal calls give equal bits.
  * ---------------------------------------------------------------------------------------- */

@@ -1133,6 +1133,7 @@ extern "C" int mtxc_block_norm(int dtype, const mtxc_block_norm_args* a) {
     if ((a->normed || a->next_rstd) && !a->next_weight)
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": normed and next_rstd need next_weight");
     if (a->post_rstd && !a->post_weight) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": post_rstd needs post_weight");
+    if (int rc = distinct(who, {a->residual_out, a->normed, a->post_rstd, a->next_rstd})) return rc;
     f.x = a->residual;
     f.xs = a->residual_stride;
     f.b = a->branch;
@@ -1198,6 +1199,7 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     if (!a->residual_out && (a->next_weight || a->branch)) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null residual_out");
     if ((a->next_weight && !a->next_rstd) || (a->post_weight && !a->post_rstd))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": a norm's rstd is missing");
+    if (int rc = distinct(who, {a->d_residual, a->d_branch, a->d_post_weight, a->d_next_weight, a->d_gate})) return rc;
     f.dh = a->d_residual_out;
     f.dhs = a->d_residual_out_stride;
     f.da = a->d_normed;

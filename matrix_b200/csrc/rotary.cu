@@ -225,6 +225,7 @@ extern "C" int mtxc_rotary(int dtype, const mtxc_rotary_args* a) {
             in_place = in_place && r.ss[k][i] == r.ds[k][i];
         }
     }
+    if (int rc = distinct(who, {r.dst[0], r.dst[1]})) return rc;
     if (r.half && (!a->positions || !a->frequencies))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null positions or frequencies");
     const uint32_t copied = in_place ? 0 : rest;

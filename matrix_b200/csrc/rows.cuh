@@ -3,6 +3,8 @@
 #pragma once
 
 #include <cmath>
+#include <initializer_list>
+#include <string>
 
 #include "mtxc_internal.cuh"
 
@@ -16,6 +18,14 @@ bool dispatch_float(int dtype, Fn&& fn) {
         case MTXC_BFLOAT16: fn((__nv_bfloat16*)nullptr); return true;
         default: return false;
     }
+}
+
+// Refuses one tensor for two outputs (NULL: not wanted); returns MTXC_OK or an error status.
+inline int distinct(const std::string& who, std::initializer_list<const void*> outputs) {
+    for (auto a = outputs.begin(); a != outputs.end(); ++a)
+        for (auto b = outputs.begin(); *a && b != a; ++b)
+            if (*a == *b) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": one tensor for two outputs");
+    return MTXC_OK;
 }
 
 inline bool is_float_like(int dtype) { return dtype == MTXC_FLOAT || dtype == MTXC_FLOAT16 || dtype == MTXC_BFLOAT16; }

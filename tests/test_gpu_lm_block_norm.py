@@ -559,3 +559,21 @@ def test_calls_from_two_threads(lm, gpu):
     for _, got, want, _ in jobs:
         for g, w in zip(got, (want.residual, want.branch, want.post_weight, want.next_weight)):
             assert torch.equal(g, w)
+
+
+def test_one_tensor_for_two_outputs_is_refused(lm):
+    from matrix_b200 import MtxcError, _abi
+
+    c = Case((4, 64), torch.float32)
+    x, b, out = c.x.cuda(), c.b.cuda(), torch.empty(4, 64, device="cuda")
+    with pytest.raises(MtxcError) as e:
+        lm.block_norm(x, b, **c.params(), out=out, normed_out=out)
+    assert e.value.code == _abi.ERR_INVALID_ARGUMENT
+    h, r, s = (t.cuda() for t in c.stored())
+    at = lambda t: (t.data_ptr(), 64)  # noqa: E731
+    dh, da, post, next = c.dh.cuda(), c.da.cuda(), c.post.cuda(), c.next.cuda()
+    sums = torch.empty(64, device="cuda")
+    for gradients in ((*at(out), *at(out), 0, 0), (0, 0, 0, 0, sums.data_ptr(), sums.data_ptr())):
+        assert _abi.lib().mtxc_block_norm_backward(0, _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
+            4, 64, *at(dh), *at(da), *at(h), *at(b), r.data_ptr(), s.data_ptr(), post.data_ptr(), next.data_ptr(), 0, 0, 0,
+            *gradients, 0, 0, 0, 0, 1.0, 1.0, 0.0, 0.0, 0, 0, 0)) == _abi.ERR_INVALID_ARGUMENT

@@ -242,3 +242,14 @@ def test_outputs_that_overlap_are_refused(lm):
         out = torch.as_strided(torch.zeros(4096, device="cuda"), q.shape, strides)
         assert lm.rotary(q + 1, None, pos, freq, out=(out, None))[0] is out
         assert torch.equal(out, lm.rotary(q + 1, None, pos, freq)[0])
+
+
+def test_one_tensor_for_queries_and_keys_is_refused(lm):
+    from matrix_b200 import MtxcError, _abi
+
+    freq, pos = lm.rotary_frequencies(64)[0], torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 3, 4, 64, device="cuda")
+    out = torch.empty_like(q)
+    with pytest.raises(MtxcError) as e:
+        lm.rotary(q, q, pos, freq, out=(out, out))
+    assert e.value.code == _abi.ERR_INVALID_ARGUMENT

@@ -97,6 +97,9 @@ int mtxc_abi_version(void);
  * GPUManager constructor (Mods/GPUManager.h:53-54) and its lazy init* calls. */
 int mtxc_init(int device);
 
+/* The device that the calling thread is bound to (MTXC_ERR_NOT_INITIALIZED: none). */
+int mtxc_get_device(int* device);
+
 /* Releases the calling thread's stream (if the runtime created it) and workspace (if the
  * runtime allocated it). */
 int mtxc_shutdown(void);
@@ -393,6 +396,7 @@ int mtxc_softmax_lastdim(int dtype, void* dst, const void* src, uint64_t rows, u
  * Common to all: dtype is MTXC_FLOAT, MTXC_FLOAT16 or MTXC_BFLOAT16 (others: MTXC_ERR_UNSUPPORTED_DTYPE).
  * Arithmetic, sums and statistics are in 32 bits; a result is rounded once, when it is stored.  Strides are
  * in elements and 64-bit; the innermost axis has unit stride, except where a stride for it is given.
+ * Tensors are in the memory of the thread's device, which is the caller's to see to (mtxc_get_device).
  * Addresses, sizes and strides need no alignment beyond the element's.  An output may be the very tensor
  * (pointer and strides) of an input of the same shape; outputs and inputs must not overlap otherwise (one pointer
  * for two outputs: MTXC_ERR_INVALID_ARGUMENT).

@@ -135,6 +135,7 @@ def lib() -> C.CDLL:
             "mtxc_comm_status": (i32, [C.POINTER(i32), C.POINTER(i32)]),
             "mtxc_reduce_sharded": (i32, [i32, i32, vp, vp, u32, u32, u32, U32P, U32P, U32P, C.POINTER(C.c_int64)]),
             "mtxc_allreduce": (i32, [i32, i32, vp, u64]),
+            "mtxc_get_device": (i32, [C.POINTER(i32)]),
             "mtxc_arange": (i32, [i32, vp, vp, vp, u64]),
             "mtxc_dropout": (i32, [i32, vp, vp, u64, u64, u64, u64, C.c_char_p]),
             "mtxc_block_norm": (i32, [i32, C.c_char_p]),

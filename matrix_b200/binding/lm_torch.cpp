@@ -31,6 +31,9 @@ using invalid = std::invalid_argument;  // ValueError in Python
 // Arguments
 // ------------------------------------------------------------------------------------------
 struct PythonError {};  // a Python exception is already set
+struct Refused {        // by the C ABI
+    int status;
+};
 
 const Tensor* maybe(PyObject* o, const char* what) {
     if (o == Py_None) return nullptr;
@@ -86,13 +89,18 @@ int code_of(const Tensor& t) {
     }
 }
 
-// The CUDA device that all the tensors (NULL: absent) are on.
+// The CUDA device that all the tensors (NULL: absent) are on: the one that the thread is bound to, whose stream the
+// kernels run on.
 c10::DeviceIndex device_of(const Tensor& x, std::initializer_list<const Tensor*> others) {
     if (!x.is_cuda()) throw invalid("expected tensors on a CUDA device");
     for (const Tensor* t : others)
         if (t && (!t->is_cuda() || t->get_device() != x.get_device()))
             throw invalid("expected all tensors on the same CUDA device");
-    return (c10::DeviceIndex)x.get_device();
+    int bound;
+    if (const int status = mtxc_get_device(&bound)) throw Refused{status};
+    if (x.get_device() != bound)
+        throw invalid("expected tensors on cuda:" + std::to_string(bound) + ", the device that the thread is bound to");
+    return (c10::DeviceIndex)bound;
 }
 
 // New tensors come from the memory of the stream that the kernels run on.
@@ -188,6 +196,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return F(args);
     } catch (const PythonError&) {
         return nullptr;
+    } catch (const Refused& e) {
+        return PyLong_FromLong(e.status);
     } catch (const std::invalid_argument& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const c10::OutOfMemoryError& e) {

@@ -103,6 +103,13 @@ int mtxc_init(int device) {
     return MTXC_OK;
 }
 
+int mtxc_get_device(int* device) {
+    if (!device) return fail(MTXC_ERR_INVALID_ARGUMENT, "mtxc_get_device: null pointer");
+    *device = ctx().device;
+    if (*device < 0) return fail(MTXC_ERR_NOT_INITIALIZED, "mtxc_init was not called on this thread");
+    return MTXC_OK;
+}
+
 int mtxc_shutdown(void) {
     ThreadCtx& c = ctx();
     if (c.device < 0) return MTXC_OK;

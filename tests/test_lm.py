@@ -3,6 +3,7 @@ of the argument structs, and the refusals that need no device."""
 import ctypes as C
 import math
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -106,4 +107,56 @@ def test_host_tensors_are_refused():
              lambda: lm.rotary(x[None], None, torch.zeros(1, dtype=torch.int32), f), lambda: lm.logits_rules(x)]
     for call in calls:
         with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+class Claimed(torch.Tensor):
+    """A tensor that claims a device and has no memory."""
+
+    @staticmethod
+    def __new__(cls, device, *shape, dtype=torch.float32):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device=device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} of a tensor without memory")
+
+
+def calls_on(device):
+    x, q = Claimed(device, 4, 8), Claimed(device, 4, 1, 8)
+    f, pos = Claimed(device, 4, dtype=torch.float64), Claimed(device, 4, dtype=torch.int32)
+    return [lambda: lm.dropout(x, 0.5, 0, 0), lambda: lm.block_norm(x, x), lambda: lm.block_norm_backward(x, None, x, x),
+            lambda: lm.rotary(q, None, pos, f), lambda: lm.logits_rules(x)]
+
+
+def test_a_thread_without_a_device_is_refused():
+    """Before anything is allocated or read: on a thread that is bound to no device."""
+    caught = []
+
+    def work():
+        device = C.c_int(7)
+        caught.append(_abi.lib().mtxc_get_device(C.byref(device)))
+        for call in calls_on("cuda:0"):
+            try:
+                caught.append(call())
+            except MtxcError as e:
+                caught.append(e.code)
+            except Exception as e:
+                caught.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert caught == [_abi.ERR_NOT_INITIALIZED] * 6
+
+
+@pytest.mark.gpu
+def test_tensors_of_another_device_are_refused(gpu):
+    """Tensors on cuda:1, from a thread bound to cuda:0: their pointers must not reach a kernel, and nothing is
+    allocated for them."""
+    device = C.c_int(7)
+    _abi.check(_abi.lib().mtxc_get_device(C.byref(device)))
+    assert device.value == 0
+    for call in calls_on("cuda:1"):
+        with pytest.raises(ValueError, match="cuda:0, the device that the thread is bound to"):
             call()

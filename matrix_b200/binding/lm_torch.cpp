@@ -135,12 +135,18 @@ uint64_t row_stride(const Tensor& t, const char* what, bool written = false) {
     return (uint64_t)stride;
 }
 
+// A tensor that a call writes in place: raises its version, by which autograd notices that a saved tensor has changed.
+const Tensor& written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return t;
+}
+
 Tensor output(const Memory& memory, const Tensor& x, const Tensor* out, const char* what) {
     if (!out) return memory.like(x);
     if (out->sizes() != x.sizes() || out->scalar_type() != x.scalar_type() || !out->is_cuda() ||
         out->get_device() != x.get_device())
         throw invalid(quoted(what, "expected a tensor of the input's shape, dtype and device"));
-    return *out;
+    return written(*out);
 }
 
 void same(const Tensor* t, const Tensor& x, const char* what) {
@@ -446,7 +452,7 @@ PyObject* rotary(PyObject* const* a) {
                 given->get_device() != dev || (x->size(-1) > 1 && given->stride(-1) != 1))
                 throw invalid(quoted(names[i], "expected an output of its shape, dtype and device, with unit stride in its last axis"));
             no_overlap(*given, names[i]);
-            out[i] = *given;
+            out[i] = written(*given);
         }
         m.heads[i] = (uint32_t)x->size(-2);
         m.src[i] = x->const_data_ptr();

@@ -5,10 +5,11 @@ These functions hand a call's tensors to the C ABI (include/mtxc.h, which states
 that matrix_b200/binding compiles against torch; PyTorch only provides device memory and streams, and there is no
 autograd: an operator's backward pass is a function of its own.  ``backend.init`` binds the thread first.  Kernels
 run on the thread's stream (``backend.set_stream``), and the outputs made here come from that stream's memory;
-where it is not torch's current stream, ordering the two is the caller's, as for any two streams.
+where it is not torch's current stream, ordering the two is the caller's, as for any two streams.  A tensor given as
+an output counts as changed in place.
 
-Inputs are float32, float16 or bfloat16 tensors on the thread's device whose last axis has unit stride; the other axes of a row
-operator's inputs have to fold into one axis of rows (a constant stride from row to row).
+Inputs are float32, float16 or bfloat16 tensors on the thread's device whose last axis has unit stride; the other axes
+of a row operator's inputs have to fold into one axis of rows (a constant stride from row to row).
 """
 from __future__ import annotations
 

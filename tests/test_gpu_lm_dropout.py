@@ -179,3 +179,26 @@ def test_refusals(lm):
     assert lib.mtxc_dropout(0, x.data_ptr(), None, 4, 8, 8, 8, state) == _abi.ERR_INVALID_ARGUMENT
     assert lib.mtxc_dropout(0, x.data_ptr(), x.data_ptr(), 4, 8, 8, 8, None) == _abi.ERR_INVALID_ARGUMENT
     assert lib.mtxc_dropout(0, x.data_ptr(), x.data_ptr(), 1 << 31, 8, 8, 8, state) == _abi.ERR_SHAPE
+
+
+def test_outputs_written_in_place_are_noticed(lm):
+    """autograd refuses to use a saved tensor that a call has written over since."""
+    x = torch.ones(4, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    freq, pos = lm.rotary_frequencies(8)[0], torch.zeros(4, dtype=torch.int32, device="cuda")
+    calls = {"dropout": lambda t: lm.dropout(t, 0.5, 0, 0, out=t), "residual": lambda t: lm.block_norm(t, x, out=t),
+             "normed": lambda t: lm.block_norm(t, x, next_weight=w, normed_out=t),
+             "rotary": lambda t: lm.rotary(t[:, None], None, pos, freq, out=(t[:, None], None)),
+             "logits": lambda t: lm.logits_rules(t, out=t)}
+    for name, call in calls.items():
+        leaf = torch.ones(4, 8, device="cuda", requires_grad=True)
+        saved = leaf * 1.5
+        y = (saved * saved).sum()
+        before = saved._version
+        call(saved.detach())
+        assert saved._version > before, name
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():  # tensors without a version
+        t = torch.ones(4, 8, device="cuda")
+        assert lm.dropout(t, 0.5, 0, 0, out=t) is t

@@ -118,6 +118,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str =
     """The frequencies (float64, rotary_dim / 2 of them, on the device) and the scale that `rotary` takes, for
     a context `factor` times as long as the one trained on: scaling "none", "linear", "base" or "by_parts"
     (mtxc_rotary_frequencies states them)."""
+    if not 0 <= rotary_dim < 1 << 31:  # the C ABI takes 32 bits, and fills as many values as they say
+        raise ValueError("rotary_dim: expected 0 .. 2^31 - 1")
     values = (ctypes.c_double * max(1, rotary_dim // 2))()
     scale = ctypes.c_double()
     if scaling not in _abi.ROTARY_SCALINGS:

@@ -160,3 +160,10 @@ def test_tensors_of_another_device_are_refused(gpu):
     for call in calls_on("cuda:1"):
         with pytest.raises(ValueError, match="cuda:0, the device that the thread is bound to"):
             call()
+
+
+@pytest.mark.parametrize("rotary_dim", [-1, -2, -(1 << 32), 1 << 31, (1 << 32) + 4])
+def test_frequencies_of_no_dimension_are_refused(rotary_dim):
+    """Numbers that 32 bits do not hold: the values would be written past their buffer, or not at all."""
+    with pytest.raises(ValueError, match="rotary_dim"):
+        lm.rotary_frequencies(rotary_dim, device="cpu")

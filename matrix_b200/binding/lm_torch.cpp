@@ -537,4 +537,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lm", nullptr, -1, methods, nullpt
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__lm(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__lm(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", MTX_TORCH_VERSION)) Py_CLEAR(m);
+    return m;
+}

@@ -5,7 +5,7 @@ cross-compiles without a GPU.  Objects go to ``matrix_b200/_build/``; the librar
 ``matrix_b200/lib/libmtxc.so``, which travels with the source tree to the GPU box.  The
 CUDA runtime is linked statically so the library does not depend on which libcudart the
 host process (e.g. PyTorch) loaded.  ``binding/`` is compiled against the installed torch into the Python
-module ``lib/_lm.so``.
+module ``lib/_lm.so``, and again when another torch is installed; where there is none with CUDA it is left out.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -26,6 +27,7 @@ HOST = PKG / "host"
 HOST_LIB = LIBDIR / "libmtx.so"
 BINDING = PKG / "binding"
 BINDING_LIB = LIBDIR / "_lm.so"
+BINDING_TORCH = BUILD / "_lm.torch"  # the torch that BINDING_LIB was compiled against
 INCLUDE = REPO / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -46,6 +48,42 @@ def _stale(obj: Path, deps: list[Path]) -> bool:
         return True
     t = obj.stat().st_mtime
     return any(d.stat().st_mtime > t for d in deps)
+
+
+def _run(cmd: list[str], verbose: bool = False) -> str:
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    return res.stdout + res.stderr
+
+
+def build_binding(headers: list[Path], verbose: bool = False) -> Path | None:
+    """Compiles the Python module over torch tensors; None, with a message, where there is no torch with CUDA."""
+    try:
+        import torch
+    except (ImportError, OSError) as e:
+        missing = f"torch cannot be imported: {e}"
+    else:
+        missing = "" if torch.version.cuda else f"torch {torch.__version__} is built without CUDA"
+    if missing:
+        print(f"{BINDING_LIB.name} left out ({missing}); the C ABI does not need it", file=sys.stderr)
+        return None
+    torch_dir = Path(torch.__file__).resolve().parent
+    against = f"{torch.__version__} {torch_dir}"
+    srcs = sorted(BINDING.glob("*.cpp"))
+    if _stale(BINDING_LIB, [*srcs, LIB, *headers]) or not BINDING_TORCH.exists() or BINDING_TORCH.read_text() != against:
+        cuda_include = Path(nvcc()).resolve().parent.parent / "include"
+        _run(["g++", *CXX_FLAGS, "-shared", "-I", str(torch_dir / "include"),
+              "-I", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+              "-I", sysconfig.get_paths()["include"], "-I", str(cuda_include),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+              f'-DMTX_TORCH_VERSION="{torch.__version__}"', "-o", str(BINDING_LIB), *map(str, srcs), "-L", str(LIBDIR),
+              "-lmtxc", "-L", str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch",
+              "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"], verbose)
+        BINDING_TORCH.write_text(against)
+    return BINDING_LIB
 
 
 def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
@@ -69,12 +107,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
             jobs.append(["g++", *CXX_FLAGS, "-c", str(src), "-o", str(obj)])
 
     def run(cmd: list[str]) -> str:
-        if verbose:
-            print(" ".join(cmd), file=sys.stderr)
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
-        return res.stdout + res.stderr
+        return _run(cmd, verbose)
 
     with cf.ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 4))) as ex:
         for out in ex.map(run, jobs):
@@ -89,20 +122,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I", str(INCLUDE), "-I", str(HOST),
              "-I", str(cuda_include), "-o", str(HOST_LIB), *map(str, host_srcs), "-L", str(LIBDIR), "-lmtxc",
              "-ldl", "-Wl,-rpath,$ORIGIN"])
-    binding_srcs = sorted(BINDING.glob("*.cpp"))
-    if _stale(BINDING_LIB, [*binding_srcs, LIB, *headers]):
-        import sysconfig
-
-        import torch
-
-        torch_dir = Path(torch.__file__).resolve().parent
-        cuda_include = Path(nvcc()).resolve().parent.parent / "include"
-        run(["g++", *CXX_FLAGS, "-shared", "-I", str(torch_dir / "include"),
-             "-I", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
-             "-I", sysconfig.get_paths()["include"], "-I", str(cuda_include),
-             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-o", str(BINDING_LIB),
-             *map(str, binding_srcs), "-L", str(LIBDIR), "-lmtxc", "-L", str(torch_dir / "lib"), "-ltorch_python",
-             "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"])
+    build_binding(headers, verbose)
     return LIB
 
 

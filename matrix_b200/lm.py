@@ -34,6 +34,9 @@ def _load():
     spec = importlib.util.spec_from_file_location("matrix_b200._lm", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    if module.torch_version != torch.__version__:
+        raise ImportError(f"{path} was compiled against torch {module.torch_version}, not the installed {torch.__version__}: "
+                          "build it again with `python -m matrix_b200.build`")
     return module
 
 

@@ -577,3 +577,23 @@ def test_one_tensor_for_two_outputs_is_refused(lm):
         assert _abi.lib().mtxc_block_norm_backward(0, _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
             4, 64, *at(dh), *at(da), *at(h), *at(b), r.data_ptr(), s.data_ptr(), post.data_ptr(), next.data_ptr(), 0, 0, 0,
             *gradients, 0, 0, 0, 0, 1.0, 1.0, 0.0, 0.0, 0, 0, 0)) == _abi.ERR_INVALID_ARGUMENT
+
+
+def test_backward_on_another_stream(lm, gpu):
+    """The pass that uses the workspace and two launches, on a stream of the caller's."""
+    c = Case((640, 1024), torch.bfloat16, gate="channel", drop=0.1)
+    h, r, s = (t.cuda() for t in c.stored())
+    dh, da, b, p = c.dh.cuda(), c.da.cuda(), c.b.cuda(), c.params()
+    call = lambda: lm.block_norm_backward(dh, da, h, b, post_rstd=r, next_rstd=s, **p)  # noqa: E731
+    want = call()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    try:
+        gpu.set_stream(side)
+        got = call()
+        side.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+    finally:
+        torch.cuda.synchronize()
+        gpu.set_stream(torch.cuda.current_stream())

@@ -219,3 +219,21 @@ def test_refusals(lm):
     with pytest.raises(MtxcError) as e:
         lm.logits_rules(x.int())
     assert e.value.code == _abi.ERR_UNSUPPORTED_DTYPE
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [64, 77])
+def test_special_values_under_every_rule(lm, dtype, vocab):
+    """Infinities, NaN and the type's lowest value, in the history, biased, masked and none of these: every element
+    of the row is the formula's."""
+    d = inputs(3, vocab, 30, 4, padding=False)
+    d["tokens"] = torch.arange(30, dtype=torch.int32).expand(3, 30).contiguous()
+    d["lengths"][:], d["prompt_lengths"][:] = 30, torch.tensor([10, 0, 30])
+    d["bias_tokens"] = torch.tensor([[2, 3, 40, 43]], dtype=torch.int32).expand(3, 4).contiguous()
+    d["mask"][0], d["mask"][1], d["mask"][2] = -1, 0x55555555, 0
+    x = normal(3, vocab, dtype)
+    lowest = torch.finfo(dtype).min
+    x[:, 0:8] = torch.tensor([INF, -INF, float("nan"), lowest, INF, -INF, float("nan"), lowest], dtype=dtype)
+    x[:, 40:44] = torch.tensor([INF, -INF, float("nan"), lowest], dtype=dtype)
+    check(lm, x, d)
+    check(lm, x, {k: v for k, v in d.items() if k != "mask"})

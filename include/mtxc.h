@@ -469,8 +469,8 @@ int mtxc_block_norm(int dtype, const mtxc_block_norm_args* args);
  *     d_branch = r * u - branch * r^3 * mean(u * branch)                     (q where there is no post norm)
  *     d_next_weight = sum_t d_normed * h * s,   d_post_weight = sum_t q * branch * r          (float)
  *     d_gate[group] = sum over its rows of branch_scale * mask * n * H                     (gate_dtype)
- * d_residual and d_branch may be the very tensors of inputs (of a gate per token too, by a slower kernel); the last
- * three must not overlap anything.
+ * d_residual and d_branch may be the very tensors of inputs (of a gate per token too, with d_post_weight by a slower
+ * kernel); the last three must not overlap anything.
  * d_residual, d_branch and the last three may each be NULL: not wanted.  d_gate has gate_stride's layout with
  * its own stride d_gate_stride.  branch NULL (and with it d_branch, post_weight, gate): a norm alone.
  * The sums over rows are made in 32 bits of per-block partials in the thread's workspace

@@ -488,8 +488,9 @@ __device__ __forceinline__ void for_each_segment(const Backward& f, uint32_t run
     }
 }
 
-// Any width (in use: above 65,536, and where a gradient is written over a gate per token, which is here read before the
-// row's stores), stride and alignment: the rows are read twice and the sums over rows live in the workspace.
+// Any width (in use: above 65,536, and where a gradient is written over a gate per token that the post weight's
+// gradient needs, which is here read before the row's stores), stride and alignment: the rows are read twice and the
+// sums over rows live in the workspace.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) block_norm_backward_any_kernel(const Backward f) {
     __shared__ float part[3 * 32];
@@ -1240,9 +1241,10 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
               param_aligned(f.gate, f.gs) && eight_aligned<T>(f.dgate, f.dgs);
         plan = plan_backward<T>(f.width, vec);
     });
-    // The other kernels read a gate row once more after its rows' stores: read before them it is held across the
-    // row's work, which cost the kernels of scalar accesses 10 to 22 % in spills ([8192, 1001] f16 77 -> 93 us).
-    if (f.gate && (f.dx == f.gate || f.db == f.gate)) plan = Plan();
+    // For the post weight's gradient the other kernels read a gate row once more after its rows' stores: read before
+    // them it is held across the row's work, which cost the kernels of scalar accesses 10 to 22 % in spills ([8192,
+    // 1001] f16 77 -> 93 us).
+    if (f.gate && a->d_post_weight && (f.dx == f.gate || f.db == f.gate)) plan = Plan();
     const int sums = !!a->d_next_weight + !!a->d_post_weight + !!a->d_gate;
     const uint64_t row_bytes = (uint64_t)f.width * sizeof(float) * sums;
     // teams that the GPU holds; a block's teams share a gate row, or each has whole ones; few rows: fewer teams in a

@@ -597,3 +597,25 @@ def test_backward_on_another_stream(lm, gpu):
     finally:
         torch.cuda.synchronize()
         gpu.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("rows,width", [(1, 4096), (300, 64), (7, 1000), (300, 4096), (300, 4097), (40, 12001)])
+@pytest.mark.parametrize("over", ["branch", "residual"])
+def test_gradients_written_over_a_gate_without_the_post_weight_s(lm, gpu, rows, width, over):
+    """The same where no sum over rows needs the gate: the bits are those of separate tensors."""
+    from matrix_b200 import _abi
+
+    c = Case((rows, width), torch.bfloat16, gate="token", drop=0.1)
+    h, r, s = c.stored()
+    dh, da, hd, b, gate = (t.cuda() for t in (c.dh, c.da, h, c.b, c.gate))
+    kept = [t.cuda() for t in (r, s, c.post, c.next)]
+    want = lm.block_norm_backward(dh, da, hd, b, post_rstd=kept[0], next_rstd=kept[1], **c.params())
+    got = {"residual": torch.empty_like(hd), "branch": torch.empty_like(hd), over: gate, "gate": torch.empty_like(hd),
+           "next_weight": torch.empty(width, device="cuda")}
+    at = lambda t: (t.data_ptr(), width)  # noqa: E731
+    _abi.check(_abi.lib().mtxc_block_norm_backward(10, _abi.BLOCK_NORM_BACKWARD_ARGS.pack(
+        rows, width, *at(dh), *at(da), *at(hd), *at(b), *(t.data_ptr() for t in kept), *at(gate), 1, *at(got["residual"]),
+        *at(got["branch"]), 0, got["next_weight"].data_ptr(), *at(got["gate"]), 10, 10, 1.0, 1.0, 0.0, 0.1, SEED, OFFSET, 0)))
+    gpu.sync()
+    for name, t in got.items():
+        assert torch.equal(t, getattr(want, name)), name

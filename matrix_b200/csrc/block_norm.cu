@@ -265,8 +265,9 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* part, uint32_t thr
 }
 
 // Rows held in registers, E elements per thread: read once, written once.  WARP: a warp per row, eight rows per
-// block; else a block per row.  Bound by HBM ([8192, 4096] bf16 46 us, 5.8 TB/s), with dropout by the generator's
-// integer work ([8192, 8192] bf16 with a gate per channel 109 us, 4.9 TB/s).  A grid of resident blocks that
+// block; else a block per row.  Bound by HBM without dropout ([8192, 4096] bf16 43 us, 6.2 TB/s).  With it neither
+// issue (61 %) nor HBM is full: a block's phases follow one another, and the mask is made after the first reduction,
+// when little is on its way ([8192, 8192] bf16 with a gate per channel 108 us, 5.0 TB/s).  A grid of resident blocks that
 // copies the next row ahead was slower (47 -> 51 us, 109 -> 122): more blocks hide a row's two reductions better.
 template <typename T, int E, bool VEC, bool WARP, int BLOCK, int MIN>
 __global__ void __launch_bounds__(BLOCK, MIN) block_norm_kernel(const Forward f) {
@@ -670,7 +671,9 @@ __device__ __forceinline__ void store_sums(const Chunk<T, VEC>& ch, float* row, 
 // block, which exchange their sums through distributed shared memory: one cluster barrier per row.  A thread keeps
 // its columns' w_next' and gate * w_post' in shared memory, as floats ready for use, for the run (or the gate
 // row).  Inputs that the call does not have read as zeros, weights as ones: fewer branches.  Bound by latency at
-// 16 warps per SM: [8192, 4096] bf16 with gate and dropout 88 us with the finish, 4.6 TB/s.
+// 16 warps per SM (vectors of half types at 4,096 and 8,192 columns; 9 to 14 at most widths between): [8192, 4096] bf16
+// with gate and dropout 89 us with the finish, 4.5 TB/s.  The kernels of scalar accesses hold 64 registers and spill
+// (up to 490 bytes with several gate rows a run), as those of a warp per row with several gate rows do at 128.
 template <typename T, int E, bool VEC, bool WARP, bool MULTI, bool CLUSTER, int BLOCK, int MIN>
 __global__ void __launch_bounds__(BLOCK, MIN) block_norm_backward_kernel(const Backward f, uint32_t team_threads, uint32_t stages) {
     constexpr int K = E / 8;
@@ -1243,7 +1246,7 @@ extern "C" int mtxc_block_norm_backward(int dtype, const mtxc_block_norm_backwar
     });
     // For the post weight's gradient the other kernels read a gate row once more after its rows' stores: read before
     // them it is held across the row's work, which cost the kernels of scalar accesses 10 to 22 % in spills ([8192,
-    // 1001] f16 77 -> 93 us).
+    // 1001] f16 77 -> 93 us).  This one takes 711 us for [4096, 4096] bf16, 84 with tensors apart.
     if (f.gate && a->d_post_weight && (f.dx == f.gate || f.db == f.gate)) plan = Plan();
     const int sums = !!a->d_next_weight + !!a->d_post_weight + !!a->d_gate;
     const uint64_t row_bytes = (uint64_t)f.width * sizeof(float) * sums;

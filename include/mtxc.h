@@ -578,6 +578,143 @@ typedef struct mtxc_logits_args {
 int mtxc_logits_rules(int dtype, const mtxc_logits_args* args);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention of a language model: the norms of queries and keys with their rotation, a paged cache, and the attention of
+ * one new token over it and of whole prompts.  As above: Float, Float16, BFloat16; unit stride within a head; strides in
+ * elements.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Norms of one or two tensors of heads (queries and keys) with their rotation, in one launch; layouts, positions,
+ * frequencies, scale and interleaved as for mtxc_rotary.  For each head x, with w' = weight_offset + weight[i] (w' = 1
+ * where weight[i] is NULL; weights have head_dim elements of weight_dtype):
+ *     r = 1 / sqrt(mean(x^2) + eps),  n = x r w',  dst = n with its first rotary_dim elements turned and scaled
+ * rstd[i] (NULL: not wanted) receives r, [batch, length, heads[i]].  dst may be the very tensor of src.  head_dim at most
+ * 1,024.
+ *
+ * The backward pass: d_out holds the gradient at the forward call's dst, src and rstd its input and its r (weight, scale,
+ * positions as there); with g = d_out turned back and scaled, u = g w':
+ *     dst = r u - x r^3 mean(u x)                 (may be the very tensor of d_out or src)
+ *     d_weight[i] = sum over tokens and heads of g x r      (float, head_dim; NULL: not wanted)
+ * The sums are made of per-block partial rows, added in a fixed order, in `workspace` (device memory aligned to 256 bytes,
+ * of at least as many bytes as mtxc_head_norm_rotary_backward_workspace gives for the call) or, where that is NULL, in the
+ * thread's (MTXC_ERR_WORKSPACE where it is too small). */
+typedef struct mtxc_head_norm_args {
+    uint64_t batch, length;
+    uint32_t head_dim, rotary_dim;
+    uint32_t heads[2];
+    void* dst[2];
+    uint64_t dst_strides[2][3];
+    const void* src[2];
+    uint64_t src_strides[2][3];
+    const void* weight[2];
+    float* rstd[2];
+    const void* positions;
+    uint64_t position_strides[2];
+    const double* frequencies;
+    int position_dtype, weight_dtype;
+    float scale, weight_offset, eps;
+    int interleaved;
+    const void* d_out[2]; /* from here on: the backward pass */
+    uint64_t d_out_strides[2][3];
+    float* d_weight[2];
+    void* workspace;
+    size_t workspace_bytes;
+} mtxc_head_norm_args;
+int mtxc_head_norm_rotary(int dtype, const mtxc_head_norm_args* args);
+int mtxc_head_norm_rotary_backward(int dtype, const mtxc_head_norm_args* args);
+int mtxc_head_norm_rotary_backward_workspace(int dtype, const mtxc_head_norm_args* args, size_t* bytes);
+
+/* A paged cache of keys (index 0) and values (1): head h of slot s of page p is head_dim elements at
+ * data[i] + p * strides[i][0] + s * strides[i][1] + h * strides[i][2].  dtype: Float, Float16, BFloat16 or
+ * MTXC_FLOAT8_E4M3, of which a head is its bytes' values (e4m3, 4 significant bits, up to 448, no infinities) times
+ * 2^exponent, the exponent at exponents[i] with exponent_strides[i].  pages * page_size below 2^31. */
+enum { MTXC_FLOAT8_E4M3 = 32 }; /* of caches only */
+typedef struct mtxc_kv_cache {
+    uint64_t pages;
+    uint32_t page_size, heads, head_dim;
+    int dtype;
+    void* data[2];
+    uint64_t strides[2][3];
+    int8_t* exponents[2];
+    uint64_t exponent_strides[2][3];
+} mtxc_kv_cache;
+
+/* Stores the keys rows[0] and values rows[1] of tokens (head h of token t at t * row_strides[i][0] + h *
+ * row_strides[i][1]) at the cache's slots slots[t * slot_stride] (slot_dtype Int32 or Int64; slot s: page s / page_size,
+ * slot s % page_size of it).  Slots outside the cache are passed over; of the tokens that name the same slot the last
+ * counts.  To 8 bits: with e the least integer such that the largest finite magnitude of the row is at most 448 * 2^e (0
+ * for none; at least -96, at most 96), the bytes are x * 2^-e rounded to nearest even, larger ones +-448, NaN and
+ * infinities NaN.  Other caches hold rows of their own dtype.  head_dim at most 1,024.
+ *
+ * mtxc_cache_read is the way back: rows[i] receives what the cache holds at the slots (of 8 bits rounded to dtype),
+ * zeros for a slot outside it. */
+typedef struct mtxc_cache_rows_args {
+    mtxc_kv_cache cache;
+    uint64_t tokens;
+    void* rows[2];
+    uint64_t row_strides[2][2];
+    const void* slots;
+    uint64_t slot_stride;
+    int slot_dtype;
+} mtxc_cache_rows_args;
+int mtxc_cache_write(int dtype, const mtxc_cache_rows_args* args);
+int mtxc_cache_read(int dtype, const mtxc_cache_rows_args* args);
+
+/* Attention of one new token of each of `batch` sequences over a cache: for sequence b and query head h, which reads key
+ * head h / (heads / cache.heads),
+ *     out[b, h] = sum_j p_j v_j,   p = softmax(scale * q[b, h] . k_j)
+ * over its lengths[b] first tokens (cut to 0 .. max_pages * page_size); token j lies in page page_table[b *
+ * page_table_stride + j / page_size] at slot j % page_size.  Tokens of a page that the cache does not have are passed
+ * over; where none is left the output is 0.  The queries' dtype is the cache's, or any for a cache in 8 bits.  q and out
+ * at b * strides[0] + h * strides[1].  head_dim at most 256, batch at most 65,535.  Scores, sums and the join of what the
+ * blocks share are in 32 bits; products of half types and of a cache in 8 bits take the weights p rounded to 16 bits.
+ * The shares' sums are in `workspace` (aligned to 256 bytes, of at least as many bytes as
+ * mtxc_decode_attention_workspace gives) or, where that is NULL, in the thread's. */
+typedef struct mtxc_decode_attention_args {
+    mtxc_kv_cache cache;
+    uint64_t batch, max_pages;
+    uint32_t heads;
+    float scale;
+    const void* q;
+    uint64_t q_strides[2];
+    void* out;
+    uint64_t out_strides[2];
+    const int32_t* page_table;
+    uint64_t page_table_stride;
+    const int32_t* lengths;
+    void* workspace;
+    size_t workspace_bytes;
+} mtxc_decode_attention_args;
+int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args* args);
+int mtxc_decode_attention_workspace(int dtype, const mtxc_decode_attention_args* args, size_t* bytes);
+
+/* Attention over whole prompts, packed one after another: sequence s has the queries starts[s] .. starts[s + 1] - 1 and
+ * the keys and values k_starts[s] .. k_starts[s + 1] - 1 (NULL: as starts).  starts, k_starts: sequences + 1 ascending
+ * int32, cut to 0 .. tokens (k_tokens); rows in no sequence are not read as far as they have a say, and their outputs are
+ * left as they were.  Of a sequence with n queries and m keys query i sees the keys j <= i + m - n (causal != 0; a prefix
+ * of m - n keys comes from elsewhere) or all:
+ *     out_i = sum_j p_j v_j,  p = softmax(scale * q_i . k_j) over the keys seen, 0 where there is none
+ * Query head h reads key head h / (heads / kv_heads).  Token t, head h of a tensor at t * strides[0] + h * strides[1].
+ * head_dim at most 256; tokens, k_tokens and sequences below 2^30.  Sums are in 32 bits; for half types the weights are
+ * rounded to 16 bits before they meet the values. */
+typedef struct mtxc_prompt_attention_args {
+    uint64_t tokens, k_tokens, sequences;
+    uint32_t heads, kv_heads, head_dim;
+    float scale;
+    const void* q;
+    uint64_t q_strides[2];
+    const void* k;
+    uint64_t k_strides[2];
+    const void* v;
+    uint64_t v_strides[2];
+    void* out;
+    uint64_t out_strides[2];
+    const int32_t* starts;
+    const int32_t* k_starts;
+    int causal;
+} mtxc_prompt_attention_args;
+int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args* args);
+
+/* ------------------------------------------------------------------------------------------
  * Multi-GPU: one communicator per GPU for reductions over an axis sharded across the GPUs of a node
  * (benchmark configs 4 and 5b).  The reference drives a single Metal device through one GPUManager
  * (Mods/GPUManager.h:53-54); these entry points are the multi-device half of the layer that replaces
@@ -648,6 +785,8 @@ int mtxc_allreduce(int op, int dtype, void* buf, uint64_t count);
 
 /* Starts capturing the calling thread's stream into a CUDA graph. */
 int mtxc_graph_begin(void);
+/* *recording: 1 between mtxc_graph_begin and mtxc_graph_end on the calling thread, else 0. */
+int mtxc_graph_recording(int* recording);
 /* Ends the capture and instantiates it; *graph receives an opaque handle. */
 int mtxc_graph_end(void** graph);
 /* Replays a captured graph on the calling thread's stream. */

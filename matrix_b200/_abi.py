@@ -64,6 +64,29 @@ LOGITS_FIELDS = (
     "lengths:P", "prompt_lengths:P", "repetition:P", "frequency:P", "presence:P", "bias_tokens:P",
     "bias_tokens_stride:Q", "bias_values:P", "bias_values_stride:Q", "biases:Q", "mask:P", "mask_stride:Q")
 LOGITS_ARGS = _layout(*LOGITS_FIELDS)
+HEAD_NORM_FIELDS = (
+    "batch:Q", "length:Q", "head_dim:I", "rotary_dim:I", "heads:2I", "dst:2P", "dst_strides:6Q", "src:2P",
+    "src_strides:6Q", "weight:2P", "rstd:2P", "positions:P", "position_strides:2Q", "frequencies:P", "position_dtype:i",
+    "weight_dtype:i", "scale:f", "weight_offset:f", "eps:f", "interleaved:i", "d_out:2P", "d_out_strides:6Q",
+    "d_weight:2P", "workspace:P", "workspace_bytes:N")
+HEAD_NORM_ARGS = _layout(*HEAD_NORM_FIELDS)
+KV_CACHE_FIELDS = (
+    "pages:Q", "page_size:I", "heads:I", "head_dim:I", "dtype:i", "data:2P", "strides:6Q", "exponents:2P",
+    "exponent_strides:6Q")
+KV_CACHE = _layout(*KV_CACHE_FIELDS)
+CACHE_ROWS_FIELDS = (
+    *("cache." + f for f in KV_CACHE_FIELDS), "tokens:Q", "rows:2P", "row_strides:4Q", "slots:P", "slot_stride:Q",
+    "slot_dtype:i")
+CACHE_ROWS_ARGS = _layout(*CACHE_ROWS_FIELDS)
+DECODE_ATTENTION_FIELDS = (
+    *("cache." + f for f in KV_CACHE_FIELDS), "batch:Q", "max_pages:Q", "heads:I", "scale:f", "q:P", "q_strides:2Q",
+    "out:P", "out_strides:2Q", "page_table:P", "page_table_stride:Q", "lengths:P", "workspace:P", "workspace_bytes:N")
+DECODE_ATTENTION_ARGS = _layout(*DECODE_ATTENTION_FIELDS)
+PROMPT_ATTENTION_FIELDS = (
+    "tokens:Q", "k_tokens:Q", "sequences:Q", "heads:I", "kv_heads:I", "head_dim:I", "scale:f", "q:P", "q_strides:2Q",
+    "k:P", "k_strides:2Q", "v:P", "v_strides:2Q", "out:P", "out_strides:2Q", "starts:P", "k_starts:P", "causal:i")
+PROMPT_ATTENTION_ARGS = _layout(*PROMPT_ATTENTION_FIELDS)
+FLOAT8_E4M3 = 32  # of caches only
 ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "by_parts": 3}
 
 
@@ -144,7 +167,16 @@ def lib() -> C.CDLL:
             "mtxc_rotary_frequencies": (i32, [i32, u32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double,
                                               C.POINTER(C.c_double), C.POINTER(C.c_double)]),
             "mtxc_logits_rules": (i32, [i32, C.c_char_p]),
+            "mtxc_head_norm_rotary": (i32, [i32, C.c_char_p]),
+            "mtxc_head_norm_rotary_backward": (i32, [i32, C.c_char_p]),
+            "mtxc_head_norm_rotary_backward_workspace": (i32, [i32, C.c_char_p, C.POINTER(sz)]),
+            "mtxc_cache_write": (i32, [i32, C.c_char_p]),
+            "mtxc_cache_read": (i32, [i32, C.c_char_p]),
+            "mtxc_decode_attention": (i32, [i32, C.c_char_p]),
+            "mtxc_decode_attention_workspace": (i32, [i32, C.c_char_p, C.POINTER(sz)]),
+            "mtxc_prompt_attention": (i32, [i32, C.c_char_p]),
             "mtxc_graph_begin": (i32, []),
+            "mtxc_graph_recording": (i32, [C.POINTER(i32)]),
             "mtxc_graph_end": (i32, [C.POINTER(vp)]),
             "mtxc_graph_launch": (i32, [vp]),
             "mtxc_graph_destroy": (i32, [vp]),

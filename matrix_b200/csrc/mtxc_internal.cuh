@@ -28,6 +28,7 @@ struct ThreadCtx {
     void* workspace = nullptr;
     size_t workspace_bytes = 0;
     bool own_workspace = false;
+    bool recording = false;              // between mtxc_graph_begin and mtxc_graph_end
     int sm_count = 148;
     CommState* comm = nullptr;           // set by mtxc_comm_init
     std::string last_error;

@@ -244,12 +244,20 @@ int mtxc_graph_begin(void) {
     if (int rc = require_init()) return rc;
     cudaError_t err = cudaStreamBeginCapture(ctx().stream(), cudaStreamCaptureModeThreadLocal);
     if (err != cudaSuccess) return cuda_fail(err, "cudaStreamBeginCapture");
+    ctx().recording = true;
+    return MTXC_OK;
+}
+
+int mtxc_graph_recording(int* recording) {
+    if (!recording) return fail(MTXC_ERR_INVALID_ARGUMENT, "mtxc_graph_recording: null pointer");
+    *recording = ctx().recording;
     return MTXC_OK;
 }
 
 int mtxc_graph_end(void** graph) {
     if (int rc = require_init()) return rc;
     if (!graph) return fail(MTXC_ERR_INVALID_ARGUMENT, "mtxc_graph_end: null pointer");
+    ctx().recording = false;
     cudaGraph_t g = nullptr;
     cudaError_t err = cudaStreamEndCapture(ctx().stream(), &g);
     if (err != cudaSuccess) return cuda_fail(err, "cudaStreamEndCapture");

@@ -1,5 +1,7 @@
-"""Row operators of a language model on device tensors: the norms around a block with its gate, dropout and
-residual, dropout by itself, rotary positions, and the rules on logits before a token is chosen.
+"""Operators of a language model on device tensors: the norms around a block with its gate, dropout and residual,
+dropout by itself, rotary positions, the norms of queries and keys together with them, a paged cache of keys and values
+(plain or in 8 bits), the attention of one new token over it and of whole prompts, and the rules on logits before a token
+is chosen.
 
 These functions hand a call's tensors to the C ABI (include/mtxc.h, which states the formulas) through the module
 that matrix_b200/binding compiles against torch; PyTorch only provides device memory and streams, and there is no
@@ -9,7 +11,8 @@ where it is not torch's current stream, ordering the two is the caller's, as for
 an output counts as changed in place.
 
 Inputs are float32, float16 or bfloat16 tensors on the thread's device whose last axis has unit stride; the other axes
-of a row operator's inputs have to fold into one axis of rows (a constant stride from row to row).
+of a row operator's inputs have to fold into one axis of rows (a constant stride from row to row), while those of heads
+and of a cache may have any strides.
 """
 from __future__ import annotations
 
@@ -22,8 +25,9 @@ import torch
 from . import _abi
 from ._abi import check, lib
 
-__all__ = ["BlockNorm", "BlockNormGradients", "block_norm", "block_norm_backward", "dropout", "logits_rules", "rotary",
-           "rotary_frequencies"]
+__all__ = ["BlockNorm", "BlockNormGradients", "HeadNorm", "HeadNormGradients", "KVCache", "block_norm",
+           "block_norm_backward", "cache_read", "cache_write", "decode_attention", "dropout", "head_norm_rotary",
+           "head_norm_rotary_backward", "kv_cache", "logits_rules", "prompt_attention", "rotary", "rotary_frequencies"]
 
 
 def _load():
@@ -158,3 +162,113 @@ def logits_rules(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, le
     v % 32 of word v / 32).  Lists may hold padding outside the vocabulary.  out may be logits."""
     return _done(_lm.logits_rules(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias_tokens,
                                   bias_values, mask, out))[0]
+
+
+class HeadNorm(NamedTuple):
+    """What head_norm_rotary returns; None where the call has no such output."""
+
+    q: torch.Tensor
+    k: torch.Tensor | None
+    q_rstd: torch.Tensor | None
+    k_rstd: torch.Tensor | None
+
+
+class HeadNormGradients(NamedTuple):
+    """Gradients of head_norm_rotary's inputs; None where the call has no such input."""
+
+    q: torch.Tensor
+    k: torch.Tensor | None
+    q_weight: torch.Tensor | None
+    k_weight: torch.Tensor | None
+
+
+def head_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *,
+                     q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                     weight_offset: float = 0.0, eps: float = 1e-6, scale: float = 1.0, interleaved: bool = False,
+                     save_rstd: bool = True, out: tuple | None = None) -> HeadNorm:
+    """Each head of the queries and keys normed (x / sqrt(mean(x^2) + eps) * (weight_offset + weight), one weight of the
+    head's width for all heads, None: none) and then turned as by `rotary`, in one pass (mtxc_head_norm_rotary); layouts,
+    positions, frequencies, scale and interleaved as there.  No frequencies: the norm alone.  save_rstd: keep the
+    norms' reciprocal deviations (one float per head, [batch, length, heads]) for head_norm_rotary_backward.
+    out=(q, k) writes in place."""
+    q_out, k_out = out if out is not None else (None, None)
+    return HeadNorm._make(_done(_lm.head_norm_rotary(q, k, positions, frequencies, q_weight, k_weight, weight_offset, eps,
+                                                     scale, interleaved, save_rstd, q_out, k_out)))
+
+
+def head_norm_rotary_backward(d_q: torch.Tensor, d_k: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor | None,
+                              positions: torch.Tensor, frequencies: torch.Tensor, *, q_rstd: torch.Tensor,
+                              k_rstd: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                              k_weight: torch.Tensor | None = None, weight_offset: float = 0.0, scale: float = 1.0,
+                              interleaved: bool = False, parameters: bool = True) -> HeadNormGradients:
+    """The gradients of head_norm_rotary's inputs (mtxc_head_norm_rotary_backward), given those of its outputs, its
+    inputs q and k, the saved rstds and its other arguments.  The weights' gradients are float32; parameters=False:
+    they are not wanted."""
+    return HeadNormGradients._make(_done(_lm.head_norm_rotary_backward(
+        d_q, d_k, q, k, positions, frequencies, q_rstd, k_rstd, q_weight, k_weight, weight_offset, scale, interleaved,
+        parameters)))
+
+
+class KVCache(NamedTuple):
+    """A paged cache: keys and values [pages, page_size, heads, head_dim] with any strides but unit stride within a head,
+    float32, float16, bfloat16 or float8_e4m3fn.  Of the last a head's elements are its bytes' values times 2^exponent,
+    exponents int8 [pages, page_size, heads] (None for the other types).  Slot s is slot s % page_size of page
+    s // page_size."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_exponents: torch.Tensor | None = None
+    value_exponents: torch.Tensor | None = None
+
+
+def kv_cache(pages: int, page_size: int, heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
+             device="cuda") -> KVCache:
+    """An empty cache (zeros), the slots of a head of a page next to each other in memory."""
+    def zeros(*shape, dtype):
+        return torch.zeros(pages, heads, page_size, *shape, dtype=dtype, device=device).transpose(1, 2)
+
+    small = dtype == torch.float8_e4m3fn
+    data = [zeros(head_dim, dtype=torch.int8).view(dtype) if small else zeros(head_dim, dtype=dtype) for _ in range(2)]
+    return KVCache(*data, *(zeros(dtype=torch.int8) if small else None for _ in range(2)))
+
+
+def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Stores keys and values [tokens, heads, head_dim] at the cache's slots (int32 or int64 [tokens]; of tokens that name
+    one slot the last counts, slots outside the cache are passed over).  A float8_e4m3fn cache takes any of the three types
+    and rounds each head to e4m3 times the least power of two that keeps its largest element (mtxc_cache_write); other
+    caches take their own."""
+    _done(_lm.cache_write(*cache, k, v, slots))
+
+
+def cache_read(cache: KVCache, slots: torch.Tensor, *, dtype: torch.dtype | None = None,
+               out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values [tokens, heads, head_dim] at the cache's slots (int32 or int64 [tokens]), zeros for slots
+    outside it.  dtype: the cache's, for float8_e4m3fn any of the three (bfloat16 where none is given, which holds its
+    values exactly).  out=(k, v): tensors to write."""
+    if dtype is None:
+        dtype = out[0].dtype if out is not None else cache.keys.dtype
+        if dtype == torch.float8_e4m3fn:
+            dtype = torch.bfloat16
+    k, v = out if out is not None else (None, None)
+    return _done(_lm.cache_read(*cache, slots, dtype, k, v))
+
+
+def decode_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, lengths: torch.Tensor, *,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token of each sequence over the cache (mtxc_decode_attention): q [batch, heads, head_dim], of
+    which heads / cache heads share a key head; page_table int32 [batch, pages of a sequence], lengths int32 [batch]: the
+    tokens of a sequence, the new one's key and value among them if it sees itself.  scale: 1 / sqrt(head_dim) where None.
+    A sequence without tokens gives 0.  The work is shared out by the lengths on the device: a captured call may be
+    replayed with others."""
+    return _done(_lm.decode_attention(q, *cache, page_table, lengths, scale, out))[0]
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, *,
+                     k_starts: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over whole prompts packed one after another (mtxc_prompt_attention): q [tokens, heads, head_dim], k and v
+    [tokens, kv_heads, head_dim]; sequence s is rows starts[s] .. starts[s + 1] - 1 (int32 [sequences + 1], ascending).
+    k_starts: the same for keys and values where a sequence has more of them than queries (a prefix from the cache):
+    its last query sees all.  causal=False: every query sees every key of its sequence.  scale: 1 / sqrt(head_dim) where
+    None.  Rows in no sequence are left as they were."""
+    return _done(_lm.prompt_attention(q, k, v, starts, k_starts, scale, causal, out))[0]

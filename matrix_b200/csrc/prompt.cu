@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "attention.cuh"
+#include "tensor.cuh"
 
 namespace mtxc {
 namespace {
@@ -179,6 +180,412 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// Half types on the tensor cores.
+//
+// A block has NT tiles of 128 queries of one head (NT = 2 for heads of up to 128 elements) and runs along the keys in tiles
+// of 128.  Roles: four warps for each tile of queries, a thread a row, have its softmax; one thread issues the products,
+// one the copies, and two warps clean values (below).  The scores S = Q K' of a tile lie in tensor memory; a row's thread
+// reads them, writes the weights over them in 16 bits, and the product with V takes them from there, so that neither
+// passes through shared memory.  While one tile of queries is with its softmax the tensor cores work for the other:
+//     S0(j)  softmax 0        | P0(j) V(j), S0(j+1)
+//     S1(j)        softmax 1        | P1(j) V(j), S1(j+1)
+//
+// The output is rescaled only where the maximum has grown by more than 2^8 since it last was: until then weights stay below
+// 2^8 (the sums are exact whatever the reference point is), and nearly all tiles keep the first one's.  S(j + 1) is issued
+// behind P(j) V(j), so a thread that sees S(j + 1) may touch the output.
+//
+// What a row does not see gets the weight 0, which is not enough where the value is NaN or infinite (another sequence's
+// row, a later token).  The two cleaning warps look through the tiles of values that some row does not see whole: rows
+// behind the sequence are zeroed, and a non-finite element of a later token is zeroed and its first key noted for each
+// element of the head, so that rows that do see it receive it at the end.
+// ------------------------------------------------------------------------------------------
+constexpr int kThreads = 384;
+constexpr uint32_t kTile = 128;
+
+struct Maps {
+    CUtensorMap q, k, v;
+    uint32_t tokens_last;  // bit 0, 1, 2: of q, k, v the token is the outermost axis (else the head)
+};
+
+template <int D, int NT>
+struct Layout {
+    static constexpr uint32_t kRowTile = kTile * 128;             // 64 elements of 128 rows
+    static constexpr uint32_t kTileBytes = kRowTile * (D / 64);
+    static constexpr uint32_t kSlots = D == 256 ? 2 : 4;          // keys and values in turn
+    static constexpr uint32_t kBytes = kTileBytes * (NT + kSlots) + 1024;  // the tiles start at a multiple of 1,024
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// Whether any of the two elements of each of the words is NaN or infinite: their products with 0 are added up.
+template <typename T>
+__device__ __forceinline__ bool all_finite(const uint4& w) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 zero = __float2half2_rn(0.0f);
+        __half2 s = __hmul2(*reinterpret_cast<const __half2*>(&w.x), zero);
+        s = __hfma2(*reinterpret_cast<const __half2*>(&w.y), zero, s);
+        s = __hfma2(*reinterpret_cast<const __half2*>(&w.z), zero, s);
+        s = __hfma2(*reinterpret_cast<const __half2*>(&w.w), zero, s);
+        return __hbeq2(s, zero);
+    } else {
+        const __nv_bfloat162 zero = __float2bfloat162_rn(0.0f);
+        __nv_bfloat162 s = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w.x), zero);
+        s = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.y), zero, s);
+        s = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.z), zero, s);
+        s = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.w), zero, s);
+        return __hbeq2(s, zero);
+    }
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Maps maps, const Prompt p) {
+    using L = Layout<D, NT>;
+    constexpr uint32_t kSlots = L::kSlots, kScores = 0, kOutput = NT * kTile;
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    constexpr float kLazy = 8.0f;
+    extern __shared__ uint8_t dynamic[];
+    __shared__ uint64_t buf[33];
+    __shared__ Found found;
+    __shared__ uint32_t tensor_base;
+    __shared__ alignas(8) uint64_t bars[2 + 4 * kSlots + 3 * NT];
+    __shared__ int first_bad[3][D];  // the first key with +infinity, -infinity, NaN in an element
+    __shared__ int any_bad;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t tiles = (shared_address(dynamic) + 1023) / 1024 * 1024;
+    auto q_tile = [&](uint32_t i) { return tiles + i * L::kTileBytes; };
+    auto slot = [&](uint32_t s) { return tiles + (NT + s) * L::kTileBytes; };
+    const uint32_t bar0 = shared_address(bars);
+    auto q_full = [&](uint32_t i) { return bar0 + 8 * i; };
+    auto full = [&](uint32_t s) { return bar0 + 8 * (2 + s); };
+    auto empty = [&](uint32_t s) { return bar0 + 8 * (2 + kSlots + s); };
+    auto raw = [&](uint32_t s) { return bar0 + 8 * (2 + 2 * kSlots + s); };  // values that are to be cleaned
+    auto clean = [&](uint32_t s) { return bar0 + 8 * (2 + 3 * kSlots + s); };
+    auto s_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + i); };
+    auto p_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + NT + i); };
+    auto o_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + 2 * NT + i); };
+
+    // the last sequence first, and in each the last tile first: of causal ones the longest; all heads of a tile in turn
+    constexpr uint32_t kRows = NT * kTile;
+    const uint32_t piece = blockIdx.x / p.heads, h = blockIdx.x - piece * p.heads, kh = p.group_div.div(h);
+    auto count = [&](uint32_t i) {
+        uint32_t first, n;
+        rows_of(p.starts, p.sequences - 1 - i, p.tokens, first, n);
+        return (uint64_t)(n + kRows - 1) / kRows;
+    };
+    const Found f = find(p.sequences, piece, count, buf, &found);
+    if (!f.any) return;
+    const uint32_t seq = p.sequences - 1 - f.i;
+    uint32_t q_first, n, k_first, m;
+    rows_of(p.starts, seq, p.tokens, q_first, n);
+    rows_of(p.k_starts, seq, p.k_tokens, k_first, m);
+    const uint32_t row0 = ((n + kRows - 1) / kRows - 1 - (uint32_t)(piece - f.first)) * kRows;
+    const int ahead = (int)m - (int)n;  // a query sees keys up to its own index plus this
+    // tiles of keys that tile i of the queries sees
+    uint32_t steps[2] = {0, 0}, most = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < NT; ++i) {
+        const uint32_t lo = row0 + i * kTile;
+        if (lo >= n) continue;
+        const int seen = p.causal ? max(0, min((int)m, (int)min(lo + kTile, n) + ahead)) : (int)m;
+        steps[i] = ((uint32_t)seen + kTile - 1) / kTile;
+        most = max(most, steps[i]);
+    }
+    // the first tile of keys that some row does not see whole
+    const uint32_t partial = p.causal ? (uint32_t)max(0, min((int)m, (int)row0 + ahead + 1)) / kTile : m / kTile;
+
+    if (warp == 0) tensor_alloc(shared_address(&tensor_base), 512);
+    if (threadIdx.x == 32) {
+        for (uint32_t i = 0; i < 2; ++i) barrier_init(q_full(i), 1);
+        for (uint32_t s = 0; s < kSlots; ++s) barrier_init(full(s), 1), barrier_init(empty(s), 1), barrier_init(raw(s), 1), barrier_init(clean(s), 2);
+        for (uint32_t i = 0; i < NT; ++i) barrier_init(s_full(i), 1), barrier_init(p_full(i), 4), barrier_init(o_full(i), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        any_bad = 0;
+    }
+    for (uint32_t e = threadIdx.x; e < 3 * D; e += kThreads) (&first_bad[0][0])[e] = 0x7FFFFFFF;
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = tensor_base;
+
+    if (warp >= 8) {
+        registers_down<88>();
+        if (warp == 8 && lane == 0) {  // copies
+            auto load = [&](uint32_t to, uint32_t bar, const CUtensorMap* map, bool token_last, uint32_t token, uint32_t head) {
+                barrier_expect(bar, L::kTileBytes);
+                for (uint32_t x = 0; x < D / 64; ++x)
+                    copy_tile(to + x * L::kRowTile, map, bar, (int)(x * 64), (int)(token_last ? head : token), (int)(token_last ? token : head));
+            };
+            bool ok = true;
+            uint32_t item = 0;
+            for (; item < 2 * most; ++item) {
+                const uint32_t j = item / 2, kv = item % 2, s = item % kSlots, use = item / kSlots;
+                if (use) ok = barrier_wait(empty(s), (use - 1) & 1);
+                if (!ok) break;
+                if (item == 0 && steps[0]) load(q_tile(0), q_full(0), &maps.q, maps.tokens_last & 1, q_first + row0, h);
+                load(slot(s), kv && j >= partial ? raw(s) : full(s), kv ? &maps.v : &maps.k, maps.tokens_last >> (1 + kv) & 1,
+                     k_first + j * kTile, kh);
+                if (NT == 2 && item == 0 && steps[1]) load(q_tile(1), q_full(1), &maps.q, maps.tokens_last & 1, q_first + row0 + kTile, h);
+            }
+            // where a wait has run out, the copies under way end before the block does
+            for (uint32_t i = item > kSlots ? item - kSlots : 0; !ok && i < item; ++i) {
+                const uint32_t j = i / 2, s = i % kSlots;
+                if (i % 2 && j >= partial) barrier_wait(raw(s), (j - partial) / (kSlots / 2) & 1);
+                else barrier_wait(full(s), i / kSlots & 1);
+            }
+        } else if (warp == 9 && lane == 0) {  // products
+            constexpr uint32_t kScore = product_descriptor(kBf16, kTile, kTile, false), kValue = product_descriptor(kBf16, kTile, D, true);
+            auto scores = [&](uint32_t i, uint32_t j) {
+                const uint32_t k = slot(2 * j % kSlots), q = q_tile(i);
+#pragma unroll
+                for (uint32_t d = 0; d < D / 16; ++d) {
+                    const uint32_t off = d / 4 * L::kRowTile + d % 4 * 32;
+                    product(tensor + kScores + i * kTile, tile_descriptor(q + off, 1024, 16), tile_descriptor(k + off, 1024, 16), kScore, d > 0);
+                }
+                product_commit(s_full(i));
+            };
+            bool ok = true;
+            auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && barrier_wait(bar, parity); };
+            if (most) wait(full(0), 0);
+            for (uint32_t i = 0; i < NT && ok; ++i) {
+                if (!steps[i]) continue;
+                wait(q_full(i), 0);
+                if (ok) scores(i, 0);
+            }
+            if (most && ok) product_commit(empty(0));
+            for (uint32_t j = 0; j < most && ok; ++j) {
+                const uint32_t item = 2 * j + 1, s = item % kSlots;
+                if (j < partial) wait(full(s), item / kSlots & 1);
+                else wait(clean(s), (j - partial) / (kSlots / 2) & 1);
+                for (uint32_t i = 0; i < NT && ok; ++i) {
+                    if (j >= steps[i]) continue;
+                    wait(p_full(i), j & 1);
+                    if (!ok) break;
+                    tensor_fence_after();
+#pragma unroll
+                    for (uint32_t d = 0; d < kTile / 16; ++d)
+                        product(tensor + kOutput + i * D, tensor + kScores + i * kTile + d * 8, tile_descriptor(slot(s) + d * 2048, 1024, L::kRowTile),
+                                kValue, j > 0 || d > 0);
+                    if (j + 1 < steps[i]) {
+                        wait(full((item + 1) % kSlots), (item + 1) / kSlots & 1);
+                        if (ok) scores(i, j + 1);
+                    } else product_commit(o_full(i));
+                }
+                if (!ok) break;
+                product_commit(empty(s));
+                if (j + 1 < most) product_commit(empty((item + 1) % kSlots));
+            }
+        } else if (warp >= 10) {  // values
+            bool ok = true;
+            for (uint32_t j = partial; j < most && ok; ++j) {
+                const uint32_t s = (2 * j + 1) % kSlots, rows = min(kTile, m - j * kTile);
+                ok = __all_sync(~0u, barrier_wait(raw(s), (j - partial) / (kSlots / 2) & 1));
+                if (!ok) break;
+                for (uint32_t e = threadIdx.x - 320; e < kTile * (D / 8); e += 64) {
+                    const uint32_t r = e / (D / 8), c = e % (D / 8);  // 16-byte units: eight elements
+                    const uint32_t at = slot(s) + c / 8 * L::kRowTile + r * 128 + (c % 8 ^ r % 8) * 16;
+                    uint4 w;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at));
+                    if (r < rows && all_finite<T>(w)) continue;
+                    uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (uint32_t x = 0; x < 8; ++x) {
+                        const uint32_t bits = v[x / 2] >> (x % 2 * 16) & 0xFFFFu;
+                        constexpr uint32_t kTop = kBf16 ? 0x7F80u : 0x7C00u;
+                        if (r < rows && (bits & kTop) != kTop) continue;
+                        v[x / 2] &= x % 2 ? 0xFFFFu : 0xFFFF0000u;
+                        if (r >= rows) continue;
+                        const int kind = (bits & 0x7FFFu) != kTop ? 2 : bits >> 15;
+                        atomicMin(&first_bad[kind][c * 8 + x], (int)(j * kTile + r));
+                        any_bad = 1;
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(clean(s));
+            }
+        }
+        __syncwarp();
+    } else {
+        registers_up<208>();
+        const uint32_t i = warp / 4, row = row0 + threadIdx.x;  // threads 128 i .. of tile i
+        const uint32_t lanes = (warp % 4 * 32) << 16;
+        const uint32_t scores = tensor + lanes + kScores + i * kTile, output = tensor + lanes + kOutput + i * D;
+        const uint32_t my_steps = i < NT ? steps[i] : 0;
+        const int limit = min((int)m - 1, p.causal ? (int)row + ahead : (int)m - 1);  // the last key that this row sees
+        const int least = min((int)m - 1, p.causal ? (int)(row0 + i * kTile) + ahead : (int)m - 1);
+        float top = -INFINITY, sum = 0.0f;  // top: what the weights so far refer to
+        bool ok = true;
+        for (uint32_t j = 0; j < my_steps; ++j) {
+            ok = __all_sync(~0u, barrier_wait(s_full(i), j & 1));
+            if (!ok) break;
+            tensor_fence_after();
+            float s[kTile];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tensor_load32(scores + 32 * c, s, 32 * c);
+            tensor_wait_load();
+            const int last = limit - (int)(j * kTile);
+            if (least - (int)(j * kTile) < (int)kTile - 1) {
+#pragma unroll
+                for (int c = 0; c < (int)kTile; ++c)
+                    if (c > last) s[c] = -INFINITY;
+            }
+            float most4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int c = 4; c < (int)kTile; c += 4)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) most4[d] = fmaxf(most4[d], s[c + d]);
+            const float now = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
+            if (j == 0) top = now;
+            else {
+                const bool grown = (now - top) * p.scale > kLazy;  // from -infinity too; not where both are
+                if (__any_sync(~0u, grown)) {
+                    const float factor = grown ? exp2_fast((top - now) * p.scale) : 1.0f;
+                    if (grown) top = now;
+                    sum *= factor;
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        tensor_load32(output + c, o, 0);
+                        tensor_wait_load();
+#pragma unroll
+                        for (int d = 0; d < 32; ++d) o[d] *= factor;
+                        tensor_store32(output + c, o, 0);
+                    }
+                }
+            }
+            const float from = top == -INFINITY ? 0.0f : -top * p.scale;
+            float part[2] = {0.0f, 0.0f};
+            uint32_t w[kTile / 2];
+#pragma unroll
+            for (int c = 0; c < (int)kTile; c += 2) {
+                const float a = exp2_fast(fmaf(s[c], p.scale, from)), b = exp2_fast(fmaf(s[c + 1], p.scale, from));
+                part[0] += a;
+                part[1] += b;
+                w[c / 2] = pack2<T>(a, b);
+            }
+            sum += part[0] + part[1];
+            tensor_store32(scores, w, 0);
+            tensor_store32(scores + 32, w, 32);
+            tensor_wait_store();
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(p_full(i));
+        }
+        if (my_steps && ok) ok = __all_sync(~0u, barrier_wait(o_full(i), 0));
+        tensor_fence_after();
+        const bool mine = i < NT && row < n;
+        T* out = static_cast<T*>(p.out) + (uint64_t)(q_first + row) * p.os[0] + h * p.os[1];
+        const float inverse = !ok ? NAN : limit < 0 ? 0.0f : 1.0f / sum;
+        if (i < NT) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                float o[32] = {};
+                __syncwarp();
+                if (my_steps && ok) {
+                    tensor_load32(output + c, o, 0);
+                    tensor_wait_load();
+                }
+                if (!mine) continue;
+                const bool extra = any_bad != 0;
+#pragma unroll
+                for (int d = 0; d < 32; ++d) {
+                    o[d] = limit < 0 ? 0.0f : o[d] * inverse;
+                    if (extra) {
+                        if (first_bad[0][c + d] <= limit) o[d] += INFINITY;
+                        if (first_bad[1][c + d] <= limit) o[d] -= INFINITY;
+                        if (first_bad[2][c + d] <= limit) o[d] = NAN;
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < 32; d += 8) {
+                    if (c + d >= (int)p.head) break;
+                    Few<T, 8> y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y.set2(e, o[d + 2 * e], o[d + 2 * e + 1]);
+                    *reinterpret_cast<uint4*>(out + c + d) = make_uint4(y.w[0], y.w[1], y.w[2], y.w[3]);
+                }
+            }
+        }
+    }
+    tensor_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tensor_fence_after();
+        tensor_free(tensor, 512);
+    }
+}
+
+// The driver's encoder of tiled copies, which the runtime finds.
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                            const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                            CUtensorMapFloatOOBfill);
+Encode encoder() {
+    static const Encode found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return (Encode) nullptr;
+        }
+        return reinterpret_cast<Encode>(f);
+    }();
+    return found;
+}
+
+// Heads [tokens, heads, head] by tiles of 128 tokens and 64 elements; false: not with these strides.
+bool encode(CUtensorMap* map, bool* tokens_last, int dtype, const void* data, uint64_t tokens, uint64_t heads, uint32_t head,
+            const uint64_t (&s)[2]) {
+    // a stride that no coordinate multiplies counts for nothing
+    const uint64_t token = tokens > 1 ? s[0] : std::max<uint64_t>(s[1], head) * heads, hs = heads > 1 ? s[1] : head;
+    if (reinterpret_cast<uintptr_t>(data) % 16 || !token || !hs || token % 8 || hs % 8 || token >> 38 || hs >> 38) return false;
+    *tokens_last = token >= hs;
+    const bool last = *tokens_last;
+    const cuuint64_t dims[3] = {head, last ? heads : tokens, last ? tokens : heads};
+    const cuuint64_t strides[2] = {2 * (last ? hs : token), 2 * (last ? token : hs)};
+    const cuuint32_t box[3] = {64, last ? 1u : kTile, last ? kTile : 1u}, ones[3] = {1, 1, 1};
+    return encoder()(map, dtype == MTXC_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                     const_cast<void*>(data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether the tensor cores take the call; fills the maps.
+bool prepare_maps(int dtype, const mtxc_prompt_attention_args* a, const Prompt& p, Maps* maps) {
+    if (dtype == MTXC_FLOAT || a->head_dim % 8 || !(p.scale > 0.0f && p.scale < INFINITY) || !a->k_tokens || !encoder()) return false;
+    if (reinterpret_cast<uintptr_t>(a->out) % 16 || a->out_strides[0] % 8 || a->out_strides[1] % 8) return false;
+    bool last[3];
+    if (!encode(&maps->q, &last[0], dtype, a->q, a->tokens, a->heads, a->head_dim, a->q_strides) ||
+        !encode(&maps->k, &last[1], dtype, a->k, a->k_tokens, a->kv_heads, a->head_dim, a->k_strides) ||
+        !encode(&maps->v, &last[2], dtype, a->v, a->k_tokens, a->kv_heads, a->head_dim, a->v_strides))
+        return false;
+    maps->tokens_last = last[0] | last[1] << 1 | last[2] << 2;
+    return true;
+}
+
+template <typename T, int D, int NT>
+int launch(const mtxc_prompt_attention_args* a, const Maps& maps, const Prompt& p) {
+    using L = Layout<D, NT>;
+    // the same limit in every call: calls from several threads do not undo each other's
+    cudaError_t err = cudaFuncSetAttribute(prompt_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
+    if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
+    // as many tiles as the sequences can have: one each may be part filled
+    const uint64_t tiles = a->tokens / (NT * kTile) + std::min(a->sequences, a->tokens);
+    if (tiles * a->heads >> 31) return fail(MTXC_ERR_SHAPE, "mtxc_prompt_attention: too many tiles of queries and heads");
+    prompt_kernel<T, D, NT><<<(unsigned)(tiles * a->heads), kThreads, L::kBytes, ctx().stream()>>>(maps, p);
+    return check_launch("prompt_kernel");
+}
+
 }  // namespace
 }  // namespace mtxc
 
@@ -217,6 +624,13 @@ extern "C" int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args
     int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        if constexpr (!std::is_same_v<T, float>) {
+            Maps maps;
+            if (prepare_maps(dtype, a, p, &maps)) {
+                rc = p.head <= 64 ? launch<T, 64, 2>(a, maps, p) : p.head <= 128 ? launch<T, 128, 2>(a, maps, p) : launch<T, 256, 1>(a, maps, p);
+                return;
+            }
+        }
         auto smem = [](uint32_t head) { return sizeof(float) * (2 * kAnyTile * pitch_of(head) + kAnyTile * (kAnyTile + 4)); };
         // the same limit in every call: calls from several threads do not undo each other's
         cudaError_t err = cudaFuncSetAttribute(prompt_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem(kMaxHead));

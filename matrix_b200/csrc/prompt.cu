@@ -184,16 +184,19 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
 // Half types on the tensor cores.
 //
 // A block has NT tiles of 128 queries of one head (NT = 2 for heads of up to 128 elements) and runs along the keys in tiles
-// of 128.  Roles: four warps for each tile of queries, a thread a row, have its softmax; one thread issues the products,
-// one the copies, and two warps clean values (below).  The scores S = Q K' of a tile lie in tensor memory; a row's thread
-// reads them, writes the weights over them in 16 bits, and the product with V takes them from there, so that neither
-// passes through shared memory.  While one tile of queries is with its softmax the tensor cores work for the other:
-//     S0(j)  softmax 0        | P0(j) V(j), S0(j+1)
-//     S1(j)        softmax 1        | P1(j) V(j), S1(j+1)
+// of 128.  Roles: four warps for each tile of queries, a thread a row, have its softmax; one warp issues the products, one
+// the copies, and two clean values (below).  The scores S = Q K' of a tile lie in tensor memory; a row's thread reads
+// them, writes the weights P over them in 16 bits, and the product with V takes them from there, so that neither passes
+// through shared memory.  While one tile of queries is with its softmax the tensor cores work for the other, and the product
+// of the first half of the keys' weights starts while the second half is made:
+//     S0(j)  softmax 0         | P0 V(j), S0(j+1)
+//     S1(j)         softmax 1         | P1 V(j), S1(j+1)
+// (Scores 64 keys at a time, with two places in turn for each tile: 780 us for the two prompts of 8,192 tokens, because a
+// product of 64 columns takes the tensor cores as long as one of 128.)
 //
 // The output is rescaled only where the maximum has grown by more than 2^8 since it last was: until then weights stay below
 // 2^8 (the sums are exact whatever the reference point is), and nearly all tiles keep the first one's.  S(j + 1) is issued
-// behind P(j) V(j), so a thread that sees S(j + 1) may touch the output.
+// behind P V(j), so a thread that sees S(j + 1) may touch the output.
 //
 // What a row does not see gets the weight 0, which is not enough where the value is NaN or infinite (another sequence's
 // row, a later token).  The two cleaning warps look through the tiles of values that some row does not see whole: rows
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
 // element of the head, so that rows that do see it receive it at the end.
 // ------------------------------------------------------------------------------------------
 constexpr int kThreads = 384;
-constexpr uint32_t kTile = 128;
+constexpr uint32_t kTile = 128, kHalf = 64;
 
 struct Maps {
     CUtensorMap q, k, v;
@@ -247,6 +250,35 @@ __device__ __forceinline__ bool all_finite(const uint4& w) {
     }
 }
 
+// 2^x on the multipliers, for a share of the weights: the unit that has the function makes 16 a clock, which is what a tile's
+// two products take.  x = n + f with n whole and |f| <= 1/2; 2^f by the polynomial of least largest relative error that is 1 at
+// 0 (found by exchange of its extrema: 1.0e-4 of degree 3, 3.6e-6 of degree 4, to bfloat16's 2^-9 and float16's 2^-12 of
+// rounding), n added to its exponent.  From -127 down, -infinity and NaN included, exactly 0: 1's exponent less 127.
+#ifndef MTX_POLY
+#define MTX_POLY 2
+#endif
+constexpr int kPolynomial = MTX_POLY;  // of eight pairs
+template <typename T>
+__device__ __forceinline__ float2 exp2_polynomial(float2 x) {
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    const auto two = [](float v) { return make_float2(v, v); };
+    x.x = fmaxf(x.x, -127.0f), x.y = fmaxf(x.y, -127.0f);
+    const float2 t = __fadd2_rn(x, two(12582912.0f));  // 1.5 * 2^23: the whole part in the last bits
+    const float2 f = __fadd2_rn(x, __ffma2_rn(t, two(-1.0f), two(12582912.0f)));
+    float2 y;
+    if constexpr (kBf16) {
+        y = __ffma2_rn(f, two(0.05500893294811249f), two(0.24221095442771912f));
+        y = __ffma2_rn(f, y, two(0.6932829022407532f));
+    } else {
+        y = __ffma2_rn(f, two(0.009782912209630013f), two(0.055976882576942444f));
+        y = __ffma2_rn(f, y, two(0.24020710587501526f));
+        y = __ffma2_rn(f, y, two(0.6931136250495911f));
+    }
+    y = __ffma2_rn(f, y, two(1.0f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Maps maps, const Prompt p) {
     using L = Layout<D, NT>;
@@ -257,9 +289,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     __shared__ uint64_t buf[33];
     __shared__ Found found;
     __shared__ uint32_t tensor_base;
-    __shared__ alignas(8) uint64_t bars[2 + 4 * kSlots + 3 * NT];
+    __shared__ alignas(8) uint64_t bars[2 + 4 * kSlots + 4 * NT];
     __shared__ int first_bad[3][D];  // the first key with +infinity, -infinity, NaN in an element
-    __shared__ int any_bad;
+    __shared__ int any_bad, failed;
+    auto wait = [&](uint32_t bar, uint32_t parity) { barrier_wait(bar, parity, &failed); };
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles = (shared_address(dynamic) + 1023) / 1024 * 1024;
     auto q_tile = [&](uint32_t i) { return tiles + i * L::kTileBytes; };
@@ -271,8 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto raw = [&](uint32_t s) { return bar0 + 8 * (2 + 2 * kSlots + s); };  // values that are to be cleaned
     auto clean = [&](uint32_t s) { return bar0 + 8 * (2 + 3 * kSlots + s); };
     auto s_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + i); };
-    auto p_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + NT + i); };
-    auto o_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + 2 * NT + i); };
+    auto p_full = [&](uint32_t i, uint32_t half) { return bar0 + 8 * (2 + 4 * kSlots + NT + 2 * i + half); };
+    auto o_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + 3 * NT + i); };
 
     // the last sequence first, and in each the last tile first: of causal ones the longest; all heads of a tile in turn
     constexpr uint32_t kRows = NT * kTile;
@@ -307,9 +340,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (threadIdx.x == 32) {
         for (uint32_t i = 0; i < 2; ++i) barrier_init(q_full(i), 1);
         for (uint32_t s = 0; s < kSlots; ++s) barrier_init(full(s), 1), barrier_init(empty(s), 1), barrier_init(raw(s), 1), barrier_init(clean(s), 2);
-        for (uint32_t i = 0; i < NT; ++i) barrier_init(s_full(i), 1), barrier_init(p_full(i), 4), barrier_init(o_full(i), 1);
+        for (uint32_t i = 0; i < NT; ++i)
+            barrier_init(s_full(i), 1), barrier_init(p_full(i, 0), 4), barrier_init(p_full(i, 1), 4), barrier_init(o_full(i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        any_bad = 0;
+        any_bad = failed = 0;
     }
     for (uint32_t e = threadIdx.x; e < 3 * D; e += kThreads) (&first_bad[0][0])[e] = 0x7FFFFFFF;
     tensor_fence_before();
@@ -319,77 +353,77 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (warp >= 8) {
         registers_down<88>();
-        if (warp == 8 && lane == 0) {  // copies
+        if (warp == 8) {  // copies
             auto load = [&](uint32_t to, uint32_t bar, const CUtensorMap* map, bool token_last, uint32_t token, uint32_t head) {
                 barrier_expect(bar, L::kTileBytes);
                 for (uint32_t x = 0; x < D / 64; ++x)
                     copy_tile(to + x * L::kRowTile, map, bar, (int)(x * 64), (int)(token_last ? head : token), (int)(token_last ? token : head));
             };
-            bool ok = true;
-            uint32_t item = 0;
-            for (; item < 2 * most; ++item) {
+            if (elected()) for (uint32_t item = 0; item < 2 * most; ++item) {
                 const uint32_t j = item / 2, kv = item % 2, s = item % kSlots, use = item / kSlots;
-                if (use) ok = barrier_wait(empty(s), (use - 1) & 1);
-                if (!ok) break;
+                if (use) wait(empty(s), (use - 1) & 1);
                 if (item == 0 && steps[0]) load(q_tile(0), q_full(0), &maps.q, maps.tokens_last & 1, q_first + row0, h);
                 load(slot(s), kv && j >= partial ? raw(s) : full(s), kv ? &maps.v : &maps.k, maps.tokens_last >> (1 + kv) & 1,
                      k_first + j * kTile, kh);
                 if (NT == 2 && item == 0 && steps[1]) load(q_tile(1), q_full(1), &maps.q, maps.tokens_last & 1, q_first + row0 + kTile, h);
             }
-            // where a wait has run out, the copies under way end before the block does
-            for (uint32_t i = item > kSlots ? item - kSlots : 0; !ok && i < item; ++i) {
-                const uint32_t j = i / 2, s = i % kSlots;
-                if (i % 2 && j >= partial) barrier_wait(raw(s), (j - partial) / (kSlots / 2) & 1);
-                else barrier_wait(full(s), i / kSlots & 1);
-            }
-        } else if (warp == 9 && lane == 0) {  // products
+            // every copy ends before the block does, even where a wait has run out
+            for (uint32_t item = 2 * most - min(2 * most, kSlots); failed && item < 2 * most; ++item)
+                for (uint32_t i = 0; i < 1000 && !barrier_try(full(item % kSlots), item / kSlots & 1); ++i) {}
+            __syncwarp();
+        } else if (warp == 9) {  // products
             constexpr uint32_t kScore = product_descriptor(kBf16, kTile, kTile, false), kValue = product_descriptor(kBf16, kTile, D, true);
             auto scores = [&](uint32_t i, uint32_t j) {
-                const uint32_t k = slot(2 * j % kSlots), q = q_tile(i);
+                const uint64_t k = tile_descriptor(slot(2 * j % kSlots), 1024, 16), q = tile_descriptor(q_tile(i), 1024, 16);
 #pragma unroll
                 for (uint32_t d = 0; d < D / 16; ++d) {
-                    const uint32_t off = d / 4 * L::kRowTile + d % 4 * 32;
-                    product(tensor + kScores + i * kTile, tile_descriptor(q + off, 1024, 16), tile_descriptor(k + off, 1024, 16), kScore, d > 0);
+                    const uint32_t off = (d / 4 * L::kRowTile + d % 4 * 32) / 16;
+                    product(tensor + kScores + i * kTile, q + off, k + off, kScore, d > 0);
                 }
                 product_commit(s_full(i));
             };
-            bool ok = true;
-            auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && barrier_wait(bar, parity); };
             if (most) wait(full(0), 0);
-            for (uint32_t i = 0; i < NT && ok; ++i) {
+            for (uint32_t i = 0; i < NT; ++i) {
                 if (!steps[i]) continue;
                 wait(q_full(i), 0);
-                if (ok) scores(i, 0);
+                __syncwarp();
+                if (elected()) scores(i, 0);
             }
-            if (most && ok) product_commit(empty(0));
-            for (uint32_t j = 0; j < most && ok; ++j) {
-                const uint32_t item = 2 * j + 1, s = item % kSlots;
-                if (j < partial) wait(full(s), item / kSlots & 1);
+            __syncwarp();
+            if (most && elected()) product_commit(empty(0));
+            for (uint32_t j = 0; j < most; ++j) {
+                const uint32_t s = (2 * j + 1) % kSlots;
+                if (j < partial) wait(full(s), (2 * j + 1) / kSlots & 1);
                 else wait(clean(s), (j - partial) / (kSlots / 2) & 1);
-                for (uint32_t i = 0; i < NT && ok; ++i) {
-                    if (j >= steps[i]) continue;
-                    wait(p_full(i), j & 1);
-                    if (!ok) break;
-                    tensor_fence_after();
+                if (j + 1 < most) wait(full((2 * j + 2) % kSlots), (2 * j + 2) / kSlots & 1);
+                const uint64_t v = tile_descriptor(slot(s), 1024, L::kRowTile);
 #pragma unroll
-                    for (uint32_t d = 0; d < kTile / 16; ++d)
-                        product(tensor + kOutput + i * D, tensor + kScores + i * kTile + d * 8, tile_descriptor(slot(s) + d * 2048, 1024, L::kRowTile),
-                                kValue, j > 0 || d > 0);
-                    if (j + 1 < steps[i]) {
-                        wait(full((item + 1) % kSlots), (item + 1) / kSlots & 1);
-                        if (ok) scores(i, j + 1);
-                    } else product_commit(o_full(i));
+                for (uint32_t i = 0; i < NT; ++i) {
+                    if (j >= steps[i]) continue;
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; ++half) {
+                        wait(p_full(i, half), j & 1);
+                        __syncwarp();
+                        tensor_fence_after();
+                        if (elected()) {
+#pragma unroll
+                            for (uint32_t d = half * 4; d < half * 4 + 4; ++d)
+                                product(tensor + kOutput + i * D, tensor + kScores + i * kTile + d * 8, v + d * (2048 / 16), kValue, j > 0 || d > 0);
+                            if (half && j + 1 < steps[i]) scores(i, j + 1);
+                            else if (half) product_commit(o_full(i));
+                        }
+                    }
                 }
-                if (!ok) break;
-                product_commit(empty(s));
-                if (j + 1 < most) product_commit(empty((item + 1) % kSlots));
+                __syncwarp();
+                if (elected()) {
+                    product_commit(empty(s));
+                    if (j + 1 < most) product_commit(empty((2 * j + 2) % kSlots));
+                }
             }
         } else if (warp >= 10) {  // values
-            bool ok = true;
-            for (uint32_t j = partial; j < most && ok; ++j) {
+            for (uint32_t j = partial; j < most; ++j) {
                 const uint32_t s = (2 * j + 1) % kSlots, rows = min(kTile, m - j * kTile);
-                ok = __all_sync(~0u, barrier_wait(raw(s), (j - partial) / (kSlots / 2) & 1));
-                if (!ok) break;
+                wait(raw(s), (j - partial) / (kSlots / 2) & 1);
                 for (uint32_t e = threadIdx.x - 320; e < kTile * (D / 8); e += 64) {
                     const uint32_t r = e / (D / 8), c = e % (D / 8);  // 16-byte units: eight elements
                     const uint32_t at = slot(s) + c / 8 * L::kRowTile + r * 128 + (c % 8 ^ r % 8) * 16;
@@ -420,19 +454,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         registers_up<208>();
         const uint32_t i = warp / 4, row = row0 + threadIdx.x;  // threads 128 i .. of tile i
         const uint32_t lanes = (warp % 4 * 32) << 16;
-        const uint32_t scores = tensor + lanes + kScores + i * kTile, output = tensor + lanes + kOutput + i * D;
+        const uint32_t output = tensor + lanes + kOutput + i * D;
         const uint32_t my_steps = i < NT ? steps[i] : 0;
         const int limit = min((int)m - 1, p.causal ? (int)row + ahead : (int)m - 1);  // the last key that this row sees
         const int least = min((int)m - 1, p.causal ? (int)(row0 + i * kTile) + ahead : (int)m - 1);
         float top = -INFINITY, sum = 0.0f;  // top: what the weights so far refer to
-        bool ok = true;
+        const uint32_t scores = tensor + lanes + kScores + i * kTile;
         for (uint32_t j = 0; j < my_steps; ++j) {
-            ok = __all_sync(~0u, barrier_wait(s_full(i), j & 1));
-            if (!ok) break;
+            wait(s_full(i), j & 1);
+            __syncwarp();
             tensor_fence_after();
             float s[kTile];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tensor_load32(scores + 32 * c, s, 32 * c);
+            for (int c = 0; c < (int)kTile; c += 32) tensor_load32(scores + c, s, c);
             tensor_wait_load();
             const int last = limit - (int)(j * kTile);
             if (least - (int)(j * kTile) < (int)kTile - 1) {
@@ -440,14 +474,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 for (int c = 0; c < (int)kTile; ++c)
                     if (c > last) s[c] = -INFINITY;
             }
+            // a NaN among the scores stays: it is not for the polynomial to show it
             float most4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 4; c < (int)kTile; c += 4)
+            for (int c = 4; c < (int)kTile - 4; c += 8)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) most4[d] = fmaxf(most4[d], s[c + d]);
-            const float now = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-            if (j == 0) top = now;
-            else {
+                for (int d = 0; d < 4; ++d) most4[d] = max3(most4[d], s[c + d], s[c + 4 + d]);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) most4[d] = max3(most4[d], s[kTile - 4 + d], most4[d]);
+            const float now = max3(max3(most4[0], most4[1], most4[2]), most4[3], most4[3]);
+            if (j == 0 || now != now) top = now;
+            if (j) {
                 const bool grown = (now - top) * p.scale > kLazy;  // from -infinity too; not where both are
                 if (__any_sync(~0u, grown)) {
                     const float factor = grown ? exp2_fast((top - now) * p.scale) : 1.0f;
@@ -465,34 +502,38 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
             const float from = top == -INFINITY ? 0.0f : -top * p.scale;
-            float part[2] = {0.0f, 0.0f};
-            uint32_t w[kTile / 2];
+            float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            const float2 scale2 = make_float2(p.scale, p.scale), from2 = make_float2(from, from);
 #pragma unroll
-            for (int c = 0; c < (int)kTile; c += 2) {
-                const float a = exp2_fast(fmaf(s[c], p.scale, from)), b = exp2_fast(fmaf(s[c + 1], p.scale, from));
-                part[0] += a;
-                part[1] += b;
-                w[c / 2] = pack2<T>(a, b);
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[kHalf / 2];
+#pragma unroll
+                for (int c = 0; c < (int)kHalf; c += 2) {
+                    const float2 x = __ffma2_rn(make_float2(s[half * kHalf + c], s[half * kHalf + c + 1]), scale2, from2);
+                    const float2 y = c / 2 % 8 < kPolynomial ? exp2_polynomial<T>(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                    part[c / 2 % 2] = __fadd2_rn(part[c / 2 % 2], y);
+                    w[c / 2] = pack2<T>(y.x, y.y);
+                }
+                tensor_store32(scores + half * (kHalf / 2), w, 0);
+                tensor_wait_store();
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(p_full(i, half));
             }
-            sum += part[0] + part[1];
-            tensor_store32(scores, w, 0);
-            tensor_store32(scores + 32, w, 32);
-            tensor_wait_store();
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(p_full(i));
+            sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         }
-        if (my_steps && ok) ok = __all_sync(~0u, barrier_wait(o_full(i), 0));
+        if (my_steps) wait(o_full(i), 0);
+        __syncwarp();
         tensor_fence_after();
         const bool mine = i < NT && row < n;
         T* out = static_cast<T*>(p.out) + (uint64_t)(q_first + row) * p.os[0] + h * p.os[1];
-        const float inverse = !ok ? NAN : limit < 0 ? 0.0f : 1.0f / sum;
+        const float inverse = failed ? NAN : limit < 0 ? 0.0f : 1.0f / sum;
         if (i < NT) {
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 float o[32] = {};
                 __syncwarp();
-                if (my_steps && ok) {
+                if (my_steps) {
                     tensor_load32(output + c, o, 0);
                     tensor_wait_load();
                 }

@@ -10,6 +10,14 @@ namespace mtxc {
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// True in one thread of a converged warp, the same one each time.  The compiler knows it for one thread: behind a
+// comparison of lanes it wraps each product in a loop over the lanes that might be there.
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // ------------------------------------------------------------------------------------------
 // Barriers
 // ------------------------------------------------------------------------------------------
@@ -22,20 +30,24 @@ __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for the phase of this parity to end; false: it did not within some seconds (each try itself waits a while).
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < 1u << 20; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {  // the hardware waits a while itself
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// Waits for the phase of this parity to end.  Where it does not within some seconds, *failed is set, and no thread waits
+// for anything any more: the block runs to its end, with outputs that count for nothing.
+__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+    if (barrier_try(bar, parity)) return;
+    for (uint32_t i = 0; i < 1u << 20; ++i)
+        if (barrier_try(bar, parity) || *failed) return;
+    *failed = 1;
 }
 // What threads have written to shared memory becomes visible to copies and products.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -131,6 +143,11 @@ __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sy
 template <int N>
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN where one of them is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -64,7 +64,7 @@ struct Found {
     bool any;        // false: there are not so many pieces
 };
 
-// The pieces of sequences 0 .. n - 1, added by the whole block (of at most 1,024 threads; buf: 33 words).
+// The pieces of sequences 0 .. n - 1, added by the whole block (buf: a word for each of its warps).
 template <typename Fn>
 __device__ __forceinline__ uint64_t total_of(uint32_t n, Fn&& count, uint64_t* buf) {
     uint64_t sum = 0;

@@ -215,7 +215,8 @@ template <int D, int NT>
 struct Layout {
     static constexpr uint32_t kRowTile = kTile * 128;             // 64 elements of 128 rows
     static constexpr uint32_t kTileBytes = kRowTile * (D / 64);
-    static constexpr uint32_t kSlots = D == 256 ? 2 : 4;          // keys and values in turn
+    static constexpr uint32_t kSlots = D == 256 ? 2 : D == 128 ? 5 : 8;  // keys and values in turn
+    static constexpr uint32_t kAgain = kSlots % 2 ? kSlots : kSlots / 2;  // tiles from one whose values have a slot to the next
     static constexpr uint32_t kBytes = kTileBytes * (NT + kSlots) + 1024;  // the tiles start at a multiple of 1,024
 };
 
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     constexpr float kLazy = 8.0f;
     extern __shared__ uint8_t dynamic[];
-    __shared__ uint64_t buf[33];
+    __shared__ uint64_t buf[kThreads / 32];
     __shared__ Found found;
     __shared__ uint32_t tensor_base;
     __shared__ alignas(8) uint64_t bars[2 + 4 * kSlots + 4 * NT];
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (uint32_t j = 0; j < most; ++j) {
                 const uint32_t s = (2 * j + 1) % kSlots;
                 if (j < partial) wait(full(s), (2 * j + 1) / kSlots & 1);
-                else wait(clean(s), (j - partial) / (kSlots / 2) & 1);
+                else wait(clean(s), (j - partial) / L::kAgain & 1);
                 if (j + 1 < most) wait(full((2 * j + 2) % kSlots), (2 * j + 2) / kSlots & 1);
                 const uint64_t v = tile_descriptor(slot(s), 1024, L::kRowTile);
 #pragma unroll
@@ -409,21 +410,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
                             for (uint32_t d = half * 4; d < half * 4 + 4; ++d)
                                 product(tensor + kOutput + i * D, tensor + kScores + i * kTile + d * 8, v + d * (2048 / 16), kValue, j > 0 || d > 0);
+                            if (half && j + 1 == steps[i]) product_commit(o_full(i));
+                            if (half && (i + 1 == NT || j >= steps[NT - 1])) product_commit(empty(s));
                             if (half && j + 1 < steps[i]) scores(i, j + 1);
-                            else if (half) product_commit(o_full(i));
                         }
                     }
                 }
                 __syncwarp();
-                if (elected()) {
-                    product_commit(empty(s));
-                    if (j + 1 < most) product_commit(empty((2 * j + 2) % kSlots));
-                }
+                if (j + 1 < most && elected()) product_commit(empty((2 * j + 2) % kSlots));
             }
         } else if (warp >= 10) {  // values
             for (uint32_t j = partial; j < most; ++j) {
                 const uint32_t s = (2 * j + 1) % kSlots, rows = min(kTile, m - j * kTile);
-                wait(raw(s), (j - partial) / (kSlots / 2) & 1);
+                wait(raw(s), (j - partial) / L::kAgain & 1);
                 for (uint32_t e = threadIdx.x - 320; e < kTile * (D / 8); e += 64) {
                     const uint32_t r = e / (D / 8), c = e % (D / 8);  // 16-byte units: eight elements
                     const uint32_t at = slot(s) + c / 8 * L::kRowTile + r * 128 + (c % 8 ^ r % 8) * 16;

@@ -110,4 +110,35 @@ __device__ __forceinline__ Found find(uint32_t n, uint64_t target, Fn&& count, u
     return *found;
 }
 
+// The same for a warp by itself.
+template <typename Fn>
+__device__ __forceinline__ uint64_t warp_total(uint32_t n, Fn&& count) {
+    uint64_t sum = 0;
+    for (uint32_t i = threadIdx.x % 32; i < n; i += 32) sum += count(i);
+#pragma unroll
+    for (int m = 16; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+    return sum;
+}
+template <typename Fn>
+__device__ __forceinline__ Found warp_find(uint32_t n, uint64_t target, Fn&& count) {
+    const uint32_t lane = threadIdx.x % 32;
+    uint64_t before = 0;
+    for (uint32_t base = 0; base < n; base += 32) {
+        const uint64_t mine = base + lane < n ? count(base + lane) : 0;
+        uint64_t sum = mine;
+#pragma unroll
+        for (int m = 1; m < 32; m *= 2) {
+            const uint64_t v = __shfl_up_sync(~0u, sum, m);
+            if (lane >= (uint32_t)m) sum += v;
+        }
+        const uint32_t passed = __ballot_sync(~0u, before + sum > target);
+        if (passed) {
+            const int l = __ffs((int)passed) - 1;
+            return Found{base + l, before + __shfl_sync(~0u, sum - mine, l), true};
+        }
+        before += __shfl_sync(~0u, sum, 31);
+    }
+    return Found{0, 0, false};
+}
+
 }  // namespace mtxc

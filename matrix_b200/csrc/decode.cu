@@ -2,10 +2,11 @@
 //
 //   o = sum_j w_j v_j / sum_j w_j,  w_j = 2^(s_j - m),  s_j = scale log2(e) q . k_j,  m a running maximum
 //
-// The keys and values are read once: bound by HBM.  The work -- a tile of keys for each key head and each 16 of its query
-// heads, of all sequences one after another -- is shared out evenly over a fixed number of blocks, whatever the lengths are
-// (which only the device knows).  A unit (sequence, heads) that lies within one block is written there; of one that blocks
-// share, each leaves its sums and maxima in the workspace, and a second launch joins them in order.
+// The keys and values are read once: bound by HBM.  The work -- tiles of keys for each key head and each 16 of its query
+// heads, of all sequences one after another -- is shared out evenly over a fixed number of workers (warps; blocks of the
+// kernel for any head), whatever the lengths are, which only the device knows.  A unit (sequence, heads) that lies within one
+// worker is written there; of one that workers share, each leaves its sums and maxima in the workspace, and a second launch
+// joins them in order.
 #include <algorithm>
 #include <cmath>
 
@@ -22,7 +23,8 @@ constexpr float kLowest = -3.402823466e+38f;
 
 struct Decode {
     Cache cache;
-    uint32_t batch, heads, kv_heads, group, groups, units, head, max_pages, tile, blocks;  // groups: of 16 query heads
+    uint32_t batch, heads, kv_heads, group, groups, units, head, max_pages, tile, workers;  // groups: of 16 query heads
+    FastDiv groups_div;
     const void* q;
     void* out;
     uint64_t qs[2], os[2];
@@ -30,7 +32,9 @@ struct Decode {
     uint64_t table_stride;
     const int* lengths;
     float scale;      // times log2(e)
-    float* partial;   // [2 * blocks][kRows][head + 2]: sums, maximum, sum of weights
+    bool vector;      // the kernel of 16-byte units
+    float* partial;   // [2 * workers][rows][head + 2]: sums, maximum, sum of weights
+    uint32_t rows;    // of a unit
 };
 
 __device__ __forceinline__ uint32_t length_of(const Decode& d, uint32_t b) {
@@ -39,8 +43,13 @@ __device__ __forceinline__ uint32_t length_of(const Decode& d, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t tiles_of(const Decode& d, uint32_t b) { return (length_of(d, b) + d.tile - 1) / d.tile; }
 
-// The blocks that share the work: each has some.
-__device__ __forceinline__ uint64_t sharing(const Decode& d, uint64_t work) { return min(work, (uint64_t)d.blocks); }
+// The workers that share the work: each has some.
+__device__ __forceinline__ uint64_t sharing(const Decode& d, uint64_t work) { return min(work, (uint64_t)d.workers); }
+
+// Where a worker leaves its part of a unit: one that it begins (and another worker ends), or one that was begun before.
+__device__ __forceinline__ float* part_of(const Decode& d, uint64_t worker, bool begins) {
+    return d.partial + (2 * worker + begins) * d.rows * (d.head + 2);
+}
 
 // The page and slot of key j of sequence b; false: the table names no page of the cache.
 __device__ __forceinline__ bool place_of(const Decode& d, uint32_t b, uint32_t j, uint32_t& page, uint32_t& slot) {
@@ -52,7 +61,7 @@ __device__ __forceinline__ bool place_of(const Decode& d, uint32_t b, uint32_t j
 
 // Rows of a unit: query heads first .. first + count - 1.
 __device__ __forceinline__ uint32_t rows_of(const Decode& d, uint32_t unit, uint32_t& head, uint32_t& first) {
-    head = unit / d.groups;
+    head = d.groups_div.div(unit);
     const uint32_t g = unit - head * d.groups;
     first = head * d.group + g * kRows;
     return min(kRows, d.group - g * kRows);
@@ -164,7 +173,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
         }
         __syncthreads();
         const bool whole = tile0 == 0 && tile == tiles;
-        float* const part = d.partial + (2ull * blockIdx.x + (tile0 == 0)) * kRows * (d.head + 2);
+        float* const part = part_of(d, blockIdx.x, tile0 == 0);
         if (column < d.head) {
 #pragma unroll
             for (uint32_t i = 0; i < kRows; ++i) {
@@ -188,42 +197,462 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
     }
 }
 
-// Joins the parts of a row that blocks share: block (query head, sequence), a thread a column.  A sequence without keys
+// ------------------------------------------------------------------------------------------
+// Half types, and caches in 8 bits under half queries, by 16-byte units.
+//
+// A warp works by itself: it copies the keys and values of its tile (16 of a half type, 32 of 8 bits) into a ring of its own
+// in shared memory, kStages ahead of use (192 KB an SM in flight and in use), and multiplies them on the tensor cores, 16
+// rows of queries (those that a unit lacks are zeros) x 16 or 32 keys: they pass once, and 16 rows cost what one does.  There is no
+// barrier between warps, and the copies run on across the borders of units and sequences.  The page numbers of a tile are
+// loaded one tile before its copies are issued.
+//
+// In 8 bits the bytes become float16, which holds them exactly, beside queries as float16 of a magnitude below 2 (their rows'
+// powers of two, like the keys' scales, come back into the scores).  The values' scales 2^e go into the weights: those are
+// 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are, and the weights that are summed
+// for the denominator 2^(s - m).
+// ------------------------------------------------------------------------------------------
+constexpr int kStages = 3;
+
+constexpr uint32_t warps_of(uint32_t steps) { return steps > 8 ? 4 : 8; }  // a ring of 24 to 26 or 50 KB each
+uint32_t steps_of(uint32_t head) {  // of 16 elements, as the kernel is built for
+    for (uint32_t s : {4u, 5u, 6u, 8u, 12u})
+        if (head <= 16 * s) return s;
+    return 16;
+}
+
+template <int STEPS, bool SMALL>
+struct Ring {
+    static constexpr uint32_t kKeys = SMALL ? 32 : 16;
+    static constexpr uint32_t kUnits = SMALL ? STEPS : 2 * STEPS;     // 16-byte units of a row
+    static constexpr uint32_t kPitch = (kUnits | 1) * 16;             // an odd number of them: rows in different banks
+    static constexpr uint32_t kSide = kKeys * kPitch, kStage = 2 * kSide;
+    static constexpr uint32_t kWarp = kStages * (kStage + 128);       // the last: which keys count, and their exponents
+    static constexpr uint32_t kBytes = warps_of(STEPS) * kWarp;
+};
+
+__device__ __forceinline__ void matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void matrices_turned(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    Few<T, 4> f;
+    f.set2(0, a, b);
+    return f.w[0];
+}
+__device__ __forceinline__ uint32_t halves_of(uint32_t bytes) {  // two bytes of e4m3 as two float16
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)bytes, __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float power(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A place in the stream of tiles.
+struct Place {
+    uint32_t b, unit, tile, tiles, length;
+    __device__ __forceinline__ void next(const Decode& d) {  // there is one
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++unit < d.units) return;
+        unit = 0;
+        do {
+            ++b;
+            length = length_of(d, b);
+            tiles = (length + d.tile - 1) / d.tile;
+        } while (tiles == 0);
+    }
+};
+
+template <typename T, int STEPS, bool SMALL>
+__global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(const Decode d) {
+    using R = Ring<STEPS, SMALL>;
+    using M = std::conditional_t<SMALL, __half, T>;  // the products' type
+    constexpr uint32_t kKeys = R::kKeys, kTiles = kKeys / 8;
+    extern __shared__ uint4 smem4[];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem4) + warp * R::kWarp;
+    uint32_t* const notes = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(smem4) + warp * R::kWarp + kStages * R::kStage);
+    auto count = [&](uint32_t b) { return (uint64_t)tiles_of(d, b) * d.units; };
+    const uint64_t work = warp_total(d.batch, count), workers = sharing(d, work);
+    const uint64_t worker = (uint64_t)warp * gridDim.x + blockIdx.x;  // little work: one warp of each block first
+    if (worker >= workers) return;
+    uint64_t left = work * (worker + 1) / workers - work * worker / workers;
+    Place now;
+    {
+        const uint64_t first = work * worker / workers;
+        const Found f = warp_find(d.batch, first, count);
+        now.b = f.i;
+        now.length = length_of(d, f.i);
+        now.tiles = (now.length + kKeys - 1) / kKeys;
+        now.unit = (uint32_t)((first - f.first) / now.tiles);
+        now.tile = (uint32_t)((first - f.first) - (uint64_t)now.unit * now.tiles);
+    }
+    // elements that the heads lack stay zeros: no copy reaches them
+    for (uint32_t i = lane; i < kStages * R::kStage / 16; i += 32)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i * 16), "r"(0) : "memory");
+    __syncwarp();
+
+    // the tile to be copied next: its page, slot and head (a lane a key), and what is left to look at
+    Place ahead = now;
+    uint64_t unseen = left;
+    uint32_t page = ~0u, slot = 0, head = 0;
+    auto look = [&]() {
+        page = ~0u;
+        if (unseen == 0) return;
+        --unseen;
+        const uint32_t key = ahead.tile * kKeys + lane;
+        head = d.groups_div.div(ahead.unit);
+        if (lane < kKeys && key < ahead.length) {
+            uint32_t i;
+            d.cache.page_div.divmod(key, i, slot);
+            page = (uint32_t)d.table[ahead.b * d.table_stride + i];
+        }
+        if (unseen) ahead.next(d);
+    };
+    const uint32_t units = d.head * (SMALL ? 1 : 2) / 16;  // of a row that are copied
+    uint32_t note = 0, note_to = 0;  // on its way to stage note_to
+    auto copy = [&](uint32_t stage) {
+        const bool ok = page < d.cache.pages;
+        uint64_t from[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const CacheSide& c = d.cache.side[k];
+            from[k] = ok ? (page * c.s[0] + slot * c.s[1] + head * c.s[2]) * (SMALL ? 1 : 2) : ~0ull;
+        }
+        notes[note_to * 32 + lane] = note;  // that of the tile before has come
+        note = ok;
+        if constexpr (SMALL)
+            if (ok) {
+                const CacheSide &c = d.cache.side[0], &v = d.cache.side[1];
+                const int8_t key = c.exponents[page * c.es[0] + slot * c.es[1] + head * c.es[2]];
+                const int8_t value = v.exponents[page * v.es[0] + slot * v.es[1] + head * v.es[2]];
+                note = 1u | (uint32_t)(uint8_t)key << 8 | (uint32_t)(uint8_t)value << 16;
+            }
+        note_to = stage;
+        // lanes side by side along a row, and rows in turn
+        const uint32_t to = ring + stage * R::kStage;
+#pragma unroll
+        for (uint32_t e = 0; e < kKeys * R::kUnits; e += 32) {
+            const uint32_t i = e + lane, row = i / R::kUnits, unit = i - row * R::kUnits;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint64_t at = __shfl_sync(~0u, from[k], row);
+                const void* src = static_cast<const uint8_t*>(d.cache.side[k].data) + (at == ~0ull ? 0 : at + unit * 16);
+                if (unit < units)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * R::kSide + row * R::kPitch + unit * 16), "l"(src),
+                                 "r"(at == ~0ull ? 0 : 16)
+                                 : "memory");
+            }
+        }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    look();
+    for (uint32_t s = 0; s + 1 < kStages; ++s) {
+        copy(s);
+        commit();
+        look();
+    }
+
+    uint32_t stage = 0;
+    while (left) {
+        // a unit, as far as this worker has it
+        uint32_t h, first;
+        const uint32_t rows = rows_of(d, now.unit, h, first), b = now.b, tile0 = now.tile, tiles = now.tiles;
+        uint32_t q[STEPS][4];
+        float factor[2] = {d.scale, d.scale};
+        {
+            // row r of the first operand: the registers' elements 2 t, 2 t + 1 and 8 further (of 8 bits: 4 t .. 4 t + 3, as a
+            // thread finds four bytes of a key side by side)
+            const T* base = static_cast<const T*>(d.q) + b * d.qs[0] + first * d.qs[1];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t row = g + 8 * r;
+                const T* x = base + row * d.qs[1];
+                if constexpr (!SMALL) {
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t c = 16 * s + 8 * e + 2 * t;
+                            const bool there = row < rows && c < d.head;
+                            q[s][r + 2 * e] = there ? pack2<T>(to_float(x[c]), to_float(x[c + 1])) : 0u;
+                        }
+                } else {
+                    uint32_t top = 0;
+                    float v[STEPS][4];
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t c = 16 * s + 4 * t + e;
+                            v[s][e] = row < rows && c < d.head ? to_float(x[c]) : 0.0f;
+                            const uint32_t bits = __float_as_uint(v[s][e]) & 0x7FFFFFFFu;
+                            top = max(top, bits < 0x7F800000u ? bits : 0u);
+                        }
+                    top = max(top, __shfl_xor_sync(~0u, top, 1));
+                    top = max(top, __shfl_xor_sync(~0u, top, 2));
+                    const int e = top ? max(-126, min(126, (int)(top >> 23) - 127)) : 0;
+                    factor[r] *= power_of_two(e);
+                    const float down = power_of_two(-e);
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) q[s][r + 2 * i] = pack2<__half>(v[s][2 * i] * down, v[s][2 * i + 1] * down);
+                }
+            }
+        }
+        float o[2 * STEPS][4];
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        bool ends, done;  // done: with the unit's last tile
+        do {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncwarp();
+            // this tile has come; the one after those on their way goes where the last one was
+            copy(stage == 0 ? kStages - 1 : stage - 1);
+            commit();
+            look();
+            const uint32_t keys = ring + stage * R::kStage, values = keys + R::kSide;
+            float s[kTiles][4];
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < STEPS; ++c) {
+                uint32_t r[4];
+                if constexpr (!SMALL) {
+                    matrices(r, keys + (lane / 16 * 8 + lane % 8) * R::kPitch + (2 * c + lane / 8 % 2) * 16);
+                    multiply<M>(s[0], q[c], r[0], r[1]);
+                    multiply<M>(s[1], q[c], r[2], r[3]);
+                } else {
+                    matrices(r, keys + lane * R::kPitch + c * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) multiply<M>(s[i], q[c], halves_of(r[i] & 0xFFFFu), halves_of(r[i] >> 16));
+                }
+            }
+            // scores in powers of two; a key that counts lifts the maximum off -infinity even where its score is
+            const uint32_t mine = notes[stage * 32 + lane], counting = __ballot_sync(~0u, mine & 1);
+            float most[2] = {-INFINITY, -INFINITY}, shift[kTiles][2];  // shift: the values' scales
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t key = 8 * i + 2 * t + e;
+                    const bool counts = counting >> key & 1;
+                    float scale = 1.0f;
+                    shift[i][e] = 0.0f;
+                    if constexpr (SMALL) {
+                        const uint32_t x = __shfl_sync(~0u, mine, key);
+                        scale = power_of_two((int8_t)(x >> 8 & 0xFFu));
+                        shift[i][e] = (float)(int8_t)(x >> 16 & 0xFFu);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float& x = s[i][2 * r + e];
+                        x = counts ? x * (factor[r] * scale) : -INFINITY;
+                        if (counts) most[r] = fmaxf(most[r], fmaxf(x + shift[i][e], kLowest));
+                    }
+                }
+            bool grown = false;
+            float old[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                most[r] = fmaxf(most[r], __shfl_xor_sync(~0u, most[r], 1));
+                most[r] = fmaxf(most[r], __shfl_xor_sync(~0u, most[r], 2));
+                old[r] = top[r];
+                top[r] = fmaxf(top[r], most[r]);
+                grown = grown || top[r] != old[r];
+            }
+            if (__any_sync(~0u, grown)) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float by = top[r] == old[r] ? 1.0f : power(old[r] - top[r]);
+                    sum[r] *= by;
+#pragma unroll
+                    for (int i = 0; i < 2 * STEPS; ++i) o[i][2 * r] *= by, o[i][2 * r + 1] *= by;
+                }
+            }
+            uint32_t w[kTiles / 2][4];
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float from = top[r] == -INFINITY ? 0.0f : top[r];
+                    float v[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = s[i][2 * r + e];
+                        v[e] = power(x + (shift[i][e] - from));
+                        sum[r] += SMALL ? power(x - from) : v[e];
+                    }
+                    w[i / 2][i % 2 * 2 + r] = pack2<M>(v[0], v[1]);
+                }
+#pragma unroll
+            for (int c = 0; c < STEPS; ++c) {
+                uint32_t r[4];
+                if constexpr (!SMALL) {
+                    matrices_turned(r, values + (lane / 8 % 2 * 8 + lane % 8) * R::kPitch + (2 * c + lane / 16) * 16);
+                    multiply<M>(o[2 * c], w[0], r[0], r[1]);
+                    multiply<M>(o[2 * c + 1], w[0], r[2], r[3]);
+                } else {
+                    // a register has two elements of two keys: keys together, the even elements, then the odd ones
+                    matrices_turned(r, values + lane * R::kPitch + c * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r[i] = __byte_perm(r[i], 0, 0x3120);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        multiply<M>(o[2 * c], w[i], halves_of(r[2 * i] & 0xFFFFu), halves_of(r[2 * i + 1] & 0xFFFFu));
+                        multiply<M>(o[2 * c + 1], w[i], halves_of(r[2 * i] >> 16), halves_of(r[2 * i + 1] >> 16));
+                    }
+                }
+            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            done = now.tile + 1 == tiles;
+            ends = --left == 0 || done;
+            if (left) now.next(d);
+        } while (!ends);
+        // the end of the unit, or of this worker's part of it
+        const bool whole = tile0 == 0 && done;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
+            sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
+            const uint32_t row = g + 8 * r;
+            if (row >= rows) continue;
+            const float by = whole ? (top[r] == -INFINITY ? 0.0f : 1.0f / sum[r]) : 1.0f;
+            T* const out = static_cast<T*>(d.out) + b * d.os[0] + (first + row) * d.os[1];
+            float* const part = part_of(d, worker, tile0 == 0) + row * (d.head + 2);
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t c = SMALL ? i / 2 * 16 + 4 * t + 2 * e + i % 2 : 8 * i + 2 * t + e;
+                    if (c >= d.head) continue;
+                    if (whole) out[c] = from_float<T>(o[i][2 * r + e] * by);
+                    else part[c] = o[i][2 * r + e];
+                }
+            if (!whole && t == 0) part[d.head] = top[r], part[d.head + 1] = sum[r];
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <typename T, bool SMALL, int STEPS>
+int launch_steps(const Decode& d) {
+    using R = Ring<STEPS, SMALL>;
+    // the same limit in every call: calls from several threads do not undo each other's
+    cudaError_t err = cudaFuncSetAttribute(decode_units_kernel<T, STEPS, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)R::kBytes);
+    if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
+    decode_units_kernel<T, STEPS, SMALL><<<ctx().sm_count, warps_of(STEPS) * 32, R::kBytes, ctx().stream()>>>(d);
+    return check_launch("decode_units_kernel");
+}
+
+template <typename T, bool SMALL>
+int launch_units(const Decode& d) {
+    switch (steps_of(d.head)) {
+        case 4: return launch_steps<T, SMALL, 4>(d);
+        case 5: return launch_steps<T, SMALL, 5>(d);
+        case 6: return launch_steps<T, SMALL, 6>(d);
+        case 8: return launch_steps<T, SMALL, 8>(d);
+        case 12: return launch_steps<T, SMALL, 12>(d);
+        default: return launch_steps<T, SMALL, 16>(d);
+    }
+}
+
+// Joins the parts of a row that workers share: block (query head, sequence), a thread a column.  A sequence without keys
 // gets zeros here.
 template <typename T>
 __global__ void __launch_bounds__(128) decode_join_kernel(const Decode d) {
-    __shared__ uint64_t buf[33];
+    constexpr uint32_t kThreads = 128, kColumns = kMaxHead / kThreads;
+    __shared__ uint64_t buf[kThreads / 32];
+    __shared__ float factors[kThreads], wide[kThreads / 32];
     const uint32_t b = blockIdx.y, query = blockIdx.x, h = query / d.group, g = (query - h * d.group) / kRows;
     const uint32_t unit = h * d.groups + g, row = query - h * d.group - g * kRows, tiles = tiles_of(d, b);
     T* const out = static_cast<T*>(d.out) + b * d.os[0] + query * d.os[1];
     if (tiles == 0) {
-        for (uint32_t c = threadIdx.x; c < d.head; c += blockDim.x) out[c] = from_float<T>(0.0f);
+        for (uint32_t c = threadIdx.x; c < d.head; c += kThreads) out[c] = from_float<T>(0.0f);
         return;
     }
     auto count = [&](uint32_t i) { return (uint64_t)tiles_of(d, i) * d.units; };
-    const uint64_t before = total_of(b, count, buf), work = total_of(d.batch, count, buf);
-    const uint64_t first = before + (uint64_t)unit * tiles, blocks = sharing(d, work);
-    const uint32_t c0 = (uint32_t)(((first + 1) * blocks - 1) / work), c1 = (uint32_t)(((first + tiles) * blocks - 1) / work);
+    const uint64_t before = total_of(b, count, buf), work = before + (uint64_t)tiles * d.units + [&] {
+        auto behind = [&](uint32_t i) { return (uint64_t)tiles_of(d, b + 1 + i) * d.units; };
+        return total_of(d.batch - b - 1, behind, buf);
+    }();
+    const uint64_t first = before + (uint64_t)unit * tiles, workers = sharing(d, work);
+    const uint32_t c0 = (uint32_t)(((first + 1) * workers - 1) / work), c1 = (uint32_t)(((first + tiles) * workers - 1) / work);
     if (c0 == c1) return;
-    auto part = [&](uint32_t c) { return d.partial + ((2ull * c + (c == c0)) * kRows + row) * (d.head + 2); };
+    auto part = [&](uint32_t c) { return part_of(d, c, c == c0) + row * (d.head + 2); };
     float top = -INFINITY;
-    for (uint32_t c = c0; c <= c1; ++c) top = fmaxf(top, part(c)[d.head]);
-    float sum = 0.0f, acc[(kMaxHead + 127) / 128] = {};
-    for (uint32_t c = c0; c <= c1; ++c) {
-        const float* p = part(c);
-        const float m = p[d.head], factor = m == top ? 1.0f : exp2f(m - top);
-        sum = fmaf(p[d.head + 1], factor, sum);
+    for (uint32_t c = c0 + threadIdx.x; c <= c1; c += kThreads) top = fmaxf(top, part(c)[d.head]);
 #pragma unroll
-        for (uint32_t i = 0; i < (kMaxHead + 127) / 128; ++i) {
-            const uint32_t column = threadIdx.x + i * 128;
-            if (column < d.head) acc[i] = fmaf(p[column], factor, acc[i]);
+    for (int m = 16; m; m /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
+    if (threadIdx.x % 32 == 0) wide[threadIdx.x / 32] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 32; ++w) top = fmaxf(top, wide[w]);
+    float sum = 0.0f, acc[kColumns] = {};
+    for (uint32_t base = c0; base <= c1; base += kThreads) {
+        const uint32_t n = min(kThreads, c1 + 1 - base);
+        __syncthreads();
+        if (threadIdx.x < n) {
+            const float* p = part(base + threadIdx.x);
+            const float m = p[d.head], factor = m == top ? 1.0f : exp2f(m - top);
+            factors[threadIdx.x] = factor;
+            sum = fmaf(p[d.head + 1], factor, sum);
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kColumns; ++k) {
+            const uint32_t column = threadIdx.x + k * kThreads;
+            if (column >= d.head) continue;
+            float a = acc[k];
+#pragma unroll 8
+            for (uint32_t i = 0; i < n; ++i) a = fmaf(part(base + i)[column], factors[i], a);
+            acc[k] = a;
         }
     }
 #pragma unroll
-    for (uint32_t i = 0; i < (kMaxHead + 127) / 128; ++i) {
-        const uint32_t column = threadIdx.x + i * 128;
-        if (column < d.head) out[column] = from_float<T>(top == -INFINITY ? 0.0f : acc[i] / sum);
+    for (int m = 16; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) wide[threadIdx.x / 32] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 32; ++w) sum += wide[w];
+#pragma unroll
+    for (uint32_t k = 0; k < kColumns; ++k) {
+        const uint32_t column = threadIdx.x + k * kThreads;
+        if (column < d.head) out[column] = from_float<T>(top == -INFINITY ? 0.0f : acc[k] / sum);
     }
+}
+
+// Whether the kernel of 16-byte units takes the call.
+bool by_units(const Decode& d, int dtype, const mtxc_decode_attention_args* a) {
+    const bool small = a->cache.dtype == MTXC_FLOAT8_E4M3;
+    const uint64_t unit = small ? 16 : 8;
+    if (dtype == MTXC_FLOAT || d.head % unit) return false;
+    for (int k = 0; k < 2; ++k) {
+        if (reinterpret_cast<uintptr_t>(a->cache.data[k]) % 16) return false;
+        for (int i = 0; i < 3; ++i)
+            if (a->cache.strides[k][i] % unit) return false;
+    }
+    return true;
 }
 
 int prepare(const std::string& who, int dtype, const mtxc_decode_attention_args* a, Decode* out) {
@@ -257,12 +686,15 @@ int prepare(const std::string& who, int dtype, const mtxc_decode_attention_args*
     d.table_stride = a->page_table_stride;
     d.lengths = a->lengths;
     d.scale = a->scale * 1.4426950408889634f;
-    d.tile = kAnyTile;
-    d.blocks = 2u * ctx().sm_count;
+    d.groups_div = FastDiv(std::max(1u, d.groups));
+    d.rows = std::min(kRows, std::max(1u, d.group));
+    d.vector = by_units(d, dtype, a);
+    d.tile = d.vector ? (a->cache.dtype == MTXC_FLOAT8_E4M3 ? 32 : 16) : kAnyTile;
+    d.workers = ctx().sm_count * (d.vector ? warps_of(steps_of(d.head)) : 2u);
     return MTXC_OK;
 }
 
-size_t partial_bytes(const Decode& d) { return ((size_t)2 * d.blocks * kRows * (d.head + 2) * sizeof(float) + 255) / 256 * 256; }
+size_t partial_bytes(const Decode& d) { return ((size_t)2 * d.workers * d.rows * (d.head + 2) * sizeof(float) + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace mtxc
@@ -295,6 +727,15 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
     int rc = MTXC_OK;
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        if constexpr (!std::is_same_v<T, float>) {
+            if (d.vector) {
+                rc = small ? launch_units<T, true>(d) : launch_units<T, false>(d);
+                if (rc) return;
+                decode_join_kernel<T><<<dim3(d.heads, d.batch), 128, 0, ctx().stream()>>>(d);
+                rc = check_launch("decode_join_kernel");
+                return;
+            }
+        }
         const size_t smem = sizeof(float) * (kRows * d.head + 2 * kAnyTile * (d.head + 1) + kRows * kAnyTile);
         constexpr int kMost = sizeof(float) * (kRows * kMaxHead + 2 * kAnyTile * (kMaxHead + 1) + kRows * kAnyTile);
         auto kernel = small ? decode_any_kernel<T, true> : decode_any_kernel<T, false>;
@@ -304,7 +745,7 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
             rc = cuda_fail(err, "cudaFuncSetAttribute");
             return;
         }
-        kernel<<<d.blocks, kAnyThreads, smem, ctx().stream()>>>(d);
+        kernel<<<d.workers, kAnyThreads, smem, ctx().stream()>>>(d);
         if ((rc = check_launch("decode_any_kernel"))) return;
         decode_join_kernel<T><<<dim3(d.heads, d.batch), 128, 0, ctx().stream()>>>(d);
         rc = check_launch("decode_join_kernel");

@@ -110,6 +110,25 @@ __device__ __forceinline__ Found find(uint32_t n, uint64_t target, Fn&& count, u
     return *found;
 }
 
+// A kernel that is launched as the next one's predecessor lets it start; the next one waits until all that the first has
+// written is there.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Args>
+cudaError_t launch_next(void (*kernel)(Args...), dim3 grid, unsigned threads, cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // The same for a warp by itself.
 template <typename Fn>
 __device__ __forceinline__ uint64_t warp_total(uint32_t n, Fn&& count) {

@@ -33,8 +33,9 @@ struct Decode {
     const int* lengths;
     float scale;      // times log2(e)
     bool vector;      // the kernel of 16-byte units
-    float* partial;   // [2 * workers][rows][head + 2]: sums, maximum, sum of weights
+    float* partial;   // [2 * workers][rows][pitch]: sums; at pitch - 4 the maximum and the sum of weights
     uint32_t rows;    // of a unit
+    uint32_t pitch;   // a multiple of four
 };
 
 __device__ __forceinline__ uint32_t length_of(const Decode& d, uint32_t b) {
@@ -48,7 +49,7 @@ __device__ __forceinline__ uint64_t sharing(const Decode& d, uint64_t work) { re
 
 // Where a worker leaves its part of a unit: one that it begins (and another worker ends), or one that was begun before.
 __device__ __forceinline__ float* part_of(const Decode& d, uint64_t worker, bool begins) {
-    return d.partial + (2 * worker + begins) * d.rows * (d.head + 2);
+    return d.partial + (2 * worker + begins) * d.rows * d.pitch;
 }
 
 // The page and slot of key j of sequence b; false: the table names no page of the cache.
@@ -90,6 +91,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
     float* const values = keys + kAnyTile * pitch;
     float* const weights = values + kAnyTile * pitch;  // [kRows][kAnyTile]
     auto count = [&](uint32_t b) { return (uint64_t)tiles_of(d, b) * d.units; };
+    let_next_start();
     const uint64_t work = total_of(d.batch, count, buf), blocks = sharing(d, work);
     if (blockIdx.x >= blocks) return;
     uint64_t at = work * blockIdx.x / blocks;
@@ -183,8 +185,9 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
                         const float o = row_max[r] == -INFINITY ? 0.0f : acc[i] / row_sum[r];
                         static_cast<T*>(d.out)[b * d.os[0] + (first + r) * d.os[1] + column] = from_float<T>(o);
                     } else {
-                        part[r * (d.head + 2) + column] = acc[i];
-                        if (column == 0) part[r * (d.head + 2) + d.head] = row_max[r], part[r * (d.head + 2) + d.head + 1] = row_sum[r];
+                        float* const p = part + r * d.pitch;
+                        p[column] = acc[i];
+                        if (column == 0) p[d.pitch - 4] = row_max[r], p[d.pitch - 3] = row_sum[r];
                     }
                 }
             }
@@ -201,19 +204,26 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // Half types, and caches in 8 bits under half queries, by 16-byte units.
 //
 // A warp works by itself: it copies the keys and values of its tile (16 of a half type, 32 of 8 bits) into a ring of its own
-// in shared memory, kStages ahead of use (192 KB an SM in flight and in use), and multiplies them on the tensor cores, 16
-// rows of queries (those that a unit lacks are zeros) x 16 or 32 keys: they pass once, and 16 rows cost what one does.  There is no
-// barrier between warps, and the copies run on across the borders of units and sequences.  The page numbers of a tile are
-// loaded one tile before its copies are issued.
+// in shared memory, kStages ahead of use (192 KB an SM in flight and in use), and multiplies them on the tensor cores: 16
+// keys are the rows and 8 or 16 queries (those that a unit lacks are zeros) the columns of K Q', 16 elements of the head are
+// the rows of V' P'.  (With the queries as 16 rows, half of them zeros for a group of 8, both took twice the products,
+// registers and exponentials: 228 us for [4 x 91k] e4m3.)  There is no barrier between warps, and the copies run on across
+// the borders of units and sequences.  The page numbers of a tile are loaded one tile before its copies are issued.
 //
 // In 8 bits the bytes become float16, which holds them exactly, beside queries as float16 of a magnitude below 2 (their rows'
 // powers of two, like the keys' scales, come back into the scores).  The values' scales 2^e go into the weights: those are
 // 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are, and the weights that are summed
 // for the denominator 2^(s - m).
 // ------------------------------------------------------------------------------------------
-constexpr int kStages = 3;
-
-constexpr uint32_t warps_of(uint32_t steps) { return steps > 8 ? 4 : 8; }  // a ring of 24 to 26 or 50 KB each
+#ifndef MTX_W
+#define MTX_W 8
+#define MTX_S 3
+#define MTX_WS 12
+#define MTX_SS 2
+#endif
+// Warps of a block, one block an SM, and tiles of a warp's ring: what 227 KB hold.
+constexpr uint32_t warps_of(uint32_t steps, bool small) { return steps > 8 ? 4 : small ? MTX_WS : MTX_W; }
+constexpr int stages_of(uint32_t steps, bool small) { return steps > 8 ? 3 : small ? MTX_SS : MTX_S; }
 uint32_t steps_of(uint32_t head) {  // of 16 elements, as the kernel is built for
     for (uint32_t s : {4u, 5u, 6u, 8u, 12u})
         if (head <= 16 * s) return s;
@@ -226,8 +236,9 @@ struct Ring {
     static constexpr uint32_t kUnits = SMALL ? STEPS : 2 * STEPS;     // 16-byte units of a row
     static constexpr uint32_t kPitch = (kUnits | 1) * 16;             // an odd number of them: rows in different banks
     static constexpr uint32_t kSide = kKeys * kPitch, kStage = 2 * kSide;
+    static constexpr int kStages = stages_of(STEPS, SMALL);
     static constexpr uint32_t kWarp = kStages * (kStage + 128);       // the last: which keys count, and their exponents
-    static constexpr uint32_t kBytes = warps_of(STEPS) * kWarp;
+    static constexpr uint32_t kBytes = warps_of(STEPS, SMALL) * kWarp;
 };
 
 __device__ __forceinline__ void matrices(uint32_t (&r)[4], uint32_t at) {
@@ -246,6 +257,12 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], 
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// An 8 x 8 matrix of 16-bit elements over a warp, its columns made rows.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -279,15 +296,17 @@ struct Place {
     }
 };
 
-template <typename T, int STEPS, bool SMALL>
-__global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(const Decode d) {
+template <typename T, int STEPS, bool SMALL, int COLUMNS>  // COLUMNS: of queries, in eights
+__global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_kernel(const Decode d) {
     using R = Ring<STEPS, SMALL>;
     using M = std::conditional_t<SMALL, __half, T>;  // the products' type
-    constexpr uint32_t kKeys = R::kKeys, kTiles = kKeys / 8;
+    constexpr uint32_t kKeys = R::kKeys, kTiles = kKeys / 16;
+    constexpr int kStages = R::kStages;
     extern __shared__ uint4 smem4[];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem4) + warp * R::kWarp;
     uint32_t* const notes = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(smem4) + warp * R::kWarp + kStages * R::kStage);
+    let_next_start();
     auto count = [&](uint32_t b) { return (uint64_t)tiles_of(d, b) * d.units; };
     const uint64_t work = warp_total(d.batch, count), workers = sharing(d, work);
     const uint64_t worker = (uint64_t)warp * gridDim.x + blockIdx.x;  // little work: one warp of each block first
@@ -304,7 +323,8 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
         now.tile = (uint32_t)((first - f.first) - (uint64_t)now.unit * now.tiles);
     }
     // elements that the heads lack stay zeros: no copy reaches them
-    for (uint32_t i = lane; i < kStages * R::kStage / 16; i += 32)
+    const uint32_t units = d.head * (SMALL ? 1 : 2) / 16;  // of a row that are copied
+    for (uint32_t i = lane; units < R::kUnits && i < kStages * R::kStage / 16; i += 32)
         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i * 16), "r"(0) : "memory");
     __syncwarp();
 
@@ -325,7 +345,6 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
         }
         if (unseen) ahead.next(d);
     };
-    const uint32_t units = d.head * (SMALL ? 1 : 2) / 16;  // of a row that are copied
     uint32_t note = 0, note_to = 0;  // on its way to stage note_to
     auto copy = [&](uint32_t stage) {
         const bool ok = page < d.cache.pages;
@@ -374,27 +393,27 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
         // a unit, as far as this worker has it
         uint32_t h, first;
         const uint32_t rows = rows_of(d, now.unit, h, first), b = now.b, tile0 = now.tile, tiles = now.tiles;
-        uint32_t q[STEPS][4];
-        float factor[2] = {d.scale, d.scale};
+        uint32_t q[STEPS][COLUMNS][2];
+        float factor[COLUMNS][2];  // of this thread's columns 2 t, 2 t + 1
         {
-            // row r of the first operand: the registers' elements 2 t, 2 t + 1 and 8 further (of 8 bits: 4 t .. 4 t + 3, as a
-            // thread finds four bytes of a key side by side)
+            // column g of the second operand: elements 2 t, 2 t + 1 and 8 further (of 8 bits: 4 t .. 4 t + 3, as a thread finds
+            // four bytes of a key side by side)
             const T* base = static_cast<const T*>(d.q) + b * d.qs[0] + first * d.qs[1];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint32_t row = g + 8 * r;
+            for (int n = 0; n < COLUMNS; ++n) {
+                const uint32_t row = g + 8 * n;
                 const T* x = base + row * d.qs[1];
+                factor[n][0] = factor[n][1] = d.scale;
                 if constexpr (!SMALL) {
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const uint32_t c = 16 * s + 8 * e + 2 * t;
-                            const bool there = row < rows && c < d.head;
-                            q[s][r + 2 * e] = there ? pack2<T>(to_float(x[c]), to_float(x[c + 1])) : 0u;
+                            q[s][n][e] = row < rows && c < d.head ? pack2<T>(to_float(x[c]), to_float(x[c + 1])) : 0u;
                         }
                 } else {
-                    uint32_t top = 0;
+                    uint32_t most = 0;
                     float v[STEPS][4];
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s)
@@ -403,24 +422,28 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
                             const uint32_t c = 16 * s + 4 * t + e;
                             v[s][e] = row < rows && c < d.head ? to_float(x[c]) : 0.0f;
                             const uint32_t bits = __float_as_uint(v[s][e]) & 0x7FFFFFFFu;
-                            top = max(top, bits < 0x7F800000u ? bits : 0u);
+                            most = max(most, bits < 0x7F800000u ? bits : 0u);
                         }
-                    top = max(top, __shfl_xor_sync(~0u, top, 1));
-                    top = max(top, __shfl_xor_sync(~0u, top, 2));
-                    const int e = top ? max(-126, min(126, (int)(top >> 23) - 127)) : 0;
-                    factor[r] *= power_of_two(e);
-                    const float down = power_of_two(-e);
+                    most = max(most, __shfl_xor_sync(~0u, most, 1));
+                    most = max(most, __shfl_xor_sync(~0u, most, 2));
+                    const int e = most ? max(-126, min(126, (int)(most >> 23) - 127)) : 0;
+                    const float down = power_of_two(-e), up = power_of_two(e);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) factor[n][i] *= __shfl_sync(~0u, up, 4 * (2 * t + i));
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) q[s][r + 2 * i] = pack2<__half>(v[s][2 * i] * down, v[s][2 * i + 1] * down);
+                        for (int i = 0; i < 2; ++i) q[s][n][i] = pack2<__half>(v[s][2 * i] * down, v[s][2 * i + 1] * down);
                 }
             }
         }
-        float o[2 * STEPS][4];
+        float o[STEPS][COLUMNS][4], top[COLUMNS][2], sum[COLUMNS][2];
 #pragma unroll
-        for (int i = 0; i < 2 * STEPS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        for (int n = 0; n < COLUMNS; ++n) {
+            top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+        }
         bool ends, done;  // done: with the unit's last tile
         do {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -430,95 +453,116 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
             commit();
             look();
             const uint32_t keys = ring + stage * R::kStage, values = keys + R::kSide;
-            float s[kTiles][4];
+            float s[kTiles][COLUMNS][4];  // keys g, g + 8 of 16 x columns 2 t, 2 t + 1
 #pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+            for (uint32_t i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int n = 0; n < COLUMNS; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.0f;
 #pragma unroll
             for (int c = 0; c < STEPS; ++c) {
                 uint32_t r[4];
                 if constexpr (!SMALL) {
-                    matrices(r, keys + (lane / 16 * 8 + lane % 8) * R::kPitch + (2 * c + lane / 8 % 2) * 16);
-                    multiply<M>(s[0], q[c], r[0], r[1]);
-                    multiply<M>(s[1], q[c], r[2], r[3]);
+                    matrices(r, keys + lane % 16 * R::kPitch + (2 * c + lane / 16) * 16);
+#pragma unroll
+                    for (int n = 0; n < COLUMNS; ++n) multiply<M>(s[0][n], r, q[c][n][0], q[c][n][1]);
                 } else {
                     matrices(r, keys + lane * R::kPitch + c * 16);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) multiply<M>(s[i], q[c], halves_of(r[i] & 0xFFFFu), halves_of(r[i] >> 16));
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t a[4] = {halves_of(r[2 * i] & 0xFFFFu), halves_of(r[2 * i + 1] & 0xFFFFu),
+                                               halves_of(r[2 * i] >> 16), halves_of(r[2 * i + 1] >> 16)};
+#pragma unroll
+                        for (int n = 0; n < COLUMNS; ++n) multiply<M>(s[i][n], a, q[c][n][0], q[c][n][1]);
+                    }
                 }
             }
             // scores in powers of two; a key that counts lifts the maximum off -infinity even where its score is
             const uint32_t mine = notes[stage * 32 + lane], counting = __ballot_sync(~0u, mine & 1);
-            float most[2] = {-INFINITY, -INFINITY}, shift[kTiles][2];  // shift: the values' scales
+            float most[COLUMNS][2], shift[kTiles][2];  // shift: the values' scales
+#pragma unroll
+            for (int n = 0; n < COLUMNS; ++n) most[n][0] = most[n][1] = -INFINITY;
 #pragma unroll
             for (uint32_t i = 0; i < kTiles; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t key = 8 * i + 2 * t + e;
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t key = 16 * i + 8 * r + g;
                     const bool counts = counting >> key & 1;
                     float scale = 1.0f;
-                    shift[i][e] = 0.0f;
+                    shift[i][r] = 0.0f;
                     if constexpr (SMALL) {
                         const uint32_t x = __shfl_sync(~0u, mine, key);
                         scale = power_of_two((int8_t)(x >> 8 & 0xFFu));
-                        shift[i][e] = (float)(int8_t)(x >> 16 & 0xFFu);
+                        shift[i][r] = (float)(int8_t)(x >> 16 & 0xFFu);
                     }
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float& x = s[i][2 * r + e];
-                        x = counts ? x * (factor[r] * scale) : -INFINITY;
-                        if (counts) most[r] = fmaxf(most[r], fmaxf(x + shift[i][e], kLowest));
-                    }
+                    for (int n = 0; n < COLUMNS; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& x = s[i][n][2 * r + e];
+                            x = counts ? x * (factor[n][e] * scale) : -INFINITY;
+                            if (counts) most[n][e] = fmaxf(most[n][e], fmaxf(x + shift[i][r], kLowest));
+                        }
                 }
             bool grown = false;
-            float old[2];
+            float old[COLUMNS][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                most[r] = fmaxf(most[r], __shfl_xor_sync(~0u, most[r], 1));
-                most[r] = fmaxf(most[r], __shfl_xor_sync(~0u, most[r], 2));
-                old[r] = top[r];
-                top[r] = fmaxf(top[r], most[r]);
-                grown = grown || top[r] != old[r];
-            }
+            for (int n = 0; n < COLUMNS; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int m = 4; m < 32; m *= 2) most[n][e] = fmaxf(most[n][e], __shfl_xor_sync(~0u, most[n][e], m));
+                    old[n][e] = top[n][e];
+                    top[n][e] = fmaxf(top[n][e], most[n][e]);
+                    grown = grown || top[n][e] != old[n][e];
+                }
             if (__any_sync(~0u, grown)) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float by = top[r] == old[r] ? 1.0f : power(old[r] - top[r]);
-                    sum[r] *= by;
-#pragma unroll
-                    for (int i = 0; i < 2 * STEPS; ++i) o[i][2 * r] *= by, o[i][2 * r + 1] *= by;
-                }
-            }
-            uint32_t w[kTiles / 2][4];
-#pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float from = top[r] == -INFINITY ? 0.0f : top[r];
-                    float v[2];
+                for (int n = 0; n < COLUMNS; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float x = s[i][2 * r + e];
-                        v[e] = power(x + (shift[i][e] - from));
-                        sum[r] += SMALL ? power(x - from) : v[e];
+                        const float by = top[n][e] == old[n][e] ? 1.0f : power(old[n][e] - top[n][e]);
+                        sum[n][e] *= by;
+#pragma unroll
+                        for (int i = 0; i < STEPS; ++i) o[i][n][e] *= by, o[i][n][2 + e] *= by;
                     }
-                    w[i / 2][i % 2 * 2 + r] = pack2<M>(v[0], v[1]);
-                }
+            }
+            uint32_t w[kTiles][COLUMNS][2];
+#pragma unroll
+            for (int n = 0; n < COLUMNS; ++n) {
+                const float from[2] = {top[n][0] == -INFINITY ? 0.0f : top[n][0], top[n][1] == -INFINITY ? 0.0f : top[n][1]};
+#pragma unroll
+                for (uint32_t i = 0; i < kTiles; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float v[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float x = s[i][n][2 * r + e];
+                            v[e] = power(x + (shift[i][r] - from[e]));
+                            sum[n][e] += SMALL ? power(x - from[e]) : v[e];
+                        }
+                        w[i][n][r] = turned(pack2<M>(v[0], v[1]));
+                    }
+            }
 #pragma unroll
             for (int c = 0; c < STEPS; ++c) {
                 uint32_t r[4];
                 if constexpr (!SMALL) {
-                    matrices_turned(r, values + (lane / 8 % 2 * 8 + lane % 8) * R::kPitch + (2 * c + lane / 16) * 16);
-                    multiply<M>(o[2 * c], w[0], r[0], r[1]);
-                    multiply<M>(o[2 * c + 1], w[0], r[2], r[3]);
+                    matrices_turned(r, values + (lane / 16 * 8 + lane % 8) * R::kPitch + (2 * c + lane / 8 % 2) * 16);
+#pragma unroll
+                    for (int n = 0; n < COLUMNS; ++n) multiply<M>(o[c][n], r, w[0][n][0], w[0][n][1]);
                 } else {
-                    // a register has two elements of two keys: keys together, the even elements, then the odd ones
+                    // a register has two elements of two keys: keys together, and the even elements are rows 0 to 7, the odd
+                    // ones rows 8 to 15
                     matrices_turned(r, values + lane * R::kPitch + c * 16);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) r[i] = __byte_perm(r[i], 0, 0x3120);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        multiply<M>(o[2 * c], w[i], halves_of(r[2 * i] & 0xFFFFu), halves_of(r[2 * i + 1] & 0xFFFFu));
-                        multiply<M>(o[2 * c + 1], w[i], halves_of(r[2 * i] >> 16), halves_of(r[2 * i + 1] >> 16));
+                        const uint32_t a[4] = {halves_of(r[2 * i] & 0xFFFFu), halves_of(r[2 * i] >> 16), halves_of(r[2 * i + 1] & 0xFFFFu),
+                                               halves_of(r[2 * i + 1] >> 16)};
+#pragma unroll
+                        for (int n = 0; n < COLUMNS; ++n) multiply<M>(o[c][n], a, w[i][n][0], w[i][n][1]);
                     }
                 }
             }
@@ -530,25 +574,27 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
         // the end of the unit, or of this worker's part of it
         const bool whole = tile0 == 0 && done;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
-            sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
-            const uint32_t row = g + 8 * r;
-            if (row >= rows) continue;
-            const float by = whole ? (top[r] == -INFINITY ? 0.0f : 1.0f / sum[r]) : 1.0f;
-            T* const out = static_cast<T*>(d.out) + b * d.os[0] + (first + row) * d.os[1];
-            float* const part = part_of(d, worker, tile0 == 0) + row * (d.head + 2);
+        for (int n = 0; n < COLUMNS; ++n)
 #pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i)
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t c = SMALL ? i / 2 * 16 + 4 * t + 2 * e + i % 2 : 8 * i + 2 * t + e;
-                    if (c >= d.head) continue;
-                    if (whole) out[c] = from_float<T>(o[i][2 * r + e] * by);
-                    else part[c] = o[i][2 * r + e];
-                }
-            if (!whole && t == 0) part[d.head] = top[r], part[d.head + 1] = sum[r];
-        }
+                for (int m = 4; m < 32; m *= 2) sum[n][e] += __shfl_xor_sync(~0u, sum[n][e], m);
+                const uint32_t row = 8 * n + 2 * t + e;
+                if (row >= rows) continue;
+                const float by = whole ? (top[n][e] == -INFINITY ? 0.0f : 1.0f / sum[n][e]) : 1.0f;
+                T* const out = static_cast<T*>(d.out) + b * d.os[0] + (first + row) * d.os[1];
+                float* const part = part_of(d, worker, tile0 == 0) + row * d.pitch;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t c = 16 * i + (SMALL ? 2 * g + r : 8 * r + g);
+                        if (c >= d.head) continue;
+                        if (whole) out[c] = from_float<T>(o[i][n][2 * r + e] * by);
+                        else part[c] = o[i][n][2 * r + e];
+                    }
+                if (!whole && g == 0) part[d.pitch - 4] = top[n][e], part[d.pitch - 3] = sum[n][e];
+            }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -556,10 +602,11 @@ __global__ void __launch_bounds__(warps_of(STEPS) * 32, 1) decode_units_kernel(c
 template <typename T, bool SMALL, int STEPS>
 int launch_steps(const Decode& d) {
     using R = Ring<STEPS, SMALL>;
+    auto kernel = d.rows <= 8 ? decode_units_kernel<T, STEPS, SMALL, 1> : decode_units_kernel<T, STEPS, SMALL, 2>;
     // the same limit in every call: calls from several threads do not undo each other's
-    cudaError_t err = cudaFuncSetAttribute(decode_units_kernel<T, STEPS, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)R::kBytes);
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)R::kBytes);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
-    decode_units_kernel<T, STEPS, SMALL><<<ctx().sm_count, warps_of(STEPS) * 32, R::kBytes, ctx().stream()>>>(d);
+    kernel<<<ctx().sm_count, warps_of(STEPS, SMALL) * 32, R::kBytes, ctx().stream()>>>(d);
     return check_launch("decode_units_kernel");
 }
 
@@ -575,71 +622,100 @@ int launch_units(const Decode& d) {
     }
 }
 
-// Joins the parts of a row that workers share: block (query head, sequence), a thread a column.  A sequence without keys
-// gets zeros here.
-template <typename T>
-__global__ void __launch_bounds__(128) decode_join_kernel(const Decode d) {
-    constexpr uint32_t kThreads = 128, kColumns = kMaxHead / kThreads;
-    __shared__ uint64_t buf[kThreads / 32];
-    __shared__ float factors[kThreads], wide[kThreads / 32];
+// Joins the parts of a row that workers share: block (query head, sequence), warps take parts in turn, a lane four columns
+// (and four more 128 further), so that all of up to 64 parts are on their way at once.  A sequence without keys gets zeros here.
+template <typename T, uint32_t kJoinThreads>
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Decode d) {
+    constexpr uint32_t kWarps = kJoinThreads / 32;
+    __shared__ uint64_t buf[kWarps];
+    __shared__ float factors[kJoinThreads], wide[kWarps];
+    __shared__ float4 sums[kWarps][kMaxHead / 4];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t b = blockIdx.y, query = blockIdx.x, h = query / d.group, g = (query - h * d.group) / kRows;
     const uint32_t unit = h * d.groups + g, row = query - h * d.group - g * kRows, tiles = tiles_of(d, b);
     T* const out = static_cast<T*>(d.out) + b * d.os[0] + query * d.os[1];
+    auto before = [&](uint32_t i) { return (uint64_t)tiles_of(d, i) * d.units; };
+    auto behind = [&](uint32_t i) { return (uint64_t)tiles_of(d, b + 1 + i) * d.units; };
+    const uint64_t start = total_of(b, before, buf), work = start + (uint64_t)tiles * d.units + total_of(d.batch - b - 1, behind, buf);
+    wait_for_previous();  // every block: what follows in the stream follows the first kernel too
     if (tiles == 0) {
-        for (uint32_t c = threadIdx.x; c < d.head; c += kThreads) out[c] = from_float<T>(0.0f);
+        for (uint32_t c = threadIdx.x; c < d.head; c += kJoinThreads) out[c] = from_float<T>(0.0f);
         return;
     }
-    auto count = [&](uint32_t i) { return (uint64_t)tiles_of(d, i) * d.units; };
-    const uint64_t before = total_of(b, count, buf), work = before + (uint64_t)tiles * d.units + [&] {
-        auto behind = [&](uint32_t i) { return (uint64_t)tiles_of(d, b + 1 + i) * d.units; };
-        return total_of(d.batch - b - 1, behind, buf);
-    }();
-    const uint64_t first = before + (uint64_t)unit * tiles, workers = sharing(d, work);
+    const uint64_t first = start + (uint64_t)unit * tiles, workers = sharing(d, work);
     const uint32_t c0 = (uint32_t)(((first + 1) * workers - 1) / work), c1 = (uint32_t)(((first + tiles) * workers - 1) / work);
     if (c0 == c1) return;
-    auto part = [&](uint32_t c) { return part_of(d, c, c == c0) + row * (d.head + 2); };
-    float top = -INFINITY;
-    for (uint32_t c = c0 + threadIdx.x; c <= c1; c += kThreads) top = fmaxf(top, part(c)[d.head]);
-#pragma unroll
-    for (int m = 16; m; m /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
-    if (threadIdx.x % 32 == 0) wide[threadIdx.x / 32] = top;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kThreads / 32; ++w) top = fmaxf(top, wide[w]);
-    float sum = 0.0f, acc[kColumns] = {};
-    for (uint32_t base = c0; base <= c1; base += kThreads) {
-        const uint32_t n = min(kThreads, c1 + 1 - base);
-        __syncthreads();
+    auto part = [&](uint32_t c) { return part_of(d, c, c == c0) + row * d.pitch; };
+    const uint32_t quads = d.pitch / 4 - 1;
+    float top = -INFINITY, sum = 0.0f;
+    float4 acc[kMaxHead / 128] = {};
+    for (uint32_t base = c0; base <= c1; base += kJoinThreads) {
+        // the sums so far follow the maximum, as in the kernels before
+        const uint32_t n = min(kJoinThreads, c1 + 1 - base);
+        float m = -INFINITY, l = 0.0f;
         if (threadIdx.x < n) {
-            const float* p = part(base + threadIdx.x);
-            const float m = p[d.head], factor = m == top ? 1.0f : exp2f(m - top);
-            factors[threadIdx.x] = factor;
-            sum = fmaf(p[d.head + 1], factor, sum);
+            const float2 ml = *reinterpret_cast<const float2*>(part(base + threadIdx.x) + d.pitch - 4);
+            m = ml.x, l = ml.y;
         }
+        float now = m;
+#pragma unroll
+        for (int x = 16; x; x /= 2) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+        __syncthreads();
+        if (lane == 0) wide[warp] = now;
+        __syncthreads();
+        now = top;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, wide[w]);
+        const float by = top == now ? 1.0f : exp2f(top - now);
+        top = now;
+        const float factor = m == top ? 1.0f : exp2f(m - top);
+        sum = sum * by + l * factor;
+        factors[threadIdx.x] = factor;
         __syncthreads();
 #pragma unroll
-        for (uint32_t k = 0; k < kColumns; ++k) {
-            const uint32_t column = threadIdx.x + k * kThreads;
-            if (column >= d.head) continue;
-            float a = acc[k];
-#pragma unroll 8
-            for (uint32_t i = 0; i < n; ++i) a = fmaf(part(base + i)[column], factors[i], a);
+        for (uint32_t k = 0; k < kMaxHead / 128; ++k) {
+            const uint32_t quad = lane + 32 * k;
+            if (quad >= quads) continue;
+            float4 a = acc[k];
+            a.x *= by, a.y *= by, a.z *= by, a.w *= by;
+#pragma unroll 4
+            for (uint32_t i = warp; i < n; i += kWarps) {
+                const float4 v = reinterpret_cast<const float4*>(part(base + i))[quad];
+                const float f = factors[i];
+                a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+            }
             acc[k] = a;
         }
     }
 #pragma unroll
     for (int m = 16; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
     __syncthreads();
-    if (threadIdx.x % 32 == 0) wide[threadIdx.x / 32] = sum;
+    if (lane == 0) wide[warp] = sum;
+#pragma unroll
+    for (uint32_t k = 0; k < kMaxHead / 128; ++k)
+        if (lane + 32 * k < quads) sums[warp][lane + 32 * k] = acc[k];
     __syncthreads();
     sum = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < kThreads / 32; ++w) sum += wide[w];
+    for (uint32_t w = 0; w < kWarps; ++w) sum += wide[w];
+    for (uint32_t c = threadIdx.x; c < d.head; c += kJoinThreads) {
+        float o = 0.0f;
 #pragma unroll
-    for (uint32_t k = 0; k < kColumns; ++k) {
-        const uint32_t column = threadIdx.x + k * kThreads;
-        if (column < d.head) out[column] = from_float<T>(top == -INFINITY ? 0.0f : acc[k] / sum);
+        for (uint32_t w = 0; w < kWarps; ++w) o += reinterpret_cast<const float*>(sums[w])[c];
+        out[c] = from_float<T>(top == -INFINITY ? 0.0f : o / sum);
     }
+}
+
+// Its start, and the sums over the lengths, behind the first kernel's work.
+template <typename T>
+int launch_join(const Decode& d) {
+    // few rows have many parts each, many rows few or none: there the blocks are small enough to start beside the first kernel's
+    // (one sequence of 1,500 tokens, 32 heads: 15 us with 512 threads, 20 with 128; 256 of 500: 178 and 117)
+    const dim3 grid(d.heads, d.batch);
+    const bool few = (uint64_t)d.heads * d.batch <= 4u * ctx().sm_count;
+    const cudaError_t err = few ? launch_next(decode_join_kernel<T, 512>, grid, 512, ctx().stream(), d)
+                                : launch_next(decode_join_kernel<T, 128>, grid, 128, ctx().stream(), d);
+    return err == cudaSuccess ? check_launch("decode_join_kernel") : cuda_fail(err, "decode_join_kernel");
 }
 
 // Whether the kernel of 16-byte units takes the call.
@@ -688,13 +764,14 @@ int prepare(const std::string& who, int dtype, const mtxc_decode_attention_args*
     d.scale = a->scale * 1.4426950408889634f;
     d.groups_div = FastDiv(std::max(1u, d.groups));
     d.rows = std::min(kRows, std::max(1u, d.group));
+    d.pitch = (d.head + 3) / 4 * 4 + 4;
     d.vector = by_units(d, dtype, a);
     d.tile = d.vector ? (a->cache.dtype == MTXC_FLOAT8_E4M3 ? 32 : 16) : kAnyTile;
-    d.workers = ctx().sm_count * (d.vector ? warps_of(steps_of(d.head)) : 2u);
+    d.workers = ctx().sm_count * (d.vector ? warps_of(steps_of(d.head), a->cache.dtype == MTXC_FLOAT8_E4M3) : 2u);
     return MTXC_OK;
 }
 
-size_t partial_bytes(const Decode& d) { return ((size_t)2 * d.workers * d.rows * (d.head + 2) * sizeof(float) + 255) / 256 * 256; }
+size_t partial_bytes(const Decode& d) { return ((size_t)2 * d.workers * d.rows * d.pitch * sizeof(float) + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace mtxc
@@ -731,8 +808,7 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
             if (d.vector) {
                 rc = small ? launch_units<T, true>(d) : launch_units<T, false>(d);
                 if (rc) return;
-                decode_join_kernel<T><<<dim3(d.heads, d.batch), 128, 0, ctx().stream()>>>(d);
-                rc = check_launch("decode_join_kernel");
+                rc = launch_join<T>(d);
                 return;
             }
         }
@@ -747,8 +823,7 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
         }
         kernel<<<d.workers, kAnyThreads, smem, ctx().stream()>>>(d);
         if ((rc = check_launch("decode_any_kernel"))) return;
-        decode_join_kernel<T><<<dim3(d.heads, d.batch), 128, 0, ctx().stream()>>>(d);
-        rc = check_launch("decode_join_kernel");
+        rc = launch_join<T>(d);
     });
     return rc;
 }

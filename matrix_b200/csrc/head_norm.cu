@@ -17,11 +17,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kMaxHead = 1024;
 constexpr uint32_t kTableEntries = 2048;  // cosines of a tile; as many sines
+constexpr uint32_t kResident = 2;         // blocks an SM of the backward pass
 
 struct Side {  // queries or keys
-    uint32_t heads, tile, blocks, first_block;  // tokens of a tile
-    uint64_t tiles;
-    FastDiv heads_div;
+    uint32_t heads, blocks, first_block;
+    uint32_t tile, tiles;  // tokens of a tile, tiles of a sequence
+    FastDiv heads_div, tiles_div;
     const void *x, *dy, *weight;
     void* out;               // y or dx
     uint64_t xs[3], ys[3], os[3];
@@ -32,7 +33,7 @@ struct Side {  // queries or keys
 struct HeadNorm {
     uint64_t tokens;
     uint64_t length;         // tokens of a sequence
-    uint32_t head, half, lanes_log, units, turned, second;  // second: from a copied unit's first access to its second
+    uint32_t batch, head, half, lanes_log;
     FastDiv half_div;
     int weight_dtype;
     const void* positions;
@@ -160,6 +161,206 @@ __global__ void __launch_bounds__(kThreads) head_norm_any_kernel(const HeadNorm 
 }
 
 // ------------------------------------------------------------------------------------------
+// Heads by accesses of N elements: a group of up to 32 lanes holds a head, a lane two accesses of it (half a head apart where
+// they are turned against each other, or, PAIRS, where each is turned in itself).  A block takes tiles of tokens of a sequence:
+// it makes their cosines and sines once, in shared memory, for all heads, with its first loads already in flight, and each group
+// loads its next head before it works on the one at hand.  Forward a tile a block; backward the blocks stay, since they keep
+// the sums for the weight's gradient in registers.
+// ------------------------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ void read_table(const float* p, float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p + i);
+            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        }
+    } else {
+        const float2 q = *reinterpret_cast<const float2*>(p);
+        v[0] = q.x, v[1] = q.y;
+    }
+}
+
+template <typename T, int N, bool PAIRS, bool BACKWARD>
+__global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(const HeadNorm r) {
+    constexpr int kAngles = PAIRS ? N / 2 : N;  // of an access
+    extern __shared__ float4 table4[];
+    float* const table = reinterpret_cast<float*>(table4);
+    const int k = blockIdx.x >= r.side[1].first_block;
+    const Side& s = r.side[k];
+    const uint32_t block = blockIdx.x - s.first_block;
+    float* const cosines = table;
+    float* const sines = table + s.tile * r.half;
+    const uint32_t lanes = 1u << r.lanes_log, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> r.lanes_log;
+    const uint32_t groups = kThreads >> r.lanes_log;
+    // this lane's accesses: their first elements, whether they are there and turned, and their first angles
+    uint32_t at[2];
+    bool there[2], turns[2];
+    if (PAIRS) {
+        const uint32_t all = r.head / N, first = (all + 1) / 2;
+        at[0] = lane * N, at[1] = (lane + first) * N;
+        there[0] = lane < first, there[1] = lane < first && lane + first < all;
+        turns[0] = at[0] < 2 * r.half, turns[1] = at[1] < 2 * r.half;
+    } else {
+        const uint32_t turned = r.half / N, rest = r.head / N - 2 * turned, first = (rest + 1) / 2, i = lane - turned;
+        const bool t = lane < turned;
+        at[0] = t ? lane * N : 2 * r.half + i * N, at[1] = at[0] + (t ? r.half : first * N);
+        there[0] = t || i < first, there[1] = t || (i < first && i + first < rest);
+        turns[0] = turns[1] = t;
+    }
+    float w[2][N], dw[2][N];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[a][i] = there[a] ? weight_at(r, s, at[a] + i) : 0.0f, dw[a][i] = 0.0f;
+
+    struct Head {
+        Few<T, N> x[2], dy[BACKWARD ? 2 : 1];
+        float rstd;
+    };
+    const uint32_t all_tiles = r.batch * s.tiles;
+    for (uint32_t tile = block; tile < all_tiles; tile += s.blocks) {
+        uint32_t b, t0;
+        s.tiles_div.divmod(tile, b, t0);
+        t0 *= s.tile;
+        const uint32_t n = (uint32_t)min((uint64_t)s.tile, r.length - t0), items = n * s.heads;
+        const T* const x = static_cast<const T*>(s.x) + b * s.xs[0] + t0 * s.xs[1];
+        const T* const dy = BACKWARD ? static_cast<const T*>(s.dy) + b * s.ys[0] + t0 * s.ys[1] : nullptr;
+        T* const out = static_cast<T*>(s.out) + b * s.os[0] + t0 * s.os[1];
+        float* const rstd = s.rstd ? s.rstd + (b * r.length + t0) * s.heads : nullptr;
+        auto load = [&](uint32_t item, Head& v) {
+            uint32_t token, h;
+            s.heads_div.divmod(item, token, h);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                if (!there[a]) continue;
+                v.x[a].load(x + token * s.xs[1] + h * s.xs[2] + at[a]);
+                if constexpr (BACKWARD) v.dy[a].load(dy + token * s.ys[1] + h * s.ys[2] + at[a]);
+            }
+            if constexpr (BACKWARD) v.rstd = rstd[item];
+        };
+        // the angles of access a, of which `first` is the value in the first place of its pair
+        auto turn_all = [&](uint32_t token, float (&v)[2][N]) {
+            float cs[kAngles], sn[kAngles];
+            if constexpr (PAIRS) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    if (!turns[a] || !there[a]) continue;
+                    read_table(cosines + token * r.half + at[a] / 2, cs);
+                    read_table(sines + token * r.half + at[a] / 2, sn);
+#pragma unroll
+                    for (int j = 0; j < kAngles; ++j) {
+                        const float p = v[a][2 * j], q = v[a][2 * j + 1];
+                        v[a][2 * j] = p * cs[j] - q * sn[j];
+                        v[a][2 * j + 1] = p * sn[j] + q * cs[j];
+                    }
+                }
+            } else if (turns[0]) {
+                read_table(cosines + token * r.half + at[0], cs);
+                read_table(sines + token * r.half + at[0], sn);
+#pragma unroll
+                for (int j = 0; j < kAngles; j += 2) {
+                    const float2 p = make_float2(v[0][j], v[0][j + 1]), q = make_float2(v[1][j], v[1][j + 1]);
+                    const float2 c = make_float2(cs[j], cs[j + 1]), d = make_float2(sn[j], sn[j + 1]);
+                    const float2 y = __ffma2_rn(p, c, __fmul2_rn(q, make_float2(-d.x, -d.y))), z = __ffma2_rn(p, d, __fmul2_rn(q, c));
+                    v[0][j] = y.x, v[0][j + 1] = y.y, v[1][j] = z.x, v[1][j + 1] = z.y;
+                }
+            }
+        };
+        Head next;
+        if (group < items) load(group, next);
+        __syncthreads();  // the tile before is done with the table
+        for (uint32_t e = threadIdx.x; e < n * r.half; e += kThreads) {
+            uint32_t token, j;
+            r.half_div.divmod(e, token, j);
+            turn(r, position_of(r, b, t0 + token), j, cosines[e], sines[e]);
+        }
+        __syncthreads();
+        for (uint32_t base = 0; base < items; base += groups) {  // the same for all lanes of a warp
+            const uint32_t item = base + group;
+            const bool mine = item < items;
+            Head v = next;
+            if (item + groups < items) load(item + groups, next);
+            uint32_t token, h;
+            s.heads_div.divmod(item, token, h);
+            float y[2][N];
+            float sum = 0.0f;
+            if constexpr (!BACKWARD) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        y[a][i] = mine && there[a] ? v.x[a].get(i) : 0.0f;
+                        sum = fmaf(y[a][i], y[a][i], sum);
+                    }
+                for (uint32_t m = lanes / 2; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+                const float scale = rsqrtf(fmaf(sum, r.inv_head, r.eps));
+                if (!mine) continue;
+                if (rstd && lane == 0) rstd[item] = scale;
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) y[a][i] *= scale * w[a][i];
+                turn_all(token, y);
+            } else {
+                float e[2][N];
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        y[a][i] = mine && there[a] ? v.dy[a].get(i) : 0.0f;
+                        e[a][i] = mine && there[a] ? v.x[a].get(i) * v.rstd : 0.0f;
+                    }
+                if (mine) turn_all(token, y);
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        dw[a][i] = fmaf(y[a][i], e[a][i], dw[a][i]);
+                        y[a][i] *= w[a][i];
+                        sum = fmaf(y[a][i], e[a][i], sum);
+                    }
+                for (uint32_t m = lanes / 2; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+                if (!mine) continue;
+                sum *= r.inv_head;
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) y[a][i] = v.rstd * fmaf(-e[a][i], sum, y[a][i]);
+            }
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                if (!there[a]) continue;
+                Few<T, N> o;
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) o.set2(i, y[a][2 * i], y[a][2 * i + 1]);
+                o.store(out + token * s.os[1] + h * s.os[2] + at[a]);
+            }
+        }
+    }
+    if constexpr (BACKWARD) {
+        if (!s.d_weight) return;
+        // the groups of a warp, then the warps, in order
+        const uint32_t warp = threadIdx.x / 32;
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float v = dw[a][i];
+                for (uint32_t m = 16; m >= lanes; m /= 2) v += __shfl_xor_sync(~0u, v, m);
+                if (threadIdx.x % 32 < lanes && there[a]) table[warp * r.head + at[a] + i] = v;
+            }
+        __syncthreads();
+        for (uint32_t d = threadIdx.x; d < r.head; d += kThreads) {
+            float sum = 0.0f;
+            for (uint32_t i = 0; i < kThreads / 32; ++i) sum += table[i * r.head + d];
+            s.d_weight[(uint64_t)block * r.head + d] = sum;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
 // The weights' gradients from the blocks' partial rows, added in a fixed order: 32 columns a block, 32 threads a
 // column.
 // ------------------------------------------------------------------------------------------
@@ -202,20 +403,36 @@ int check_args(const std::string& who, int dtype, const mtxc_head_norm_args* a) 
     return distinct(who, {a->heads[0] ? a->dst[0] : nullptr, a->heads[1] ? a->dst[1] : nullptr});
 }
 
-// The call's arguments as the kernels take them, and its plan; blocks: all that the launch needs.
+// The call's arguments as the kernels take them, and its plan; blocks: all that the launch needs; access: elements, 0: any.
 struct Plan {
     HeadNorm r{};
-    bool vector = false;
-    uint32_t blocks = 0;
+    uint32_t access = 0, blocks = 0;
 };
+
+// Whether a call's heads go by accesses of N elements.
+template <typename T, int N>
+bool fits(const mtxc_head_norm_args* a, bool backward) {
+    const uint32_t half = a->rotary_dim / 2, head = a->head_dim;
+    if (head % N || (a->interleaved ? a->rotary_dim % N : half % N)) return false;
+    const uint32_t lanes = a->interleaved ? (head / N + 1) / 2 : half / N + (head / N - 2 * (half / N) + 1) / 2;
+    bool ok = lanes <= 32 && a->length < 1ull << 31 && a->batch < 1ull << 31;
+    for (int k = 0; k < 2; ++k)
+        for (int i = 0; a->heads[k] && i < 3; ++i) {
+            ok = ok && few_aligned<T, N>(a->src[k], a->src_strides[k][i]) && few_aligned<T, N>(a->dst[k], a->dst_strides[k][i]);
+            if (backward) ok = ok && few_aligned<T, N>(a->d_out[k], a->d_out_strides[k][i]);
+        }
+    return ok;
+}
 
 Plan plan(int dtype, const mtxc_head_norm_args* a, bool backward) {
     Plan p;
     HeadNorm& r = p.r;
     r.tokens = a->batch * a->length;
     r.length = std::max<uint64_t>(1, a->length);
+    r.batch = (uint32_t)a->batch;
     r.head = a->head_dim;
     r.half = a->rotary_dim / 2;
+    r.half_div = FastDiv(std::max(1u, r.half));
     r.weight_dtype = a->weight_dtype;
     r.positions = a->positions;
     r.wide_positions = a->position_dtype == MTXC_INT64;
@@ -227,6 +444,18 @@ Plan plan(int dtype, const mtxc_head_norm_args* a, bool backward) {
     r.weight_offset = a->weight_offset;
     r.eps = a->eps;
     r.inv_head = 1.0f / (float)std::max(1u, r.head);
+    dispatch_float(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        p.access = fits<T, 8>(a, backward) ? 8 : fits<T, 4>(a, backward) ? 4 : 0;
+    });
+    if (!r.tokens || !r.head) p.access = 0;
+    uint32_t lanes = 1;
+    if (p.access) {
+        const uint32_t n = p.access, turned = r.half / n;
+        const uint32_t want = a->interleaved ? (r.head / n + 1) / 2 : turned + (r.head / n - 2 * turned + 1) / 2;
+        while (lanes < want) lanes *= 2, ++r.lanes_log;
+    }
+    const uint32_t groups = kThreads / lanes, all_heads = a->heads[0] + a->heads[1], sms = (uint32_t)ctx().sm_count;
     for (int k = 0; k < 2; ++k) {
         Side& s = r.side[k];
         s.heads = a->heads[k];
@@ -238,8 +467,30 @@ Plan plan(int dtype, const mtxc_head_norm_args* a, bool backward) {
         s.rstd = a->rstd[k];
         for (int i = 0; i < 3; ++i)
             s.xs[i] = a->src_strides[k][i], s.ys[i] = a->d_out_strides[k][i], s.os[i] = a->dst_strides[k][i];
-        const uint64_t warps = r.tokens * s.heads;
-        s.blocks = (uint32_t)std::min<uint64_t>((warps + kThreads / 32 - 1) / (kThreads / 32), 4u * ctx().sm_count);
+        s.tile = s.tiles = 1;
+        if (!s.heads || !r.tokens) {
+            s.blocks = 0;
+        } else if (p.access) {
+            // tokens of a tile: eight heads a group, while every SM has four blocks and the table fits
+            uint64_t tile = std::max<uint64_t>(1, 8 * groups / s.heads);
+            tile = std::min(tile, std::max<uint64_t>(1, r.tokens * s.heads / (4ull * sms * all_heads)));
+            tile = std::min<uint64_t>({tile, std::max(1u, kTableEntries / std::max(1u, r.half)), r.length});
+            s.tile = (uint32_t)tile;
+            s.tiles = (uint32_t)((r.length + tile - 1) / tile);
+            const uint64_t all = (uint64_t)s.tiles * a->batch;
+            if (all >> 31) p.access = 0;
+            // backward: as many blocks as are resident, shared by heads
+            const uint64_t most = backward ? std::max<uint64_t>(1, (uint64_t)kResident * sms * s.heads / all_heads) : 1u << 30;
+            s.blocks = (uint32_t)std::min(all, most);
+        }
+        s.tiles_div = FastDiv(s.tiles);
+    }
+    for (int k = 0; k < 2; ++k) {
+        Side& s = r.side[k];
+        if (!p.access) {
+            const uint64_t warps = r.tokens * s.heads;
+            s.blocks = (uint32_t)std::min<uint64_t>((warps + kThreads / 32 - 1) / (kThreads / 32), 4u * sms);
+        }
         s.first_block = p.blocks;
         p.blocks += s.blocks;
     }
@@ -249,11 +500,19 @@ Plan plan(int dtype, const mtxc_head_norm_args* a, bool backward) {
 template <bool BACKWARD>
 int launch(int dtype, const mtxc_head_norm_args* a, const Plan& p) {
     const HeadNorm& r = p.r;
-    const size_t smem = BACKWARD ? sizeof(float) * (kThreads / 32) * r.head : 0;
+    const size_t sums = BACKWARD ? sizeof(float) * (kThreads / 32) * r.head : 0;
+    const size_t table = 2 * sizeof(float) * r.half * std::max(r.side[0].tile, r.side[1].tile);
     dispatch_float(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (a->interleaved) head_norm_any_kernel<T, true, BACKWARD><<<p.blocks, kThreads, smem, ctx().stream()>>>(r);
-        else head_norm_any_kernel<T, false, BACKWARD><<<p.blocks, kThreads, smem, ctx().stream()>>>(r);
+        cudaStream_t st = ctx().stream();
+        auto run = [&](auto pairs) {
+            constexpr bool P = decltype(pairs)::value;
+            if (p.access == 8) head_norm_kernel<T, 8, P, BACKWARD><<<p.blocks, kThreads, std::max(sums, table), st>>>(r);
+            else if (p.access == 4) head_norm_kernel<T, 4, P, BACKWARD><<<p.blocks, kThreads, std::max(sums, table), st>>>(r);
+            else head_norm_any_kernel<T, P, BACKWARD><<<p.blocks, kThreads, sums, st>>>(r);
+        };
+        if (a->interleaved) run(std::true_type());
+        else run(std::false_type());
     });
     return check_launch("head_norm_kernel");
 }

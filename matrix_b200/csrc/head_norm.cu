@@ -28,6 +28,7 @@ struct Side {  // queries or keys
     uint64_t xs[3], ys[3], os[3];
     float* rstd;             // written forward (or NULL), read backward
     float* d_weight;         // partial rows [blocks][head], or NULL
+    bool whole_weight;       // of the heads' dtype and aligned as they are
 };
 
 struct HeadNorm {
@@ -212,7 +213,23 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[a][i] = there[a] ? weight_at(r, s, at[a] + i) : 0.0f, dw[a][i] = 0.0f;
+        for (int i = 0; i < N; ++i) w[a][i] = s.weight ? 0.0f : 1.0f, dw[a][i] = 0.0f;
+    if (s.weight && s.whole_weight) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            Few<T, N> v;
+            if (!there[a]) continue;
+            v.load(static_cast<const T*>(s.weight) + at[a]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[a][i] = r.weight_offset + v.get(i);
+        }
+    } else if (s.weight) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (there[a]) w[a][i] = weight_at(r, s, at[a] + i);
+    }
 
     struct Head {
         Few<T, N> x[2], dy[BACKWARD ? 2 : 1];
@@ -449,6 +466,8 @@ Plan plan(int dtype, const mtxc_head_norm_args* a, bool backward) {
         p.access = fits<T, 8>(a, backward) ? 8 : fits<T, 4>(a, backward) ? 4 : 0;
     });
     if (!r.tokens || !r.head) p.access = 0;
+    for (int k = 0; k < 2; ++k)
+        r.side[k].whole_weight = a->weight_dtype == dtype && reinterpret_cast<uintptr_t>(a->weight[k]) % 32 == 0;
     uint32_t lanes = 1;
     if (p.access) {
         const uint32_t n = p.access, turned = r.half / n;
@@ -473,7 +492,7 @@ Plan plan(int dtype, const mtxc_head_norm_args* a, bool backward) {
         } else if (p.access) {
             // tokens of a tile: eight heads a group, while every SM has four blocks and the table fits
             uint64_t tile = std::max<uint64_t>(1, 8 * groups / s.heads);
-            tile = std::min(tile, std::max<uint64_t>(1, r.tokens * s.heads / (4ull * sms * all_heads)));
+            tile = std::min(tile, std::max<uint64_t>(1, r.tokens * all_heads / (4ull * sms * s.heads)));
             tile = std::min<uint64_t>({tile, std::max(1u, kTableEntries / std::max(1u, r.half)), r.length});
             s.tile = (uint32_t)tile;
             s.tiles = (uint32_t)((r.length + tile - 1) / tile);

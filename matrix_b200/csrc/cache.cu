@@ -12,6 +12,9 @@ namespace mtxc {
 namespace {
 
 constexpr int kThreads = 256;
+#ifndef MTX_WB
+#define MTX_WB 4
+#endif
 constexpr uint32_t kMaxTile = 64;
 constexpr uint32_t kChunk = 16384;  // tokens of a launch of the write
 constexpr uint32_t kMaxHead = 1024;
@@ -23,7 +26,7 @@ struct Rows {
     void* rows[2];
     uint64_t rs[2][2];
     const void* slots;
-    bool wide_slots;
+    bool wide_slots, four_slots;  // four_slots: 32 bits, one after another, aligned to four
     uint64_t slot_stride;
 };
 
@@ -72,123 +75,224 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, const float (&y)[N]) {
     } else *p = (uint8_t)to_e4m3(y[0], 0.0f);
 }
 
-// A group of 2^lanes_log lanes stores the key and the value of one head of one token, a lane every N elements.  Of the
-// tokens that name one slot the last is stored: a block looks for its slots among those of the tokens behind it (a bit for
-// each of its slots modulo 2,048 tells nearly all of them apart at once).
-template <typename T, int N, bool SMALL>
+// Where a row lies in the cache: its elements and its exponents, of keys (0) or values (1).
+__device__ __forceinline__ uint64_t row_at(const Rows& r, int k, int slot, uint32_t h) {
+    uint32_t page, at;
+    r.cache.page_div.divmod((uint32_t)slot, page, at);
+    const CacheSide& c = r.cache.side[k];
+    return page * c.s[0] + at * c.s[1] + h * c.s[2];
+}
+__device__ __forceinline__ int8_t* exponent_at(const Rows& r, int k, int slot, uint32_t h) {
+    uint32_t page, at;
+    r.cache.page_div.divmod((uint32_t)slot, page, at);
+    const CacheSide& c = r.cache.side[k];
+    return c.exponents + page * c.es[0] + at * c.es[1] + h * c.es[2];
+}
+
+// A group of 2^lanes_log lanes stores the key and the value of one head of one token, a lane every N elements, kAhead heads on
+// their way at a time.  Of the tokens that name one slot the last is stored: a block looks for its slots among those of the
+// tokens behind it (a bit for each of its slots modulo kBits tells nearly all of them apart at once; modulo 2,048, where one in
+// 70 was mistaken, the search took most of the time: 70 us for [16384 tokens, 8 heads of 128]), while its first rows come.
+// Bound by HBM.
+constexpr int kAhead = 4;
+constexpr uint32_t kBits = 32768;
+
+// The largest finite magnitude of a group's row, as a float's bits; bad: some row of the warp has others.  (Of half types the
+// magnitudes are compared two at a time as they are, and only where one is not finite each by itself.)
+template <typename T, int N, bool ONE>
+__device__ __forceinline__ uint32_t largest(const Piece<T, N>& x, const T* src, uint32_t lane, uint32_t lanes, uint32_t pieces, bool& bad) {
+    if constexpr (ONE && N == 8 && sizeof(T) == 2) {
+        constexpr uint32_t kInfinite = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, x.v.w[i] & 0x7FFF7FFFu);
+        if (lane >= pieces) m = 0;
+#pragma unroll
+        for (uint32_t d = 16; d; d /= 2)
+            if (d < lanes) m = __vmaxu2(m, __shfl_xor_sync(~0u, m, d));
+        m = max(m & 0xFFFFu, m >> 16);
+        bad = __any_sync(~0u, m >= kInfinite);
+        if (!bad) return std::is_same_v<T, __half> ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))) : m << 16;
+    }
+    uint32_t top = 0;
+    bad = true;
+    for (uint32_t p = lane; p < pieces; p += lanes) {
+        Piece<T, N> y = x;
+        if (!ONE && p != lane) y.load(src + p * N);
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = max(top, finite_bits(y.get(i)));
+    }
+    __syncwarp();
+    for (uint32_t d = lanes / 2; d; d /= 2) top = max(top, __shfl_xor_sync(~0u, top, d));
+    return top;
+}
+
+template <typename T, int N, bool SMALL, bool ONE>  // ONE: no lane has more than one piece
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const Rows r) {
     __shared__ int slots[kMaxTile];
     __shared__ bool again[kMaxTile];
-    __shared__ uint32_t seen[64];
+    __shared__ uint64_t places[2][kMaxTile], exponents[2][kMaxTile];  // of a token's slot
+    __shared__ uint32_t seen[kBits / 32];
     const uint32_t t0 = blockIdx.x * r.tile, n = min(r.tile, r.tokens - t0);
-    if (threadIdx.x < 64) seen[threadIdx.x] = 0;
+    const uint32_t lanes = 1u << r.lanes_log, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> r.lanes_log;
+    const uint32_t groups = kThreads >> r.lanes_log, pieces = r.head / N, items = n * r.heads;
+    Piece<T, N> x[kAhead][2];
+    auto row = [&](int k, uint32_t token, uint32_t h) {
+        return static_cast<const T*>(r.rows[k]) + (uint64_t)(t0 + token) * r.rs[k][0] + h * r.rs[k][1];
+    };
+    auto load = [&](uint32_t first) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t item = first + a * groups + group;
+            uint32_t token, h;
+            r.heads_div.divmod(item, token, h);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (item < items && lane < pieces) x[a][k].load(row(k, token, h) + lane * N);
+        }
+    };
+    load(0);
+    for (uint32_t i = threadIdx.x; i < kBits / 32; i += kThreads) seen[i] = 0;
     __syncthreads();
     if (threadIdx.x < n) {
         const int s = slot_of(r, t0 + threadIdx.x);
         slots[threadIdx.x] = s;
         again[threadIdx.x] = false;
-        if (s >= 0) atomicOr(&seen[s % 2048 / 32], 1u << (s % 32));
+        if (s >= 0) {
+            atomicOr(&seen[s % kBits / 32], 1u << (s % 32));
+            uint32_t page, at;
+            r.cache.page_div.divmod((uint32_t)s, page, at);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const CacheSide& c = r.cache.side[k];
+                places[k][threadIdx.x] = page * c.s[0] + at * c.s[1];
+                exponents[k][threadIdx.x] = page * c.es[0] + at * c.es[1];
+            }
+        }
     }
     __syncthreads();
-    for (uint32_t t = t0 + 1 + threadIdx.x; t < r.tokens; t += kThreads) {
-        const int s = slot_of(r, t);
-        if (s >= 0 && (seen[s % 2048 / 32] >> (s % 32) & 1))
+    auto look = [&](uint32_t t, int s) {
+        if (seen[(uint32_t)s % kBits / 32] >> (s & 31) & 1)
             for (uint32_t i = 0; i < n && t0 + i < t; ++i)
                 if (slots[i] == s) again[i] = true;
-    }
-    __syncthreads();
-    const uint32_t lanes = 1u << r.lanes_log, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> r.lanes_log;
-    const uint32_t groups = kThreads >> r.lanes_log, pieces = r.head / N, items = n * r.heads;
-    for (uint32_t base = 0; base < items; base += groups) {
-        const uint32_t item = base + group;
-        uint32_t token, h;
-        r.heads_div.divmod(item, token, h);
-        const int slot = item < items && !again[token] ? slots[token] : -1;
-        uint32_t page = 0, at = 0;
-        if (slot >= 0) r.cache.page_div.divmod((uint32_t)slot, page, at);
-        const T* src[2];
-        Piece<T, N> x[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            src[k] = static_cast<const T*>(r.rows[k]) + (uint64_t)(t0 + token) * r.rs[k][0] + h * r.rs[k][1];
-            if (slot >= 0 && lane < pieces) x[k].load(src[k] + lane * N);
+    };
+    uint32_t from = t0 + 1;
+    if (r.four_slots) {
+        // four at a time, sixteen on their way
+        const uint32_t end = r.tokens / 4;
+#pragma unroll 4
+        for (uint32_t q = (from + 3) / 4 + threadIdx.x; q < end; q += kThreads) {
+            const int4 v = __ldg(static_cast<const int4*>(r.slots) + q);
+            look(4 * q, v.x), look(4 * q + 1, v.y), look(4 * q + 2, v.z), look(4 * q + 3, v.w);
         }
+        // what is left at both ends: fewer than eight
+        const uint32_t t = threadIdx.x < 4 ? from + threadIdx.x : 4 * end + threadIdx.x - 4;
+        if (threadIdx.x < 8 && t < r.tokens && (threadIdx.x >= 4 ? t >= from : t < (from + 3) / 4 * 4)) look(t, slot_of(r, t));
+        from = r.tokens;
+    }
+#pragma unroll 4
+    for (uint32_t t = from + threadIdx.x; t < r.tokens; t += kThreads) look(t, slot_of(r, t));
+    __syncthreads();
+    for (uint32_t first = 0; first < items; first += kAhead * groups) {
+        if (first) load(first);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const CacheSide& c = r.cache.side[k];
-            const uint64_t to = page * c.s[0] + at * c.s[1] + h * c.s[2];
-            if constexpr (SMALL) {
-                uint32_t top = 0;
-                if (slot >= 0)
+        for (int a = 0; a < kAhead; ++a) {
+            if (first + a * groups >= items) break;  // for the whole block
+            const uint32_t item = first + a * groups + group;
+            uint32_t token, h;
+            r.heads_div.divmod(item, token, h);
+            const bool stored = item < items && !again[token] && slots[token] >= 0;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const CacheSide& c = r.cache.side[k];
+                const T* const src = ONE ? nullptr : row(k, token, h);
+                const uint32_t mine = stored ? pieces : 0;
+                if constexpr (SMALL) {
+                    bool bad;
+                    const int e = exponent_of(largest<T, N, ONE>(x[a][k], src, lane, lanes, mine, bad));
+                    if (!stored) continue;
+                    const float scale = power_of_two(-e);
+                    uint8_t* const to = static_cast<uint8_t*>(c.data) + places[k][token] + h * c.s[2];
                     for (uint32_t p = lane; p < pieces; p += lanes) {
-                        Piece<T, N> y = x[k];
-                        if (p != lane) y.load(src[k] + p * N);
+                        Piece<T, N> y = x[a][k];
+                        if (!ONE && p != lane) y.load(src + p * N);
+                        float q[N];
 #pragma unroll
-                        for (int i = 0; i < N; ++i) top = max(top, finite_bits(y.get(i)));
+                        for (int i = 0; i < N; ++i) {
+                            const float v = y.get(i);
+                            q[i] = bad ? fmaf(v, scale, v - v) : v * scale;  // an infinity becomes NaN: the type has none
+                        }
+                        store_bytes<N>(to + p * N, q);
+                        if (ONE) break;
                     }
-                for (uint32_t m = lanes / 2; m; m /= 2) top = max(top, __shfl_xor_sync(~0u, top, m));
-                if (slot < 0) continue;
-                const int e = exponent_of(top);
-                const float scale = power_of_two(-e);
-                for (uint32_t p = lane; p < pieces; p += lanes) {
-                    Piece<T, N> y = x[k];
-                    if (p != lane) y.load(src[k] + p * N);
-                    float q[N];
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float v = y.get(i);
-                        q[i] = fmaf(v, scale, v - v);  // an infinity becomes NaN: the type has none
+                    if (lane == 0) c.exponents[exponents[k][token] + h * c.es[2]] = (int8_t)e;
+                } else {
+                    T* const to = static_cast<T*>(c.data) + places[k][token] + h * c.s[2];
+                    for (uint32_t p = lane; p < mine; p += lanes) {
+                        Piece<T, N> y = x[a][k];
+                        if (!ONE && p != lane) y.load(src + p * N);
+                        y.store(to + p * N);
+                        if (ONE) break;
                     }
-                    store_bytes<N>(static_cast<uint8_t*>(c.data) + to + p * N, q);
-                }
-                if (lane == 0) c.exponents[page * c.es[0] + at * c.es[1] + h * c.es[2]] = (int8_t)e;
-            } else {
-                if (slot < 0) continue;
-                for (uint32_t p = lane; p < pieces; p += lanes) {
-                    Piece<T, N> y = x[k];
-                    if (p != lane) y.load(src[k] + p * N);
-                    y.store(static_cast<T*>(c.data) + to + p * N);
                 }
             }
         }
     }
 }
 
+// The way back: the slots of kAhead heads, then their rows, then what is stored.
 template <typename T, int N, bool SMALL>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const Rows r) {
+    using Held = std::conditional_t<SMALL, uint8_t, T>;
+    struct Eight {  // eight bytes, or what a Piece has
+        Piece<T, N> v;
+        uint2 w;
+    };
     const uint32_t lanes = 1u << r.lanes_log, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> r.lanes_log;
     const uint32_t groups = kThreads >> r.lanes_log, pieces = r.head / N;
-    const uint64_t items = (uint64_t)r.tokens * r.heads;
-    for (uint64_t item = (uint64_t)blockIdx.x * groups + group; item < items; item += (uint64_t)gridDim.x * groups) {
-        const uint32_t token = (uint32_t)(item / r.heads), h = (uint32_t)(item - (uint64_t)token * r.heads);
-        const int slot = slot_of(r, token);
-        uint32_t page = 0, at = 0;
-        if (slot >= 0) r.cache.page_div.divmod((uint32_t)slot, page, at);
+    const uint64_t items = (uint64_t)r.tokens * r.heads, step = (uint64_t)gridDim.x * groups;
+    for (uint64_t first = (uint64_t)blockIdx.x * groups + group; first < items; first += kAhead * step) {
+        int slot[kAhead];
+        uint32_t token[kAhead], h[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint64_t item = first + a * step;
+            token[a] = (uint32_t)(item / r.heads), h[a] = (uint32_t)(item - (uint64_t)token[a] * r.heads);
+            slot[a] = item < items ? slot_of(r, token[a]) : -2;
+        }
         for (uint32_t p = lane; p < pieces; p += lanes) {
+            Eight x[kAhead][2] = {};
+            int8_t e[kAhead][2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const CacheSide& c = r.cache.side[k];
-                T* dst = static_cast<T*>(r.rows[k]) + (uint64_t)token * r.rs[k][0] + h * r.rs[k][1] + p * N;
-                const uint64_t from = page * c.s[0] + at * c.s[1] + h * c.s[2] + p * N;
-                if constexpr (!SMALL) {
-                    Piece<T, N> y{};
-                    if (slot >= 0) y.load(static_cast<const T*>(c.data) + from);
-                    y.store(dst);
-                } else {
-                    float scale = 0.0f;
-                    if (slot >= 0) scale = power_of_two(c.exponents[page * c.es[0] + at * c.es[1] + h * c.es[2]]);
-                    const uint8_t* bytes = static_cast<const uint8_t*>(c.data) + from;
-                    if constexpr (N == 8) {
-                        uint2 w = make_uint2(0, 0);
-                        if (slot >= 0) w = *reinterpret_cast<const uint2*>(bytes);
-                        Few<T, 8> y;
+            for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 v = from_e4m3((i < 2 ? w.x : w.y) >> (i % 2 * 16) & 0xFFFFu);
-                            y.set2(i, v.x * scale, v.y * scale);
-                        }
-                        y.store(dst);
-                    } else *dst = from_float<T>(slot >= 0 ? from_e4m3(*bytes).x * scale : 0.0f);
+                for (int k = 0; k < 2; ++k) {
+                    if (slot[a] < 0) continue;
+                    const Held* const from = static_cast<const Held*>(r.cache.side[k].data) + row_at(r, k, slot[a], h[a]) + p * N;
+                    if constexpr (SMALL) {
+                        e[a][k] = *exponent_at(r, k, slot[a], h[a]);
+                        if constexpr (N == 8) x[a][k].w = *reinterpret_cast<const uint2*>(from);
+                        else x[a][k].w.x = *from;
+                    } else x[a][k].v.load(from);
+                }
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                if (slot[a] == -2) continue;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    T* const dst = static_cast<T*>(r.rows[k]) + (uint64_t)token[a] * r.rs[k][0] + h[a] * r.rs[k][1] + p * N;
+                    if constexpr (SMALL) {
+                        const float scale = slot[a] < 0 ? 0.0f : power_of_two(e[a][k]);
+                        if constexpr (N == 8) {
+                            Few<T, 8> y;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 v = from_e4m3((i < 2 ? x[a][k].w.x : x[a][k].w.y) >> (i % 2 * 16) & 0xFFFFu);
+                                y.set2(i, v.x * scale, v.y * scale);
+                            }
+                            y.store(dst);
+                        } else *dst = from_float<T>(from_e4m3(x[a][k].w.x).x * scale);
+                    } else x[a][k].v.store(dst);
                 }
             }
         }
@@ -262,16 +366,22 @@ extern "C" int mtxc_cache_write(int dtype, const mtxc_cache_rows_args* a) {
             c.tokens = (uint32_t)std::min<uint64_t>(kChunk, a->tokens - first);
             for (int k = 0; k < 2; ++k) c.rows[k] = static_cast<T*>(r.rows[k]) + first * r.rs[k][0];
             c.slots = static_cast<const char*>(r.slots) + first * r.slot_stride * (r.wide_slots ? 8 : 4);
-            c.tile = std::max(1u, std::min(kMaxTile, c.tokens / (4u * ctx().sm_count)));
+            c.four_slots = !c.wide_slots && c.slot_stride == 1 && aligned16(c.slots);
+            // one wave of MTX_WB blocks an SM where the tiles allow
+            c.tile = std::min(kMaxTile, (c.tokens + MTX_WB * ctx().sm_count - 1) / (MTX_WB * ctx().sm_count));
             const unsigned blocks = (c.tokens + c.tile - 1) / c.tile;
             cudaStream_t st = ctx().stream();
+            const bool one = c.head / (eights ? 8 : 1) <= 1u << c.lanes_log;
             auto run = [&](auto n, auto s) {
-                cache_write_kernel<T, decltype(n)::value, decltype(s)::value><<<blocks, kThreads, 0, st>>>(c);
+                constexpr int N = decltype(n)::value;
+                constexpr bool S = decltype(s)::value;
+                if (one) cache_write_kernel<T, N, S, true><<<blocks, kThreads, 0, st>>>(c);
+                else cache_write_kernel<T, N, S, false><<<blocks, kThreads, 0, st>>>(c);
             };
-            using one = std::integral_constant<int, 1>;
+            using single = std::integral_constant<int, 1>;
             using eight = std::integral_constant<int, 8>;
-            if (small) eights ? run(eight(), std::true_type()) : run(one(), std::true_type());
-            else eights ? run(eight(), std::false_type()) : run(one(), std::false_type());
+            if (small) eights ? run(eight(), std::true_type()) : run(single(), std::true_type());
+            else eights ? run(eight(), std::false_type()) : run(single(), std::false_type());
             rc = check_launch("cache_write_kernel");
         }
     });
@@ -289,7 +399,7 @@ extern "C" int mtxc_cache_read(int dtype, const mtxc_cache_rows_args* a) {
         using T = std::remove_pointer_t<decltype(t)>;
         const bool eights = by_eights<T>(r, small);
         const uint64_t groups = kThreads >> r.lanes_log, items = (uint64_t)r.tokens * r.heads;
-        const unsigned blocks = (unsigned)std::min<uint64_t>((items + groups - 1) / groups, 8u * ctx().sm_count);
+        const unsigned blocks = (unsigned)std::min<uint64_t>((items + groups - 1) / groups, 4u * ctx().sm_count);
         cudaStream_t st = ctx().stream();
         auto run = [&](auto n, auto s) {
             cache_read_kernel<T, decltype(n)::value, decltype(s)::value><<<blocks, kThreads, 0, st>>>(r);

@@ -12,9 +12,7 @@ namespace mtxc {
 namespace {
 
 constexpr int kThreads = 256;
-#ifndef MTX_WB
-#define MTX_WB 4
-#endif
+constexpr uint32_t kBlocksPerSm = 4;
 constexpr uint32_t kMaxTile = 64;
 constexpr uint32_t kChunk = 16384;  // tokens of a launch of the write
 constexpr uint32_t kMaxHead = 1024;
@@ -94,7 +92,7 @@ __device__ __forceinline__ int8_t* exponent_at(const Rows& r, int k, int slot, u
 // tokens behind it (a bit for each of its slots modulo kBits tells nearly all of them apart at once; modulo 2,048, where one in
 // 70 was mistaken, the search took most of the time: 70 us for [16384 tokens, 8 heads of 128]), while its first rows come.
 // Bound by HBM.
-constexpr int kAhead = 4;
+constexpr int kAhead = 2;
 constexpr uint32_t kBits = 32768;
 
 // The largest finite magnitude of a group's row, as a float's bits; bad: some row of the warp has others.  (Of half types the
@@ -367,8 +365,9 @@ extern "C" int mtxc_cache_write(int dtype, const mtxc_cache_rows_args* a) {
             for (int k = 0; k < 2; ++k) c.rows[k] = static_cast<T*>(r.rows[k]) + first * r.rs[k][0];
             c.slots = static_cast<const char*>(r.slots) + first * r.slot_stride * (r.wide_slots ? 8 : 4);
             c.four_slots = !c.wide_slots && c.slot_stride == 1 && aligned16(c.slots);
-            // one wave of MTX_WB blocks an SM where the tiles allow
-            c.tile = std::min(kMaxTile, (c.tokens + MTX_WB * ctx().sm_count - 1) / (MTX_WB * ctx().sm_count));
+            // one wave of blocks where the tiles allow
+            const uint32_t wave = kBlocksPerSm * ctx().sm_count;
+            c.tile = std::min(kMaxTile, (c.tokens + wave - 1) / wave);
             const unsigned blocks = (c.tokens + c.tile - 1) / c.tile;
             cudaStream_t st = ctx().stream();
             const bool one = c.head / (eights ? 8 : 1) <= 1u << c.lanes_log;
@@ -399,7 +398,7 @@ extern "C" int mtxc_cache_read(int dtype, const mtxc_cache_rows_args* a) {
         using T = std::remove_pointer_t<decltype(t)>;
         const bool eights = by_eights<T>(r, small);
         const uint64_t groups = kThreads >> r.lanes_log, items = (uint64_t)r.tokens * r.heads;
-        const unsigned blocks = (unsigned)std::min<uint64_t>((items + groups - 1) / groups, 4u * ctx().sm_count);
+        const unsigned blocks = (unsigned)std::min<uint64_t>((items + groups - 1) / groups, (uint64_t)kBlocksPerSm * ctx().sm_count);
         cudaStream_t st = ctx().stream();
         auto run = [&](auto n, auto s) {
             cache_read_kernel<T, decltype(n)::value, decltype(s)::value><<<blocks, kThreads, 0, st>>>(r);

@@ -36,25 +36,33 @@ __device__ __forceinline__ void rows_of(const int* starts, uint32_t i, uint32_t 
 }
 
 // ------------------------------------------------------------------------------------------
-// Any head and type: 64 queries and 64 keys at a time, products in 32 bits.
+// Any head and type: 16 ROWS queries and 64 keys at a time, products in 32 bits on the multipliers, a thread ROWS rows by 4 keys
+// of the scores and by up to 16 elements of the output.  The next keys come while the weights meet the values, the next values
+// while the scores are made.  ROWS = 2 where there would be fewer than four blocks of 64 rows an SM: its blocks are half as long
+// ([500, 228, 381] f32, 8 heads of 80: a row of tiles of 64 keys is all that the longest block has).
 // ------------------------------------------------------------------------------------------
 __host__ __device__ inline uint32_t pitch_of(uint32_t head) { return (head + 3) / 8 * 8 + 4; }  // an odd number of 16-byte units
+constexpr uint32_t kTilePitch = kAnyTile + 4;
 
-template <typename T>
+template <int ROWS>
+uint32_t any_bytes(uint32_t head) { return (uint32_t)sizeof(float) * ((16 * ROWS + 2 * kAnyTile) * pitch_of(head) + 16 * ROWS * kTilePitch); }
+
+template <typename T, int ROWS, bool WHOLE>  // WHOLE: float, by 16-byte units
 __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p) {
     extern __shared__ float4 smem4[];
-    __shared__ uint64_t buf[33];
+    __shared__ uint64_t buf[kAnyThreads / 32];
     __shared__ Found found;
-    constexpr uint32_t kTilePitch = kAnyTile + 4;
+    constexpr uint32_t kRows = 16 * ROWS;
     const uint32_t pitch = pitch_of(p.head), quads = (p.head + 3) / 4;
-    float* const q = reinterpret_cast<float*>(smem4);    // [64][pitch]
-    float* const kv = q + kAnyTile * pitch;              // [64][pitch]: keys, then values
-    float* const weights = kv + kAnyTile * pitch;        // [64][kTilePitch]
+    float* const q = reinterpret_cast<float*>(smem4);    // [kRows][pitch]
+    float* const keys = q + kRows * pitch;               // [64][pitch]
+    float* const values = keys + kAnyTile * pitch;       // [64][pitch]
+    float* const weights = values + kAnyTile * pitch;    // [kRows][kTilePitch]
     // the last sequence first, and in each the last tile first: of causal ones the longest
     auto count = [&](uint32_t i) {
         uint32_t first, n;
         rows_of(p.starts, p.sequences - 1 - i, p.tokens, first, n);
-        return (uint64_t)(n + kAnyTile - 1) / kAnyTile;
+        return (uint64_t)(n + kRows - 1) / kRows;
     };
     const Found f = find(p.sequences, blockIdx.x, count, buf, &found);
     if (!f.any) return;
@@ -62,40 +70,53 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
     uint32_t q_first, n, k_first, m;
     rows_of(p.starts, i, p.tokens, q_first, n);
     rows_of(p.k_starts, i, p.k_tokens, k_first, m);
-    const uint32_t row0 = ((n + kAnyTile - 1) / kAnyTile - 1 - (uint32_t)(blockIdx.x - f.first)) * kAnyTile;
+    const uint32_t row0 = ((n + kRows - 1) / kRows - 1 - (uint32_t)(blockIdx.x - f.first)) * kRows;
     const int64_t ahead = (int64_t)m - n;  // a query sees keys up to its own index plus this
-    auto load = [&](float* to, const void* from, const uint64_t (&s)[2], uint32_t first, uint32_t head, uint32_t rows) {
-        const T* x = static_cast<const T*>(from) + head * s[1];
-        for (uint32_t e = threadIdx.x; e < kAnyTile * quads * 4; e += kAnyThreads) {
-            const uint32_t r = e / (quads * 4), c = e - r * (quads * 4);
-            to[r * pitch + c] = r < rows && c < p.head ? to_float(x[(uint64_t)(first + r) * s[0] + c]) : 0.0f;
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    // a warp a row; rows and elements that are not there are zeros
+    auto load = [&](float* to, const void* from, const uint64_t (&s)[2], uint32_t first, uint32_t head, uint32_t rows, uint32_t all) {
+        const T* x = static_cast<const T*>(from) + head * s[1] + (uint64_t)first * s[0];
+        for (uint32_t r = warp; r < all; r += kAnyThreads / 32) {
+            if constexpr (WHOLE) {
+                for (uint32_t c = lane; c < quads; c += 32)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + r * pitch + 4 * c)),
+                                 "l"(r < rows ? x + (uint64_t)r * s[0] + 4 * c : static_cast<const T*>(from)), "r"(r < rows ? 16 : 0)
+                                 : "memory");
+            } else {
+                for (uint32_t c = lane; c < 4 * quads; c += 32)
+                    to[r * pitch + c] = r < rows && c < p.head ? to_float(x[(uint64_t)r * s[0] + c]) : 0.0f;
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    load(q, p.q, p.qs, q_first + row0, h, min(kAnyTile, n - row0));
-    const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // rows 4 ty .., keys tx + 16 j, columns 4 tx + 64 c
-    float top[4], sum[4];
-    float4 acc[4][kMaxHead / 64];
+    const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // rows ROWS ty .., keys tx + 16 j, columns 4 tx + 64 c
+    float top[ROWS], sum[ROWS];
+    float4 acc[ROWS][kMaxHead / 64];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
+    for (int a = 0; a < ROWS; ++a) {
         top[a] = -INFINITY, sum[a] = 0.0f;
 #pragma unroll
         for (uint32_t c = 0; c < kMaxHead / 64; ++c) acc[a][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    int64_t last = p.causal ? min((int64_t)m, (int64_t)min(row0 + kAnyTile, n) + ahead) : (int64_t)m;  // keys seen by any row
+    const int64_t last = p.causal ? min((int64_t)m, (int64_t)min(row0 + kRows, n) + ahead) : (int64_t)m;  // keys seen by any row
+    auto keys_of = [&](int64_t k0) { return (uint32_t)max((int64_t)0, min((int64_t)kAnyTile, m - k0)); };
+    load(q, p.q, p.qs, q_first + row0, h, min(kRows, n - row0), kRows);
+    load(keys, p.k, p.ks, k_first, kh, last > 0 ? keys_of(0) : 0, kAnyTile);
+    load(values, p.v, p.vs, k_first, kh, last > 0 ? keys_of(0) : 0, kAnyTile);
     for (int64_t k0 = 0; k0 < last; k0 += kAnyTile) {
-        const uint32_t keys = (uint32_t)min((int64_t)kAnyTile, m - k0);
+        const uint32_t there = keys_of(k0);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the values
         __syncthreads();
-        load(kv, p.k, p.ks, k_first + (uint32_t)k0, kh, keys);
-        __syncthreads();
-        float s[4][4] = {};
+        float s[ROWS][4] = {};
+#pragma unroll 2
         for (uint32_t c = 0; c < quads; ++c) {
-            float4 x[4], y[4];
+            float4 x[ROWS], y[4];
 #pragma unroll
-            for (int a = 0; a < 4; ++a) x[a] = *reinterpret_cast<const float4*>(q + (4 * ty + a) * pitch + 4 * c);
+            for (int a = 0; a < ROWS; ++a) x[a] = *reinterpret_cast<const float4*>(q + (ROWS * ty + a) * pitch + 4 * c);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) y[b] = *reinterpret_cast<const float4*>(kv + (tx + 16 * b) * pitch + 4 * c);
+            for (int b = 0; b < 4; ++b) y[b] = *reinterpret_cast<const float4*>(keys + (tx + 16 * b) * pitch + 4 * c);
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < ROWS; ++a)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     s[a][b] = fmaf(x[a].x, y[b].x, s[a][b]);
@@ -104,20 +125,19 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
                     s[a][b] = fmaf(x[a].w, y[b].w, s[a][b]);
                 }
         }
-        __syncthreads();
-        load(kv, p.v, p.vs, k_first + (uint32_t)k0, kh, keys);
+        int limit[ROWS];  // the last key of this tile that a row sees
+        bool all = true;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int64_t limit = p.causal ? (int64_t)row0 + 4 * ty + a + ahead : (int64_t)m - 1;
+        for (int a = 0; a < ROWS; ++a) {
+            const int64_t sees = (p.causal ? min((int64_t)m - 1, (int64_t)row0 + ROWS * ty + a + ahead) : (int64_t)m - 1) - k0;
+            limit[a] = (int)max((int64_t)-1, min((int64_t)kAnyTile - 1, sees));
+            all = all && limit[a] == kAnyTile - 1;
             float now = -INFINITY;
-            bool seen[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int64_t j = k0 + tx + 16 * b;
-                seen[b] = j < m && j <= limit;
                 s[a][b] *= p.scale;
                 // a key that counts lifts the maximum off -infinity even where its score is -infinity
-                if (seen[b]) now = fmaxf(now, fmaxf(s[a][b], kLowest));
+                if ((int)tx + 16 * b <= limit[a]) now = fmaxf(now, fmaxf(s[a][b], kLowest));
             }
 #pragma unroll
             for (int d = 8; d; d /= 2) now = fmaxf(now, __shfl_xor_sync(~0u, now, d));
@@ -127,9 +147,9 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
             float part = 0.0f;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const float w = seen[b] ? exp2f(s[a][b] - now) : 0.0f;
+                const float w = (int)tx + 16 * b <= limit[a] ? exp2f(s[a][b] - now) : 0.0f;
                 part += w;
-                weights[(4 * ty + a) * kTilePitch + tx + 16 * b] = w;
+                weights[(ROWS * ty + a) * kTilePitch + tx + 16 * b] = w;
             }
             sum[a] = sum[a] * factor + part;
 #pragma unroll
@@ -137,35 +157,48 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
                 acc[a][c].x *= factor, acc[a][c].y *= factor, acc[a][c].z *= factor, acc[a][c].w *= factor;
             }
         }
-        __syncthreads();
-        int seen_to[4];  // what a row does not see may hold anything
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the scores are made, the values have come
+        const int64_t next = k0 + kAnyTile;
+        load(keys, p.k, p.ks, k_first + (uint32_t)next, kh, next < last ? keys_of(next) : 0, next < last ? kAnyTile : 0);
+        auto add = [&](float w, const float4& y, float4& o) {
+            o.x = fmaf(w, y.x, o.x), o.y = fmaf(w, y.y, o.y), o.z = fmaf(w, y.z, o.z), o.w = fmaf(w, y.w, o.w);
+        };
+        for (uint32_t j = 0; j < there; j += 4) {
+            float4 w[ROWS];
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
-            seen_to[a] = p.causal ? (int)max((int64_t)-1, min((int64_t)kAnyTile, (int64_t)row0 + 4 * ty + a + ahead - k0)) : (int)kAnyTile;
-        for (uint32_t j = 0; j < keys; ++j) {
-            float w[4];
-#pragma unroll
-            for (int a = 0; a < 4; ++a) w[a] = weights[(4 * ty + a) * kTilePitch + j];
+            for (int a = 0; a < ROWS; ++a) w[a] = *reinterpret_cast<const float4*>(weights + (ROWS * ty + a) * kTilePitch + j);
 #pragma unroll
             for (uint32_t c = 0; c < kMaxHead / 64; ++c) {
                 if (tx + 16 * c >= quads) break;
-                const float4 y = *reinterpret_cast<const float4*>(kv + j * pitch + 4 * (tx + 16 * c));
+                const float* const v = values + j * pitch + 4 * (tx + 16 * c);
+                float4 y[4];
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    if ((int)j > seen_to[a]) continue;
-                    acc[a][c].x = fmaf(w[a], y.x, acc[a][c].x);
-                    acc[a][c].y = fmaf(w[a], y.y, acc[a][c].y);
-                    acc[a][c].z = fmaf(w[a], y.z, acc[a][c].z);
-                    acc[a][c].w = fmaf(w[a], y.w, acc[a][c].w);
+                for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const float4*>(v + e * pitch);
+                if (all) {
+#pragma unroll
+                    for (int a = 0; a < ROWS; ++a) add(w[a].x, y[0], acc[a][c]), add(w[a].y, y[1], acc[a][c]), add(w[a].z, y[2], acc[a][c]), add(w[a].w, y[3], acc[a][c]);
+                } else {
+                    // what a row does not see may hold anything
+#pragma unroll
+                    for (int a = 0; a < ROWS; ++a) {
+                        if ((int)j <= limit[a]) add(w[a].x, y[0], acc[a][c]);
+                        if ((int)j + 1 <= limit[a]) add(w[a].y, y[1], acc[a][c]);
+                        if ((int)j + 2 <= limit[a]) add(w[a].z, y[2], acc[a][c]);
+                        if ((int)j + 3 <= limit[a]) add(w[a].w, y[3], acc[a][c]);
+                    }
                 }
             }
         }
+        __syncthreads();
+        load(values, p.v, p.vs, k_first + (uint32_t)next, kh, next < last ? keys_of(next) : 0, next < last ? kAnyTile : 0);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
+    for (int a = 0; a < ROWS; ++a) {
 #pragma unroll
         for (int d = 8; d; d /= 2) sum[a] += __shfl_xor_sync(~0u, sum[a], d);
-        const uint32_t row = row0 + 4 * ty + a;
+        const uint32_t row = row0 + ROWS * ty + a;
         if (row >= n) continue;
         T* out = static_cast<T*>(p.out) + (uint64_t)(q_first + row) * p.os[0] + h * p.os[1];
         const bool any = top[a] != -INFINITY;
@@ -178,6 +211,29 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
                 if (at + e < p.head) out[at + e] = from_float<T>(any ? o[e] / sum[a] : 0.0f);
         }
     }
+}
+
+template <typename T, int ROWS, bool WHOLE>
+int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
+    // the same limit in every call: calls from several threads do not undo each other's
+    cudaError_t err = cudaFuncSetAttribute(prompt_any_kernel<T, ROWS, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_bytes<ROWS>(kMaxHead));
+    if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
+    // as many tiles as the sequences can have: one each may be part filled
+    const uint64_t tiles = a->tokens / (16 * ROWS) + std::min(a->sequences, a->tokens);
+    prompt_any_kernel<T, ROWS, WHOLE><<<dim3((unsigned)tiles, a->heads), kAnyThreads, any_bytes<ROWS>(p.head), ctx().stream()>>>(p);
+    return check_launch("prompt_any_kernel");
+}
+
+template <typename T>
+int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
+    const bool few = (a->tokens / 64 + std::min(a->sequences, a->tokens)) * a->heads < 4u * ctx().sm_count;
+    if constexpr (std::is_same_v<T, float>) {
+        bool whole = a->head_dim % 4 == 0;
+        for (const void* x : {a->q, a->k, a->v}) whole = whole && aligned16(x);
+        for (int i = 0; i < 2; ++i) whole = whole && a->q_strides[i] % 4 == 0 && a->k_strides[i] % 4 == 0 && a->v_strides[i] % 4 == 0;
+        if (whole) return few ? launch_any<T, 2, true>(a, p) : launch_any<T, 4, true>(a, p);
+    }
+    return few ? launch_any<T, 2, false>(a, p) : launch_any<T, 4, false>(a, p);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -671,17 +727,7 @@ extern "C" int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args
                 return;
             }
         }
-        auto smem = [](uint32_t head) { return sizeof(float) * (2 * kAnyTile * pitch_of(head) + kAnyTile * (kAnyTile + 4)); };
-        // the same limit in every call: calls from several threads do not undo each other's
-        cudaError_t err = cudaFuncSetAttribute(prompt_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem(kMaxHead));
-        if (err != cudaSuccess) {
-            rc = cuda_fail(err, "cudaFuncSetAttribute");
-            return;
-        }
-        // as many tiles as the sequences can have: one each may be part filled
-        const uint64_t tiles = a->tokens / kAnyTile + std::min(a->sequences, a->tokens);
-        prompt_any_kernel<T><<<dim3((unsigned)tiles, a->heads), kAnyThreads, smem(p.head), ctx().stream()>>>(p);
-        rc = check_launch("prompt_any_kernel");
+        rc = launch_any<T>(a, p);
     });
     return rc;
 }

@@ -47,7 +47,7 @@ constexpr uint32_t kTilePitch = kAnyTile + 4;
 template <int ROWS>
 uint32_t any_bytes(uint32_t head) { return (uint32_t)sizeof(float) * ((16 * ROWS + 2 * kAnyTile) * pitch_of(head) + 16 * ROWS * kTilePitch); }
 
-template <typename T, int ROWS, bool WHOLE>  // WHOLE: float, by 16-byte units
+template <typename T, int ROWS, int COLUMNS, bool WHOLE>  // COLUMNS: 64 elements each; WHOLE: float, by 16-byte units
 __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p) {
     extern __shared__ float4 smem4[];
     __shared__ uint64_t buf[kAnyThreads / 32];
@@ -91,12 +91,12 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
     };
     const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // rows ROWS ty .., keys tx + 16 j, columns 4 tx + 64 c
     float top[ROWS], sum[ROWS];
-    float4 acc[ROWS][kMaxHead / 64];
+    float2 acc[ROWS][COLUMNS][2];
 #pragma unroll
     for (int a = 0; a < ROWS; ++a) {
         top[a] = -INFINITY, sum[a] = 0.0f;
 #pragma unroll
-        for (uint32_t c = 0; c < kMaxHead / 64; ++c) acc[a][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int c = 0; c < COLUMNS; ++c) acc[a][c][0] = acc[a][c][1] = make_float2(0.0f, 0.0f);
     }
     const int64_t last = p.causal ? min((int64_t)m, (int64_t)min(row0 + kRows, n) + ahead) : (int64_t)m;  // keys seen by any row
     auto keys_of = [&](int64_t k0) { return (uint32_t)max((int64_t)0, min((int64_t)kAnyTile, m - k0)); };
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
         const uint32_t there = keys_of(k0);
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the values
         __syncthreads();
-        float s[ROWS][4] = {};
+        float2 even_odd[ROWS][4] = {};  // the products of even and of odd elements: two at a time
 #pragma unroll 2
         for (uint32_t c = 0; c < quads; ++c) {
             float4 x[ROWS], y[4];
@@ -119,12 +119,15 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
             for (int a = 0; a < ROWS; ++a)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    s[a][b] = fmaf(x[a].x, y[b].x, s[a][b]);
-                    s[a][b] = fmaf(x[a].y, y[b].y, s[a][b]);
-                    s[a][b] = fmaf(x[a].z, y[b].z, s[a][b]);
-                    s[a][b] = fmaf(x[a].w, y[b].w, s[a][b]);
+                    even_odd[a][b] = __ffma2_rn(make_float2(x[a].x, x[a].y), make_float2(y[b].x, y[b].y), even_odd[a][b]);
+                    even_odd[a][b] = __ffma2_rn(make_float2(x[a].z, x[a].w), make_float2(y[b].z, y[b].w), even_odd[a][b]);
                 }
         }
+        float s[ROWS][4];
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) s[a][b] = even_odd[a][b].x + even_odd[a][b].y;
         int limit[ROWS];  // the last key of this tile that a row sees
         bool all = true;
 #pragma unroll
@@ -153,23 +156,24 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
             }
             sum[a] = sum[a] * factor + part;
 #pragma unroll
-            for (uint32_t c = 0; c < kMaxHead / 64; ++c) {
-                acc[a][c].x *= factor, acc[a][c].y *= factor, acc[a][c].z *= factor, acc[a][c].w *= factor;
-            }
+            for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) acc[a][c][e] = __fmul2_rn(acc[a][c][e], make_float2(factor, factor));
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();  // the scores are made, the values have come
         const int64_t next = k0 + kAnyTile;
         load(keys, p.k, p.ks, k_first + (uint32_t)next, kh, next < last ? keys_of(next) : 0, next < last ? kAnyTile : 0);
-        auto add = [&](float w, const float4& y, float4& o) {
-            o.x = fmaf(w, y.x, o.x), o.y = fmaf(w, y.y, o.y), o.z = fmaf(w, y.z, o.z), o.w = fmaf(w, y.w, o.w);
+        auto add = [&](float w, const float4& y, float2 (&o)[2]) {
+            o[0] = __ffma2_rn(make_float2(w, w), make_float2(y.x, y.y), o[0]);
+            o[1] = __ffma2_rn(make_float2(w, w), make_float2(y.z, y.w), o[1]);
         };
         for (uint32_t j = 0; j < there; j += 4) {
             float4 w[ROWS];
 #pragma unroll
             for (int a = 0; a < ROWS; ++a) w[a] = *reinterpret_cast<const float4*>(weights + (ROWS * ty + a) * kTilePitch + j);
 #pragma unroll
-            for (uint32_t c = 0; c < kMaxHead / 64; ++c) {
+            for (int c = 0; c < COLUMNS; ++c) {
                 if (tx + 16 * c >= quads) break;
                 const float* const v = values + j * pitch + 4 * (tx + 16 * c);
                 float4 y[4];
@@ -203,9 +207,9 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
         T* out = static_cast<T*>(p.out) + (uint64_t)(q_first + row) * p.os[0] + h * p.os[1];
         const bool any = top[a] != -INFINITY;
 #pragma unroll
-        for (uint32_t c = 0; c < kMaxHead / 64; ++c) {
+        for (int c = 0; c < COLUMNS; ++c) {
             const uint32_t at = 4 * (tx + 16 * c);
-            const float o[4] = {acc[a][c].x, acc[a][c].y, acc[a][c].z, acc[a][c].w};
+            const float o[4] = {acc[a][c][0].x, acc[a][c][0].y, acc[a][c][1].x, acc[a][c][1].y};
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
                 if (at + e < p.head) out[at + e] = from_float<T>(any ? o[e] / sum[a] : 0.0f);
@@ -216,11 +220,12 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
 template <typename T, int ROWS, bool WHOLE>
 int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
     // the same limit in every call: calls from several threads do not undo each other's
-    cudaError_t err = cudaFuncSetAttribute(prompt_any_kernel<T, ROWS, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_bytes<ROWS>(kMaxHead));
+    auto kernel = p.head <= 64 ? prompt_any_kernel<T, ROWS, 1, WHOLE> : p.head <= 128 ? prompt_any_kernel<T, ROWS, 2, WHOLE> : prompt_any_kernel<T, ROWS, 4, WHOLE>;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_bytes<ROWS>(kMaxHead));
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
     // as many tiles as the sequences can have: one each may be part filled
     const uint64_t tiles = a->tokens / (16 * ROWS) + std::min(a->sequences, a->tokens);
-    prompt_any_kernel<T, ROWS, WHOLE><<<dim3((unsigned)tiles, a->heads), kAnyThreads, any_bytes<ROWS>(p.head), ctx().stream()>>>(p);
+    kernel<<<dim3((unsigned)tiles, a->heads), kAnyThreads, any_bytes<ROWS>(p.head), ctx().stream()>>>(p);
     return check_launch("prompt_any_kernel");
 }
 

@@ -1,9 +1,10 @@
-"""The row operators of matrix_b200.lm as a language model uses them: training steps of a small decoder with hand-
-written backward passes, and a decode loop that chooses tokens under penalties and a grammar mask.
+"""The operators of matrix_b200.lm as a language model uses them: training steps of a small decoder with hand-
+written backward passes, a decode loop that chooses tokens under penalties and a grammar mask, and the same model served:
+prompts of different lengths packed into one pass, then a token at a time for all of them over a paged cache.
 
-The matrix products are torch's; every other pass over the activations is this framework's: the norms around a block
-with its gate, dropout and residual, rotary positions, dropout, the softmax over the scores, the rules on the logits and
-the ArgMax that chooses.  Run it with
+The matrix products of the weights are torch's; every other pass over the activations is this framework's: the norms
+around a block with its gate, dropout and residual, the norms of the heads and their rotary positions, dropout, the softmax
+over the scores, the cache and the attention over it, the rules on the logits and the ArgMax that chooses.  Run it with
 
     python examples/language_model.py
 """
@@ -28,9 +29,10 @@ def softmax(x: torch.Tensor) -> torch.Tensor:
 
 class Decoder:
     """Embedding, one attention block, one feed-forward block (each between two norms, with a gate per channel), and
-    logits from the embedding's transpose.  All parameters float32."""
+    logits from the embedding's transpose.  head_norm: queries and keys are normed for each head before they are turned.
+    All parameters float32."""
 
-    def __init__(self, vocab=256, width=64, heads=4, kv_heads=2, hidden=128, p=0.1, seed=0, device="cuda"):
+    def __init__(self, vocab=256, width=64, heads=4, kv_heads=2, hidden=128, p=0.1, seed=0, device="cuda", head_norm=False):
         g = torch.Generator().manual_seed(seed)
 
         def normal(*shape, std):
@@ -44,12 +46,33 @@ class Decoder:
             "gate1": torch.full((width,), 0.5, device=device), "norm1": torch.ones(width, device=device),
             "post2": torch.ones(width, device=device), "gate2": torch.full((width,), 0.5, device=device),
             "norm2": torch.ones(width, device=device)}
+        self.head_norm = head_norm
+        if head_norm:
+            self.w |= {"q_norm": torch.ones(self.head, device=device), "k_norm": torch.ones(self.head, device=device)}
         self.frequencies, self.scale = lm.rotary_frequencies(self.head, device=device)
 
     def split(self, qkv):
         q, k, v = qkv.split([self.heads * self.head, self.kv_heads * self.head, self.kv_heads * self.head], -1)
         shape = (*qkv.shape[:-1], -1, self.head)
         return q.reshape(shape), k.reshape(shape), v.reshape(shape)
+
+    def turn(self, q, k, positions, save=False):
+        """Queries and keys normed, if the model does, and turned: (q, k, what the backward pass needs)."""
+        if not self.head_norm:
+            return *lm.rotary(q, k, positions, self.frequencies, scale=self.scale), None
+        o = lm.head_norm_rotary(q, k, positions, self.frequencies, q_weight=self.w["q_norm"], k_weight=self.w["k_norm"],
+                                scale=self.scale, save_rstd=save)
+        return o.q, o.k, (q, k, o.q_rstd, o.k_rstd)
+
+    def turn_backward(self, d_q, d_k, positions, saved, g):
+        """The gradients at turn's inputs; those of its weights go into g."""
+        if not self.head_norm:
+            return lm.rotary(d_q, d_k, positions, self.frequencies, scale=self.scale, inverse=True)
+        q, k, q_rstd, k_rstd = saved
+        d = lm.head_norm_rotary_backward(d_q, d_k, q, k, positions, self.frequencies, q_rstd=q_rstd, k_rstd=k_rstd,
+                                         q_weight=self.w["q_norm"], k_weight=self.w["k_norm"], scale=self.scale)
+        g["q_norm"], g["k_norm"] = d.q_weight, d.k_weight
+        return d.q, d.k
 
     # -- training ----------------------------------------------------------------------------
     def step(self, tokens: torch.Tensor, seed: int):
@@ -63,7 +86,7 @@ class Decoder:
         a0 = lm.block_norm(x0, next_weight=w["norm0"])
 
         q, k, v = self.split(a0.normed @ w["qkv"])
-        q, k = lm.rotary(q, k, positions, self.frequencies, scale=self.scale)
+        q, k, saved = self.turn(q, k, positions, save=True)
         group = self.heads // self.kv_heads
         qh, kh, vh = q.transpose(1, 2), *(t.repeat_interleave(group, 2).transpose(1, 2) for t in (k, v))
         causal = torch.ones(n, n, dtype=torch.bool, device=tokens.device).tril()
@@ -106,7 +129,7 @@ class Decoder:
         d_q = (d_scores @ kh).transpose(1, 2).contiguous()
         d_k = (d_scores.mT @ qh).transpose(1, 2).reshape(shared).sum(3)
         d_v = (probs.mT @ d_mixed).transpose(1, 2).reshape(shared).sum(3)
-        d_q, d_k = lm.rotary(d_q, d_k, positions, self.frequencies, scale=self.scale, inverse=True)
+        d_q, d_k = self.turn_backward(d_q, d_k, positions, saved, g)
         d_qkv = torch.cat([t.flatten(2) for t in (d_q, d_k, d_v)], -1)
         g["qkv"] = torch.einsum("bnd,bnc->dc", a0.normed, d_qkv)
         d0 = lm.block_norm_backward(d1.residual, d_qkv @ w["qkv"].mT, x0, next_rstd=a0.next_rstd, next_weight=w["norm0"])
@@ -137,8 +160,7 @@ class Decoder:
             x = w["embed"][tokens[:, t].long()][:, None]  # [batch, 1, width]
             a = lm.block_norm(x, next_weight=w["norm0"], save_rstd=False)
             q, k, v = self.split(a.normed @ w["qkv"])
-            at = torch.full((1,), t, dtype=torch.int32, device=dev)
-            lm.rotary(q, k, at, self.frequencies, scale=self.scale, out=(q, k))
+            q, k, _ = self.turn(q, k, torch.full((1,), t, dtype=torch.int32, device=dev))
             keys[:, :, t] = k[:, 0].repeat_interleave(group, 1)
             values[:, :, t] = v[:, 0].repeat_interleave(group, 1)
             scores = (q.transpose(1, 2) @ keys.mT / self.head ** 0.5)[:, :, 0]
@@ -157,6 +179,66 @@ class Decoder:
         return tokens[:, length:]
 
 
+    def attend(self, x, positions, cache, slots, attention):
+        """One pass of tokens [tokens, width] through the model: their keys and values go to the cache's slots, and
+        attention(q, k, v) is what their queries see.  Returns the last norm's output."""
+        w = self.w
+        a = lm.block_norm(x, next_weight=w["norm0"], save_rstd=False)
+        q, k, v = self.split(a.normed @ w["qkv"])
+        q, k, _ = self.turn(q, k, positions)
+        lm.cache_write(cache, k, v, slots)
+        mixed = attention(q, k, v).flatten(1)
+        a = lm.block_norm(x, mixed @ w["out"], post_weight=w["post1"], gate=w["gate1"], next_weight=w["norm1"], save_rstd=False)
+        return lm.block_norm(a.residual, (a.normed @ w["up"]).relu() @ w["down"], post_weight=w["post2"], gate=w["gate2"],
+                             next_weight=w["norm2"], save_rstd=False).normed
+
+    def generate(self, prompts: list, count: int, cache_dtype=torch.float32, page=8, prefix=0) -> tuple:
+        """`count` tokens more for each of prompts (token tensors of any lengths), all at once: the prompts packed into one
+        pass, then one pass a token over a paged cache.  The first `prefix` tokens of each prompt (fewer than it has) make a
+        pass of their own, and the rest of the prompt reads their keys and values back from the cache.  Returns the tokens
+        [prompts, count] and the logits that chose them [prompts, count, vocab]."""
+        w, dev, n = self.w, prompts[0].device, len(prompts)
+        lengths = [len(t) for t in prompts]
+        pages = -(-(max(lengths) + count) // page)
+        table = torch.randperm(n * pages, device=dev).to(torch.int32).view(n, pages)  # in any order
+        cache = lm.kv_cache(n * pages, page, self.kv_heads, self.head, cache_dtype, device=dev)
+
+        def slots(sequence, position):
+            return table[sequence, position // page] * page + position % page
+
+        def starts(values):
+            return torch.tensor([0, *values], device=dev).cumsum(0).to(torch.int32)
+
+        def prompt_pass(first, last):  # tokens first[i] .. last[i] - 1 of prompt i
+            tokens = torch.cat([t[a:b] for t, a, b in zip(prompts, first, last)])
+            at = torch.cat([torch.arange(a, b, device=dev) for a, b in zip(first, last)])
+            of = torch.cat([torch.full((b - a,), i, device=dev) for i, (a, b) in enumerate(zip(first, last))])
+            every = torch.cat([slots(i, torch.arange(b, device=dev)) for i, b in enumerate(last)])
+
+            def attention(q, k, v):
+                if any(first):  # what came before is in the cache
+                    k, v = lm.cache_read(cache, every, dtype=q.dtype)
+                return lm.prompt_attention(q, k, v, starts([b - a for a, b in zip(first, last)]), k_starts=starts(last))
+
+            return self.attend(w["embed"][tokens], at, cache, slots(of, at), attention)
+
+        if prefix:
+            prompt_pass([0] * n, [prefix] * n)
+        hidden = prompt_pass([prefix] * n, lengths)
+        hidden = hidden[starts([m - prefix for m in lengths])[1:].long() - 1]  # of each prompt's last token
+        tokens, chosen = torch.empty(n, count, dtype=torch.int32, device=dev), []
+        sequence, length = torch.arange(n, device=dev), torch.tensor(lengths, dtype=torch.int32, device=dev)
+        for step in range(count):
+            logits = hidden @ w["embed"].mT
+            chosen.append(logits)
+            tokens[:, step] = backend.reduce("argmax", logits, 1)
+            if step + 1 < count:
+                at = length + step
+                hidden = self.attend(w["embed"][tokens[:, step].long()], at, cache, slots(sequence, at),
+                                     lambda q, k, v: lm.decode_attention(q, cache, table, at + 1))
+        return tokens, torch.stack(chosen, 1)
+
+
 def main() -> None:
     torch.cuda.set_device(0)
     backend.init(0)
@@ -171,6 +253,7 @@ def main() -> None:
     mask = torch.zeros(8, dtype=torch.int32, device="cuda")
     mask[:2] = -1  # a grammar that allows tokens 0 .. 63
     print(model.decode(cycle[:2, :6], 10, repetition=1.0, frequency=0.0, presence=0.0, allowed=mask).tolist())
+    print(model.generate([cycle[0, :6], cycle[1, :11], cycle[2, :3]], 10)[0].tolist())
 
 
 if __name__ == "__main__":

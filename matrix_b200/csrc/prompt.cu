@@ -26,6 +26,7 @@ struct Prompt {
     FastDiv group_div;
     float scale;  // times log2(e)
     bool causal;
+    bool pairs;   // the tensor cores' kernel: two heads of a group a block, and not two tiles of a head
 };
 
 // Rows [first, first + count) of a sequence, within what there is.
@@ -244,8 +245,8 @@ int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
 // ------------------------------------------------------------------------------------------
 // Half types on the tensor cores.
 //
-// A block has NT tiles of 128 queries of one head (NT = 2 for heads of up to 128 elements) and runs along the keys in tiles
-// of 128.  Roles: four warps for each tile of queries, a thread a row, have its softmax; one warp issues the products, one
+// A block has NT tiles of 128 queries (NT = 2 for heads of up to 128 elements: of two heads that share keys, or, where groups
+// are odd, one behind the other of one head) and runs along the keys in tiles of 128.  Roles: four warps for each tile of queries, a thread a row, have its softmax; one warp issues the products, one
 // the copies, and two clean values (below).  The scores S = Q K' of a tile lie in tensor memory; a row's thread reads
 // them, writes the weights P over them in 16 bits, and the product with V takes them from there, so that neither passes
 // through shared memory.  While one tile of queries is with its softmax the tensor cores work for the other, and the product
@@ -370,8 +371,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto o_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + 3 * NT + i); };
 
     // the last sequence first, and in each the last tile first: of causal ones the longest; all heads of a tile in turn
-    constexpr uint32_t kRows = NT * kTile;
-    const uint32_t piece = blockIdx.x / p.heads, h = blockIdx.x - piece * p.heads, kh = p.group_div.div(h);
+    const uint32_t per = p.pairs ? p.heads / 2 : p.heads;
+    const uint32_t kRows = p.pairs ? kTile : NT * kTile, next_row = p.pairs ? 0 : kTile;  // from a tile of queries to the next
+    const uint32_t piece = blockIdx.x / per, which = blockIdx.x - piece * per, h = p.pairs ? 2 * which : which, kh = p.group_div.div(h);
     auto count = [&](uint32_t i) {
         uint32_t first, n;
         rows_of(p.starts, p.sequences - 1 - i, p.tokens, first, n);
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     uint32_t steps[2] = {0, 0}, most = 0;
 #pragma unroll
     for (uint32_t i = 0; i < NT; ++i) {
-        const uint32_t lo = row0 + i * kTile;
+        const uint32_t lo = row0 + i * next_row;
         if (lo >= n) continue;
         const int seen = p.causal ? max(0, min((int)m, (int)min(lo + kTile, n) + ahead)) : (int)m;
         steps[i] = ((uint32_t)seen + kTile - 1) / kTile;
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (item == 0 && steps[0]) load(q_tile(0), q_full(0), &maps.q, maps.tokens_last & 1, q_first + row0, h);
                 load(slot(s), kv && j >= partial ? raw(s) : full(s), kv ? &maps.v : &maps.k, maps.tokens_last >> (1 + kv) & 1,
                      k_first + j * kTile, kh);
-                if (NT == 2 && item == 0 && steps[1]) load(q_tile(1), q_full(1), &maps.q, maps.tokens_last & 1, q_first + row0 + kTile, h);
+                if (NT == 2 && item == 0 && steps[1]) load(q_tile(1), q_full(1), &maps.q, maps.tokens_last & 1, q_first + row0 + next_row, h + p.pairs);
             }
             // every copy ends before the block does, even where a wait has run out
             for (uint32_t item = 2 * most - min(2 * most, kSlots); failed && item < 2 * most; ++item)
@@ -484,25 +486,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (uint32_t j = partial; j < most; ++j) {
                 const uint32_t s = (2 * j + 1) % kSlots, rows = min(kTile, m - j * kTile);
                 wait(raw(s), (j - partial) / L::kAgain & 1);
-                for (uint32_t e = threadIdx.x - 320; e < kTile * (D / 8); e += 64) {
-                    const uint32_t r = e / (D / 8), c = e % (D / 8);  // 16-byte units: eight elements
-                    const uint32_t at = slot(s) + c / 8 * L::kRowTile + r * 128 + (c % 8 ^ r % 8) * 16;
-                    uint4 w;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at));
-                    if (r < rows && all_finite<T>(w)) continue;
-                    uint32_t v[4] = {w.x, w.y, w.z, w.w};
+                constexpr uint32_t kUnits = 8;  // of 16 bytes, eight elements, on their way
+                for (uint32_t e0 = threadIdx.x - 320; e0 < kTile * (D / 8); e0 += 64 * kUnits) {
+                    uint4 w[kUnits];
+                    uint32_t at[kUnits];
 #pragma unroll
-                    for (uint32_t x = 0; x < 8; ++x) {
-                        const uint32_t bits = v[x / 2] >> (x % 2 * 16) & 0xFFFFu;
-                        constexpr uint32_t kTop = kBf16 ? 0x7F80u : 0x7C00u;
-                        if (r < rows && (bits & kTop) != kTop) continue;
-                        v[x / 2] &= x % 2 ? 0xFFFFu : 0xFFFF0000u;
-                        if (r >= rows) continue;
-                        const int kind = (bits & 0x7FFFu) != kTop ? 2 : bits >> 15;
-                        atomicMin(&first_bad[kind][c * 8 + x], (int)(j * kTile + r));
-                        any_bad = 1;
+                    for (uint32_t u = 0; u < kUnits; ++u) {
+                        const uint32_t e = e0 + 64 * u, r = e / (D / 8), c = e % (D / 8);
+                        at[u] = slot(s) + c / 8 * L::kRowTile + r * 128 + (c % 8 ^ r % 8) * 16;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[u].x), "=r"(w[u].y), "=r"(w[u].z), "=r"(w[u].w) : "r"(at[u]));
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+#pragma unroll
+                    for (uint32_t u = 0; u < kUnits; ++u) {
+                        const uint32_t e = e0 + 64 * u, r = e / (D / 8), c = e % (D / 8);
+                        if (r < rows && all_finite<T>(w[u])) continue;
+                        uint32_t v[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+                        for (uint32_t x = 0; x < 8 && r < rows; ++x) {
+                            const uint32_t bits = v[x / 2] >> (x % 2 * 16) & 0xFFFFu;
+                            constexpr uint32_t kTop = kBf16 ? 0x7F80u : 0x7C00u;
+                            if ((bits & kTop) != kTop) continue;
+                            v[x / 2] &= x % 2 ? 0xFFFFu : 0xFFFF0000u;
+                            const int kind = (bits & 0x7FFFu) != kTop ? 2 : bits >> 15;
+                            atomicMin(&first_bad[kind][c * 8 + x], (int)(j * kTile + r));
+                            any_bad = 1;
+                        }
+                        if (r >= rows) v[0] = v[1] = v[2] = v[3] = 0;
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at[u]), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                    }
                 }
                 fence_async();
                 __syncwarp();
@@ -512,12 +522,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         __syncwarp();
     } else {
         registers_up<208>();
-        const uint32_t i = warp / 4, row = row0 + threadIdx.x;  // threads 128 i .. of tile i
+        const uint32_t i = warp / 4, row = row0 + i * next_row + threadIdx.x % kTile;  // threads 128 i .. of tile i
         const uint32_t lanes = (warp % 4 * 32) << 16;
         const uint32_t output = tensor + lanes + kOutput + i * D;
         const uint32_t my_steps = i < NT ? steps[i] : 0;
         const int limit = min((int)m - 1, p.causal ? (int)row + ahead : (int)m - 1);  // the last key that this row sees
-        const int least = min((int)m - 1, p.causal ? (int)(row0 + i * kTile) + ahead : (int)m - 1);
+        const int least = min((int)m - 1, p.causal ? (int)(row0 + i * next_row) + ahead : (int)m - 1);
         float top = -INFINITY, sum = 0.0f;  // top: what the weights so far refer to
         const uint32_t scores = tensor + lanes + kScores + i * kTile;
         for (uint32_t j = 0; j < my_steps; ++j) {
@@ -586,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         __syncwarp();
         tensor_fence_after();
         const bool mine = i < NT && row < n;
-        T* out = static_cast<T*>(p.out) + (uint64_t)(q_first + row) * p.os[0] + h * p.os[1];
+        T* out = static_cast<T*>(p.out) + (uint64_t)(q_first + row) * p.os[0] + (h + (p.pairs ? i : 0)) * p.os[1];
         const float inverse = failed ? NAN : limit < 0 ? 0.0f : 1.0f / sum;
         if (i < NT) {
 #pragma unroll
@@ -681,9 +691,10 @@ int launch(const mtxc_prompt_attention_args* a, const Maps& maps, const Prompt& 
     cudaError_t err = cudaFuncSetAttribute(prompt_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
     // as many tiles as the sequences can have: one each may be part filled
-    const uint64_t tiles = a->tokens / (NT * kTile) + std::min(a->sequences, a->tokens);
-    if (tiles * a->heads >> 31) return fail(MTXC_ERR_SHAPE, "mtxc_prompt_attention: too many tiles of queries and heads");
-    prompt_kernel<T, D, NT><<<(unsigned)(tiles * a->heads), kThreads, L::kBytes, ctx().stream()>>>(maps, p);
+    const uint64_t tiles = a->tokens / (p.pairs ? kTile : NT * kTile) + std::min(a->sequences, a->tokens);
+    const uint64_t per = p.pairs ? a->heads / 2 : a->heads;
+    if (tiles * per >> 31) return fail(MTXC_ERR_SHAPE, "mtxc_prompt_attention: too many tiles of queries and heads");
+    prompt_kernel<T, D, NT><<<(unsigned)(tiles * per), kThreads, L::kBytes, ctx().stream()>>>(maps, p);
     return check_launch("prompt_kernel");
 }
 
@@ -728,6 +739,8 @@ extern "C" int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args
         if constexpr (!std::is_same_v<T, float>) {
             Maps maps;
             if (prepare_maps(dtype, a, p, &maps)) {
+                // two heads that share keys see the same of them: no step has one tile of queries only
+                p.pairs = p.head <= 128 && p.group % 2 == 0;
                 rc = p.head <= 64 ? launch<T, 64, 2>(a, maps, p) : p.head <= 128 ? launch<T, 128, 2>(a, maps, p) : launch<T, 256, 1>(a, maps, p);
                 return;
             }

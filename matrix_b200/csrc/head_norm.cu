@@ -209,11 +209,11 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
         there[0] = t || i < first, there[1] = t || (i < first && i + first < rest);
         turns[0] = turns[1] = t;
     }
-    float w[2][N], dw[2][N];
+    float2 w[2][N / 2], dw[2][N / 2];  // two elements at a time: two products an instruction
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[a][i] = s.weight ? 0.0f : 1.0f, dw[a][i] = 0.0f;
+        for (int i = 0; i < N / 2; ++i) w[a][i] = s.weight ? make_float2(0.0f, 0.0f) : make_float2(1.0f, 1.0f), dw[a][i] = make_float2(0.0f, 0.0f);
     if (s.weight && s.whole_weight) {
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
@@ -221,14 +221,14 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
             if (!there[a]) continue;
             v.load(static_cast<const T*>(s.weight) + at[a]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) w[a][i] = r.weight_offset + v.get(i);
+            for (int i = 0; i < N / 2; ++i) w[a][i] = __fadd2_rn(make_float2(r.weight_offset, r.weight_offset), v.get2(i));
         }
     } else if (s.weight) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (there[a]) w[a][i] = weight_at(r, s, at[a] + i);
+            for (int i = 0; i < N / 2; ++i)
+                if (there[a]) w[a][i] = make_float2(weight_at(r, s, at[a] + 2 * i), weight_at(r, s, at[a] + 2 * i + 1));
     }
 
     struct Head {
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
             if constexpr (BACKWARD) v.rstd = rstd[item];
         };
         // the angles of access a, of which `first` is the value in the first place of its pair
-        auto turn_all = [&](uint32_t token, float (&v)[2][N]) {
+        auto turn_all = [&](uint32_t token, float2 (&v)[2][N / 2]) {
             float cs[kAngles], sn[kAngles];
             if constexpr (PAIRS) {
 #pragma unroll
@@ -267,20 +267,19 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
                     read_table(sines + token * r.half + at[a] / 2, sn);
 #pragma unroll
                     for (int j = 0; j < kAngles; ++j) {
-                        const float p = v[a][2 * j], q = v[a][2 * j + 1];
-                        v[a][2 * j] = p * cs[j] - q * sn[j];
-                        v[a][2 * j + 1] = p * sn[j] + q * cs[j];
+                        const float2 q = v[a][j];
+                        v[a][j] = __ffma2_rn(make_float2(q.x, q.x), make_float2(cs[j], sn[j]),
+                                             __fmul2_rn(make_float2(q.y, q.y), make_float2(-sn[j], cs[j])));
                     }
                 }
             } else if (turns[0]) {
                 read_table(cosines + token * r.half + at[0], cs);
                 read_table(sines + token * r.half + at[0], sn);
 #pragma unroll
-                for (int j = 0; j < kAngles; j += 2) {
-                    const float2 p = make_float2(v[0][j], v[0][j + 1]), q = make_float2(v[1][j], v[1][j + 1]);
-                    const float2 c = make_float2(cs[j], cs[j + 1]), d = make_float2(sn[j], sn[j + 1]);
-                    const float2 y = __ffma2_rn(p, c, __fmul2_rn(q, make_float2(-d.x, -d.y))), z = __ffma2_rn(p, d, __fmul2_rn(q, c));
-                    v[0][j] = y.x, v[0][j + 1] = y.y, v[1][j] = z.x, v[1][j + 1] = z.y;
+                for (int j = 0; j < kAngles / 2; ++j) {
+                    const float2 p = v[0][j], q = v[1][j], c = make_float2(cs[2 * j], cs[2 * j + 1]), d = make_float2(sn[2 * j], sn[2 * j + 1]);
+                    v[0][j] = __ffma2_rn(p, c, __fmul2_rn(q, make_float2(-d.x, -d.y)));
+                    v[1][j] = __ffma2_rn(p, d, __fmul2_rn(q, c));
                 }
             }
         };
@@ -300,57 +299,64 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
             if (item + groups < items) load(item + groups, next);
             uint32_t token, h;
             s.heads_div.divmod(item, token, h);
-            float y[2][N];
-            float sum = 0.0f;
+            float2 y[2][N / 2], sums = make_float2(0.0f, 0.0f);
+            const float2 none = make_float2(0.0f, 0.0f);
             if constexpr (!BACKWARD) {
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        y[a][i] = mine && there[a] ? v.x[a].get(i) : 0.0f;
-                        sum = fmaf(y[a][i], y[a][i], sum);
+                    for (int i = 0; i < N / 2; ++i) {
+                        y[a][i] = mine && there[a] ? v.x[a].get2(i) : none;
+                        sums = __ffma2_rn(y[a][i], y[a][i], sums);
                     }
-                for (uint32_t m = lanes / 2; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+                float sum = sums.x + sums.y;
+#pragma unroll
+                for (uint32_t m = 16; m; m /= 2)
+                    if (m < lanes) sum += __shfl_xor_sync(~0u, sum, m);
                 const float scale = rsqrtf(fmaf(sum, r.inv_head, r.eps));
                 if (!mine) continue;
                 if (rstd && lane == 0) rstd[item] = scale;
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) y[a][i] *= scale * w[a][i];
+                    for (int i = 0; i < N / 2; ++i) y[a][i] = __fmul2_rn(__fmul2_rn(y[a][i], make_float2(scale, scale)), w[a][i]);
                 turn_all(token, y);
             } else {
-                float e[2][N];
+                float2 e[2][N / 2];
+                const float2 scale = make_float2(v.rstd, v.rstd);
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        y[a][i] = mine && there[a] ? v.dy[a].get(i) : 0.0f;
-                        e[a][i] = mine && there[a] ? v.x[a].get(i) * v.rstd : 0.0f;
+                    for (int i = 0; i < N / 2; ++i) {
+                        y[a][i] = mine && there[a] ? v.dy[a].get2(i) : none;
+                        e[a][i] = mine && there[a] ? __fmul2_rn(v.x[a].get2(i), scale) : none;
                     }
                 if (mine) turn_all(token, y);
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        dw[a][i] = fmaf(y[a][i], e[a][i], dw[a][i]);
-                        y[a][i] *= w[a][i];
-                        sum = fmaf(y[a][i], e[a][i], sum);
+                    for (int i = 0; i < N / 2; ++i) {
+                        dw[a][i] = __ffma2_rn(y[a][i], e[a][i], dw[a][i]);
+                        y[a][i] = __fmul2_rn(y[a][i], w[a][i]);
+                        sums = __ffma2_rn(y[a][i], e[a][i], sums);
                     }
-                for (uint32_t m = lanes / 2; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+                float sum = sums.x + sums.y;
+#pragma unroll
+                for (uint32_t m = 16; m; m /= 2)
+                    if (m < lanes) sum += __shfl_xor_sync(~0u, sum, m);
                 if (!mine) continue;
-                sum *= r.inv_head;
+                sum *= -r.inv_head;
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) y[a][i] = v.rstd * fmaf(-e[a][i], sum, y[a][i]);
+                    for (int i = 0; i < N / 2; ++i) y[a][i] = __fmul2_rn(scale, __ffma2_rn(e[a][i], make_float2(sum, sum), y[a][i]));
             }
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 if (!there[a]) continue;
                 Few<T, N> o;
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) o.set2(i, y[a][2 * i], y[a][2 * i + 1]);
+                for (int i = 0; i < N / 2; ++i) o.set2(i, y[a][i].x, y[a][i].y);
                 o.store(out + token * s.os[1] + h * s.os[2] + at[a]);
             }
         }
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                float v = dw[a][i];
+                float v = i % 2 ? dw[a][i / 2].y : dw[a][i / 2].x;
                 for (uint32_t m = 16; m >= lanes; m /= 2) v += __shfl_xor_sync(~0u, v, m);
                 if (threadIdx.x % 32 < lanes && there[a]) table[warp * r.head + at[a] + i] = v;
             }

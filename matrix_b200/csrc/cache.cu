@@ -181,6 +181,9 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const Rows r) {
 #pragma unroll 4
         for (uint32_t q = (from + 3) / 4 + threadIdx.x; q < end; q += kThreads) {
             const int4 v = __ldg(static_cast<const int4*>(r.slots) + q);
+            // most often four slots of a page, one after another: their bits lie in one word
+            const bool row = v.y == v.x + 1 && v.z == v.x + 2 && v.w == v.x + 3 && (v.x & 31) <= 28;
+            if (row && !(seen[(uint32_t)v.x % kBits / 32] >> (v.x & 31) & 15)) continue;
             look(4 * q, v.x), look(4 * q + 1, v.y), look(4 * q + 2, v.z), look(4 * q + 3, v.w);
         }
         // what is left at both ends: fewer than eight

@@ -235,6 +235,10 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
         Few<T, N> x[2], dy[BACKWARD ? 2 : 1];
         float rstd;
     };
+    // accesses that are not there stay zeros
+    Head next{};
+    uint32_t token_step, head_step;  // from a group's head to its next one
+    s.heads_div.divmod(groups, token_step, head_step);
     const uint32_t all_tiles = r.batch * s.tiles;
     for (uint32_t tile = block; tile < all_tiles; tile += s.blocks) {
         uint32_t b, t0;
@@ -245,14 +249,14 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
         const T* const dy = BACKWARD ? static_cast<const T*>(s.dy) + b * s.ys[0] + t0 * s.ys[1] : nullptr;
         T* const out = static_cast<T*>(s.out) + b * s.os[0] + t0 * s.os[1];
         float* const rstd = s.rstd ? s.rstd + (b * r.length + t0) * s.heads : nullptr;
-        auto load = [&](uint32_t item, Head& v) {
-            uint32_t token, h;
-            s.heads_div.divmod(item, token, h);
+        auto load = [&](uint32_t item, uint32_t token, uint32_t h, Head& v) {
+            const T* const px = x + token * s.xs[1] + h * s.xs[2];
+            const T* const py = BACKWARD ? dy + token * s.ys[1] + h * s.ys[2] : nullptr;
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 if (!there[a]) continue;
-                v.x[a].load(x + token * s.xs[1] + h * s.xs[2] + at[a]);
-                if constexpr (BACKWARD) v.dy[a].load(dy + token * s.ys[1] + h * s.ys[2] + at[a]);
+                v.x[a].load(px + at[a]);
+                if constexpr (BACKWARD) v.dy[a].load(py + at[a]);
             }
             if constexpr (BACKWARD) v.rstd = rstd[item];
         };
@@ -283,30 +287,31 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
                 }
             }
         };
-        Head next;
-        if (group < items) load(group, next);
+        uint32_t token, h;
+        s.heads_div.divmod(group, token, h);
+        if (group < items) load(group, token, h, next);
         __syncthreads();  // the tile before is done with the table
         for (uint32_t e = threadIdx.x; e < n * r.half; e += kThreads) {
-            uint32_t token, j;
-            r.half_div.divmod(e, token, j);
-            turn(r, position_of(r, b, t0 + token), j, cosines[e], sines[e]);
+            uint32_t t, j;
+            r.half_div.divmod(e, t, j);
+            turn(r, position_of(r, b, t0 + t), j, cosines[e], sines[e]);
         }
         __syncthreads();
         for (uint32_t base = 0; base < items; base += groups) {  // the same for all lanes of a warp
             const uint32_t item = base + group;
             const bool mine = item < items;
-            Head v = next;
-            if (item + groups < items) load(item + groups, next);
-            uint32_t token, h;
-            s.heads_div.divmod(item, token, h);
+            const Head v = next;
+            const uint32_t token_now = token, h_now = h;
+            token += token_step, h += head_step;
+            if (h >= s.heads) h -= s.heads, ++token;
+            if (item + groups < items) load(item + groups, token, h, next);
             float2 y[2][N / 2], sums = make_float2(0.0f, 0.0f);
-            const float2 none = make_float2(0.0f, 0.0f);
             if constexpr (!BACKWARD) {
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int i = 0; i < N / 2; ++i) {
-                        y[a][i] = mine && there[a] ? v.x[a].get2(i) : none;
+                        y[a][i] = v.x[a].get2(i);
                         sums = __ffma2_rn(y[a][i], y[a][i], sums);
                     }
                 float sum = sums.x + sums.y;
@@ -320,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int i = 0; i < N / 2; ++i) y[a][i] = __fmul2_rn(__fmul2_rn(y[a][i], make_float2(scale, scale)), w[a][i]);
-                turn_all(token, y);
+                turn_all(token_now, y);
             } else {
                 float2 e[2][N / 2];
                 const float2 scale = make_float2(v.rstd, v.rstd);
@@ -328,18 +333,20 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int i = 0; i < N / 2; ++i) {
-                        y[a][i] = mine && there[a] ? v.dy[a].get2(i) : none;
-                        e[a][i] = mine && there[a] ? __fmul2_rn(v.x[a].get2(i), scale) : none;
+                        y[a][i] = v.dy[a].get2(i);
+                        e[a][i] = __fmul2_rn(v.x[a].get2(i), scale);
                     }
-                if (mine) turn_all(token, y);
+                if (mine) {
+                    turn_all(token_now, y);
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
+                    for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < N / 2; ++i) {
-                        dw[a][i] = __ffma2_rn(y[a][i], e[a][i], dw[a][i]);
-                        y[a][i] = __fmul2_rn(y[a][i], w[a][i]);
-                        sums = __ffma2_rn(y[a][i], e[a][i], sums);
-                    }
+                        for (int i = 0; i < N / 2; ++i) {
+                            dw[a][i] = __ffma2_rn(y[a][i], e[a][i], dw[a][i]);
+                            y[a][i] = __fmul2_rn(y[a][i], w[a][i]);
+                            sums = __ffma2_rn(y[a][i], e[a][i], sums);
+                        }
+                }
                 float sum = sums.x + sums.y;
 #pragma unroll
                 for (uint32_t m = 16; m; m /= 2)
@@ -351,13 +358,14 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? 2 : 3) head_norm_kernel(c
 #pragma unroll
                     for (int i = 0; i < N / 2; ++i) y[a][i] = __fmul2_rn(scale, __ffma2_rn(e[a][i], make_float2(sum, sum), y[a][i]));
             }
+            T* const to = out + token_now * s.os[1] + h_now * s.os[2];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 if (!there[a]) continue;
                 Few<T, N> o;
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) o.set2(i, y[a][i].x, y[a][i].y);
-                o.store(out + token * s.os[1] + h * s.os[2] + at[a]);
+                o.store(to + at[a]);
             }
         }
     }

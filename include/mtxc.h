@@ -587,8 +587,8 @@ int mtxc_logits_rules(int dtype, const mtxc_logits_args* args);
  * frequencies, scale and interleaved as for mtxc_rotary.  For each head x, with w' = weight_offset + weight[i] (w' = 1
  * where weight[i] is NULL; weights have head_dim elements of weight_dtype):
  *     r = 1 / sqrt(mean(x^2) + eps),  n = x r w',  dst = n with its first rotary_dim elements turned and scaled
- * rstd[i] (NULL: not wanted) receives r, [batch, length, heads[i]].  dst may be the very tensor of src.  head_dim at most
- * 1,024.
+ * rstd[i] (NULL: not wanted) receives r, [batch, length, heads[i]].  dst[i] may be the very tensor of src[i], and must not
+ * overlap anything else.  head_dim at most 1,024.
  *
  * The backward pass: d_out holds the gradient at the forward call's dst, src and rstd its input and its r (weight, scale,
  * positions as there); with g = d_out turned back and scaled, u = g w':
@@ -626,7 +626,7 @@ int mtxc_head_norm_rotary_backward_workspace(int dtype, const mtxc_head_norm_arg
 /* A paged cache of keys (index 0) and values (1): head h of slot s of page p is head_dim elements at
  * data[i] + p * strides[i][0] + s * strides[i][1] + h * strides[i][2].  dtype: Float, Float16, BFloat16 or
  * MTXC_FLOAT8_E4M3, of which a head is its bytes' values (e4m3, 4 significant bits, up to 448, no infinities) times
- * 2^exponent, the exponent at exponents[i] with exponent_strides[i].  pages * page_size below 2^31. */
+ * 2^exponent, the exponent (-126 .. 127) at exponents[i] with exponent_strides[i].  pages * page_size below 2^31. */
 enum { MTXC_FLOAT8_E4M3 = 32 }; /* of caches only */
 typedef struct mtxc_kv_cache {
     uint64_t pages;
@@ -643,7 +643,7 @@ typedef struct mtxc_kv_cache {
  * slot s % page_size of it).  Slots outside the cache are passed over; of the tokens that name the same slot the last
  * counts.  To 8 bits: with e the least integer such that the largest finite magnitude of the row is at most 448 * 2^e (0
  * for none; at least -96, at most 96), the bytes are x * 2^-e rounded to nearest even, larger ones +-448, NaN and
- * infinities NaN.  Other caches hold rows of their own dtype.  head_dim at most 1,024.
+ * infinities NaN.  Other caches hold rows of their own dtype.  head_dim at most 1,024.  Rows must not overlap the cache.
  *
  * mtxc_cache_read is the way back: rows[i] receives what the cache holds at the slots (of 8 bits rounded to dtype),
  * zeros for a slot outside it. */
@@ -665,7 +665,7 @@ int mtxc_cache_read(int dtype, const mtxc_cache_rows_args* args);
  * over its lengths[b] first tokens (cut to 0 .. max_pages * page_size); token j lies in page page_table[b *
  * page_table_stride + j / page_size] at slot j % page_size.  Tokens of a page that the cache does not have are passed
  * over; where none is left the output is 0.  The queries' dtype is the cache's, or any for a cache in 8 bits.  q and out
- * at b * strides[0] + h * strides[1].  head_dim at most 256, batch at most 65,535.  Scores, sums and the join of what the
+ * (which may be q, and must not overlap anything else) at b * strides[0] + h * strides[1].  head_dim at most 256, batch at most 65,535.  Scores, sums and the join of what the
  * blocks share are in 32 bits; products of half types and of a cache in 8 bits take the weights p rounded to 16 bits.
  * The shares' sums are in `workspace` (aligned to 256 bytes, of at least as many bytes as
  * mtxc_decode_attention_workspace gives) or, where that is NULL, in the thread's. */
@@ -694,7 +694,7 @@ int mtxc_decode_attention_workspace(int dtype, const mtxc_decode_attention_args*
  * of m - n keys comes from elsewhere) or all:
  *     out_i = sum_j p_j v_j,  p = softmax(scale * q_i . k_j) over the keys seen, 0 where there is none
  * Query head h reads key head h / (heads / kv_heads).  Token t, head h of a tensor at t * strides[0] + h * strides[1].
- * head_dim at most 256; tokens, k_tokens and sequences below 2^30.  Sums are in 32 bits; for half types the weights are
+ * out may be q, and must not overlap anything else.  head_dim at most 256; tokens, k_tokens and sequences below 2^30.  Sums are in 32 bits; for half types the weights are
  * rounded to 16 bits before they meet the values. */
 typedef struct mtxc_prompt_attention_args {
     uint64_t tokens, k_tokens, sequences;

@@ -314,6 +314,9 @@ int prepare(const std::string& who, int dtype, const mtxc_cache_rows_args* a, Ro
         return fail(MTXC_ERR_UNSUPPORTED_DTYPE, who + ": slots must be Int32 or Int64");
     if (a->tokens && a->cache.heads && a->cache.head_dim && (!a->rows[0] || !a->rows[1] || !a->slots))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null rows or slots");
+    for (int k = 0; k < 2; ++k)
+        if (a->rows[k] && (a->rows[k] == a->cache.data[0] || a->rows[k] == a->cache.data[1]))
+            return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": rows that are the cache itself");
     r.tokens = (uint32_t)a->tokens;
     r.heads = a->cache.heads;
     r.head = a->cache.head_dim;

@@ -796,6 +796,8 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
     if (!d.batch || !d.heads) return MTXC_OK;
     if (!a->q || !a->out || !a->lengths || (a->max_pages && !a->page_table))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
+    if (a->out == a->cache.data[0] || a->out == a->cache.data[1])
+        return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over the cache");
     const size_t bytes = partial_bytes(d);
     d.partial = static_cast<float*>(a->workspace ? a->workspace : ctx().workspace);
     if (bytes > (a->workspace ? a->workspace_bytes : ctx().workspace_bytes))

@@ -429,6 +429,8 @@ int check_args(const std::string& who, int dtype, const mtxc_head_norm_args* a) 
     const uint64_t tokens = a->batch * a->length;
     for (int k = 0; k < 2 && tokens && a->head_dim; ++k)
         if (a->heads[k] && (!a->src[k] || !a->dst[k])) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
+    if (a->heads[0] && a->heads[1] && a->dst[0] && a->dst[1] && (a->dst[0] == a->src[1] || a->dst[1] == a->src[0]))
+        return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over the other tensor's input");
     if (tokens && a->rotary_dim && (!a->positions || !a->frequencies))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null positions or frequencies");
     return distinct(who, {a->heads[0] ? a->dst[0] : nullptr, a->heads[1] ? a->dst[1] : nullptr});

@@ -718,6 +718,7 @@ extern "C" int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args
     if (!a->tokens || !a->sequences || !a->heads) return MTXC_OK;
     if (!a->q || !a->out || !a->starts || (a->k_tokens && (!a->k || !a->v)))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
+    if (a->out == a->k || a->out == a->v) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over keys or values");
     Prompt p{};
     p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out;
     for (int i = 0; i < 2; ++i)

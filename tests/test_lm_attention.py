@@ -126,7 +126,7 @@ def cuda(*shape, dtype=torch.float32):
 @pytest.mark.gpu
 def test_head_norm_refusals(gpu):
     q, k, pos, f = cuda(2, 4, 3, 8), cuda(2, 4, 1, 8), cuda(4, dtype=torch.int32), cuda(4, dtype=torch.float64)
-    w, r = cuda(8), cuda(2, 4, 3)
+    w, r, other = cuda(8), cuda(2, 4, 3), cuda(2, 4, 3, 8)
     bad = [
         lambda: lm.head_norm_rotary(cuda(4, 8), None, pos, f),
         lambda: lm.head_norm_rotary(q, cuda(2, 4, 1, 6), pos, f),
@@ -158,6 +158,7 @@ def test_head_norm_refusals(gpu):
                        (lambda: lm.head_norm_rotary(q.double(), None, pos, f), _abi.ERR_UNSUPPORTED_DTYPE),
                        (lambda: lm.head_norm_rotary(q, k, pos, f, q_weight=w.int()), _abi.ERR_UNSUPPORTED_DTYPE),
                        (lambda: lm.head_norm_rotary(q, q, pos, f, out=(q, q)), _abi.ERR_INVALID_ARGUMENT),
+                       (lambda: lm.head_norm_rotary(q, other, pos, f, out=(other, q)), _abi.ERR_INVALID_ARGUMENT),
                        (lambda: lm.head_norm_rotary(cuda(1, 1, 1, 1025), None, pos[:1], f), _abi.ERR_SHAPE)]:
         with pytest.raises(MtxcError) as e:
             call()
@@ -167,6 +168,7 @@ def test_head_norm_refusals(gpu):
 @pytest.mark.gpu
 def test_cache_refusals(gpu):
     cache, small = lm.kv_cache(3, 4, 2, 8, torch.float32), lm.kv_cache(3, 4, 2, 8, torch.float8_e4m3fn)
+    one = lm.KVCache(*(cuda(1, 4, 2, 8) for _ in range(2)))
     k, slots = cuda(5, 2, 8), cuda(5, dtype=torch.int32)
     bad = [
         lambda: lm.cache_write(cache, k, k, slots.float()),
@@ -197,6 +199,8 @@ def test_cache_refusals(gpu):
                        (lambda: lm.cache_write(lm.KVCache(cache.keys, cache.keys), k, k, slots), _abi.ERR_INVALID_ARGUMENT),
                        (lambda: lm.cache_read(cache, slots, dtype=torch.float16), _abi.ERR_UNSUPPORTED_DTYPE),
                        (lambda: lm.cache_read(cache, slots, out=(k, k)), _abi.ERR_INVALID_ARGUMENT),
+                       (lambda: lm.cache_read(one, slots[:4], out=(one.keys[0], k[:4])), _abi.ERR_INVALID_ARGUMENT),
+                       (lambda: lm.cache_write(one, one.keys[0], k[:4], slots[:4]), _abi.ERR_INVALID_ARGUMENT),
                        (lambda: lm.cache_write(lm.kv_cache(1, 1, 1, 1025, torch.float32), cuda(5, 1, 1025), cuda(5, 1, 1025), slots),
                         _abi.ERR_SHAPE)]:
         with pytest.raises(MtxcError) as e:
@@ -210,6 +214,7 @@ def test_cache_refusals(gpu):
 def test_decode_refusals(gpu):
     cache, q = lm.kv_cache(3, 4, 2, 8, torch.float32), cuda(2, 4, 8)
     table, n = cuda(2, 3, dtype=torch.int32), cuda(2, dtype=torch.int32)
+    one = lm.KVCache(*(cuda(1, 4, 2, 8) for _ in range(2)))
     bad = [
         lambda: lm.decode_attention(q[0], cache, table, n),
         lambda: lm.decode_attention(cuda(2, 4, 6), cache, table, n),
@@ -230,6 +235,7 @@ def test_decode_refusals(gpu):
     for call, code in [(lambda: lm.decode_attention(q.half(), cache, table, n), _abi.ERR_UNSUPPORTED_DTYPE),
                        (lambda: lm.decode_attention(q.double(), cache, table, n), _abi.ERR_UNSUPPORTED_DTYPE),
                        (lambda: lm.decode_attention(cuda(2, 3, 8), cache, table, n), _abi.ERR_SHAPE),
+                       (lambda: lm.decode_attention(cuda(1, 2, 8), one, table[:1], n[:1], out=one.values[0, :1]), _abi.ERR_INVALID_ARGUMENT),
                        (lambda: lm.decode_attention(cuda(2, 2, 257), lm.kv_cache(1, 1, 1, 257, torch.float32), table, n), _abi.ERR_SHAPE),
                        (lambda: lm.decode_attention(q, lm.kv_cache(1, 0, 2, 8, torch.float32), table, n), _abi.ERR_SHAPE)]:
         with pytest.raises(MtxcError) as e:
@@ -239,7 +245,7 @@ def test_decode_refusals(gpu):
 
 @pytest.mark.gpu
 def test_prompt_refusals(gpu):
-    q, k, starts = cuda(6, 4, 8), cuda(6, 2, 8), cuda(3, dtype=torch.int32)
+    q, k, starts, other = cuda(6, 4, 8), cuda(6, 2, 8), cuda(3, dtype=torch.int32), cuda(6, 4, 8)
     bad = [
         lambda: lm.prompt_attention(q[0], k, k, starts),
         lambda: lm.prompt_attention(q, cuda(6, 2, 6), k, starts),
@@ -262,6 +268,7 @@ def test_prompt_refusals(gpu):
             call()
     for call, code in [(lambda: lm.prompt_attention(q.double(), k.double(), k.double(), starts), _abi.ERR_UNSUPPORTED_DTYPE),
                        (lambda: lm.prompt_attention(cuda(6, 3, 8), k, k, starts), _abi.ERR_SHAPE),
+                       (lambda: lm.prompt_attention(q, q, other, starts, out=other), _abi.ERR_INVALID_ARGUMENT),
                        (lambda: lm.prompt_attention(cuda(6, 2, 257), cuda(6, 2, 257), cuda(6, 2, 257), starts), _abi.ERR_SHAPE)]:
         with pytest.raises(MtxcError) as e:
             call()

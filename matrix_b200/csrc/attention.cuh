@@ -129,26 +129,40 @@ cudaError_t launch_next(void (*kernel)(Args...), dim3 grid, unsigned threads, cu
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-// The same for a warp by itself.
-template <typename Fn>
-__device__ __forceinline__ uint64_t warp_total(uint32_t n, Fn&& count) {
-    uint64_t sum = 0;
-    for (uint32_t i = threadIdx.x % 32; i < n; i += 32) sum += count(i);
+// The same for a warp by itself.  Where one round takes all sequences their counts are read once for both.
+struct Counts {
+    uint64_t mine, sum;  // of sequence `lane`, and of those up to it (of at most 32 sequences)
+    uint64_t total;
+};
+__device__ __forceinline__ uint64_t warp_sums(uint64_t sum) {
+    const uint32_t lane = threadIdx.x % 32;
 #pragma unroll
-    for (int m = 16; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+    for (int m = 1; m < 32; m *= 2) {
+        const uint64_t v = __shfl_up_sync(~0u, sum, m);
+        if (lane >= (uint32_t)m) sum += v;
+    }
     return sum;
 }
 template <typename Fn>
-__device__ __forceinline__ Found warp_find(uint32_t n, uint64_t target, Fn&& count) {
+__device__ __forceinline__ Counts warp_counts(uint32_t n, Fn&& count) {
     const uint32_t lane = threadIdx.x % 32;
-    uint64_t before = 0;
+    Counts c;
+    c.mine = lane < n ? count(lane) : 0;
+    c.sum = warp_sums(c.mine);
+    c.total = __shfl_sync(~0u, c.sum, 31);
+    uint64_t rest = 0;
+    for (uint32_t i = 32 + lane; i < n; i += 32) rest += count(i);
+    if (n > 32) c.total += __shfl_sync(~0u, warp_sums(rest), 31);
+    return c;
+}
+template <typename Fn>
+__device__ __forceinline__ Found warp_find(uint32_t n, uint64_t target, const Counts& c, Fn&& count) {
+    const uint32_t lane = threadIdx.x % 32;
+    uint64_t before = 0, mine = c.mine, sum = c.sum;
     for (uint32_t base = 0; base < n; base += 32) {
-        const uint64_t mine = base + lane < n ? count(base + lane) : 0;
-        uint64_t sum = mine;
-#pragma unroll
-        for (int m = 1; m < 32; m *= 2) {
-            const uint64_t v = __shfl_up_sync(~0u, sum, m);
-            if (lane >= (uint32_t)m) sum += v;
+        if (base) {
+            mine = base + lane < n ? count(base + lane) : 0;
+            sum = warp_sums(mine);
         }
         const uint32_t passed = __ballot_sync(~0u, before + sum > target);
         if (passed) {

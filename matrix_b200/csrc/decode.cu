@@ -308,14 +308,15 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
     uint32_t* const notes = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(smem4) + warp * R::kWarp + kStages * R::kStage);
     let_next_start();
     auto count = [&](uint32_t b) { return (uint64_t)tiles_of(d, b) * d.units; };
-    const uint64_t work = warp_total(d.batch, count), workers = sharing(d, work);
+    const Counts counts = warp_counts(d.batch, count);
+    const uint64_t work = counts.total, workers = sharing(d, work);
     const uint64_t worker = (uint64_t)warp * gridDim.x + blockIdx.x;  // little work: one warp of each block first
     if (worker >= workers) return;
     uint64_t left = work * (worker + 1) / workers - work * worker / workers;
     Place now;
     {
         const uint64_t first = work * worker / workers;
-        const Found f = warp_find(d.batch, first, count);
+        const Found f = warp_find(d.batch, first, counts, count);
         now.b = f.i;
         now.length = length_of(d, f.i);
         now.tiles = (now.length + kKeys - 1) / kKeys;
@@ -657,6 +658,16 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Decode 
             const float2 ml = *reinterpret_cast<const float2*>(part(base + threadIdx.x) + d.pitch - 4);
             m = ml.x, l = ml.y;
         }
+        // the first parts of each warp are on their way before it is known what they count (few rows: 14.7 -> 10.7 us for one
+        // sequence of 1,500 tokens; many rows have next to none, and the registers would cost blocks)
+        constexpr uint32_t kFirst = kJoinThreads > 128 ? 6 : 0;
+        float4 parts[kMaxHead / 128][kFirst + 1];
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxHead / 128; ++k)
+#pragma unroll
+            for (uint32_t i = 0; i < kFirst; ++i)
+                if (warp + i * kWarps < n && lane + 32 * k < quads)
+                    parts[k][i] = reinterpret_cast<const float4*>(part(base + warp + i * kWarps))[lane + 32 * k];
         float now = m;
 #pragma unroll
         for (int x = 16; x; x /= 2) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
@@ -678,12 +689,14 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Decode 
             if (quad >= quads) continue;
             float4 a = acc[k];
             a.x *= by, a.y *= by, a.z *= by, a.w *= by;
-#pragma unroll 4
-            for (uint32_t i = warp; i < n; i += kWarps) {
-                const float4 v = reinterpret_cast<const float4*>(part(base + i))[quad];
-                const float f = factors[i];
+            auto add = [&](const float4& v, float f) {
                 a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
-            }
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < kFirst; ++i)
+                if (warp + i * kWarps < n) add(parts[k][i], factors[warp + i * kWarps]);
+#pragma unroll 4
+            for (uint32_t i = warp + kFirst * kWarps; i < n; i += kWarps) add(reinterpret_cast<const float4*>(part(base + i))[quad], factors[i]);
             acc[k] = a;
         }
     }

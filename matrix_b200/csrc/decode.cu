@@ -623,111 +623,122 @@ int launch_units(const Decode& d) {
     }
 }
 
-// Joins the parts of a row that workers share: block (query head, sequence), warps take parts in turn, a lane four columns
-// (and four more 128 further), so that all of up to 64 parts are on their way at once.  A sequence without keys gets zeros here.
-template <typename T, uint32_t kJoinThreads>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Decode d) {
+// Joins the parts of the units that workers share: block (unit, sequence), or, where there are few (FEW), (query head,
+// sequence); warps take parts in turn, a lane four columns (and four more 128 further).  A sequence without keys gets zeros here.
+template <typename T, bool FEW>
+__global__ void __launch_bounds__(FEW ? 512 : 128) decode_join_kernel(const Decode d) {
+    constexpr uint32_t kJoinThreads = FEW ? 512 : 128;
     constexpr uint32_t kWarps = kJoinThreads / 32;
     __shared__ uint64_t buf[kWarps];
     __shared__ float factors[kJoinThreads], wide[kWarps];
     __shared__ float4 sums[kWarps][kMaxHead / 4];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const uint32_t b = blockIdx.y, query = blockIdx.x, h = query / d.group, g = (query - h * d.group) / kRows;
-    const uint32_t unit = h * d.groups + g, row = query - h * d.group - g * kRows, tiles = tiles_of(d, b);
-    T* const out = static_cast<T*>(d.out) + b * d.os[0] + query * d.os[1];
+    const uint32_t b = blockIdx.y, tiles = tiles_of(d, b);
+    uint32_t unit = blockIdx.x, row0 = 0;
+    if (FEW) {
+        const uint32_t h = blockIdx.x / d.group, in = blockIdx.x - h * d.group;
+        unit = h * d.groups + in / kRows, row0 = in % kRows;
+    }
+    uint32_t h, query;
+    const uint32_t rows = rows_of(d, unit, h, query), row1 = FEW ? row0 + 1 : rows;
     auto before = [&](uint32_t i) { return (uint64_t)tiles_of(d, i) * d.units; };
     auto behind = [&](uint32_t i) { return (uint64_t)tiles_of(d, b + 1 + i) * d.units; };
     const uint64_t start = total_of(b, before, buf), work = start + (uint64_t)tiles * d.units + total_of(d.batch - b - 1, behind, buf);
     wait_for_previous();  // every block: what follows in the stream follows the first kernel too
+    T* const base_out = static_cast<T*>(d.out) + b * d.os[0] + query * d.os[1];
     if (tiles == 0) {
-        for (uint32_t c = threadIdx.x; c < d.head; c += kJoinThreads) out[c] = from_float<T>(0.0f);
+        for (uint32_t row = row0; row < row1; ++row)
+            for (uint32_t c = threadIdx.x; c < d.head; c += kJoinThreads) base_out[row * d.os[1] + c] = from_float<T>(0.0f);
         return;
     }
     const uint64_t first = start + (uint64_t)unit * tiles, workers = sharing(d, work);
     const uint32_t c0 = (uint32_t)(((first + 1) * workers - 1) / work), c1 = (uint32_t)(((first + tiles) * workers - 1) / work);
     if (c0 == c1) return;
-    auto part = [&](uint32_t c) { return part_of(d, c, c == c0) + row * d.pitch; };
-    const uint32_t quads = d.pitch / 4 - 1;
-    float top = -INFINITY, sum = 0.0f;
-    float4 acc[kMaxHead / 128] = {};
-    for (uint32_t base = c0; base <= c1; base += kJoinThreads) {
-        // the sums so far follow the maximum, as in the kernels before
-        const uint32_t n = min(kJoinThreads, c1 + 1 - base);
-        float m = -INFINITY, l = 0.0f;
-        if (threadIdx.x < n) {
-            const float2 ml = *reinterpret_cast<const float2*>(part(base + threadIdx.x) + d.pitch - 4);
-            m = ml.x, l = ml.y;
+    for (uint32_t row = row0; row < row1; ++row) {
+        T* const out = base_out + row * d.os[1];
+        auto part = [&](uint32_t c) { return part_of(d, c, c == c0) + row * d.pitch; };
+        const uint32_t quads = d.pitch / 4 - 1;
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc[kMaxHead / 128] = {};
+        for (uint32_t base = c0; base <= c1; base += kJoinThreads) {
+            // the sums so far follow the maximum, as in the kernels before
+            const uint32_t n = min(kJoinThreads, c1 + 1 - base);
+            float m = -INFINITY, l = 0.0f;
+            if (threadIdx.x < n) {
+                const float2 ml = *reinterpret_cast<const float2*>(part(base + threadIdx.x) + d.pitch - 4);
+                m = ml.x, l = ml.y;
+            }
+            // the first parts of each warp are on their way before it is known what they count (few rows: 14.7 -> 10.7 us for one
+            // sequence of 1,500 tokens; many rows have next to none, and the registers would cost blocks)
+            constexpr uint32_t kFirst = FEW ? 6 : 0;
+            float4 parts[kMaxHead / 128][kFirst + 1];
+#pragma unroll
+            for (uint32_t k = 0; k < kMaxHead / 128; ++k)
+#pragma unroll
+                for (uint32_t i = 0; i < kFirst; ++i)
+                    if (warp + i * kWarps < n && lane + 32 * k < quads)
+                        parts[k][i] = reinterpret_cast<const float4*>(part(base + warp + i * kWarps))[lane + 32 * k];
+            float now = m;
+#pragma unroll
+            for (int x = 16; x; x /= 2) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+            __syncthreads();
+            if (lane == 0) wide[warp] = now;
+            __syncthreads();
+            now = top;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, wide[w]);
+            const float by = top == now ? 1.0f : exp2f(top - now);
+            top = now;
+            const float factor = m == top ? 1.0f : exp2f(m - top);
+            sum = sum * by + l * factor;
+            factors[threadIdx.x] = factor;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t k = 0; k < kMaxHead / 128; ++k) {
+                const uint32_t quad = lane + 32 * k;
+                if (quad >= quads) continue;
+                float4 a = acc[k];
+                a.x *= by, a.y *= by, a.z *= by, a.w *= by;
+                auto add = [&](const float4& v, float f) {
+                    a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+                };
+#pragma unroll
+                for (uint32_t i = 0; i < kFirst; ++i)
+                    if (warp + i * kWarps < n) add(parts[k][i], factors[warp + i * kWarps]);
+#pragma unroll 4
+                for (uint32_t i = warp + kFirst * kWarps; i < n; i += kWarps) add(reinterpret_cast<const float4*>(part(base + i))[quad], factors[i]);
+                acc[k] = a;
+            }
         }
-        // the first parts of each warp are on their way before it is known what they count (few rows: 14.7 -> 10.7 us for one
-        // sequence of 1,500 tokens; many rows have next to none, and the registers would cost blocks)
-        constexpr uint32_t kFirst = kJoinThreads > 128 ? 6 : 0;
-        float4 parts[kMaxHead / 128][kFirst + 1];
+#pragma unroll
+        for (int m = 16; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
+        __syncthreads();
+        if (lane == 0) wide[warp] = sum;
 #pragma unroll
         for (uint32_t k = 0; k < kMaxHead / 128; ++k)
-#pragma unroll
-            for (uint32_t i = 0; i < kFirst; ++i)
-                if (warp + i * kWarps < n && lane + 32 * k < quads)
-                    parts[k][i] = reinterpret_cast<const float4*>(part(base + warp + i * kWarps))[lane + 32 * k];
-        float now = m;
-#pragma unroll
-        for (int x = 16; x; x /= 2) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+            if (lane + 32 * k < quads) sums[warp][lane + 32 * k] = acc[k];
         __syncthreads();
-        if (lane == 0) wide[warp] = now;
-        __syncthreads();
-        now = top;
+        sum = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, wide[w]);
-        const float by = top == now ? 1.0f : exp2f(top - now);
-        top = now;
-        const float factor = m == top ? 1.0f : exp2f(m - top);
-        sum = sum * by + l * factor;
-        factors[threadIdx.x] = factor;
-        __syncthreads();
+        for (uint32_t w = 0; w < kWarps; ++w) sum += wide[w];
+        for (uint32_t c = threadIdx.x; c < d.head; c += kJoinThreads) {
+            float o = 0.0f;
 #pragma unroll
-        for (uint32_t k = 0; k < kMaxHead / 128; ++k) {
-            const uint32_t quad = lane + 32 * k;
-            if (quad >= quads) continue;
-            float4 a = acc[k];
-            a.x *= by, a.y *= by, a.z *= by, a.w *= by;
-            auto add = [&](const float4& v, float f) {
-                a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
-            };
-#pragma unroll
-            for (uint32_t i = 0; i < kFirst; ++i)
-                if (warp + i * kWarps < n) add(parts[k][i], factors[warp + i * kWarps]);
-#pragma unroll 4
-            for (uint32_t i = warp + kFirst * kWarps; i < n; i += kWarps) add(reinterpret_cast<const float4*>(part(base + i))[quad], factors[i]);
-            acc[k] = a;
+            for (uint32_t w = 0; w < kWarps; ++w) o += reinterpret_cast<const float*>(sums[w])[c];
+            out[c] = from_float<T>(top == -INFINITY ? 0.0f : o / sum);
         }
-    }
-#pragma unroll
-    for (int m = 16; m; m /= 2) sum += __shfl_xor_sync(~0u, sum, m);
-    __syncthreads();
-    if (lane == 0) wide[warp] = sum;
-#pragma unroll
-    for (uint32_t k = 0; k < kMaxHead / 128; ++k)
-        if (lane + 32 * k < quads) sums[warp][lane + 32 * k] = acc[k];
-    __syncthreads();
-    sum = 0.0f;
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) sum += wide[w];
-    for (uint32_t c = threadIdx.x; c < d.head; c += kJoinThreads) {
-        float o = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) o += reinterpret_cast<const float*>(sums[w])[c];
-        out[c] = from_float<T>(top == -INFINITY ? 0.0f : o / sum);
+        __syncthreads();  // before the next row's
     }
 }
 
 // Its start, and the sums over the lengths, behind the first kernel's work.
 template <typename T>
 int launch_join(const Decode& d) {
-    // few rows have many parts each, many rows few or none: there the blocks are small enough to start beside the first kernel's
-    // (one sequence of 1,500 tokens, 32 heads: 15 us with 512 threads, 20 with 128; 256 of 500: 178 and 117)
-    const dim3 grid(d.heads, d.batch);
+    // few rows have many parts each, many units few or none: there the blocks are small enough to start beside the first
+    // kernel's (one sequence of 1,500 tokens, 32 heads: 15 us with 512 threads, 20 with 128; 256 of 500: 178 and 117, and 113 by units)
     const bool few = (uint64_t)d.heads * d.batch <= 4u * ctx().sm_count;
-    const cudaError_t err = few ? launch_next(decode_join_kernel<T, 512>, grid, 512, ctx().stream(), d)
-                                : launch_next(decode_join_kernel<T, 128>, grid, 128, ctx().stream(), d);
+    const cudaError_t err = few ? launch_next(decode_join_kernel<T, true>, dim3(d.heads, d.batch), 512, ctx().stream(), d)
+                                : launch_next(decode_join_kernel<T, false>, dim3(d.units, d.batch), 128, ctx().stream(), d);
     return err == cudaSuccess ? check_launch("decode_join_kernel") : cuda_fail(err, "decode_join_kernel");
 }
 

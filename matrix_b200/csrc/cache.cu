@@ -91,7 +91,8 @@ __device__ __forceinline__ int8_t* exponent_at(const Rows& r, int k, int slot, u
 // their way at a time.  Of the tokens that name one slot the last is stored: a block looks for its slots among those of the
 // tokens behind it (a bit for each of its slots modulo kBits tells nearly all of them apart at once; modulo 2,048, where one in
 // 70 was mistaken, the search took most of the time: 70 us for [16384 tokens, 8 heads of 128]), while its first rows come.
-// Bound by HBM.
+// [16,384 tokens, 8 heads of 128] bf16 to 8 bits 41 us, 2.4 TB/s: 11 us of it is that search, and the rest is bound by its
+// instructions (issue 57 %); to bf16 34 us, 4.0 TB/s.
 constexpr int kAhead = 2;
 constexpr uint32_t kBits = 32768;
 
@@ -241,7 +242,8 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const Rows r) {
     }
 }
 
-// The way back: the slots of kAhead heads, then their rows, then what is stored.
+// The way back: the slots of kAhead heads, then their rows, then what is stored.  [16,384 tokens, 8 heads of 128] 8 bits to bf16
+// 21 us, 4.8 TB/s, bf16 23 us, 5.9; four heads on their way took 25.
 template <typename T, int N, bool SMALL>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const Rows r) {
     using Held = std::conditional_t<SMALL, uint8_t, T>;

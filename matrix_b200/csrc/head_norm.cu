@@ -3,9 +3,11 @@
 //   n = x r w',  r = 1 / sqrt(mean(x^2) + eps),  w' = weight_offset + w;   y = scale * turn(n), the rest of the head n
 //   backward: g = turn back (scale included) of dy, u = g w':  dx = r (u - x r^2 mean(u x)),  dw = sum of g x r
 //
-// Bound by HBM: x (and dy) read once, y (dx) written once.  A group of lanes holds a head in registers between the
-// reduction and the store; its blocks work on queries alone or keys alone, so that a lane meets one piece of one weight
-// (and adds to one piece of its gradient) for all its heads.
+// x (and dy) are read once, y (dx) written once.  A group of lanes holds a head in registers between the reduction and the
+// store; its blocks work on queries alone or keys alone, so that a lane meets one piece of one weight (and adds to one piece of
+// its gradient) for all its heads.  Measured: 16,384 tokens x 40 heads of 128 bf16 forward 70 us, 4.8 TB/s, backward 107 us, 4.7;
+// f32 8,192 tokens 58 and 91 us, 5.7 and 5.5.  Half types are bound by their instructions (issue 57 and 52 %, about 260 and 350
+// for a warp's four heads) behind one another's latency at 24 and 16 warps an SM; 32 warps of 64 registers measured the same.
 #include <algorithm>
 #include <cmath>
 

@@ -204,9 +204,10 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // Half types, and caches in 8 bits under half queries, by 16-byte units.
 //
 // A warp works by itself: it copies the keys and values of its tile (16 of a half type, 32 of 8 bits) into a ring of its own
-// in shared memory, kStages ahead of use (192 KB an SM in flight and in use), and multiplies them on the tensor cores: 16
+// in shared memory, up to kStages of them (192 KB an SM in flight and in use), and multiplies them on the tensor cores: 16
 // keys are the rows and 8 or 16 queries (those that a unit lacks are zeros) the columns of K Q', 16 elements of the head are
-// the rows of V' P'.  (With the queries as 16 rows, half of them zeros for a group of 8, both took twice the products,
+// the rows of V' P'.  Warp-wide products, since the keys pass once and HBM bounds them (the tensor pipe is busy for 10 to 15 %):
+// tcgen05's tiles of 128 rows would be filled by waiting for 128 keys.  (With the queries as 16 rows, half of them zeros for a group of 8, both took twice the products,
 // registers and exponentials: 228 us for [4 x 91k] e4m3.)  There is no barrier between warps, and the copies run on across
 // the borders of units and sequences.  The page numbers of a tile are loaded one tile before its copies are issued.
 //
@@ -220,15 +221,9 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are, and the weights that are summed
 // for the denominator 2^(s - m).
 // ------------------------------------------------------------------------------------------
-#ifndef MTX_W
-#define MTX_W 8
-#define MTX_S 3
-#define MTX_WS 12
-#define MTX_SS 2
-#endif
 // Warps of a block, one block an SM, and tiles of a warp's ring: what 227 KB hold.
-constexpr uint32_t warps_of(uint32_t steps, bool small) { return steps > 8 ? 4 : small ? MTX_WS : MTX_W; }
-constexpr int stages_of(uint32_t steps, bool small) { return steps > 8 ? 3 : small ? MTX_SS : MTX_S; }
+constexpr uint32_t warps_of(uint32_t steps, bool small) { return steps > 8 ? 4 : small ? 12 : 8; }
+constexpr int stages_of(uint32_t steps, bool small) { return steps > 8 || !small ? 3 : 2; }
 uint32_t steps_of(uint32_t head) {  // of 16 elements, as the kernel is built for
     for (uint32_t s : {4u, 5u, 6u, 8u, 12u})
         if (head <= 16 * s) return s;

@@ -220,8 +220,10 @@ __global__ void __launch_bounds__(kAnyThreads) prompt_any_kernel(const Prompt p)
 
 template <typename T, int ROWS, bool WHOLE>
 int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
+    auto kernel = p.head <= 64    ? prompt_any_kernel<T, ROWS, 1, WHOLE>
+                  : p.head <= 128 ? prompt_any_kernel<T, ROWS, 2, WHOLE>
+                                  : prompt_any_kernel<T, ROWS, 4, WHOLE>;
     // the same limit in every call: calls from several threads do not undo each other's
-    auto kernel = p.head <= 64 ? prompt_any_kernel<T, ROWS, 1, WHOLE> : p.head <= 128 ? prompt_any_kernel<T, ROWS, 2, WHOLE> : prompt_any_kernel<T, ROWS, 4, WHOLE>;
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_bytes<ROWS>(kMaxHead));
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
     // as many tiles as the sequences can have: one each may be part filled
@@ -246,11 +248,12 @@ int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
 // Half types on the tensor cores.
 //
 // A block has NT tiles of 128 queries (NT = 2 for heads of up to 128 elements: of two heads that share keys, or, where groups
-// are odd, one behind the other of one head) and runs along the keys in tiles of 128.  Roles: four warps for each tile of queries, a thread a row, have its softmax; one warp issues the products, one
-// the copies, and two clean values (below).  The scores S = Q K' of a tile lie in tensor memory; a row's thread reads
-// them, writes the weights P over them in 16 bits, and the product with V takes them from there, so that neither passes
-// through shared memory.  While one tile of queries is with its softmax the tensor cores work for the other, and the product
-// of the first half of the keys' weights starts while the second half is made:
+// are odd, one behind the other of one head) and runs along the keys in tiles of 128.  Roles: four warps for each tile of
+// queries, a thread a row, have its softmax; one warp issues the products, one the copies, and two clean values (below).  The
+// scores S = Q K' of a tile lie in tensor memory; a row's thread reads them, writes the weights P over them in 16 bits, and the
+// product with V takes them from there, so that neither passes through shared memory.  While one tile of queries is with its
+// softmax the tensor cores work for the other, and the product of the first half of the keys' weights starts while the second
+// half is made:
 //     S0(j)  softmax 0         | P0 V(j), S0(j+1)
 //     S1(j)         softmax 1         | P1 V(j), S1(j+1)
 // (Scores 64 keys at a time, with two places in turn for each tile: 780 us for prompts of 8,192 and 3,903 tokens where 128 keys
@@ -299,7 +302,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// Whether any of the two elements of each of the words is NaN or infinite: their products with 0 are added up.
+// Whether none of eight elements is NaN or infinite: their products with 0 are added up.
 template <typename T>
 __device__ __forceinline__ bool all_finite(const uint4& w) {
     if constexpr (std::is_same_v<T, __half>) {
@@ -323,10 +326,8 @@ __device__ __forceinline__ bool all_finite(const uint4& w) {
 // two products take.  x = n + f with n whole and |f| <= 1/2; 2^f by the polynomial of least largest relative error that is 1 at
 // 0 (found by exchange of its extrema: 1.0e-4 of degree 3, 3.6e-6 of degree 4, to bfloat16's 2^-9 and float16's 2^-12 of
 // rounding), n added to its exponent.  From -127 down, -infinity and NaN included, exactly 0: 1's exponent less 127.
-#ifndef MTX_POLY
-#define MTX_POLY 2
-#endif
-constexpr int kPolynomial = MTX_POLY;  // of eight pairs
+// Of eight pairs 0, 1, 2, 3, 4 by it: four prompts of 4,096 tokens, 16 heads of 64, 237, 227, 226, 230, 242 us.
+constexpr int kPolynomial = 2;
 template <typename T>
 __device__ __forceinline__ float2 exp2_polynomial(float2 x) {
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
@@ -599,6 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         }
         if (my_steps) wait(o_full(i), 0);
+        if (partial < most) wait(clean((2 * most - 1) % kSlots), (most - 1 - partial) / L::kAgain & 1);  // what was noted is there
         __syncwarp();
         tensor_fence_after();
         const bool mine = i < NT && row < n;

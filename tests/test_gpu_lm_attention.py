@@ -431,7 +431,7 @@ def test_prompt_prefixes(lm, dtype, head, causal):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("head", [64, 128, 256])
 def test_prompt_long(lm, dtype, head):
     """Many tiles of keys, on both sides of the diagonal, with peaked scores."""
     check_prompt(lm, dtype, [1500, 1100], 2, 1, head, [1900, 1100])
@@ -441,7 +441,7 @@ def test_prompt_long(lm, dtype, head):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("head", [64, 128, 256])
 def test_prompt_a_growing_maximum(lm, dtype, head):
     """Scores that rise along the keys by far more than any bound on what is kept between maxima: every tile rescales."""
     n = 700
@@ -456,7 +456,7 @@ def test_prompt_a_growing_maximum(lm, dtype, head):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("head", [64, 128, 100])
+@pytest.mark.parametrize("head", [64, 128, 100, 256])
 def test_prompt_what_is_not_seen_does_not_count(lm, dtype, head):
     """NaN and infinities in later tokens, in other sequences and behind the last one."""
     lengths = [200, 150, 64]
@@ -486,7 +486,7 @@ def test_prompt_what_is_not_seen_does_not_count(lm, dtype, head):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("head", [64, 128, 256])
 def test_prompt_infinite_values_that_are_seen(lm, dtype, head):
     """An infinity among the values reaches the elements of the rows that see it, and no others."""
     n = 300
@@ -650,3 +650,26 @@ def test_threads(lm, gpu):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("qh,kh", [(4, 2), (3, 1), (6, 2)])
+def test_prompt_an_infinite_value_for_some_heads(lm, dtype, qh, kh):
+    """Non-finite values of one key head, seen by the second of the heads that share it too, beside another key head's finite
+    ones."""
+    n, head = 200, 64
+    q, k, v = normal(n, qh, head, dtype=dtype), normal(n, kh, head, dtype=dtype, seed=1), normal(n, kh, head, dtype=dtype, seed=2)
+    clean = v.clone()
+    v[150, 0, 3], v[199, 0, 9] = float("inf"), float("nan")
+    got = lm.prompt_attention(q.cuda(), k.cuda(), v.cuda(), torch.tensor([0, n], dtype=torch.int32).cuda())
+    want, bound = att.prompt(q.double(), k.double(), clean.double(), [0, n], [0, n], head ** -0.5, True, dtype)
+    group = qh // kh
+    want[150:, :group, 3], want[199:, :group, 9] = torch.inf, torch.nan
+    att.assert_close(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+def test_decode_many_rows_of_long_sequences(lm, dtype, kind):
+    """More rows than a join by rows takes, and sequences long enough to be shared: joined by units, several rows each."""
+    check_decode(lm, dtype, kind, [700] * 20 + [0, 3, 2000], 40, 2, 64, 16, pages=64)
+    check_decode(lm, dtype, kind, [900] * 25, 28, 4, 128, 24, pages=40)

@@ -665,10 +665,10 @@ int mtxc_cache_read(int dtype, const mtxc_cache_rows_args* args);
  * over its lengths[b] first tokens (cut to 0 .. max_pages * page_size); token j lies in page page_table[b *
  * page_table_stride + j / page_size] at slot j % page_size.  Tokens of a page that the cache does not have are passed
  * over; where none is left the output is 0.  The queries' dtype is the cache's, or any for a cache in 8 bits.  q and out
- * (which may be q, and must not overlap anything else) at b * strides[0] + h * strides[1].  head_dim at most 256, batch at most 65,535.  Scores, sums and the join of what the
- * blocks share are in 32 bits; products of half types and of a cache in 8 bits take the weights p rounded to 16 bits.
- * The shares' sums are in `workspace` (aligned to 256 bytes, of at least as many bytes as
- * mtxc_decode_attention_workspace gives) or, where that is NULL, in the thread's. */
+ * (which may be q, and must not overlap anything else) at b * strides[0] + h * strides[1].  head_dim at most 256, batch at
+ * most 65,535.  Scores, sums and the join of what the workers share are in 32 bits; under queries of half types the weights
+ * p are rounded to 16 bits before they meet the values.  The shares' sums are in `workspace` (aligned to 256 bytes, of at
+ * least as many bytes as mtxc_decode_attention_workspace gives) or, where that is NULL, in the thread's. */
 typedef struct mtxc_decode_attention_args {
     mtxc_kv_cache cache;
     uint64_t batch, max_pages;

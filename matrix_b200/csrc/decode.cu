@@ -220,6 +220,10 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // powers of two, like the keys' scales, come back into the scores).  The values' scales 2^e go into the weights: those are
 // 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are, and the weights that are summed
 // for the denominator 2^(s - m).
+//
+// float16 weights are taken 2^15 times: the largest is 2^15 (65,504 is the type's last), and what is rounded to multiples of
+// 2^-24 is the part of them below 2^-29 of it.  Without, a key with nearly all the weight rounded 131,071 others of 2^-25.2 to
+// nothing, and those are the output where its value is 0.  It costs nothing: the factor is in the exponent.
 // ------------------------------------------------------------------------------------------
 // Warps of a block, one block an SM, and tiles of a warp's ring: what 227 KB hold.
 constexpr uint32_t warps_of(uint32_t steps, bool small) { return steps > 8 ? 4 : small ? 12 : 8; }
@@ -302,6 +306,8 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
     using M = std::conditional_t<SMALL, __half, T>;  // the products' type
     constexpr uint32_t kKeys = R::kKeys, kTiles = kKeys / 16;
     constexpr int kStages = R::kStages;
+    constexpr float kLifted = std::is_same_v<M, __half> ? 15.0f : 0.0f;  // weights as operands: 2^kLifted times
+    constexpr float kLower = SMALL ? 1.0f / 32768 : 1.0f;                // the denominator's weights are not
     extern __shared__ uint4 smem4[];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem4) + warp * R::kWarp;
@@ -539,7 +545,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const float x = s[i][n][2 * r + e];
-                            v[e] = power(x + (shift[i][r] - from[e]));
+                            v[e] = power(x + (shift[i][r] - from[e] + kLifted));
                             sum[n][e] += SMALL ? power(x - from[e]) : v[e];
                         }
                         w[i][n][r] = turned(pack2<M>(v[0], v[1]));
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                 for (int m = 4; m < 32; m *= 2) sum[n][e] += __shfl_xor_sync(~0u, sum[n][e], m);
                 const uint32_t row = 8 * n + 2 * t + e;
                 if (row >= rows) continue;
-                const float by = whole ? (top[n][e] == -INFINITY ? 0.0f : 1.0f / sum[n][e]) : 1.0f;
+                const float by = whole ? (top[n][e] == -INFINITY ? 0.0f : kLower / sum[n][e]) : kLower;
                 T* const out = static_cast<T*>(d.out) + b * d.os[0] + (first + row) * d.os[1];
                 float* const part = part_of(d, worker, tile0 == 0) + row * d.pitch;
 #pragma unroll
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                         const uint32_t c = 16 * i + (SMALL ? 2 * g + r : 8 * r + g);
                         if (c >= d.head) continue;
                         if (whole) out[c] = from_float<T>(o[i][n][2 * r + e] * by);
-                        else part[c] = o[i][n][2 * r + e];
+                        else part[c] = o[i][n][2 * r + e] * by;
                     }
                 if (!whole && g == 0) part[d.pitch - 4] = top[n][e], part[d.pitch - 3] = sum[n][e];
             }

@@ -1,0 +1,92 @@
+"""Attention whose weights, scales and queries span a wide range: what contributes least to the maximum, or beside it, has to
+reach the output all the same (mtxc_decode_attention, mtxc_prompt_attention, against the formulas in 64 bits).
+
+Bounds, for a row whose exact weights are p_j, with the terms that attention_reference derives for scores (d), exponentials (e),
+the rounding of weights to 16 bits (r) and of the result.  Sums: a product of 16 keys adds to a sum in 32 bits once, a truncation
+of 2^-23, so m keys take m / 16 of them (m in the kernels for any head) and 16 for their own sum and the joins.  float16 weights
+are multiples of 2^-24, 2^15 (prompts: 2^11) for the largest one or more: off by another 2^-25 / 2^15 of it, whatever their size.
+Over 8 bits a weight carries its value's scale a_j = 2^exponent, and stands beside v_j / a_j:
+    |got - exact| <= 2^-p |exact| + (2 d + 2 e + r + 2 (m / 16 + 16) 2^-23) sum_j p_j |v_j|
+                     + 2^-40 max_j(p_j a_j) sum_j |v_j| / a_j
+(a_j = 1 elsewhere; 2^-36 in prompts; no such term for other types), and exponents of up to E beside scores in powers of two
+round by 2^-22 E more in d.
+"""
+import math
+
+import pytest
+import torch
+
+from tests import attention_reference as att
+from tests.lm_reference import ROUND, TINY
+
+pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
+KINDS = [(t, k) for t in (torch.float32, torch.float16, torch.bfloat16) for k in (t, E4M3)]
+HALVES = [(t, k) for t, k in KINDS if t != torch.float32]
+
+
+@pytest.fixture
+def lm(gpu):
+    from matrix_b200 import lm
+
+    return lm
+
+
+def attend(q, k, v, scale, dtype, kind, exponents=None, step=2.0 ** -40, seen=None):
+    """Rows q [n, d] over k, v [m, d] (64 bits; seen [n, m]): (result, bound)."""
+    m = k.shape[0]
+    seen = torch.ones(len(q), m, dtype=torch.bool) if seen is None else seen
+    p = (q @ k.T * scale).masked_fill(~seen, -torch.inf).softmax(1)
+    o, mag = p @ v, p @ v.abs()
+    half = dtype != torch.float32
+    weights = torch.float32 if not half else torch.float16 if kind == E4M3 else kind
+    d = att.score_error(q.shape[1], (q.abs() @ k.abs().T * abs(scale)).masked_fill(~seen, 0.0).amax(1, keepdim=True))
+    a = torch.ones(m, dtype=torch.float64) if exponents is None else torch.exp2(exponents.double())
+    if exponents is not None:
+        d = d + 2.0 ** -22 * exponents.abs().max()
+    work = 2 * d + 2 * (2.0 ** -12 if half else 2.0 ** -21) + (ROUND[weights] if half else 0.0)
+    work = work + 2 * ((m / 16 if half else m) + 16) * 2.0 ** -23
+    floor = step * (p * a).amax(1, keepdim=True) * (seen.double() @ (v.abs() / a[:, None])) if weights == torch.float16 else 0.0
+    return o, ROUND[dtype] * o.abs() + work * mag + floor + TINY[dtype]
+
+
+def stored(lm, k, v, kind, page=64):
+    """A cache of one head that holds k, v [n, d] (in 8 bits: bytes of their own, with exponents 0), and its page table."""
+    n, head = k.shape
+    pages = (n + page - 1) // page
+    cache = lm.kv_cache(pages, page, 1, head, kind)
+    at = torch.randperm(pages, generator=torch.Generator().manual_seed(n))
+    slots = at[torch.arange(n) // page] * page + torch.arange(n) % page
+    for x, to in ((k, cache.keys), (v, cache.values)):
+        to.view(torch.int8 if kind == E4M3 else kind)[slots // page, slots % page, 0] = \
+            x.to(kind).view(torch.int8 if kind == E4M3 else kind).cuda()
+    return cache, at.to(torch.int32)[None].cuda(), slots
+
+
+def decode(lm, q, cache, table, n, scale):
+    return lm.decode_attention(q[None].cuda(), cache, table, torch.tensor([n], dtype=torch.int32).cuda(), scale=scale)[0]
+
+
+def powers(bits, head):
+    """The scale with which rows of ones have 2^bits times the weight of zeros."""
+    return bits * math.log(2.0) / head
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("bits", [16.3, 22.4, 24.8, 25.2])
+@pytest.mark.parametrize("n,heads,head", [(2500, 4, 64), (2500, 16, 128), (40000, 4, 64)])
+def test_decode_one_key_far_above_the_others(lm, dtype, kind, bits, n, heads, head):
+    """A key with nearly all the weight and zeros but for one element as its value: the rest of the output is what the others
+    are worth together, each of a weight 2^-bits."""
+    g = torch.Generator().manual_seed(n + heads)
+    for where in (0, n // 2, n - 1):
+        k = torch.zeros(n, head)
+        k[where] = 1.0
+        v = (torch.rand(n, head, generator=g) * 100 + 100).to(kind).float()
+        v[where, 1:] = 0.0
+        cache, table, _ = stored(lm, k, v, kind)
+        q = torch.ones(heads, head, dtype=dtype)
+        scale = powers(bits, head)
+        want, bound = attend(q.double(), k.double(), v.double(), scale, dtype, kind)
+        att.assert_close(decode(lm, q, cache, table, n, scale), want, bound, f"{dtype} {kind} {where}")

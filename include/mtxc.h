@@ -626,7 +626,8 @@ int mtxc_head_norm_rotary_backward_workspace(int dtype, const mtxc_head_norm_arg
 /* A paged cache of keys (index 0) and values (1): head h of slot s of page p is head_dim elements at
  * data[i] + p * strides[i][0] + s * strides[i][1] + h * strides[i][2].  dtype: Float, Float16, BFloat16 or
  * MTXC_FLOAT8_E4M3, of which a head is its bytes' values (e4m3, 4 significant bits, up to 448, no infinities) times
- * 2^exponent, the exponent (-126 .. 127) at exponents[i] with exponent_strides[i].  pages * page_size below 2^31. */
+ * 2^exponent, the exponent (-96 .. 96, as mtxc_cache_write makes it) at exponents[i] with exponent_strides[i].
+ * pages * page_size below 2^31. */
 enum { MTXC_FLOAT8_E4M3 = 32 }; /* of caches only */
 typedef struct mtxc_kv_cache {
     uint64_t pages;

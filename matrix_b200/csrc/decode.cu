@@ -33,7 +33,7 @@ struct Decode {
     const int* lengths;
     float scale;      // times log2(e)
     bool vector;      // the kernel of 16-byte units
-    float* partial;   // [2 * workers][rows][pitch]: sums; at pitch - 4 the maximum and the sum of weights
+    float* partial;   // [2 * workers][rows][pitch]: sums; at pitch - 4 their maximum, the sum of weights and (in 8 bits) its maximum
     uint32_t rows;    // of a unit
     uint32_t pitch;   // a multiple of four
 };
@@ -217,9 +217,11 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // warp's latency), 12 with two 168.
 //
 // In 8 bits the bytes become float16, which holds them exactly, beside queries as float16 of a magnitude below 2 (their rows'
-// powers of two, like the keys' scales, come back into the scores).  The values' scales 2^e go into the weights: those are
-// 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are, and the weights that are summed
-// for the denominator 2^(s - m).
+// powers of two, like the keys' scales, come back into the scores).  The values' scales 2^e go into the weights that meet them:
+// those are 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are.  The weights of the
+// denominator are 2^(s - m') with a maximum m' of their own: m lies up to 2^96 from it, and 2^(s - m) would lose or overflow
+// the sum.  A row of values that is all zeros (its scale is 2^0, whatever its neighbours have) does not lift m: the rows are
+// looked through in the tiles that lift it.  Both together 2 % of the time ([4 x 91k]: 167 -> 170 us).
 //
 // float16 weights are taken 2^15 times: the largest is 2^15 (65,504 is the type's last), and what is rounded to multiples of
 // 2^-24 is the part of them below 2^-29 of it.  Without, a key with nearly all the weight rounded 131,071 others of 2^-25.2 to
@@ -395,6 +397,11 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
         look();
     }
 
+    auto among = [](float x) {  // the largest of the lanes of a column
+#pragma unroll
+        for (int m = 4; m < 32; m *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, m));
+        return x;
+    };
     uint32_t stage = 0;
     while (left) {
         // a unit, as far as this worker has it
@@ -444,14 +451,17 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                 }
             }
         }
-        float o[STEPS][COLUMNS][4], top[COLUMNS][2], sum[COLUMNS][2];
+        // top: what the weights refer to, SMALL: with their values' scales; peak: what those of the denominator do, SMALL: of
+        // this thread's own keys until the end
+        float o[STEPS][COLUMNS][4], top[COLUMNS][2], peak[COLUMNS][2], sum[COLUMNS][2];
 #pragma unroll
         for (int n = 0; n < COLUMNS; ++n) {
-            top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
+            top[n][0] = top[n][1] = peak[n][0] = peak[n][1] = kLowest, sum[n][0] = sum[n][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
         }
-        bool ends, done;  // done: with the unit's last tile
+        bool any = false;  // key counts, were its score -infinity
+        bool ends, done;   // done: with the unit's last tile
         do {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             __syncwarp();
@@ -483,11 +493,14 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                     }
                 }
             }
-            // scores in powers of two; a key that counts lifts the maximum off -infinity even where its score is
+            // scores in powers of two
             const uint32_t mine = notes[stage * 32 + lane], counting = __ballot_sync(~0u, mine & 1);
-            float most[COLUMNS][2], shift[kTiles][2];  // shift: the values' scales
+            any = any || counting;
+            float most[COLUMNS][2], highest[COLUMNS][2], shift[kTiles][2];  // with and without shift: the values' scales
 #pragma unroll
-            for (int n = 0; n < COLUMNS; ++n) most[n][0] = most[n][1] = -INFINITY;
+            for (int n = 0; n < COLUMNS; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) most[n][e] = -INFINITY, highest[n][e] = SMALL ? peak[n][e] : -INFINITY;
 #pragma unroll
             for (uint32_t i = 0; i < kTiles; ++i)
 #pragma unroll
@@ -507,7 +520,8 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                         for (int e = 0; e < 2; ++e) {
                             float& x = s[i][n][2 * r + e];
                             x = counts ? x * (factor[n][e] * scale) : -INFINITY;
-                            if (counts) most[n][e] = fmaxf(most[n][e], fmaxf(x + shift[i][r], kLowest));
+                            highest[n][e] = fmaxf(highest[n][e], x);
+                            if (SMALL) most[n][e] = fmaxf(most[n][e], x + shift[i][r]);
                         }
                 }
             bool grown = false;
@@ -516,19 +530,49 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
             for (int n = 0; n < COLUMNS; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (int m = 4; m < 32; m *= 2) most[n][e] = fmaxf(most[n][e], __shfl_xor_sync(~0u, most[n][e], m));
                     old[n][e] = top[n][e];
-                    top[n][e] = fmaxf(top[n][e], most[n][e]);
+                    top[n][e] = fmaxf(top[n][e], among(SMALL ? most[n][e] : highest[n][e]));
                     grown = grown || top[n][e] != old[n][e];
+                    if (SMALL) {
+                        sum[n][e] *= power(peak[n][e] - highest[n][e]);
+                        peak[n][e] = highest[n][e];
+                    }
                 }
             if (__any_sync(~0u, grown)) {
+                if constexpr (SMALL) {
+                    uint32_t any = 0;  // of this lane's key: a value that is not 0
+#pragma unroll
+                    for (uint32_t u = 0; u < R::kUnits; ++u) {
+                        uint4 x;
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(values + lane * R::kPitch + u * 16) : "memory");
+                        any |= (x.x | x.y | x.z | x.w) & 0x7F7F7F7Fu;
+                    }
+                    const uint32_t zeros = __ballot_sync(~0u, any == 0) & counting;
+                    if (zeros) {
+#pragma unroll
+                        for (int n = 0; n < COLUMNS; ++n) most[n][0] = most[n][1] = -INFINITY;
+#pragma unroll
+                        for (uint32_t i = 0; i < kTiles; ++i)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                if (zeros >> (16 * i + 8 * r + g) & 1) shift[i][r] = -INFINITY;
+#pragma unroll
+                                for (int n = 0; n < COLUMNS; ++n)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) most[n][e] = fmaxf(most[n][e], s[i][n][2 * r + e] + shift[i][r]);
+                            }
+#pragma unroll
+                        for (int n = 0; n < COLUMNS; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) top[n][e] = fmaxf(old[n][e], among(most[n][e]));
+                    }
+                }
 #pragma unroll
                 for (int n = 0; n < COLUMNS; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float by = top[n][e] == old[n][e] ? 1.0f : power(old[n][e] - top[n][e]);
-                        sum[n][e] *= by;
+                        if (!SMALL) sum[n][e] *= by;
 #pragma unroll
                         for (int i = 0; i < STEPS; ++i) o[i][n][e] *= by, o[i][n][2 + e] *= by;
                     }
@@ -536,7 +580,6 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
             uint32_t w[kTiles][COLUMNS][2];
 #pragma unroll
             for (int n = 0; n < COLUMNS; ++n) {
-                const float from[2] = {top[n][0] == -INFINITY ? 0.0f : top[n][0], top[n][1] == -INFINITY ? 0.0f : top[n][1]};
 #pragma unroll
                 for (uint32_t i = 0; i < kTiles; ++i)
 #pragma unroll
@@ -545,8 +588,8 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const float x = s[i][n][2 * r + e];
-                            v[e] = power(x + (shift[i][r] - from[e] + kLifted));
-                            sum[n][e] += SMALL ? power(x - from[e]) : v[e];
+                            v[e] = power(x + (shift[i][r] - top[n][e] + kLifted));
+                            sum[n][e] += SMALL ? power(x - peak[n][e]) : v[e];
                         }
                         w[i][n][r] = turned(pack2<M>(v[0], v[1]));
                     }
@@ -584,11 +627,17 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
         for (int n = 0; n < COLUMNS; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                if (SMALL) {
+                    const float high = peak[n][e];
+                    peak[n][e] = among(high);
+                    sum[n][e] *= power(high - peak[n][e]);
+                } else peak[n][e] = top[n][e];
 #pragma unroll
                 for (int m = 4; m < 32; m *= 2) sum[n][e] += __shfl_xor_sync(~0u, sum[n][e], m);
                 const uint32_t row = 8 * n + 2 * t + e;
                 if (row >= rows) continue;
-                const float by = whole ? (top[n][e] == -INFINITY ? 0.0f : kLower / sum[n][e]) : kLower;
+                const float by = whole ? (any ? kLower / sum[n][e] : 0.0f) : kLower;
+                const float back = SMALL && whole ? exp2f(top[n][e] - peak[n][e]) : 1.0f;  // not in `by`: both may be far from 1
                 T* const out = static_cast<T*>(d.out) + b * d.os[0] + (first + row) * d.os[1];
                 float* const part = part_of(d, worker, tile0 == 0) + row * d.pitch;
 #pragma unroll
@@ -597,10 +646,14 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                     for (int r = 0; r < 2; ++r) {
                         const uint32_t c = 16 * i + (SMALL ? 2 * g + r : 8 * r + g);
                         if (c >= d.head) continue;
-                        if (whole) out[c] = from_float<T>(o[i][n][2 * r + e] * by);
+                        if (whole) out[c] = from_float<T>(o[i][n][2 * r + e] * by * back);
                         else part[c] = o[i][n][2 * r + e] * by;
                     }
-                if (!whole && g == 0) part[d.pitch - 4] = top[n][e], part[d.pitch - 3] = sum[n][e];
+                if (!whole && g == 0) {
+                    part[d.pitch - 4] = any || SMALL ? top[n][e] : -INFINITY;
+                    part[d.pitch - 3] = sum[n][e];
+                    part[d.pitch - 2] = any ? peak[n][e] : -INFINITY;
+                }
             }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -631,12 +684,13 @@ int launch_units(const Decode& d) {
 
 // Joins the parts of the units that workers share: block (unit, sequence), or, where there are few (FEW), (query head,
 // sequence); warps take parts in turn, a lane four columns (and four more 128 further).  A sequence without keys gets zeros here.
-template <typename T, bool FEW>
+// APART: the parts' sums and their denominators refer to maxima of their own.
+template <typename T, bool FEW, bool APART>
 __global__ void __launch_bounds__(FEW ? 512 : 128) decode_join_kernel(const Decode d) {
     constexpr uint32_t kJoinThreads = FEW ? 512 : 128;
     constexpr uint32_t kWarps = kJoinThreads / 32;
     __shared__ uint64_t buf[kWarps];
-    __shared__ float factors[kJoinThreads], wide[kWarps];
+    __shared__ float factors[kJoinThreads], wide[kWarps], wide_peak[kWarps];
     __shared__ float4 sums[kWarps][kMaxHead / 4];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t b = blockIdx.y, tiles = tiles_of(d, b);
@@ -664,15 +718,15 @@ __global__ void __launch_bounds__(FEW ? 512 : 128) decode_join_kernel(const Deco
         T* const out = base_out + row * d.os[1];
         auto part = [&](uint32_t c) { return part_of(d, c, c == c0) + row * d.pitch; };
         const uint32_t quads = d.pitch / 4 - 1;
-        float top = -INFINITY, sum = 0.0f;
+        float top = -INFINITY, peak = -INFINITY, sum = 0.0f;
         float4 acc[kMaxHead / 128] = {};
         for (uint32_t base = c0; base <= c1; base += kJoinThreads) {
             // the sums so far follow the maximum, as in the kernels before
             const uint32_t n = min(kJoinThreads, c1 + 1 - base);
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f, high = -INFINITY;
             if (threadIdx.x < n) {
-                const float2 ml = *reinterpret_cast<const float2*>(part(base + threadIdx.x) + d.pitch - 4);
-                m = ml.x, l = ml.y;
+                const float4 mlh = *reinterpret_cast<const float4*>(part(base + threadIdx.x) + d.pitch - 4);
+                m = mlh.x, l = mlh.y, high = APART ? mlh.z : mlh.x;
             }
             // the first parts of each warp are on their way before it is known what they count (few rows: 14.7 -> 10.7 us for one
             // sequence of 1,500 tokens; many rows have next to none, and the registers would cost blocks)
@@ -684,19 +738,28 @@ __global__ void __launch_bounds__(FEW ? 512 : 128) decode_join_kernel(const Deco
                 for (uint32_t i = 0; i < kFirst; ++i)
                     if (warp + i * kWarps < n && lane + 32 * k < quads)
                         parts[k][i] = reinterpret_cast<const float4*>(part(base + warp + i * kWarps))[lane + 32 * k];
-            float now = m;
+            float now = m, now_peak = high;
 #pragma unroll
-            for (int x = 16; x; x /= 2) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+            for (int x = 16; x; x /= 2) {
+                now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+                if (APART) now_peak = fmaxf(now_peak, __shfl_xor_sync(~0u, now_peak, x));
+            }
             __syncthreads();
-            if (lane == 0) wide[warp] = now;
+            if (lane == 0) wide[warp] = now, wide_peak[warp] = now_peak;
             __syncthreads();
-            now = top;
+            now = top, now_peak = peak;
 #pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, wide[w]);
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                now = fmaxf(now, wide[w]);
+                if (APART) now_peak = fmaxf(now_peak, wide_peak[w]);
+            }
             const float by = top == now ? 1.0f : exp2f(top - now);
             top = now;
             const float factor = m == top ? 1.0f : exp2f(m - top);
-            sum = sum * by + l * factor;
+            if (APART) {
+                sum = sum * (peak == now_peak ? 1.0f : exp2f(peak - now_peak)) + l * (high == now_peak ? 1.0f : exp2f(high - now_peak));
+                peak = now_peak;
+            } else sum = sum * by + l * factor;
             factors[threadIdx.x] = factor;
             __syncthreads();
 #pragma unroll
@@ -731,20 +794,22 @@ __global__ void __launch_bounds__(FEW ? 512 : 128) decode_join_kernel(const Deco
             float o = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWarps; ++w) o += reinterpret_cast<const float*>(sums[w])[c];
-            out[c] = from_float<T>(top == -INFINITY ? 0.0f : o / sum);
+            o /= sum;  // first: the other factor may be far from 1
+            if (APART) o *= exp2f(top - peak);
+            out[c] = from_float<T>((APART ? peak : top) == -INFINITY ? 0.0f : o);
         }
         __syncthreads();  // before the next row's
     }
 }
 
 // Its start, and the sums over the lengths, behind the first kernel's work.
-template <typename T>
+template <typename T, bool APART>
 int launch_join(const Decode& d) {
     // few rows have many parts each, many units few or none: there the blocks are small enough to start beside the first
     // kernel's (one sequence of 1,500 tokens, 32 heads: 15 us with 512 threads, 20 with 128; 256 of 500: 178 and 117, and 113 by units)
     const bool few = (uint64_t)d.heads * d.batch <= 4u * ctx().sm_count;
-    const cudaError_t err = few ? launch_next(decode_join_kernel<T, true>, dim3(d.heads, d.batch), 512, ctx().stream(), d)
-                                : launch_next(decode_join_kernel<T, false>, dim3(d.units, d.batch), 128, ctx().stream(), d);
+    const cudaError_t err = few ? launch_next(decode_join_kernel<T, true, APART>, dim3(d.heads, d.batch), 512, ctx().stream(), d)
+                                : launch_next(decode_join_kernel<T, false, APART>, dim3(d.units, d.batch), 128, ctx().stream(), d);
     return err == cudaSuccess ? check_launch("decode_join_kernel") : cuda_fail(err, "decode_join_kernel");
 }
 
@@ -840,7 +905,7 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
             if (d.vector) {
                 rc = small ? launch_units<T, true>(d) : launch_units<T, false>(d);
                 if (rc) return;
-                rc = launch_join<T>(d);
+                rc = small ? launch_join<T, true>(d) : launch_join<T, false>(d);
                 return;
             }
         }
@@ -855,7 +920,7 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
         }
         kernel<<<d.workers, kAnyThreads, smem, ctx().stream()>>>(d);
         if ((rc = check_launch("decode_any_kernel"))) return;
-        rc = launch_join<T>(d);
+        rc = launch_join<T, false>(d);
     });
     return rc;
 }

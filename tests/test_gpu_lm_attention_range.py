@@ -73,6 +73,49 @@ def powers(bits, head):
     return bits * math.log(2.0) / head
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("top", [1e-3, 1e-5, 1e-20])
+@pytest.mark.parametrize("head,heads", [(64, 4), (128, 12)])
+def test_decode_zero_rows_beside_small_ones(lm, dtype, top, head, heads):
+    """Values of zeros, whose scale in 8 bits is 2^0, count for the denominator alone, wherever they lie."""
+    if dtype == torch.float16 and top < 1e-5:
+        pytest.skip("no float16 of this size")
+    n, page = 900, 16
+    g = torch.Generator().manual_seed(head)
+    for zeros in (slice(0, 300), slice(600, 900), slice(1, None, 2), slice(0, 899), slice(None)):
+        k, v = torch.randn(n, 1, head, generator=g), torch.randn(n, 1, head, generator=g) * top
+        v[zeros] = 0.0
+        k, v, q = k.to(dtype), v.to(torch.bfloat16).float(), torch.randn(heads, head, generator=g).to(dtype)
+        cache = lm.kv_cache(60, page, 1, head, E4M3)
+        table = torch.arange(60, dtype=torch.int32)[None].cuda()
+        slots = torch.arange(n).cuda()
+        lm.cache_write(cache, k.float().cuda(), v.cuda(), slots)
+        (k, _), (v, e) = att.quantise(k[:, 0].double()), att.quantise(v[:, 0].double())
+        e = torch.where(v.any(1), e, -96)  # a row of zeros has no say in the weights' step
+        want, bound = attend(q.double(), k, v, head ** -0.5, dtype, E4M3, e.long())
+        att.assert_close(decode(lm, q, cache, table, n, None), want, bound, f"{dtype} {top} {zeros}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [40, 3000])
+def test_decode_scales_at_the_ends(lm, dtype, n):
+    """Keys of nearly all the weight whose values' scales are 2^-90, others with 2^90: the values of the others are the output,
+    the weights of the first the denominator."""
+    head = 64
+    g = torch.Generator().manual_seed(n)
+    for bits in (30, 100):
+        for order in (slice(0, n // 2), slice(n // 2, n), slice(0, None, 2)):
+            k, e = torch.zeros(n, head), torch.full((n,), 90)
+            k[order], e[order] = 1.0, -90
+            v = (torch.rand(n, head, generator=g) * 200 + 200).to(E4M3).double()
+            cache, table, slots = stored(lm, k, v, E4M3)
+            cache.value_exponents[slots // 64, slots % 64, 0] = e.to(torch.int8).cuda()
+            v = v * torch.exp2(e.double())[:, None]
+            q = torch.ones(4, head, dtype=dtype)
+            want, bound = attend(q.double(), k.double(), v, powers(bits, head), dtype, E4M3, e)
+            att.assert_close(decode(lm, q, cache, table, n, powers(bits, head)), want, bound, f"{bits} {order}")
+
+
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("bits", [16.3, 22.4, 24.8, 25.2])
 @pytest.mark.parametrize("n,heads,head", [(2500, 4, 64), (2500, 16, 128), (40000, 4, 64)])

@@ -216,8 +216,9 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // than others: equal shares end 157 to 191 us after the start.  In 8 bits 8 warps with three tiles took 195 us (bound by each
 // warp's latency), 12 with two 168.
 //
-// In 8 bits the bytes become float16, which holds them exactly, beside queries as float16 of a magnitude below 2 (their rows'
-// powers of two, like the keys' scales, come back into the scores).  The values' scales 2^e go into the weights that meet them:
+// In 8 bits the bytes become float16, which holds them exactly, beside queries as float16 with their largest element between
+// 2^15 and 2^16 (their rows' powers of two, like the keys' scales, come back into the scores): float16 ones keep every bit,
+// bfloat16 ones theirs down to 2^-32 of the largest.  The values' scales 2^e go into the weights that meet them:
 // those are 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are.  The weights of the
 // denominator are 2^(s - m') with a maximum m' of their own: m lies up to 2^96 from it, and 2^(s - m) would lose or overflow
 // the sum.  A row of values that is all zeros (its scale is 2^0, whatever its neighbours have) does not lift m: the rows are
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                         }
                     most = max(most, __shfl_xor_sync(~0u, most, 1));
                     most = max(most, __shfl_xor_sync(~0u, most, 2));
-                    const int e = most ? max(-126, min(126, (int)(most >> 23) - 127)) : 0;
+                    const int e = most ? max(-126, (int)(most >> 23) - 127 - 15) : 0;  // at most 112
                     const float down = power_of_two(-e), up = power_of_two(e);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) factor[n][i] *= __shfl_sync(~0u, up, 4 * (2 * t + i));

@@ -133,3 +133,19 @@ def test_decode_one_key_far_above_the_others(lm, dtype, kind, bits, n, heads, he
         scale = powers(bits, head)
         want, bound = attend(q.double(), k.double(), v.double(), scale, dtype, kind)
         att.assert_close(decode(lm, q, cache, table, n, scale), want, bound, f"{dtype} {kind} {where}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,head", [(4, 64), (12, 128)])
+def test_decode_queries_with_one_large_element_over_8_bits(lm, dtype, heads, head):
+    """A query's element of 2^12 against zeros in the keys, the others of 2^-9: those make the scores."""
+    n = 500
+    g = torch.Generator().manual_seed(head)
+    k, v = ((torch.randn(n, head, generator=g) * 2).to(E4M3).float() for _ in range(2))
+    k[:, 3] = 0.0
+    q = (torch.randn(heads, head, generator=g) * 2.0 ** -9).to(dtype)
+    q[:, 3] = 2.0 ** 12
+    cache, table, _ = stored(lm, k, v, E4M3)
+    scale = 512 / head ** 0.5
+    want, bound = attend(q.double(), k.double(), v.double(), scale, dtype, E4M3)
+    att.assert_close(decode(lm, q, cache, table, n, scale), want, bound)

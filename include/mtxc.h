@@ -698,8 +698,9 @@ int mtxc_decode_attention_workspace(int dtype, const mtxc_decode_attention_args*
  * of m - n keys comes from elsewhere) or all:
  *     out_i = sum_j p_j v_j,  p = softmax(scale * q_i . k_j) over the keys seen, 0 where there is none
  * Query head h reads key head h / (heads / kv_heads).  Token t, head h of a tensor at t * strides[0] + h * strides[1].
- * out may be q, and must not overlap anything else.  head_dim at most 256; tokens, k_tokens and sequences below 2^30.  Sums are in 32 bits; for half types the weights are
- * rounded to 16 bits before they meet the values. */
+ * out may be q, and must not overlap anything else.  head_dim at most 256; tokens, k_tokens and sequences below 2^30.  Sums are
+ * in 32 bits; for half types the weights are rounded to 16 bits before they meet the values (float16 keeps 11 bits of a weight
+ * down to 2^-25 of the largest, and multiples of 2^-35 of that below). */
 typedef struct mtxc_prompt_attention_args {
     uint64_t tokens, k_tokens, sequences;
     uint32_t heads, kv_heads, head_dim;

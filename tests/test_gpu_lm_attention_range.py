@@ -136,6 +136,25 @@ def test_decode_one_key_far_above_the_others(lm, dtype, kind, bits, n, heads, he
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [3.9, 7.9, 16.3, 22.4, 24.8])
+@pytest.mark.parametrize("head", [64, 128, 256])
+def test_prompt_one_key_far_above_the_others(lm, dtype, bits, head):
+    """The same in a prompt, with the key in the first tile of keys or a later one."""
+    n, scale = 1500, powers(bits, head)
+    g = torch.Generator().manual_seed(head)
+    for where in (0, 400):
+        q, k = torch.ones(n, 2, head, dtype=dtype), torch.zeros(n, 1, head, dtype=dtype)
+        k[where] = 1.0
+        v = (torch.rand(n, 1, head, generator=g) * 100 + 100).to(dtype)
+        v[where, :, 1:] = 0.0
+        got = lm.prompt_attention(q.cuda(), k.cuda(), v.cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), scale=scale)
+        seen = torch.ones(n, n, dtype=torch.bool).tril()
+        want, bound = attend(q[:, 0].double(), k[:, 0].double(), v[:, 0].double(), scale, dtype, dtype, None, 2.0 ** -36, seen)
+        for h in range(2):
+            att.assert_close(got[:, h], want, bound, f"{dtype} {where}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("heads,head", [(4, 64), (12, 128)])
 def test_decode_queries_with_one_large_element_over_8_bits(lm, dtype, heads, head):
     """A query's element of 2^12 against zeros in the keys, the others of 2^-9: those make the scores."""

@@ -292,6 +292,10 @@ struct Layout {
     static constexpr uint32_t kSlots = D == 256 ? 2 : D == 128 ? 5 : 8;  // keys and values in turn
     static constexpr uint32_t kAgain = kSlots % 2 ? kSlots : kSlots / 2;  // tiles from one whose values have a slot to the next
     static constexpr uint32_t kBytes = kTileBytes * (NT + kSlots) + 1024;  // the tiles start at a multiple of 1,024
+    // With an odd number of slots keys and values take turns in a slot.  Values that are to be cleaned arrive at `raw`, and the
+    // slot's `full` misses a phase that its next keys' wait counts: (kSlots + 1) / 2 tiles further, which has to be behind the
+    // last tile.  NT + 1 tiles of keys at most are seen in part by NT tiles of rows, one behind the other, and cleaned.
+    static_assert(kSlots % 2 == 0 || NT + 1 <= (kSlots + 1) / 2, "keys would be waited for at a phase that their slot does not reach");
 };
 
 template <typename T>

@@ -366,10 +366,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     __shared__ uint64_t buf[kThreads / 32];
     __shared__ Found found;
     __shared__ uint32_t tensor_base;
-    __shared__ alignas(8) uint64_t bars[2 + 4 * kSlots + 4 * NT];
+    __shared__ alignas(8) uint64_t bars[2 + 4 * kSlots + 4 * NT + 1];
     __shared__ int first_bad[3][D];  // the first key with +infinity, -infinity, NaN in an element
     __shared__ int any_bad, failed;
-    auto wait = [&](uint32_t bar, uint32_t parity) { barrier_wait(bar, parity, &failed); };
+    __shared__ uint32_t issued;  // copies of keys and values
+    auto wait = [&](uint32_t bar, uint32_t parity) { return barrier_wait(bar, parity, &failed); };
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles = (shared_address(dynamic) + 1023) / 1024 * 1024;
     auto q_tile = [&](uint32_t i) { return tiles + i * L::kTileBytes; };
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto s_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + i); };
     auto p_full = [&](uint32_t i, uint32_t half) { return bar0 + 8 * (2 + 4 * kSlots + NT + 2 * i + half); };
     auto o_full = [&](uint32_t i) { return bar0 + 8 * (2 + 4 * kSlots + 3 * NT + i); };
+    const uint32_t products_done = bar0 + 8 * (2 + 4 * kSlots + 4 * NT);  // where a wait has run out
 
     // the last sequence first, and in each the last tile first: of causal ones the longest; all heads of a tile in turn
     const uint32_t per = p.pairs ? p.heads / 2 : p.heads;
@@ -420,8 +422,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (uint32_t s = 0; s < kSlots; ++s) barrier_init(full(s), 1), barrier_init(empty(s), 1), barrier_init(raw(s), 1), barrier_init(clean(s), 2);
         for (uint32_t i = 0; i < NT; ++i)
             barrier_init(s_full(i), 1), barrier_init(p_full(i, 0), 4), barrier_init(p_full(i, 1), 4), barrier_init(o_full(i), 1);
+        barrier_init(products_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         any_bad = failed = 0;
+        issued = 0;
     }
     for (uint32_t e = threadIdx.x; e < 3 * D; e += kThreads) (&first_bad[0][0])[e] = 0x7FFFFFFF;
     tensor_fence_before();
@@ -439,15 +443,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             };
             if (elected()) for (uint32_t item = 0; item < 2 * most; ++item) {
                 const uint32_t j = item / 2, kv = item % 2, s = item % kSlots, use = item / kSlots;
-                if (use) wait(empty(s), (use - 1) & 1);
+                if (use && !wait(empty(s), (use - 1) & 1)) break;
                 if (item == 0 && steps[0]) load(q_tile(0), q_full(0), &maps.q, maps.tokens_last & 1, q_first + row0, h);
                 load(slot(s), kv && j >= partial ? raw(s) : full(s), kv ? &maps.v : &maps.k, maps.tokens_last >> (1 + kv) & 1,
                      k_first + j * kTile, kh);
                 if (NT == 2 && item == 0 && steps[1]) load(q_tile(1), q_full(1), &maps.q, maps.tokens_last & 1, q_first + row0 + next_row, h + p.pairs);
+                issued = item + 1;
             }
-            // every copy ends before the block does, even where a wait has run out
-            for (uint32_t item = 2 * most - min(2 * most, kSlots); failed && item < 2 * most; ++item)
-                for (uint32_t i = 0; i < 1000 && !barrier_try(full(item % kSlots), item / kSlots & 1); ++i) {}
             __syncwarp();
         } else if (warp == 9) {  // products
             constexpr uint32_t kScore = product_descriptor(kBf16, kTile, kTile, false), kValue = product_descriptor(kBf16, kTile, D, true);
@@ -646,6 +648,28 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     tensor_fence_before();
     __syncthreads();
+    if (failed) {
+        // no copy and no product outlasts the block: the last copy of each slot, the queries' and all products (again for some
+        // seconds at most)
+        auto drain = [](uint32_t bar, uint32_t parity) {
+            for (uint32_t i = 0; i < 1u << 20 && !barrier_try(bar, parity); ++i) {}
+        };
+        if (warp == 8 && elected()) {
+            for (uint32_t item = issued - min(issued, kSlots); item < issued; ++item) {
+                // the barrier that the copy was issued on, and how often it was used before
+                const uint32_t s = item % kSlots, j = item / 2;
+                if (item % 2 && j >= partial) drain(raw(s), (j - partial) / L::kAgain & 1);
+                else drain(full(s), item / kSlots & 1);
+            }
+            for (uint32_t i = 0; i < NT; ++i)
+                if (issued && steps[i]) drain(q_full(i), 0);
+        }
+        if (warp == 9 && elected()) {
+            product_commit(products_done);
+            drain(products_done, 0);
+        }
+        __syncthreads();
+    }
     if (warp == 0) {
         tensor_fence_after();
         tensor_free(tensor, 512);

@@ -42,12 +42,15 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {  //
     return done != 0;
 }
 // Waits for the phase of this parity to end.  Where it does not within some seconds, *failed is set, and no thread waits
-// for anything any more: the block runs to its end, with outputs that count for nothing.
-__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
-    if (barrier_try(bar, parity)) return;
-    for (uint32_t i = 0; i < 1u << 20; ++i)
-        if (barrier_try(bar, parity) || *failed) return;
+// for anything any more: the block runs to its end, with outputs that count for nothing.  False: the phase has not ended.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+    if (barrier_try(bar, parity)) return true;
+    for (uint32_t i = 0; i < 1u << 20; ++i) {
+        if (barrier_try(bar, parity)) return true;
+        if (*failed) return false;
+    }
     *failed = 1;
+    return false;
 }
 // What threads have written to shared memory becomes visible to copies and products.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

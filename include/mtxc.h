@@ -719,6 +719,11 @@ typedef struct mtxc_prompt_attention_args {
 } mtxc_prompt_attention_args;
 int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args* args);
 
+/* mtxc_prompt_attention's blocks wait for their copies and products at barriers in shared memory, about four seconds each.  One
+ * whose wait runs out ends, with NaN for its outputs, while the call has long returned: this waits for the thread's stream,
+ * then gives 1 where that has happened in a kernel of the thread's device since the last query, else 0. */
+int mtxc_waits_gave_up(int* gave_up);
+
 /* ------------------------------------------------------------------------------------------
  * Multi-GPU: one communicator per GPU for reductions over an axis sharded across the GPUs of a node
  * (benchmark configs 4 and 5b).  The reference drives a single Metal device through one GPUManager

@@ -175,6 +175,7 @@ def lib() -> C.CDLL:
             "mtxc_decode_attention": (i32, [i32, C.c_char_p]),
             "mtxc_decode_attention_workspace": (i32, [i32, C.c_char_p, C.POINTER(sz)]),
             "mtxc_prompt_attention": (i32, [i32, C.c_char_p]),
+            "mtxc_waits_gave_up": (i32, [C.POINTER(i32)]),
             "mtxc_graph_begin": (i32, []),
             "mtxc_graph_recording": (i32, [C.POINTER(i32)]),
             "mtxc_graph_end": (i32, [C.POINTER(vp)]),

@@ -356,6 +356,8 @@ __device__ __forceinline__ float2 exp2_polynomial(float2 x) {
                        __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
 
+__device__ int waits_gave_up;  // since it was last looked at, in a kernel of this device
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Maps maps, const Prompt p) {
     using L = Layout<D, NT>;
@@ -668,6 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             product_commit(products_done);
             drain(products_done, 0);
         }
+        if (threadIdx.x == 0) waits_gave_up = 1;
         __syncthreads();
     }
     if (warp == 0) {
@@ -741,6 +744,18 @@ int launch(const mtxc_prompt_attention_args* a, const Maps& maps, const Prompt& 
 }  // namespace mtxc
 
 using namespace mtxc;
+
+extern "C" int mtxc_waits_gave_up(int* gave_up) {
+    if (!gave_up) return fail(MTXC_ERR_INVALID_ARGUMENT, "mtxc_waits_gave_up: null pointer");
+    if (int rc = require_init()) return rc;
+    const int none = 0;
+    cudaStream_t st = ctx().stream();
+    cudaError_t err = cudaMemcpyFromSymbolAsync(gave_up, waits_gave_up, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(st);
+    if (err == cudaSuccess && *gave_up) err = cudaMemcpyToSymbolAsync(waits_gave_up, &none, sizeof none, 0, cudaMemcpyHostToDevice, st);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(st);
+    return err == cudaSuccess ? MTXC_OK : cuda_fail(err, "mtxc_waits_gave_up");
+}
 
 extern "C" int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args* a) {
     if (int rc = require_init()) return rc;

@@ -41,8 +41,9 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {  //
         : "memory");
     return done != 0;
 }
-// Waits for the phase of this parity to end.  Where it does not within some seconds, *failed is set, and no thread waits
-// for anything any more: the block runs to its end, with outputs that count for nothing.  False: the phase has not ended.
+// Waits for the phase of this parity to end.  Where it does not within some seconds (2^20 tries, which take 4 us each), *failed
+// is set, and no thread waits for anything any more: the block runs to its end, with outputs that count for nothing.  False: the
+// phase has not ended.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
     if (barrier_try(bar, parity)) return true;
     for (uint32_t i = 0; i < 1u << 20; ++i) {

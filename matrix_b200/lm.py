@@ -27,7 +27,8 @@ from ._abi import check, lib
 
 __all__ = ["BlockNorm", "BlockNormGradients", "HeadNorm", "HeadNormGradients", "KVCache", "block_norm",
            "block_norm_backward", "cache_read", "cache_write", "decode_attention", "dropout", "head_norm_rotary",
-           "head_norm_rotary_backward", "kv_cache", "logits_rules", "prompt_attention", "rotary", "rotary_frequencies"]
+           "head_norm_rotary_backward", "kv_cache", "logits_rules", "prompt_attention", "rotary", "rotary_frequencies",
+           "waits_gave_up"]
 
 
 def _load():
@@ -272,3 +273,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     its last query sees all.  causal=False: every query sees every key of its sequence.  scale: 1 / sqrt(head_dim) where
     None.  Rows in no sequence are left as they were."""
     return _done(_lm.prompt_attention(q, k, v, starts, k_starts, scale, causal, out))[0]
+
+
+def waits_gave_up() -> bool:
+    """Whether a wait inside a kernel of prompt_attention has run out on the thread's device since the last query, and left NaN
+    for outputs (mtxc_waits_gave_up).  Waits for the thread's stream."""
+    gave_up = ctypes.c_int()
+    check(lib().mtxc_waits_gave_up(ctypes.byref(gave_up)))
+    return bool(gave_up.value)

@@ -431,8 +431,10 @@ int check_args(const std::string& who, int dtype, const mtxc_head_norm_args* a) 
     const uint64_t tokens = a->batch * a->length;
     for (int k = 0; k < 2 && tokens && a->head_dim; ++k)
         if (a->heads[k] && (!a->src[k] || !a->dst[k])) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
-    if (a->heads[0] && a->heads[1] && a->dst[0] && a->dst[1] && (a->dst[0] == a->src[1] || a->dst[1] == a->src[0]))
-        return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over the other tensor's input");
+    // queries and keys are worked on at the same time: an output may be its own input, not the other's
+    for (int k = 0; k < 2; ++k)
+        if (a->heads[k])
+            if (int rc = apart(who, {a->dst[k]}, {a->heads[1 - k] ? a->src[1 - k] : nullptr, a->weight[0], a->weight[1]})) return rc;
     if (tokens && a->rotary_dim && (!a->positions || !a->frequencies))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null positions or frequencies");
     return distinct(who, {a->heads[0] ? a->dst[0] : nullptr, a->heads[1] ? a->dst[1] : nullptr});
@@ -571,6 +573,7 @@ extern "C" int mtxc_head_norm_rotary(int dtype, const mtxc_head_norm_args* a) {
     if (int rc = require_init()) return rc;
     if (int rc = check_args("mtxc_head_norm_rotary", dtype, a)) return rc;
     if (int rc = distinct("mtxc_head_norm_rotary", {a->dst[0], a->dst[1], a->rstd[0], a->rstd[1]})) return rc;
+    if (int rc = apart("mtxc_head_norm_rotary", {a->rstd[0], a->rstd[1]}, {a->src[0], a->src[1], a->weight[0], a->weight[1]})) return rc;
     const Plan p = plan(dtype, a, false);
     if (!p.blocks || !a->head_dim) return MTXC_OK;
     return launch<false>(dtype, a, p);
@@ -590,6 +593,12 @@ extern "C" int mtxc_head_norm_rotary_backward(int dtype, const mtxc_head_norm_ar
     const std::string who = "mtxc_head_norm_rotary_backward";
     if (int rc = check_args(who, dtype, a)) return rc;
     if (int rc = distinct(who, {a->dst[0], a->dst[1], a->d_weight[0], a->d_weight[1]})) return rc;
+    for (int k = 0; k < 2; ++k)
+        if (a->heads[k])
+            if (int rc = apart(who, {a->dst[k]}, {a->heads[1 - k] ? a->d_out[1 - k] : nullptr, a->rstd[0], a->rstd[1]})) return rc;
+    if (int rc = apart(who, {a->d_weight[0], a->d_weight[1]},
+                       {a->src[0], a->src[1], a->d_out[0], a->d_out[1], a->rstd[0], a->rstd[1], a->weight[0], a->weight[1]}))
+        return rc;
     Plan p = plan(dtype, a, true);
     for (int k = 0; k < 2; ++k) {
         if (p.r.side[k].blocks && a->head_dim && (!a->d_out[k] || !a->rstd[k]))

@@ -28,6 +28,14 @@ inline int distinct(const std::string& who, std::initializer_list<const void*> o
     return MTXC_OK;
 }
 
+// Refuses an output (NULL: not wanted) that starts where an input does.
+inline int apart(const std::string& who, std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
+    for (const void* out : outputs)
+        for (const void* in : inputs)
+            if (out && out == in) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over a tensor that the call reads");
+    return MTXC_OK;
+}
+
 inline bool is_float_like(int dtype) { return dtype == MTXC_FLOAT || dtype == MTXC_FLOAT16 || dtype == MTXC_BFLOAT16; }
 
 // ------------------------------------------------------------------------------------------

@@ -894,6 +894,7 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
     if (a->out == a->cache.data[0] || a->out == a->cache.data[1])
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over the cache");
+    if (int rc = laid_alike(who, a->out, a->out_strides, a->q, a->q_strides, {a->batch, a->heads})) return rc;
     const size_t bytes = partial_bytes(d);
     d.partial = static_cast<float*>(a->workspace ? a->workspace : ctx().workspace);
     if (bytes > (a->workspace ? a->workspace_bytes : ctx().workspace_bytes))

@@ -432,9 +432,11 @@ int check_args(const std::string& who, int dtype, const mtxc_head_norm_args* a) 
     for (int k = 0; k < 2 && tokens && a->head_dim; ++k)
         if (a->heads[k] && (!a->src[k] || !a->dst[k])) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
     // queries and keys are worked on at the same time: an output may be its own input, not the other's
-    for (int k = 0; k < 2; ++k)
-        if (a->heads[k])
-            if (int rc = apart(who, {a->dst[k]}, {a->heads[1 - k] ? a->src[1 - k] : nullptr, a->weight[0], a->weight[1]})) return rc;
+    for (int k = 0; k < 2; ++k) {
+        if (!a->heads[k]) continue;
+        if (int rc = apart(who, {a->dst[k]}, {a->heads[1 - k] ? a->src[1 - k] : nullptr, a->weight[0], a->weight[1]})) return rc;
+        if (int rc = laid_alike(who, a->dst[k], a->dst_strides[k], a->src[k], a->src_strides[k], {a->batch, a->length, a->heads[k]})) return rc;
+    }
     if (tokens && a->rotary_dim && (!a->positions || !a->frequencies))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null positions or frequencies");
     return distinct(who, {a->heads[0] ? a->dst[0] : nullptr, a->heads[1] ? a->dst[1] : nullptr});
@@ -593,9 +595,11 @@ extern "C" int mtxc_head_norm_rotary_backward(int dtype, const mtxc_head_norm_ar
     const std::string who = "mtxc_head_norm_rotary_backward";
     if (int rc = check_args(who, dtype, a)) return rc;
     if (int rc = distinct(who, {a->dst[0], a->dst[1], a->d_weight[0], a->d_weight[1]})) return rc;
-    for (int k = 0; k < 2; ++k)
-        if (a->heads[k])
-            if (int rc = apart(who, {a->dst[k]}, {a->heads[1 - k] ? a->d_out[1 - k] : nullptr, a->rstd[0], a->rstd[1]})) return rc;
+    for (int k = 0; k < 2; ++k) {
+        if (!a->heads[k]) continue;
+        if (int rc = apart(who, {a->dst[k]}, {a->heads[1 - k] ? a->d_out[1 - k] : nullptr, a->rstd[0], a->rstd[1]})) return rc;
+        if (int rc = laid_alike(who, a->dst[k], a->dst_strides[k], a->d_out[k], a->d_out_strides[k], {a->batch, a->length, a->heads[k]})) return rc;
+    }
     if (int rc = apart(who, {a->d_weight[0], a->d_weight[1]},
                        {a->src[0], a->src[1], a->d_out[0], a->d_out[1], a->rstd[0], a->rstd[1], a->weight[0], a->weight[1]}))
         return rc;

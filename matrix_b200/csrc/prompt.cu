@@ -773,6 +773,7 @@ extern "C" int mtxc_prompt_attention(int dtype, const mtxc_prompt_attention_args
     if (!a->q || !a->out || !a->starts || (a->k_tokens && (!a->k || !a->v)))
         return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": null tensor");
     if (a->out == a->k || a->out == a->v) return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over keys or values");
+    if (int rc = laid_alike(who, a->out, a->out_strides, a->q, a->q_strides, {a->tokens, a->heads})) return rc;
     Prompt p{};
     p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out;
     for (int i = 0; i < 2; ++i)

@@ -36,6 +36,18 @@ inline int apart(const std::string& who, std::initializer_list<const void*> outp
     return MTXC_OK;
 }
 
+// Refuses an output that starts where the input does that it may be, and lies otherwise: `strides` of axes of these sizes.
+inline int laid_alike(const std::string& who, const void* out, const uint64_t* out_strides, const void* in, const uint64_t* in_strides,
+                      std::initializer_list<uint64_t> sizes) {
+    if (!out || out != in) return MTXC_OK;
+    for (uint64_t size : sizes) {
+        if (size > 1 && *out_strides != *in_strides)
+            return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": an output over its input with other strides");
+        ++out_strides, ++in_strides;
+    }
+    return MTXC_OK;
+}
+
 inline bool is_float_like(int dtype) { return dtype == MTXC_FLOAT || dtype == MTXC_FLOAT16 || dtype == MTXC_BFLOAT16; }
 
 // ------------------------------------------------------------------------------------------

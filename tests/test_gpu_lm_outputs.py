@@ -3,7 +3,7 @@ refused before anything runs (through the C ABI: the Python module makes gradien
 import pytest
 import torch
 
-from matrix_b200 import _abi
+from matrix_b200 import MtxcError, _abi
 
 pytestmark = pytest.mark.gpu
 
@@ -34,11 +34,11 @@ def strides(*tensors):
     return [s for t in tensors for s in t.stride()[:3]]
 
 
-def backward_args(q, k, dq, dk, dst, rstd, weights, positions, f, interleaved, workspace, d_weight=(None, None)):
+def backward_args(q, k, dq, dk, dst, rstd, weights, positions, f, interleaved, workspace, d_weight=(None, None), dst_strides=None):
     batch, length, _, head = q.shape
     return packed(_abi.HEAD_NORM_FIELDS, _abi.HEAD_NORM_ARGS, {
         "batch": batch, "length": length, "head_dim": head, "rotary_dim": 2 * len(f), "heads": [q.shape[2], k.shape[2]],
-        "dst": dst, "dst_strides": strides(q, k), "src": [q, k], "src_strides": strides(q, k), "weight": weights, "rstd": rstd,
+        "dst": dst, "dst_strides": dst_strides or strides(q, k), "src": [q, k], "src_strides": strides(q, k), "weight": weights, "rstd": rstd,
         "positions": positions, "position_strides": positions.stride(), "frequencies": f, "position_dtype": 3,
         "weight_dtype": TYPES[q.dtype], "scale": 1.25, "weight_offset": 0.5, "eps": 1e-6, "interleaved": int(interleaved),
         "d_out": [dq, dk], "d_out_strides": strides(dq, dk), "d_weight": d_weight, "workspace": workspace,
@@ -98,3 +98,37 @@ def test_head_norm_outputs_over_other_inputs_are_refused(lm):
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip((q, k, dq, dk, *r, *w), before))
     assert backward((a, b)) == 0 and torch.isfinite(out.q).all()
+
+
+def test_outputs_over_their_input_in_another_order_are_refused(lm):
+    """Axes exchanged: elements would be written before they are read.  Strides of axes of one element do not count."""
+    q = torch.randn(4, 4, 64, device="cuda")
+    turned, before = q.transpose(0, 1), q.clone()
+    starts, positions = torch.tensor([0, 4], dtype=torch.int32).cuda(), torch.arange(4, dtype=torch.int32).cuda()
+    f = lm.rotary_frequencies(64)[0]
+    cache, table = lm.kv_cache(1, 16, 2, 64, torch.float32), torch.zeros(4, 1, dtype=torch.int32).cuda()
+    k = torch.randn(4, 2, 64, device="cuda")
+    w, r = [None, None], [torch.ones(1, 4, 4, device="cuda"), torch.ones(1, 4, 2, device="cuda")]
+    for call in (lambda: lm.head_norm_rotary(q, None, positions, f, out=(turned, None)),
+                 lambda: lm.head_norm_rotary(k, q, positions, f, out=(torch.empty_like(k), turned)),
+                 lambda: lm.decode_attention(q, cache, table, positions, out=turned),
+                 lambda: lm.prompt_attention(q, k, k, starts, out=turned)):
+        with pytest.raises(MtxcError) as e:
+            call()
+        assert e.value.code == _abi.ERR_INVALID_ARGUMENT
+    dq, dk = torch.randn(1, 4, 4, 64, device="cuda"), torch.randn(1, 4, 2, 64, device="cuda")
+    before_dq, workspace = dq.clone(), torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+    for q4 in (q[None], dq):  # over src, over d_out
+        args = {"q": q[None], "k": k[None], "dq": dq, "dk": dk, "rstd": r, "weights": w, "positions": positions[None], "f": f,
+                "interleaved": False, "workspace": workspace}
+        over = torch.as_strided(q4, (1, 4, 4, 64), (1024, 64, 256, 1))
+        packed_args = backward_args(dst=(over, torch.empty_like(dk)), dst_strides=strides(over, dk), **args)
+        assert _abi.lib().mtxc_head_norm_rotary_backward(0, packed_args) == _abi.ERR_INVALID_ARGUMENT
+    torch.cuda.synchronize()
+    assert torch.equal(q, before) and torch.equal(dq, before_dq)
+    one = torch.randn(1, 4, 64, device="cuda")
+    want = lm.prompt_attention(one, one, one, starts[:2] // 4)
+    assert torch.equal(lm.prompt_attention(one.clone(), one, one, starts // 4, out=None), want)
+    again = one.clone()
+    odd = torch.as_strided(again, (1, 4, 64), (7, 64, 1))
+    assert torch.equal(lm.prompt_attention(again, one, one, starts // 4, out=odd), want)

@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const Rows r) {
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
                             const float v = y.get(i);
-                            q[i] = bad ? fmaf(v, scale, v - v) : v * scale;  // an infinity becomes NaN: the type has none
+                            q[i] = bad && isinf(v) ? NAN : v * scale;  // the type has no infinities
                         }
                         store_bytes<N>(to + p * N, q);
                         if (ONE) break;

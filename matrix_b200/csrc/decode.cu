@@ -309,8 +309,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
     using M = std::conditional_t<SMALL, __half, T>;  // the products' type
     constexpr uint32_t kKeys = R::kKeys, kTiles = kKeys / 16;
     constexpr int kStages = R::kStages;
-    constexpr float kLifted = std::is_same_v<M, __half> ? 15.0f : 0.0f;  // weights as operands: 2^kLifted times
-    constexpr float kLower = SMALL ? 1.0f / 32768 : 1.0f;                // the denominator's weights are not
+    constexpr float kLifted = std::is_same_v<M, __half> ? 15.0f : 0.0f;  // the largest weight is 2^kLifted
     extern __shared__ uint4 smem4[];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem4) + warp * R::kWarp;
@@ -452,8 +451,8 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                 }
             }
         }
-        // top: what the weights refer to, SMALL: with their values' scales; peak: what those of the denominator do, SMALL: of
-        // this thread's own keys until the end
+        // top: what the weights refer to, kLifted below the largest (SMALL: with their values' scales); peak: what those of the
+        // denominator do, the largest (SMALL: of this thread's own keys until the end)
         float o[STEPS][COLUMNS][4], top[COLUMNS][2], peak[COLUMNS][2], sum[COLUMNS][2];
 #pragma unroll
         for (int n = 0; n < COLUMNS; ++n) {
@@ -532,7 +531,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     old[n][e] = top[n][e];
-                    top[n][e] = fmaxf(top[n][e], among(SMALL ? most[n][e] : highest[n][e]));
+                    top[n][e] = fmaxf(top[n][e], among(SMALL ? most[n][e] : highest[n][e]) - kLifted);
                     grown = grown || top[n][e] != old[n][e];
                     if (SMALL) {
                         sum[n][e] *= power(peak[n][e] - highest[n][e]);
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
 #pragma unroll
                         for (int n = 0; n < COLUMNS; ++n)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) top[n][e] = fmaxf(old[n][e], among(most[n][e]));
+                            for (int e = 0; e < 2; ++e) top[n][e] = fmaxf(old[n][e], among(most[n][e]) - kLifted);
                     }
                 }
 #pragma unroll
@@ -589,7 +588,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const float x = s[i][n][2 * r + e];
-                            v[e] = power(x + (shift[i][r] - top[n][e] + kLifted));
+                            v[e] = power((SMALL ? x + shift[i][r] : x) - top[n][e]);
                             sum[n][e] += SMALL ? power(x - peak[n][e]) : v[e];
                         }
                         w[i][n][r] = turned(pack2<M>(v[0], v[1]));
@@ -637,7 +636,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                 for (int m = 4; m < 32; m *= 2) sum[n][e] += __shfl_xor_sync(~0u, sum[n][e], m);
                 const uint32_t row = 8 * n + 2 * t + e;
                 if (row >= rows) continue;
-                const float by = whole ? (any ? kLower / sum[n][e] : 0.0f) : kLower;
+                const float by = whole ? (any ? 1.0f / sum[n][e] : 0.0f) : 1.0f;
                 const float back = SMALL && whole ? exp2f(top[n][e] - peak[n][e]) : 1.0f;  // not in `by`: both may be far from 1
                 T* const out = static_cast<T*>(d.out) + b * d.os[0] + (first + row) * d.os[1];
                 float* const part = part_of(d, worker, tile0 == 0) + row * d.pitch;
@@ -648,7 +647,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                         const uint32_t c = 16 * i + (SMALL ? 2 * g + r : 8 * r + g);
                         if (c >= d.head) continue;
                         if (whole) out[c] = from_float<T>(o[i][n][2 * r + e] * by * back);
-                        else part[c] = o[i][n][2 * r + e] * by;
+                        else part[c] = o[i][n][2 * r + e];
                     }
                 if (!whole && g == 0) {
                     part[d.pitch - 4] = any || SMALL ? top[n][e] : -INFINITY;

@@ -668,9 +668,10 @@ int mtxc_cache_read(int dtype, const mtxc_cache_rows_args* args);
  * over; where none is left the output is 0.  The queries' dtype is the cache's, or any for a cache in 8 bits.  q and out
  * (which may be q, and must not overlap anything else) at b * strides[0] + h * strides[1].  head_dim at most 256, batch at
  * most 65,535.  Scores, sums and the join of what the workers share are in 32 bits.  Under queries of half types the weights p
- * are rounded to 16 bits before they meet the values: to the cache's type, or, over 8 bits, to float16 together with the
- * value's scale, where the queries are float16 too (bfloat16 ones with all bits of what is 2^-32 of a head's largest element or
- * more).  float16 keeps 11 bits of a weight down to 2^-29 of the largest, and multiples of 2^-39 of that below.  The shares'
+ * meet the values as two parts of the cache's type, which keep 16 bits (bfloat16) or 22 of them, or, over 8 bits, as float16
+ * together with the value's scale, where the queries are float16 too (bfloat16 ones with all bits of what is 2^-32 of a head's
+ * largest element or more).  float16 keeps 11 bits of a weight down to 2^-29 of the largest, and multiples of 2^-39 of that
+ * below.  The shares'
  * sums are in `workspace` (aligned to 256 bytes, of at least as many bytes as mtxc_decode_attention_workspace gives) or, where
  * that is NULL, in the thread's. */
 typedef struct mtxc_decode_attention_args {

@@ -207,9 +207,15 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // in shared memory, up to kStages of them (192 KB an SM in flight and in use), and multiplies them on the tensor cores: 16
 // keys are the rows and 8 or 16 queries (those that a unit lacks are zeros) the columns of K Q', 16 elements of the head are
 // the rows of V' P'.  Warp-wide products, since the keys pass once and HBM bounds them (the tensor pipe is busy for 10 to 15 %):
-// tcgen05's tiles of 128 rows would be filled by waiting for 128 keys.  (With the queries as 16 rows, half of them zeros for a group of 8, both took twice the products,
-// registers and exponentials: 228 us for [4 x 91k] e4m3.)  There is no barrier between warps, and the copies run on across
-// the borders of units and sequences.  The page numbers of a tile are loaded one tile before its copies are issued.
+// tcgen05's tiles of 128 rows would be filled by waiting for 128 keys.  (With the queries as 16 rows, half of them zeros for a
+// group of 8, both took twice the products, registers and exponentials: 228 us for [4 x 91k] e4m3.)  There is no barrier between
+// warps, and the copies run on across the borders of units and sequences.  The page numbers of a tile are loaded one tile before
+// its copies are issued.
+//
+// Over plain caches a weight is two operands, what 16 bits hold of it and what that leaves: 16 or 22 bits for a second product.
+// The result is then as far from 64 bits as its own rounding (relative 0.0017 in bfloat16, with one operand 0.0021), for 1.5 % of
+// the time (235 us for 232).  Over 8 bits, where the issue of instructions counts, weights are float16 (2.1e-4, of which 2.0e-4
+// are the result's rounding).
 //
 // Measured, heads of 128, 32 over 8: 64 sequences of 1,024 to 8,192 tokens bf16 220 us, 5.7 TB/s (0.87 of the copy figure), 4 of
 // 16,384 to 131,072 in 8 bits under 56 heads f16 168 us, 5.6 TB/s.  Bound by HBM and, at the end, by the SMs that get less of it
@@ -276,6 +282,21 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     Few<T, 4> f;
     f.set2(0, a, b);
     return f.w[0];
+}
+// Two weights as two parts of T each, the first one rounded down from a little less: a weight that is not 0 has no part of 0, nor
+// a negative one, with which an infinite value would become NaN.
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& first, uint32_t& second) {
+    constexpr float kLess = 1.0f - 1.0f / 8192;
+    float2 kept;
+    if constexpr (std::is_same_v<T, __half>) {
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(first) : "f"(b * kLess), "f"(a * kLess));
+        kept = __half22float2(*reinterpret_cast<const __half2*>(&first));
+    } else {
+        first = __byte_perm(__float_as_uint(a * kLess), __float_as_uint(b * kLess), 0x7632);
+        kept = make_float2(__uint_as_float(first << 16), __uint_as_float(first & 0xFFFF0000u));
+    }
+    second = pack2<T>(a - kept.x, b - kept.y);
 }
 __device__ __forceinline__ uint32_t halves_of(uint32_t bytes) {  // two bytes of e4m3 as two float16
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)bytes, __NV_E4M3);
@@ -577,7 +598,7 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                         for (int i = 0; i < STEPS; ++i) o[i][n][e] *= by, o[i][n][2 + e] *= by;
                     }
             }
-            uint32_t w[kTiles][COLUMNS][2];
+            uint32_t w[kTiles][COLUMNS][2], rest[COLUMNS][2];  // rest: the second parts
 #pragma unroll
             for (int n = 0; n < COLUMNS; ++n) {
 #pragma unroll
@@ -591,7 +612,12 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                             v[e] = power((SMALL ? x + shift[i][r] : x) - top[n][e]);
                             sum[n][e] += SMALL ? power(x - peak[n][e]) : v[e];
                         }
-                        w[i][n][r] = turned(pack2<M>(v[0], v[1]));
+                        if constexpr (SMALL) w[i][n][r] = turned(pack2<M>(v[0], v[1]));
+                        else {
+                            uint32_t first, second;
+                            split2<M>(v[0], v[1], first, second);
+                            w[i][n][r] = turned(first), rest[n][r] = turned(second);
+                        }
                     }
             }
 #pragma unroll
@@ -600,7 +626,10 @@ __global__ void __launch_bounds__(warps_of(STEPS, SMALL) * 32, 1) decode_units_k
                 if constexpr (!SMALL) {
                     matrices_turned(r, values + (lane / 16 * 8 + lane % 8) * R::kPitch + (2 * c + lane / 8 % 2) * 16);
 #pragma unroll
-                    for (int n = 0; n < COLUMNS; ++n) multiply<M>(o[c][n], r, w[0][n][0], w[0][n][1]);
+                    for (int n = 0; n < COLUMNS; ++n) {
+                        multiply<M>(o[c][n], r, w[0][n][0], w[0][n][1]);
+                        multiply<M>(o[c][n], r, rest[n][0], rest[n][1]);
+                    }
                 } else {
                     // a register has two elements of two keys: keys together, and the even elements are rows 0 to 7, the odd
                     // ones rows 8 to 15

@@ -168,3 +168,44 @@ def test_decode_queries_with_one_large_element_over_8_bits(lm, dtype, heads, hea
     scale = 512 / head ** 0.5
     want, bound = attend(q.double(), k.double(), v.double(), scale, dtype, E4M3)
     att.assert_close(decode(lm, q, cache, table, n, scale), want, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,head", [(4, 64), (16, 128), (12, 200), (3, 66)])
+def test_decode_weights_keep_more_than_16_bits(lm, dtype, heads, head):
+    """Values of two keys that would cancel if the weight of one, 2^-1 and 0.4 steps of its type, were rounded to it.  The weights are
+    kept as two parts of 16 bits, so r is the square of the type's rounding, and the exponentials are those of 32 bits."""
+    n, weight = 120, 0.5 + 0.4 * ROUND[dtype]
+    k, v = torch.zeros(n, head), torch.ones(n, head)
+    k[1::2], v[1::2] = -1.0, -2.0
+    cache, table, _ = stored(lm, k, v, dtype)
+    q, scale = torch.ones(heads, head, dtype=dtype), -math.log(weight) / head
+    p = (q.double() @ k.double().T * scale).softmax(1)
+    want, mag = p @ v.double(), p @ v.abs().double()
+    d = att.score_error(head, torch.full((heads, 1), -math.log(weight), dtype=torch.float64))
+    work = 2 * d + 2 * 2.0 ** -21 + ROUND[dtype] ** 2 + 2 * (n + 16) * 2.0 ** -24
+    bound = ROUND[dtype] * want.abs() + work * mag + 2.0 ** -40 * p.amax() * n + TINY[dtype]
+    assert (want.abs() > 2 * bound).all()
+    att.assert_close(decode(lm, q, cache, table, n, scale), want, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,head", [(4, 64), (16, 128), (3, 66)])
+def test_decode_infinite_values_that_are_seen(lm, dtype, heads, head):
+    """An infinity among the values is the output's in its element, against a weight of 1, of a power of two and of neither; of both
+    signs, or with NaN, it is NaN."""
+    n = 90
+    g = torch.Generator().manual_seed(head)
+    k, v = torch.zeros(n, head), torch.randn(n, head, generator=g).to(dtype).float()
+    k[10:20], k[20:30] = -1.0, -1.3
+    inf = float("inf")
+    want_of = {1: (0, inf), 2: (15, inf), 3: (25, -inf), 4: (89, -inf), 5: (40, float("nan"))}
+    for c, (at, x) in want_of.items():
+        v[at, c] = x
+    v[3, 6], v[70, 6] = inf, -inf
+    cache, table, _ = stored(lm, k, v, dtype)
+    for scale in (math.log(2.0) / head, 9 * math.log(2.0) / head):  # 1/2 and 2^-1.3, 2^-9 and 2^-11.7
+        got = decode(lm, torch.ones(heads, head, dtype=dtype), cache, table, n, scale).float().cpu()
+        for c, (_, x) in want_of.items():
+            assert (got[:, c] == x).all() if x == x else torch.isnan(got[:, c]).all(), (c, got[:, c])
+        assert torch.isnan(got[:, 6]).all() and torch.isfinite(got[:, 7:]).all() and torch.isfinite(got[:, 0]).all()

@@ -68,6 +68,20 @@ def decode(lm, q, cache, table, n, scale):
     return lm.decode_attention(q[None].cuda(), cache, table, torch.tensor([n], dtype=torch.int32).cuda(), scale=scale)[0]
 
 
+def check_decode(lm, q, cache, table, n, scale, want, bound, what=""):
+    """As one sequence, whose tiles workers share, and as many, of which a worker has several tiles and whole sequences."""
+    att.assert_close(decode(lm, q, cache, table, n, scale), want, bound, what)
+    many = 1 + 500000 // n
+    lengths = torch.full((many,), n, dtype=torch.int32).cuda()
+    got = lm.decode_attention(q[None].expand(many, -1, -1).cuda(), cache, table.expand(many, -1), lengths, scale=scale)
+    different = (got - got[0]).abs().flatten(1).amax(1).nonzero()[:, 0].tolist()
+    for i in [0, *different[:20], many - 1]:
+        att.assert_close(got[i], want, bound, f"{what}, {i} of {many}")
+    low, high = got.amin(0), got.amax(0)
+    att.assert_close(low, want, bound, what)
+    att.assert_close(high, want, bound, what)
+
+
 def powers(bits, head):
     """The scale with which rows of ones have 2^bits times the weight of zeros."""
     return bits * math.log(2.0) / head
@@ -80,20 +94,21 @@ def test_decode_zero_rows_beside_small_ones(lm, dtype, top, head, heads):
     """Values of zeros, whose scale in 8 bits is 2^0, count for the denominator alone, wherever they lie."""
     if dtype == torch.float16 and top < 1e-5:
         pytest.skip("no float16 of this size")
-    n, page = 900, 16
+    page = 16
     g = torch.Generator().manual_seed(head)
-    for zeros in (slice(0, 300), slice(600, 900), slice(1, None, 2), slice(0, 899), slice(None)):
+    for n, zeros in ((900, slice(0, 300)), (900, slice(600, 900)), (900, slice(1, None, 2)), (900, slice(0, 899)), (900, slice(None)),
+                     (200, slice(0, 70)), (200, slice(100, 200)), (200, slice(1, None, 2)), (20, slice(0, 19))):
         k, v = torch.randn(n, 1, head, generator=g), torch.randn(n, 1, head, generator=g) * top
         v[zeros] = 0.0
         k, v, q = k.to(dtype), v.to(torch.bfloat16).float(), torch.randn(heads, head, generator=g).to(dtype)
         cache = lm.kv_cache(60, page, 1, head, E4M3)
-        table = torch.arange(60, dtype=torch.int32)[None].cuda()
+        table = torch.arange((n + page - 1) // page, dtype=torch.int32)[None].cuda()
         slots = torch.arange(n).cuda()
         lm.cache_write(cache, k.float().cuda(), v.cuda(), slots)
         (k, _), (v, e) = att.quantise(k[:, 0].double()), att.quantise(v[:, 0].double())
         e = torch.where(v.any(1), e, -96)  # a row of zeros has no say in the weights' step
         want, bound = attend(q.double(), k, v, head ** -0.5, dtype, E4M3, e.long())
-        att.assert_close(decode(lm, q, cache, table, n, None), want, bound, f"{dtype} {top} {zeros}")
+        check_decode(lm, q, cache, table, n, None, want, bound, f"{dtype} {top} {zeros}")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -113,7 +128,7 @@ def test_decode_scales_at_the_ends(lm, dtype, n):
             v = v * torch.exp2(e.double())[:, None]
             q = torch.ones(4, head, dtype=dtype)
             want, bound = attend(q.double(), k.double(), v, powers(bits, head), dtype, E4M3, e)
-            att.assert_close(decode(lm, q, cache, table, n, powers(bits, head)), want, bound, f"{bits} {order}")
+            check_decode(lm, q, cache, table, n, powers(bits, head), want, bound, f"{bits} {order}")
 
 
 @pytest.mark.parametrize("dtype,kind", KINDS)
@@ -132,7 +147,7 @@ def test_decode_one_key_far_above_the_others(lm, dtype, kind, bits, n, heads, he
         q = torch.ones(heads, head, dtype=dtype)
         scale = powers(bits, head)
         want, bound = attend(q.double(), k.double(), v.double(), scale, dtype, kind)
-        att.assert_close(decode(lm, q, cache, table, n, scale), want, bound, f"{dtype} {kind} {where}")
+        check_decode(lm, q, cache, table, n, scale, want, bound, f"{dtype} {kind} {where}")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
@@ -167,7 +182,7 @@ def test_decode_queries_with_one_large_element_over_8_bits(lm, dtype, heads, hea
     cache, table, _ = stored(lm, k, v, E4M3)
     scale = 512 / head ** 0.5
     want, bound = attend(q.double(), k.double(), v.double(), scale, dtype, E4M3)
-    att.assert_close(decode(lm, q, cache, table, n, scale), want, bound)
+    check_decode(lm, q, cache, table, n, scale, want, bound)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -186,7 +201,7 @@ def test_decode_weights_keep_more_than_16_bits(lm, dtype, heads, head):
     work = 2 * d + 2 * 2.0 ** -21 + ROUND[dtype] ** 2 + 2 * (n + 16) * 2.0 ** -24
     bound = ROUND[dtype] * want.abs() + work * mag + 2.0 ** -40 * p.amax() * n + TINY[dtype]
     assert (want.abs() > 2 * bound).all()
-    att.assert_close(decode(lm, q, cache, table, n, scale), want, bound)
+    check_decode(lm, q, cache, table, n, scale, want, bound)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])

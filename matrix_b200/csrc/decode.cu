@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // A warp works by itself: it copies the keys and values of its tile (16 of a half type, 32 of 8 bits) into a ring of its own
 // in shared memory, up to kStages of them (192 KB an SM in flight and in use), and multiplies them on the tensor cores: 16
 // keys are the rows and 8 or 16 queries (those that a unit lacks are zeros) the columns of K Q', 16 elements of the head are
-// the rows of V' P'.  Warp-wide products, since the keys pass once and HBM bounds them (the tensor pipe is busy for 10 to 15 %):
+// the rows of V' P'.  Warp-wide products, since the keys pass once and HBM bounds them (the tensor pipe is busy for 15 %):
 // tcgen05's tiles of 128 rows would be filled by waiting for 128 keys.  (With the queries as 16 rows, half of them zeros for a
 // group of 8, both took twice the products, registers and exponentials: 228 us for [4 x 91k] e4m3.)  There is no barrier between
 // warps, and the copies run on across the borders of units and sequences.  The page numbers of a tile are loaded one tile before
@@ -217,10 +217,11 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // the time (235 us for 232).  Over 8 bits, where the issue of instructions counts, weights are float16 (2.1e-4, of which 2.0e-4
 // are the result's rounding).
 //
-// Measured, heads of 128, 32 over 8: 64 sequences of 1,024 to 8,192 tokens bf16 220 us, 5.7 TB/s (0.87 of the copy figure), 4 of
-// 16,384 to 131,072 in 8 bits under 56 heads f16 168 us, 5.6 TB/s.  Bound by HBM and, at the end, by the SMs that get less of it
-// than others: equal shares end 157 to 191 us after the start.  In 8 bits 8 warps with three tiles took 195 us (bound by each
-// warp's latency), 12 with two 168.
+// Measured, heads of 128, 32 over 8: 64 sequences of 1,024 to 8,192 tokens bf16 224 us in a few calls, 5.6 TB/s (0.85 of the copy
+// figure), 235 back to back for a second, under the power limit; 4 of 16,384 to 131,072 in 8 bits under 56 heads f16 172 us, 5.4
+// TB/s, and 195.  Bound by HBM and, at the end, by the SMs that get less of it than others: equal shares of 8 bits ended 157 to
+// 191 us after the start.  In 8 bits 8 warps with three tiles took 195 us in a few calls (bound by each warp's latency) where 12
+// with two took 168.
 //
 // In 8 bits the bytes become float16, which holds them exactly, beside queries as float16 with their largest element between
 // 2^15 and 2^16 (their rows' powers of two, like the keys' scales, come back into the scores): float16 ones keep every bit,
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // those are 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are.  The weights of the
 // denominator are 2^(s - m') with a maximum m' of their own: m lies up to 2^96 from it, and 2^(s - m) would lose or overflow
 // the sum.  A row of values that is all zeros (its scale is 2^0, whatever its neighbours have) does not lift m: the rows are
-// looked through in the tiles that lift it.  Both together 2 % of the time ([4 x 91k]: 167 -> 170 us).
+// looked through in the tiles that lift it.  Both together 2 % of the time ([4 x 91k]: 191 -> 194 us).
 //
 // float16 weights are taken 2^15 times: the largest is 2^15 (65,504 is the type's last), and what is rounded to multiples of
 // 2^-24 is the part of them below 2^-29 of it.  Without, a key with nearly all the weight rounded 131,071 others of 2^-25.2 to

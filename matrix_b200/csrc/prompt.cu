@@ -267,10 +267,15 @@ int launch_any(const mtxc_prompt_attention_args* a, const Prompt& p) {
 // rounding is to multiples of 2^-24).  At 1 and 2^8 a key with nearly all the weight left others of 2^-25 as nothing or twice
 // what they are, and those are the output where its value is 0.
 //
-// Measured, 32 heads of 128 over 8, bf16: two prompts of 8,192 tokens 890 us, 1,236 TFLOP/s (0.74 of cuBLAS's burst), of 8,192
-// and 3,903 tokens 576 us, 1,171; 24 prompts of 105 to 777 tokens, 16 heads of 64, f16: 75 us, 242.  Bound by the exchange of a
-// tile between its softmax and its products: the tensor cores are busy for half of the time at heads of 128 and for a quarter at
-// 64, whose products take half as long and whose softmax as long; the exponentials' unit for 38 %.
+// Measured, 32 heads of 128 over 8, bf16: two prompts of 8,192 tokens 898 us in a few calls, 1,225 TFLOP/s (0.73 of cuBLAS's
+// burst), of 8,192 and 3,903 tokens 572 us, 1,180, and back to back for a second, under the power limit, 663 us, 1,015; 24 prompts
+// of 105 to 777 tokens, 16 heads of 64, f16: 77 us, 237.  Heads of 80 and 96 take the work of 128, of 136 to 192 that of 256 (two
+// prompts of 4,096 tokens, 16 heads of 64, 80, 96, 128, 160, 192, 256 over 4: 113, 134, 140, 140, 328, 328, 333 us).
+// Weights are operands of 16 bits, which adds to the result's own rounding (relative 0.0021 against 64 bits in bfloat16, of which
+// 0.0016 are that rounding; 2.6e-4 and 2.1e-4 in float16): a second operand, as in decode, would be half as many products again
+// and more to make for the softmax.  Bound by the exchange of a tile between its softmax and its products: the tensor cores are
+// busy for half of the time at heads of 128 and for a quarter at 64, whose products take half as long and whose softmax as long;
+// the exponentials' unit for 38 %.
 //
 // What a row does not see gets the weight 0, which is not enough where the value is NaN or infinite (another sequence's
 // row, a later token).  The two cleaning warps look through the tiles of values that some row does not see whole: rows

@@ -358,7 +358,7 @@ extern "C" int mtxc_cache_write(int dtype, const mtxc_cache_rows_args* a) {
     if (int rc = require_init()) return rc;
     Rows r{};
     if (int rc = prepare("mtxc_cache_write", dtype, a, &r)) return rc;
-    if (int rc = distinct("mtxc_cache_write", {a->cache.data[0], a->cache.data[1]})) return rc;
+    if (int rc = distinct("mtxc_cache_write", {a->cache.data[0], a->cache.data[1], a->cache.exponents[0], a->cache.exponents[1]})) return rc;
     if (!r.tokens || !r.heads || !r.head || !r.cache.slots) return MTXC_OK;
     const bool small = a->cache.dtype == MTXC_FLOAT8_E4M3;
     int rc = MTXC_OK;

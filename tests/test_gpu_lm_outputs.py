@@ -132,3 +132,24 @@ def test_outputs_over_their_input_in_another_order_are_refused(lm):
     again = one.clone()
     odd = torch.as_strided(again, (1, 4, 64), (7, 64, 1))
     assert torch.equal(lm.prompt_attention(again, one, one, starts // 4, out=odd), want)
+
+
+def test_one_tensor_for_both_exponents(lm):
+    """Read by every call, written by none: keys and values have different scales."""
+    e4m3 = torch.float8_e4m3fn
+    cache = lm.kv_cache(2, 4, 2, 64, e4m3)
+    shared = lm.KVCache(cache.keys, cache.values, cache.key_exponents, cache.key_exponents)
+    k, slots = torch.randn(8, 2, 64, device="cuda"), torch.arange(8).cuda()
+    with pytest.raises(MtxcError) as e:
+        lm.cache_write(shared, k, k * 100, slots)
+    assert e.value.code == _abi.ERR_INVALID_ARGUMENT
+    torch.cuda.synchronize()
+    assert not cache.keys.view(torch.uint8).any() and not cache.key_exponents.any()
+    lm.cache_write(cache, k, k.flip(0), slots)
+    cache.key_exponents.fill_(-7)
+    cache.value_exponents.fill_(-7)
+    for got, want in zip(lm.cache_read(shared, slots), lm.cache_read(cache, slots)):
+        assert torch.equal(got, want)
+    table, n = torch.tensor([[0, 1]], dtype=torch.int32).cuda(), torch.tensor([7], dtype=torch.int32).cuda()
+    q = torch.randn(1, 4, 64, device="cuda").half()
+    assert torch.equal(lm.decode_attention(q, shared, table, n), lm.decode_attention(q, cache, table, n))

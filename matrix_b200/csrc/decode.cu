@@ -926,6 +926,8 @@ extern "C" int mtxc_decode_attention(int dtype, const mtxc_decode_attention_args
     if (int rc = laid_alike(who, a->out, a->out_strides, a->q, a->q_strides, {a->batch, a->heads})) return rc;
     const size_t bytes = partial_bytes(d);
     d.partial = static_cast<float*>(a->workspace ? a->workspace : ctx().workspace);
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 256)
+        return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": the workspace must be aligned to 256 bytes");
     if (bytes > (a->workspace ? a->workspace_bytes : ctx().workspace_bytes))
         return fail(MTXC_ERR_WORKSPACE, who + ": the partial sums need " + std::to_string(bytes) + " bytes of workspace");
     const bool small = a->cache.dtype == MTXC_FLOAT8_E4M3;

@@ -611,6 +611,8 @@ extern "C" int mtxc_head_norm_rotary_backward(int dtype, const mtxc_head_norm_ar
     if (!a->head_dim) return MTXC_OK;
     const size_t bytes = partial_bytes(p, a);
     float* partial = static_cast<float*>(a->workspace ? a->workspace : ctx().workspace);
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 256)
+        return fail(MTXC_ERR_INVALID_ARGUMENT, who + ": the workspace must be aligned to 256 bytes");
     if (bytes > (a->workspace ? a->workspace_bytes : ctx().workspace_bytes))
         return fail(MTXC_ERR_WORKSPACE, who + ": the partial sums need " + std::to_string(bytes) + " bytes of workspace");
     const float* rows[2] = {nullptr, nullptr};

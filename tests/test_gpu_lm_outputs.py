@@ -153,3 +153,25 @@ def test_one_tensor_for_both_exponents(lm):
     table, n = torch.tensor([[0, 1]], dtype=torch.int32).cuda(), torch.tensor([7], dtype=torch.int32).cuda()
     q = torch.randn(1, 4, 64, device="cuda").half()
     assert torch.equal(lm.decode_attention(q, shared, table, n), lm.decode_attention(q, cache, table, n))
+
+
+def test_a_workspace_off_its_alignment_is_refused(lm):
+    q, k, dq, dk, w, positions, f, o, _ = heads_case(lm, torch.float32, False, 64, 64)
+    dst, dw = (torch.full_like(q, 7.0), torch.full_like(k, 7.0)), torch.empty(2, 64, device="cuda")
+    workspace = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    cache, table = lm.kv_cache(1, 16, 1, 64, torch.float32), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    x, n = torch.ones(1, 2, 64, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(x, 7.0)
+    lib = _abi.lib()
+    for off, status in ((1, _abi.ERR_INVALID_ARGUMENT), (4, _abi.ERR_INVALID_ARGUMENT), (128, _abi.ERR_INVALID_ARGUMENT), (0, 0)):
+        args = backward_args(q, k, dq, dk, dst, [o.q_rstd, o.k_rstd], w, positions, f, False, workspace[off:], (dw[0], dw[1]))
+        assert lib.mtxc_head_norm_rotary_backward(0, args) == status
+        args = packed(_abi.DECODE_ATTENTION_FIELDS, _abi.DECODE_ATTENTION_ARGS, {
+            "cache.pages": 1, "cache.page_size": 16, "cache.heads": 1, "cache.head_dim": 64, "cache.data": cache[:2],
+            "cache.strides": strides(*cache[:2]), "batch": 1, "max_pages": 1, "heads": 2, "scale": 0.125, "q": x,
+            "q_strides": x.stride()[:2], "out": out, "out_strides": out.stride()[:2], "page_table": table, "page_table_stride": 1,
+            "lengths": n, "workspace": workspace[off:], "workspace_bytes": workspace.numel() - off})
+        assert lib.mtxc_decode_attention(0, args) == status
+        torch.cuda.synchronize()
+        assert (out == 7).all() == bool(status) and (dst[0] == 7).all() == bool(status)
+    assert not out.any()

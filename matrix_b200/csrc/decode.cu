@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_any_kernel(const Decode d)
 // 2^15 and 2^16 (their rows' powers of two, like the keys' scales, come back into the scores): float16 ones keep every bit,
 // bfloat16 ones theirs down to 2^-32 of the largest.  The values' scales 2^e go into the weights that meet them:
 // those are 2^(s + e - m) with m the running maximum of s + e, at most 1 whatever the scales are.  The weights of the
-// denominator are 2^(s - m') with a maximum m' of their own: m lies up to 2^96 from it, and 2^(s - m) would lose or overflow
+// denominator are 2^(s - m') with a maximum m' of their own: m lies up to 96 from it, and 2^(s - m) would lose or overflow
 // the sum.  A row of values that is all zeros (its scale is 2^0, whatever its neighbours have) does not lift m: the rows are
 // looked through in the tiles that lift it.  Both together 2 % of the time ([4 x 91k]: 191 -> 194 us).
 //
